@@ -12,6 +12,8 @@ softmax, so nothing is gathered or compacted.
     cache tokens [0, kv_len) (+ optional tail), block-causal at chunk
     granularity (the BASELINE config-3 workload), with optional key masks and
     a one-slot cache read by every query batch.
+  * ``sparse_chunk_attention``: the same over chosen blocks of the history (the
+    lists of kv_history.select_blocks), with the rows' log-sum-exp.
   * ``causal_attention_with_cache_mp``: the reference's cached-attention entry
     point (nomas_cpt.py:335-884) for quantized caches: same arguments, same
     cache write (validate K and V, then quantize at ``cache_valid_len``, then
@@ -62,6 +64,28 @@ def chunk_attention(q: torch.Tensor, kv_cache: dict, kv_len: int, *,
                           kv_cache["v_scale"], kv_len, k_cur, v_cur, q_pos0, chunk_len,
                           None if softmax_scale is None else float(softmax_scale),
                           cache_valid, cur_valid)
+
+
+def sparse_chunk_attention(q: torch.Tensor, kv_cache: dict, kv_len: int, block_idx: Optional[torch.Tensor], *,
+                           block: int = 64, q_block: int = 128, k_cur: Optional[torch.Tensor] = None,
+                           v_cur: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
+                           cache_valid: Optional[torch.Tensor] = None,
+                           cur_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """softmax(q K^T * scale) V over chosen blocks of cache tokens [0, kv_len) then
+    k_cur/v_cur, and the rows' log-sum-exp: (out [B, Lq, Hq, D], lse fp32 [B, Hq, Lq]).
+
+    block_idx int32 [B, H, ceil(Lq / q_block), K] names the blocks of ``block``
+    tokens that each run of ``q_block`` queries reads (kv_history.select_blocks),
+    ended by the first negative entry; None reads the whole cache. Hq may be a
+    multiple of the cache's heads. Every listed key is visible to the run's queries;
+    cache_valid and cur_valid are as in chunk_attention. A query without a key gets
+    a zero row and lse -inf.
+    """
+    if not is_quantized_kv_cache(kv_cache):
+        raise TypeError("sparse_chunk_attention reads FP8/INT8 caches")
+    return ops.attn_kv_blocks(q, kv_cache["k"], kv_cache["v"], kv_cache["k_scale"], kv_cache["v_scale"], kv_len,
+                              block_idx, block, q_block, k_cur, v_cur,
+                              None if softmax_scale is None else float(softmax_scale), cache_valid, cur_valid)
 
 
 def _dense_sparse_context(sparse_context, kv_cache, update_cache):

@@ -1,0 +1,98 @@
+"""A history longer than what is read or kept: the quantized KV cache by blocks.
+
+A roll-out outlives any fixed cache, and most of a long history draws little
+attention. The reference answers with routed sparse attention and with history
+policies (nomas_cache_sparse.py, swa_cache.py, uniform_history_cache.py); here
+both work on the FP8/INT8 cache of fp8_kv_cache.py in place:
+
+  make_block_bounds / update_block_bounds
+      per block of tokens and head, the smallest and largest value of every key
+      channel: kept beside the cache, brought up to date after each write
+  select_blocks
+      the blocks that each run of queries reads: those whose bounds allow the
+      largest logits, with the first and the newest always among them;
+      cache_attention.sparse_chunk_attention attends over them
+  key_mass
+      the attention weight that every cached key drew, added up over calls
+  select_tokens / evict
+      the tokens of largest mass, moved to the front of another cache; keys carry
+      their rotation, so a moved token keeps its position
+
+The choices are exact (scores in 64 bits, ties to the lowest index): the same
+inputs give the same blocks and tokens.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import ops
+from .fp8_kv_cache import _storage
+
+STORAGE_KEYS = ("k", "v", "k_scale", "v_scale")
+
+
+def make_block_bounds(cache: dict, *, block: int = 64) -> torch.Tensor:
+    """Bounds of an empty cache: bf16 [B, ceil(cap / block), H, 2, D], +inf / -inf."""
+    codes, _ = _storage(cache, "k")
+    if block not in ops.BLOCK_SIZES:
+        raise ValueError(f"block must be one of {ops.BLOCK_SIZES}")
+    B, cap, H, D = codes.shape
+    bounds = torch.empty((B, -(-cap // block), H, 2, D), dtype=torch.bfloat16, device=codes.device)
+    bounds[:, :, :, 0].fill_(float("inf"))
+    bounds[:, :, :, 1].fill_(float("-inf"))
+    return bounds
+
+
+def update_block_bounds(bounds: torch.Tensor, cache: dict, start: int, end: int, *, block: int = 64,
+                        cache_valid: Optional[torch.Tensor] = None) -> None:
+    """Bring the blocks that tokens [start, end) fall in up to date after a write of
+    those tokens (``end`` is the cache's new length: later tokens do not count).
+    cache_valid (bool [B or 1, >= end]) leaves invalid tokens out."""
+    codes, scale = _storage(cache, "k")
+    ops.kv_block_bounds_(bounds, codes, scale, start, end, block, cache_valid)
+
+
+def select_blocks(q: torch.Tensor, bounds: torch.Tensor, kv_len: int, top_k: int, *, block: int = 64,
+                  q_block: int = 128, keep_first: int = 0, keep_last: int = 0,
+                  q_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Block lists int32 [B, H, ceil(Lq / q_block), top_k] for
+    cache_attention.sparse_chunk_attention (ops.select_kv_blocks)."""
+    return ops.select_kv_blocks(q, bounds, kv_len, top_k, block, q_block, keep_first, keep_last, q_valid)
+
+
+def key_mass(q: torch.Tensor, lse: torch.Tensor, cache: dict, kv_len: int, *,
+             prior: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
+             cache_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention weight of cached keys [0, kv_len) from queries q [B, Lq, Hq, D] with
+    log-sum-exps lse [B, Hq, Lq] (of the attention that q ran), onto ``prior``: a new
+    fp32 [B, H, kv_len] (ops.attn_key_mass)."""
+    codes, scale = _storage(cache, "k")
+    return ops.attn_key_mass(q, lse, codes, scale, kv_len, prior,
+                             None if softmax_scale is None else float(softmax_scale), cache_valid)
+
+
+def select_tokens(mass: torch.Tensor, kv_len: int, keep: int, *, keep_first: int = 0, keep_last: int = 0,
+                  cache_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The tokens of [0, kv_len) that stay in each head, int32 [B, H, keep]
+    (ops.select_kv_tokens)."""
+    return ops.select_kv_tokens(mass, kv_len, keep, keep_first, keep_last, cache_valid)
+
+
+def evict(cache: dict, out: dict, mass: torch.Tensor, kv_len: int, keep: int, *, keep_first: int = 0,
+          keep_last: int = 0, cache_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keep ``keep`` of the tokens [0, kv_len) of every head in ``out``, another cache
+    of the same heads and format: select_tokens, then codes, scales and mass of the
+    chosen ones moved to its rows [0, keep). Returns (idx, mass of the kept tokens),
+    int32 and fp32 [B, H, keep]. With fewer valid tokens than ``keep``, idx ends in
+    -1 and those rows of ``out`` stay as they are; a batch has as many in every head,
+    so ``idx[:, 0] >= 0`` is the validity of out's rows."""
+    for c in (cache, out):
+        for key in ("k", "v"):
+            _storage(c, key)
+    if mass.ndim == 3 and mass.shape[2] > cache["k"].shape[1]:
+        mass = mass[:, :, :kv_len]
+    idx = ops.select_kv_tokens(mass, kv_len, keep, keep_first, keep_last, cache_valid)
+    moved = ops.move_kv_tokens_(*(out[n] for n in STORAGE_KEYS), *(cache[n] for n in STORAGE_KEYS), mass, idx)
+    return idx, moved

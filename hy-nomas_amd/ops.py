@@ -728,3 +728,386 @@ def attn_fp8kv(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
 def _(q, k_codes, v_codes, k_scale, v_scale, kv_len, k_cur=None, v_cur=None, q_pos0=0,
       chunk_len=0, softmax_scale=None, cache_valid=None, cur_valid=None):
     return torch.empty_like(q)
+
+
+# --------------------------------------------------------------------------
+# long history: block bounds, block choice, sparse attention, key mass, eviction
+
+BLOCK_SIZES = (64, 128, 256, 512, 1024)
+
+
+def _check_block(block: int, what: str) -> None:
+    if block not in BLOCK_SIZES:
+        raise ValueError(f"{what}: block must be one of {BLOCK_SIZES}")
+
+
+def _check_keys(codes: torch.Tensor, scale: torch.Tensor, what: str) -> None:
+    """Codes [B, cap, H, D] with fp32 scales [B, cap, H, 1]."""
+    if codes.ndim != 4 or scale.dtype != torch.float32 or tuple(scale.shape) != (*codes.shape[:3], 1):
+        raise ValueError(f"{what}: codes [B, cap, H, D] with fp32 scales [B, cap, H, 1]")
+
+
+def _one_device(what: str, *tensors) -> None:
+    """Every tensor given is on a GPU, and all on the same one."""
+    _gpu(*tensors)
+    first = next(t for t in tensors if t is not None)
+    if any(t is not None and t.device != first.device for t in tensors):
+        raise RuntimeError(f"{what}: tensors are on different devices")
+
+
+def _mask_bytes(mask: Optional[torch.Tensor], rows: int, cols: int, what: str):
+    """A validity mask as (uint8 view, batch stride): bool or uint8 [rows or 1, >= cols]."""
+    if mask is None:
+        return None, 0
+    if mask.dtype not in (torch.bool, torch.uint8) or mask.ndim != 2:
+        raise TypeError(f"{what} must be a bool [B, L] mask")
+    if mask.shape[0] not in (rows, 1) or mask.shape[1] < cols:
+        raise ValueError(f"{what} must cover [{rows}, {cols}]")
+    if mask.shape[1] > 1 and mask.stride(1) != 1:
+        mask = mask.contiguous()
+    return mask.view(torch.uint8), 0 if mask.shape[0] == 1 else mask.stride(0)
+
+
+def _softmax_scale(softmax_scale: Optional[float], D: int, what: str) -> float:
+    if softmax_scale is None:
+        return D ** -0.5
+    if not (softmax_scale > 0 and math.isfinite(softmax_scale)):
+        raise ValueError(f"{what}: softmax_scale must be finite and positive")
+    return float(softmax_scale)
+
+
+def kv_block_bounds_(bounds, k_codes, k_scale, start: int, end: int, block: int = 64, valid=None) -> None:
+    """Bounds of the cached keys of the blocks that tokens [start, end) fall in,
+    per channel (see _kv_block_bounds_op)."""
+    _kv_block_bounds_op(bounds, k_codes, k_scale, start, end, block, valid)
+
+
+@eager_op("hy_nomas_amd::kv_block_bounds_", mutates_args=("bounds",))
+def _kv_block_bounds_op(bounds: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor, start: int, end: int,
+                        block: int, valid: Optional[torch.Tensor]) -> None:
+    """bounds[b, j, h, 0] = min and [..., 1] = max of bf16(code * scale) over the
+    tokens t < end of block j with valid[b, t] (bool [B or 1, >= end]; None: all),
+    for the blocks of ``block`` tokens that [start, end) touches; +inf / -inf for a
+    block without one. bounds: bf16 [B, >= ceil(end / block), H, 2, D]."""
+    what = "kv_block_bounds_"
+    fmt = _kv_fmt(k_codes)
+    _check_keys(k_codes, k_scale, what)
+    _check_block(block, what)
+    B, cap, H, D = k_codes.shape
+    if not 0 <= start <= end <= cap:
+        raise ValueError(f"{what}: tokens [{start}, {end}) outside the cache capacity {cap}")
+    if (bounds.dtype != torch.bfloat16 or bounds.ndim != 5 or bounds.shape[0] != B
+            or bounds.shape[1] * block < end or tuple(bounds.shape[2:]) != (H, 2, D)):
+        raise ValueError(f"{what}: bounds must be bf16 [B, ceil(end / block), H, 2, D]")
+    if bounds.stride(4) != 1 or bounds.stride(3) != D:
+        raise ValueError(f"{what}: the two bounds of a head must be contiguous")
+    vb, vs = _mask_bytes(valid, B, end, f"{what}: valid")
+    _one_device(what, k_codes, k_scale, bounds, vb)
+    with _on(k_codes.device):
+        L.check(L.load().hn_kv_block_bounds(
+            fmt, k_codes.data_ptr(), L.strides(k_codes), k_scale.data_ptr(), L.strides(k_scale), B, H, D, cap, start,
+            end, block, L.ptr(vb), vs, bounds.data_ptr(), L.strides(bounds), bounds.shape[1], _stream(k_codes)),
+            "hn_kv_block_bounds")
+
+
+@_kv_block_bounds_op.register_fake
+def _(bounds, k_codes, k_scale, start, end, block, valid):
+    return None
+
+
+@eager_op("hy_nomas_amd::select_kv_blocks", mutates_args=())
+def select_kv_blocks(q: torch.Tensor, bounds: torch.Tensor, kv_len: int, top_k: int, block: int = 64,
+                     q_block: int = 128, keep_first: int = 0, keep_last: int = 0,
+                     q_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The blocks that each run of ``q_block`` queries reads of tokens [0, kv_len):
+    int32 [B, H, ceil(Lq / q_block), top_k], ascending, -1 behind the last.
+
+    q: bf16 [B, Lq, Hq, D], Hq a multiple of the bounds' H; bounds as
+    kv_block_bounds_ writes them, [B or 1, n, H, 2, D]. Chosen are the first
+    ``keep_first`` and the last ``keep_last`` blocks and those of the highest score,
+    an upper bound of the run's logits; see hn_select_kv_blocks. q_valid (bool [B or 1, >= Lq]) leaves
+    padded queries out of the score."""
+    what = "select_kv_blocks"
+    _check_block(block, what)
+    if q.dtype != torch.bfloat16 or bounds.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects bf16 queries and bounds")
+    if q.ndim != 4 or bounds.ndim != 5:
+        raise ValueError(f"{what}: q [B, Lq, Hq, D] with bounds [B or 1, n, H, 2, D]")
+    B, Lq, Hq, D = q.shape
+    H = bounds.shape[2]
+    if bounds.shape[0] not in (B, 1) or tuple(bounds.shape[3:]) != (2, D) or H == 0 or Hq % H:
+        raise ValueError(f"{what}: bounds do not match q's batch, heads and dim")
+    if kv_len < 0 or bounds.shape[1] * block < kv_len:
+        raise ValueError(f"{what}: kv_len {kv_len} outside the bounds' {bounds.shape[1]} blocks")
+    if q_block < 1 or top_k < 1:
+        raise ValueError(f"{what}: q_block and top_k must be positive")
+    if keep_first < 0 or keep_last < 0 or keep_first + keep_last > top_k:
+        raise ValueError(f"{what}: keep_first + keep_last exceeds top_k")
+    if bounds.stride(4) != 1 or bounds.stride(3) != D:
+        raise ValueError(f"{what}: the two bounds of a head must be contiguous")
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if bounds.shape[0] != B:
+        bounds = bounds.expand(B, -1, -1, -1, -1)
+    vb, vs = _mask_bytes(q_valid, B, Lq, f"{what}: q_valid")
+    _one_device(what, q, bounds, vb)
+    runs, blocks = -(-Lq // q_block), -(-kv_len // block)
+    idx = torch.empty((B, H, runs, top_k), dtype=torch.int32, device=q.device)
+    with _on(q.device):
+        lib = L.load()
+        ws_bytes = lib.hn_select_kv_blocks_workspace_size(B, H, runs, blocks)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+        L.check(lib.hn_select_kv_blocks(
+            q.data_ptr(), L.strides(q), B, Lq, Hq, D, L.ptr(vb), vs, bounds.data_ptr(), L.strides(bounds), H, blocks,
+            q_block, top_k, keep_first, keep_last, idx.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)),
+            "hn_select_kv_blocks")
+    return idx
+
+
+@select_kv_blocks.register_fake
+def _(q, bounds, kv_len, top_k, block=64, q_block=128, keep_first=0, keep_last=0, q_valid=None):
+    return q.new_empty((q.shape[0], bounds.shape[2], -(-q.shape[1] // q_block), top_k), dtype=torch.int32)
+
+
+@eager_op("hy_nomas_amd::attn_kv_blocks", mutates_args=())
+def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor, kv_len: int, block_idx: Optional[torch.Tensor] = None, block: int = 64,
+                   q_block: int = 128, k_cur: Optional[torch.Tensor] = None, v_cur: Optional[torch.Tensor] = None,
+                   softmax_scale: Optional[float] = None, cache_valid: Optional[torch.Tensor] = None,
+                   cur_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of q [B, Lq, Hq, D] over the listed blocks of cache tokens [0,
+    kv_len) and the bf16 tail k_cur/v_cur [B, Lc, H, D]: out bf16 [B, Lq, Hq, D] and
+    the rows' log-sum-exp fp32 [B, Hq, Lq].
+
+    block_idx: int32 [B, H, ceil(Lq / q_block), K], the blocks that the queries of
+    each run read, ended by the first negative entry (None: every cached token).
+    Hq is a multiple of the cache's H. The cache may hold B slots or one that every
+    query batch reads. See hn_attn_kv_blocks."""
+    what = "attn_kv_blocks"
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects bf16 queries")
+    fmt = _kv_fmt(k_codes)
+    _check_keys(k_codes, k_scale, what)
+    _check_block(block, what)
+    if q.ndim != 4:
+        raise ValueError(f"{what}: q must be [B, Lq, Hq, D]")
+    B, Lq, Hq, D = q.shape
+    cap, H = k_codes.shape[1:3]
+    if k_codes.shape[0] not in (B, 1) or k_codes.shape[3] != D or H == 0 or Hq % H:
+        raise ValueError(f"{what}: cache [B or 1, cap, H, D] does not match q")
+    if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride()
+            or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape
+            or v_scale.stride() != k_scale.stride()):
+        raise ValueError(f"{what}: K and V must share dtype, shape and strides")
+    if not 0 <= kv_len <= cap:
+        raise ValueError(f"{what}: kv_len {kv_len} outside the cache capacity {cap}")
+    if q_block < 1:
+        raise ValueError(f"{what}: q_block must be positive")
+    runs = -(-Lq // q_block)
+    if block_idx is not None:
+        if block_idx.dtype != torch.int32 or block_idx.ndim != 4 or tuple(block_idx.shape[:3]) != (B, H, runs):
+            raise ValueError(f"{what}: block_idx must be int32 [B, H, ceil(Lq / q_block), K]")
+        if block_idx.shape[3] == 0:  # empty lists (a null pointer would mean no list)
+            block_idx = block_idx.new_full((B, H, runs, 1), -1)
+        elif block_idx.stride(3) != 1:
+            block_idx = block_idx.contiguous()
+    scale = _softmax_scale(softmax_scale, D, what)
+    if k_codes.shape[0] != B:  # one history slot read by every query batch
+        k_codes, v_codes = k_codes.expand(B, -1, -1, -1), v_codes.expand(B, -1, -1, -1)
+        k_scale, v_scale = k_scale.expand(B, -1, -1, -1), v_scale.expand(B, -1, -1, -1)
+    cur_len = 0 if k_cur is None else k_cur.shape[1] if k_cur.ndim == 4 else -1
+    if k_cur is not None and (k_cur.ndim != 4 or k_cur.shape[0] != B or tuple(k_cur.shape[2:]) != (H, D)):
+        raise ValueError(f"{what}: k_cur must be [B, Lc, H, D] matching the cache")
+    if (k_cur is None) != (v_cur is None) or (k_cur is not None and (
+            v_cur.shape != k_cur.shape or k_cur.dtype != torch.bfloat16 or v_cur.dtype != torch.bfloat16)):
+        raise ValueError(f"{what}: k_cur/v_cur must be matching bf16 tensors")
+    q = _head_rows(q)
+    if cur_len:
+        k_cur, v_cur = _head_rows(k_cur), _head_rows(v_cur)
+        if k_cur.stride() != v_cur.stride():
+            k_cur, v_cur = k_cur.contiguous(), v_cur.contiguous()
+    kvb, kvs = _mask_bytes(cache_valid if kv_len else None, B, kv_len, f"{what}: cache_valid")
+    uvb, uvs = _mask_bytes(cur_valid if cur_len else None, B, cur_len, f"{what}: cur_valid")
+    _one_device(what, q, k_codes, v_codes, k_scale, v_scale, block_idx, k_cur, v_cur, kvb, uvb)
+    out = torch.empty((B, Lq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+    top_k = -1 if block_idx is None else block_idx.shape[3]
+    with _on(q.device):
+        lib = L.load()
+        ws_bytes = lib.hn_attn_kv_blocks_workspace_size(B, Lq, Hq, H, kv_len, cur_len, top_k, block, q_block)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+        L.check(lib.hn_attn_kv_blocks(
+            fmt, q.data_ptr(), L.strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), L.strides(k_codes),
+            k_scale.data_ptr(), v_scale.data_ptr(), L.strides(k_scale), H, cap, kv_len, L.ptr(kvb), kvs,
+            L.ptr(block_idx), None if block_idx is None else L.strides(block_idx), max(top_k, 0),
+            block, q_block, L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
+            L.strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), L.strides(out),
+            lse.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_kv_blocks")
+    return out, lse
+
+
+@attn_kv_blocks.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, kv_len, block_idx=None, block=64, q_block=128, k_cur=None, v_cur=None,
+      softmax_scale=None, cache_valid=None, cur_valid=None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+def _head_rows(t: torch.Tensor) -> torch.Tensor:
+    """bf16 [B, L, H, D] as the kernels load it: rows of D contiguous values at
+    16-byte boundaries (a copy where it is laid out otherwise)."""
+    if t.stride(3) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(2) % 8:
+        return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+@eager_op("hy_nomas_amd::attn_key_mass", mutates_args=())
+def attn_key_mass(q: torch.Tensor, lse: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor, kv_len: int,
+                  prior: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
+                  cache_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention weight that cached keys [0, kv_len) draw from q [Bq, Lq, Hq, D]
+    whose rows have log-sum-exp lse [Bq, Hq, Lq], added to ``prior`` (fp32 [B, H, <=
+    kv_len], keys past it start at 0): a new fp32 [B, H, kv_len].
+
+    A cache of one slot (B = 1) collects the weight of every query batch. Invalid
+    keys (cache_valid bool [B or 1, >= kv_len]) and rows of infinite lse add nothing."""
+    what = "attn_key_mass"
+    if q.dtype != torch.bfloat16 or lse.dtype != torch.float32:
+        raise TypeError(f"{what} expects bf16 queries and fp32 log-sum-exps")
+    fmt = _kv_fmt(k_codes)
+    _check_keys(k_codes, k_scale, what)
+    if q.ndim != 4:
+        raise ValueError(f"{what}: q must be [B, Lq, Hq, D]")
+    Bq, Lq, Hq, D = q.shape
+    B, cap, H = k_codes.shape[:3]
+    if B not in (Bq, 1) or k_codes.shape[3] != D or H == 0 or Hq % H:
+        raise ValueError(f"{what}: cache [B or 1, cap, H, D] does not match q")
+    if tuple(lse.shape) != (Bq, Hq, Lq):
+        raise ValueError(f"{what}: lse must be [B, Hq, Lq]")
+    if not 0 <= kv_len <= cap:
+        raise ValueError(f"{what}: kv_len {kv_len} outside the cache capacity {cap}")
+    if prior is not None and (prior.dtype != torch.float32 or prior.ndim != 3 or tuple(prior.shape[:2]) != (B, H)
+                              or prior.shape[2] > kv_len):
+        raise ValueError(f"{what}: prior must be fp32 [B, H, <= kv_len]")
+    scale = _softmax_scale(softmax_scale, D, what)
+    q, lse = _head_rows(q), lse.contiguous()
+    if prior is not None and prior.stride(2) != 1:
+        prior = prior.contiguous()
+    kvb, kvs = _mask_bytes(cache_valid if kv_len else None, B, kv_len, f"{what}: cache_valid")
+    _one_device(what, q, lse, k_codes, k_scale, prior, kvb)
+    mass = torch.empty((B, H, kv_len), dtype=torch.float32, device=q.device)
+    n_prior = 0 if prior is None else prior.shape[2]
+    with _on(q.device):
+        lib = L.load()
+        ws_bytes = lib.hn_attn_key_mass_workspace_size(Bq, Lq, Hq, B, H, kv_len)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
+        L.check(lib.hn_attn_key_mass(
+            fmt, q.data_ptr(), L.strides(q), Bq, Lq, Hq, D, lse.data_ptr(), k_codes.data_ptr(), L.strides(k_codes),
+            k_scale.data_ptr(), L.strides(k_scale), B, H, cap, kv_len, L.ptr(kvb), kvs, scale,
+            L.ptr(prior) if n_prior else None, L.strides(prior) if n_prior else None, n_prior, mass.data_ptr(),
+            L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_key_mass")
+    return mass
+
+
+@attn_key_mass.register_fake
+def _(q, lse, k_codes, k_scale, kv_len, prior=None, softmax_scale=None, cache_valid=None):
+    return q.new_empty((k_codes.shape[0], k_codes.shape[2], kv_len), dtype=torch.float32)
+
+
+@eager_op("hy_nomas_amd::select_kv_tokens", mutates_args=())
+def select_kv_tokens(mass: torch.Tensor, kv_len: int, keep: int, keep_first: int = 0, keep_last: int = 0,
+                     cache_valid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The ``keep`` of tokens [0, kv_len) that stay in each head: int32 [B, H, keep],
+    ascending, -1 behind the last. Always the first ``keep_first`` and the last
+    ``keep_last``, then those of the largest mass (fp32 [B, H, >= kv_len]), ties to
+    the lowest index; only tokens that cache_valid (bool [B or 1, >= kv_len]) allows."""
+    what = "select_kv_tokens"
+    if mass.dtype != torch.float32 or mass.ndim != 3:
+        raise TypeError(f"{what} expects an fp32 [B, H, L] mass")
+    if not 0 <= kv_len <= mass.shape[2]:
+        raise ValueError(f"{what}: kv_len {kv_len} outside the mass's {mass.shape[2]} tokens")
+    if keep < 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > keep:
+        raise ValueError(f"{what}: keep_first + keep_last exceeds keep")
+    if mass.stride(2) != 1:
+        mass = mass.contiguous()
+    B, H = mass.shape[:2]
+    vb, vs = _mask_bytes(cache_valid if kv_len else None, B, kv_len, f"{what}: cache_valid")
+    _one_device(what, mass, vb)
+    idx = torch.empty((B, H, keep), dtype=torch.int32, device=mass.device)
+    if H == 0:
+        return idx
+    with _on(mass.device):
+        L.check(L.load().hn_select_kv_tokens(mass.data_ptr(), L.strides(mass), B, H, kv_len, L.ptr(vb), vs, keep,
+                                             keep_first, keep_last, idx.data_ptr(), _stream(mass)),
+                "hn_select_kv_tokens")
+    return idx
+
+
+@select_kv_tokens.register_fake
+def _(mass, kv_len, keep, keep_first=0, keep_last=0, cache_valid=None):
+    return mass.new_empty((mass.shape[0], mass.shape[1], keep), dtype=torch.int32)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges that two tensors span meet."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+@eager_op("hy_nomas_amd::move_kv_tokens_", mutates_args=("out_k", "out_v", "out_k_scale", "out_v_scale"))
+def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch.Tensor, out_v_scale: torch.Tensor,
+                    k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    mass: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
+    """Row i of each head of the output cache <- token idx[b, h, i] of the source, for
+    idx int32 [B, H, keep]; returns that token's mass, fp32 [B, H, keep]. An index
+    outside the mass's tokens leaves its row as it is (mass 0). The output cache is
+    another one than the source: [B, >= keep, H, D] of the same dtype."""
+    what = "move_kv_tokens_"
+    _kv_fmt(k_codes)
+    _check_keys(k_codes, k_scale, what)
+    _check_keys(out_k, out_k_scale, what)
+    B, cap, H, D = k_codes.shape
+    if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride()
+            or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape
+            or v_scale.stride() != k_scale.stride()):
+        raise ValueError(f"{what}: K and V must share dtype, shape and strides")
+    if (out_v.dtype != out_k.dtype or out_v.shape != out_k.shape or out_v.stride() != out_k.stride()
+            or out_v_scale.dtype != torch.float32 or out_v_scale.shape != out_k_scale.shape
+            or out_v_scale.stride() != out_k_scale.stride()):
+        raise ValueError(f"{what}: the output's K and V must share dtype, shape and strides")
+    if out_k.dtype != k_codes.dtype or (out_k.shape[0], *out_k.shape[2:]) != (B, H, D):
+        raise ValueError(f"{what}: the output cache does not match the source")
+    if mass.dtype != torch.float32 or mass.ndim != 3 or tuple(mass.shape[:2]) != (B, H) or mass.shape[2] > cap:
+        raise ValueError(f"{what}: mass must be fp32 [B, H, <= cap]")
+    if idx.dtype != torch.int32 or idx.ndim != 3 or tuple(idx.shape[:2]) != (B, H):
+        raise ValueError(f"{what}: idx must be int32 [B, H, keep]")
+    keep = idx.shape[2]
+    if keep > out_k.shape[1]:
+        raise ValueError(f"{what}: {keep} tokens exceed the output cache's capacity {out_k.shape[1]}")
+    _one_device(what, k_codes, v_codes, k_scale, v_scale, mass, idx, out_k, out_v, out_k_scale, out_v_scale)
+    for o in (out_k, out_v, out_k_scale, out_v_scale):
+        if any(_overlap(o, t) for t in (k_codes, v_codes, k_scale, v_scale, mass, idx)):
+            raise ValueError(f"{what}: the output cache overlaps the source")
+    if mass.stride(2) != 1:
+        mass = mass.contiguous()
+    idx = idx.contiguous()
+    moved = torch.empty((B, H, keep), dtype=torch.float32, device=mass.device)
+    if H == 0:
+        return moved
+    with _on(mass.device):
+        L.check(L.load().hn_move_kv_tokens(
+            k_codes.data_ptr(), v_codes.data_ptr(), L.strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(),
+            L.strides(k_scale), mass.data_ptr(), L.strides(mass), B, H, D, mass.shape[2], idx.data_ptr(), keep,
+            out_k.data_ptr(), out_v.data_ptr(), L.strides(out_k), out_k_scale.data_ptr(), out_v_scale.data_ptr(),
+            L.strides(out_k_scale), out_k.shape[1], moved.data_ptr(), _stream(mass)), "hn_move_kv_tokens")
+    return moved
+
+
+@move_kv_tokens_.register_fake
+def _(out_k, out_v, out_k_scale, out_v_scale, k_codes, v_codes, k_scale, v_scale, mass, idx):
+    return mass.new_empty(idx.shape, dtype=torch.float32)

@@ -291,6 +291,117 @@ int hn_qk_norm_rope_kv(int fmt, void *q, void *k, const void *v, const int64_t *
                        const int64_t *ss, int64_t cap, int64_t start, int32_t *status,
                        void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A long history: reading a few blocks of the cache instead of all of it, and
+ * keeping the tokens that drew attention when the cache is full. The
+ * reference's sparse routing and history policies (nomas_cache_sparse.py,
+ * swa_cache.py) are Python over other caches; these calls work on the quantized
+ * cache in place. Below, K and V are the held values bf16(code * scale), a cache
+ * has H heads, queries Hq = G H heads, query head h G + g reading cached head h.
+ * Blocks are runs of `block` tokens (64, 128, 256, 512 or 1024), block j holding
+ * tokens [j block, (j + 1) block).
+ */
+
+/* Bounds of the keys of the blocks that tokens [start, end) fall in, channel by
+ * channel: bounds[b, j, h, 0, :] = min, [.., 1, :] = max of K over the block's
+ * tokens t < end with valid[b * valid_stride + t] != 0 (valid NULL: all). A block
+ * without such a token gets +inf and -inf, by which hn_select_kv_blocks knows it.
+ *   kc, cs, ks, ss, cap: codes and scales as in hn_attn_fp8kv
+ *   bounds: bf16 [B, n_blocks, H, 2, 128], strides bs[3] of its first three dims
+ *           (multiples of 8), the last two contiguous; other blocks stay as they are
+ * The cached values are finite (the cache writers refuse others). */
+int hn_kv_block_bounds(int fmt, const void *kc, const int64_t *cs, const float *ks, const int64_t *ss,
+                       int64_t B, int64_t H, int64_t D, int64_t cap, int64_t start, int64_t end,
+                       int64_t block, const uint8_t *valid, int64_t valid_stride, void *bounds,
+                       const int64_t *bs, int64_t n_blocks, void *stream);
+
+/* The blocks that each run of q_block consecutive queries reads, of the first
+ * `blocks` blocks: with W_d = sum min(q_d, 0), U_d = sum max(q_d, 0) over the
+ * run's queries (q_valid[b * q_valid_stride + i] != 0; NULL: all) and the G query
+ * heads of a cached head, a block's score
+ *   sum_d W_d lo_d + U_d hi_d  >=  sum over the run's rows of q . K(t), any t in it,
+ * is formed in 64 bits (exact for values of the usual range) and rounded once to
+ * fp32. idx[b, h, run, :top_k] (int32, contiguous [B, H, runs, top_k]) are the
+ * blocks < keep_first and >= blocks - keep_last, then those of the highest scores,
+ * ties to the lowest index, in ascending order; empty blocks are never chosen,
+ * a NaN score ranks as -inf, and -1 fills the entries behind the last.
+ *   bounds: bf16 [B, blocks, H, 2, 128] with strides bs[3] (bs[0] == 0: one slot
+ *           read by every query batch)
+ * keep_first + keep_last <= top_k. workspace: hn_select_kv_blocks_workspace_size(B,
+ * H, ceil(Lq / q_block), blocks) bytes, 16-byte aligned. */
+int hn_select_kv_blocks(const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
+                        const uint8_t *q_valid, int64_t q_valid_stride, const void *bounds,
+                        const int64_t *bs, int64_t H, int64_t blocks, int64_t q_block, int64_t top_k,
+                        int64_t keep_first, int64_t keep_last, int32_t *idx, void *workspace,
+                        int64_t workspace_bytes, void *stream);
+
+int64_t hn_select_kv_blocks_workspace_size(int64_t B, int64_t H, int64_t runs, int64_t blocks);
+
+/* Attention of q [B, Lq, Hq, 128] over listed blocks of the cache and the bf16
+ * tail, with the rows' log-sum-exp:
+ *   out = softmax(softmax_scale q K^T) V, lse = ln sum exp(softmax_scale q . K),
+ * over the valid cached tokens t < kv_len of the blocks in idx[b, h, i / q_block]
+ * and the valid tail keys. A list ends at its first negative entry; an entry past
+ * the last block is ignored; a block that is listed twice counts twice. idx NULL:
+ * every cached token (top_k, is unused). A row without a key gets zeros and -inf.
+ * What masked keys and the cache past kv_len hold (Inf and NaN included) does not
+ * matter.
+ *   idx: int32 [B, H, runs, top_k], runs = ceil(Lq / q_block), strides is[3] of
+ *        its first three dims, the last contiguous
+ *   lse: fp32 [B, Hq, Lq] contiguous
+ * The other arguments, the fp16 rounding of the probabilities and V's range are
+ * those of hn_attn_fp8kv. */
+int hn_attn_kv_blocks(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
+                      const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
+                      const int64_t *ss, int64_t H, int64_t cache_cap, int64_t kv_len,
+                      const uint8_t *cache_valid, int64_t cache_valid_stride, const int32_t *idx,
+                      const int64_t *is, int64_t top_k, int64_t block, int64_t q_block, const void *kcur,
+                      const void *vcur, const int64_t *curs, int64_t cur_len, const uint8_t *cur_valid,
+                      int64_t cur_valid_stride, float softmax_scale, void *out, const int64_t *os, float *lse,
+                      void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace hn_attn_kv_blocks needs for these sizes on the current device
+ * (0: none); top_k < 0: without a list. */
+int64_t hn_attn_kv_blocks_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t kv_len,
+                                         int64_t cur_len, int64_t top_k, int64_t block, int64_t q_block);
+
+/* The attention weight that every cached key draws:
+ *   mass[b, h, t] = prior[b, h, t] + sum over rows of exp(softmax_scale q . K(t) - lse(row))
+ * for t < kv_len, over the Lq queries and G query heads of the Bq / B query batches
+ * that read slot b. An invalid key draws nothing (its prior stays), and so does a row
+ * whose lse is infinite. prior: fp32 [B, H, prior_len <= kv_len] with strides ps[2]
+ * (keys past it start at 0) or NULL with prior_len 0; lse: fp32 [Bq, Hq, Lq]
+ * contiguous; mass: fp32 [B, H, kv_len] contiguous, not overlapping prior. The sums are in 32 bits, in an order that only the sizes decide.
+ * workspace: hn_attn_key_mass_workspace_size() bytes, 16-byte aligned. */
+int hn_attn_key_mass(int fmt, const void *q, const int64_t *qs, int64_t Bq, int64_t Lq, int64_t Hq, int64_t D,
+                     const float *lse, const void *kc, const int64_t *cs, const float *ks, const int64_t *ss,
+                     int64_t B, int64_t H, int64_t cache_cap, int64_t kv_len, const uint8_t *cache_valid,
+                     int64_t cache_valid_stride, float softmax_scale, const float *prior, const int64_t *ps,
+                     int64_t prior_len, float *mass, void *workspace, int64_t workspace_bytes, void *stream);
+
+int64_t hn_attn_key_mass_workspace_size(int64_t Bq, int64_t Lq, int64_t Hq, int64_t B, int64_t H, int64_t kv_len);
+
+/* The `keep` tokens of each head that stay: tokens t < keep_first and t >= kv_len -
+ * keep_last, then those of the largest mass, ties to the lowest index, NaN as -inf;
+ * only tokens with valid[b * valid_stride + t] != 0 (NULL: all). idx: int32 [B, H,
+ * keep] contiguous, ascending, -1 behind the last. mass: fp32 [B, H, kv_len], strides
+ * ms[3] (ms[2] == 1). keep_first + keep_last <= keep. */
+int hn_select_kv_tokens(const float *mass, const int64_t *ms, int64_t B, int64_t H, int64_t kv_len,
+                        const uint8_t *valid, int64_t valid_stride, int64_t keep, int64_t keep_first,
+                        int64_t keep_last, int32_t *idx, void *stream);
+
+/* Moves the listed tokens of each head to the front of another cache: row i of the
+ * output (codes and scales of K and V) and out_mass[b, h, i] <- token idx[b, h, i].
+ * An index outside [0, tokens) leaves the row as it is and its mass 0. The output
+ * does not overlap the source.
+ *   cs, ss: strides of the source's codes and scales; os, ts: of the output's;
+ *   ms[2]: of the mass [B, H, tokens]; out_mass: fp32 [B, H, keep] contiguous */
+int hn_move_kv_tokens(const void *k, const void *v, const int64_t *cs, const float *ks, const float *vs,
+                      const int64_t *ss, const float *mass, const int64_t *ms, int64_t B, int64_t H, int64_t D,
+                      int64_t tokens, const int32_t *idx, int64_t keep, void *out_k, void *out_v,
+                      const int64_t *os, float *out_ks, float *out_vs, const int64_t *ts, int64_t out_cap,
+                      float *out_mass, void *stream);
+
 /* Test support; it replaces no reference interface. Writes to out[i] the e4m3
  * byte that the quantizers' hardware conversion (v_cvt_pk_fp8_f32, round to
  * nearest even) gives for the fp32 value whose bit pattern is first + i, for
