@@ -419,12 +419,13 @@ __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Key mass. A wave holds 64 keys as MFMA operands in registers; the query rows
-// stream past them through LDS, 32 at a time, and S^T = K Q^T puts one row per
-// lane column, whose log-sum-exp is one register. Each lane adds its rows'
-// probabilities per key; the 32 columns are summed once at the end. One
-// workgroup sees every row of its keys, so no two add to one key: the result
-// does not depend on their order.
+// Key mass. A wave holds 32 KB keys as MFMA operands in registers; the query rows
+// stream past them through LDS, 32 at a time. S = Q K^T puts one key per lane
+// column, so a key's mass is a sum over the lane's own registers and one exchange
+// with lane ^ 32 at the end; the rows' log-sum-exps come as four 16-byte LDS reads
+// a tile. The MFMAs of one key block run beside the exponentials of the one before.
+// One workgroup sees every row of its keys (or, split, its share of the rows, added
+// in order afterwards), so no two add to one key and the result has one order.
 struct MassParams {
     const uint16_t* q;
     const float* lse;       // [Bq, Hq, Lq]
@@ -438,38 +439,64 @@ struct MassParams {
     int64_t rows;           // query rows per cached head: batches * Lq * G
     int64_t rows_per_split; // rows of a workgroup (a multiple of MASS_ROWS)
     float* part;            // row splits: [split][B, H, kv_len] sums, or null
+    int64_t B;
     int batches;            // query batches per cache slot
-    int H, G;
+    int H, G, tiles, work, per_xcd;
     float scale_log2;
 };
 
-constexpr int MASS_KEYS = 256;  // keys per workgroup: 4 waves of 64
 constexpr int MASS_ROWS = 32;   // query rows per LDS tile
 constexpr int MASS_TILE = MASS_ROWS * KROW;
 
-template <int FMT>
+// The exponentials of block s (rows' n = -lse log2 e) beside the S of the next block.
+HN_DEVICE f32x16 mass_step(const f32x16& s, float c, const f32x16& n, float& acc, const bf16x8 (&qf)[8],
+                           const bf16x8 (&kf)[8]) {
+    f32x16 next;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) next[v] = 0.0f;
+    float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        next = mfma_bf16(qf[i], kf[i], next);
+        a0 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, n[2 * i]));
+        a1 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, n[2 * i + 1]));
+        pin(a0, a1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    acc += a0 + a1;
+    return next;
+}
+
+template <int FMT, int KB>
 __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * MASS_TILE];
-    __shared__ float nl[2][MASS_ROWS];
+    __shared__ __attribute__((aligned(16))) float nl[2][MASS_ROWS];
+    // Work order: id % 8 (the XCD) picks a contiguous range of items, heads fastest:
+    // the heads of one key range share the lines of its scales in one L2.
+    const int w = (int)(blockIdx.x & 7) * p.per_xcd + (int)(blockIdx.x >> 3);
+    if (w >= p.work) return;
+    const int64_t h = w % p.H;
+    int x = w / p.H;
+    const int tile = x % p.tiles;
+    x /= p.tiles;
+    const int64_t b = x % p.B, split = x / p.B;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    const int64_t h = blockIdx.y % p.H, b = blockIdx.y / p.H;
-    const int64_t key0 = (int64_t)blockIdx.x * MASS_KEYS + wave * 64;
+    const int64_t key0 = ((int64_t)tile * 4 + wave) * (32 * KB);
     const float c = p.scale_log2;
 
-    // K fragments of the wave's two 32-key blocks: key col, dims 16 sl + 8 half ..
-    bf16x8 kf[2][8];
+    // K fragments: key 32 kb + col, dims 64 half + 8 sl ..: 64 contiguous bytes a lane
+    bf16x8 kf[KB][8];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < KB; ++kb) {
         const int64_t key = key0 + 32 * kb + col;
-        const bool ok = key < p.kv_len && (!p.valid || p.valid[b * p.vs + key] != 0);
-        uint2 x[8];
+        uint4 y[4];
         float s = 0.0f;
 #pragma unroll
-        for (int sl = 0; sl < 8; ++sl) x[sl] = make_uint2(0u, 0u);
-        if (ok) {
-            const uint8_t* src = p.kc + b * p.cs0 + key * p.cs1 + h * p.cs2 + 8 * half;
+        for (int e = 0; e < 4; ++e) y[e] = make_uint4(0u, 0u, 0u, 0u);
+        if (key < p.kv_len && (!p.valid || p.valid[b * p.vs + key] != 0)) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.kc + b * p.cs0 + key * p.cs1 + h * p.cs2 + 64 * half);
 #pragma unroll
-            for (int sl = 0; sl < 8; ++sl) x[sl] = *reinterpret_cast<const uint2*>(src + 16 * sl);
+            for (int e = 0; e < 4; ++e) y[e] = src[e];
             s = p.ks[b * p.ss0 + key * p.ss1 + h * p.ss2];
         }
 #pragma unroll
@@ -477,7 +504,7 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
             uint32_t d[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const f32x2 f = codes2_f32<FMT>(e < 2 ? x[sl].x : x[sl].y, e & 1);
+                const f32x2 f = codes2_f32<FMT>(word(y[sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
                 d[e] = pack_bf16(f[0] * s, f[1] * s);
             }
             kf[kb][sl] = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
@@ -486,14 +513,21 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
 
     // This thread's 32 bytes of a query tile: row tid / 8, dims 16 (tid % 8) ..
     const int tr = tid >> 3, tu = tid & 7;
+    const int64_t row0 = split * p.rows_per_split;
+    const int64_t row1 = row0 + p.rows_per_split < p.rows ? row0 + p.rows_per_split : p.rows;
     uint4 x0, x1;
     float ln = 0.0f;
-    auto fetch = [&](int64_t r0) {
-        const int64_t r = r0 + tr;
+    // Row r0 + tr of the next fetch: query head g of the group, query i, batch bb; each
+    // fetch moves 32 rows on (steps dg, di, db with their carries; no division).
+    int64_t r = row0 + tr;
+    int g = (int)(r % p.G);
+    int64_t i = p.Lq > 0 ? (r / p.G) % p.Lq : 0, bb = b * p.batches + (p.Lq > 0 ? r / (p.G * p.Lq) : 0);
+    const int dg = MASS_ROWS % p.G;
+    const int64_t di = p.Lq > 0 ? (MASS_ROWS / p.G) % p.Lq : 0, db = p.Lq > 0 ? MASS_ROWS / p.G / p.Lq : 0;
+    auto fetch = [&]() {
         x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
         ln = -INFINITY;  // a row that adds nothing: exp2(0 - inf) = 0
-        if (r < p.rows) {
-            const int64_t g = r % p.G, i = (r / p.G) % p.Lq, bb = b * p.batches + r / (p.G * p.Lq);
+        if (r < row1) {
             const float lse = p.lse[(bb * p.H * p.G + h * p.G + g) * p.Lq + i];
             if (__builtin_fabsf(lse) != INFINITY) {
                 ln = -lse * 1.4426950408889634f;
@@ -502,6 +536,18 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
                 x1 = reinterpret_cast<const uint4*>(src)[1];
             }
         }
+        r += MASS_ROWS;
+        g += dg;
+        i += di;
+        bb += db;
+        if (g >= p.G) {
+            g -= p.G;
+            ++i;
+        }
+        if (i >= p.Lq) {
+            i -= p.Lq;
+            ++bb;
+        }
     };
     auto put = [&](int buf) {
         uint4* dst = reinterpret_cast<uint4*>(smem + buf * MASS_TILE + tr * KROW + 32 * tu);
@@ -509,57 +555,59 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
         dst[1] = x1;
         if (tu == 0) nl[buf][tr] = ln;
     };
-    f32x16 acc[2];
+    float acc[KB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[kb][v] = 0.0f;
-    const int64_t row0 = blockIdx.z * p.rows_per_split;
-    const int64_t row1 = row0 + p.rows_per_split < p.rows ? row0 + p.rows_per_split : p.rows;
-    fetch(row0);
+    for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.0f;
+    fetch();
     put(0);
     __syncthreads();
     int buf = 0;
     for (int64_t r0 = row0; r0 < row1; r0 += MASS_ROWS, buf ^= 1) {
         const bool more = r0 + MASS_ROWS < row1;
-        if (more) fetch(r0 + MASS_ROWS);
+        if (more) fetch();
         bf16x8 qf[8];
-        const uint8_t* qa = smem + buf * MASS_TILE + col * KROW + 16 * half;
+        const uint8_t* qa = smem + buf * MASS_TILE + col * KROW + 128 * half;
 #pragma unroll
-        for (int sl = 0; sl < 8; ++sl) qf[sl] = ld_bf16x8(qa + 32 * sl);
-        const float n = nl[buf][col];
+        for (int sl = 0; sl < 8; ++sl) qf[sl] = ld_bf16x8(qa + 16 * sl);
+        f32x16 n;  // row 8 (v / 4) + 4 half + v % 4
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            f32x16 s;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
-#pragma unroll
-            for (int sl = 0; sl < 8; ++sl) s = mfma_bf16(kf[kb][sl], qf[sl], s);
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[kb][v] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c, n));
+        for (int e = 0; e < 4; ++e) {
+            const float4 y = *reinterpret_cast<const float4*>(&nl[buf][8 * e + 4 * half]);
+            n[4 * e] = y.x;
+            n[4 * e + 1] = y.y;
+            n[4 * e + 2] = y.z;
+            n[4 * e + 3] = y.w;
         }
+        f32x16 s;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) s = mfma_bf16(qf[sl], kf[0][sl], s);
+#pragma unroll
+        for (int kb = 1; kb < KB; ++kb) s = mass_step(s, c, n, acc[kb - 1], qf, kf[kb]);
+        float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            a0 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c, n[v]));
+            a1 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], c, n[v + 1]));
+        }
+        acc[KB - 1] += a0 + a1;
         if (more) put(buf ^ 1);
         __syncthreads();
     }
-    // Sum over the 32 lane columns; key 32 kb + 8 (v / 4) + 4 half + v % 4.
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            float s = acc[kb][v];
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-            const int64_t key = key0 + 32 * kb + 8 * (v >> 2) + 4 * half + (v & 3);
-            if (col == v && key < p.kv_len) {
-                if (p.part) {
-                    p.part[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * p.kv_len + key] = s;
-                    continue;
-                }
-                const bool ok = !p.valid || p.valid[b * p.vs + key] != 0;
-                const float before = p.prior && key < p.prior_len ? p.prior[b * p.ps0 + h * p.ps1 + key] : 0.0f;
-                p.mass[(b * p.H + h) * p.kv_len + key] = ok ? before + s : before;
-            }
+    for (int kb = 0; kb < KB; ++kb) {
+        const float s = acc[kb] + __shfl_xor(acc[kb], 32, 64);
+        const int64_t key = key0 + 32 * kb + col;
+        if (half != 0 || key >= p.kv_len) continue;
+        if (p.part) {
+            p.part[((split * p.B + b) * p.H + h) * p.kv_len + key] = s;
+            continue;
         }
+        const bool ok = !p.valid || p.valid[b * p.vs + key] != 0;
+        const float before = p.prior && key < p.prior_len ? p.prior[b * p.ps0 + h * p.ps1 + key] : 0.0f;
+        p.mass[(b * p.H + h) * p.kv_len + key] = ok ? before + s : before;
+    }
 }
 
 // Sum of the row splits in order, onto the prior mass.
@@ -724,23 +772,33 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     return check_launch("hn_attn_kv_blocks (combine)");
 }
 
-// Row splits of the key mass: one workgroup per 256 keys and head sees every row;
-// where those are too few for the device (a short cache, many queries), the rows
-// are split, each split writes its sums and a second kernel adds them in order.
-static int mass_splits(int64_t rows, int64_t B, int64_t H, int64_t kv_len) {
-    const int64_t work = B * H * ((kv_len + attn::MASS_KEYS - 1) / attn::MASS_KEYS);
+// Plan of the key mass: 512 keys per workgroup (KB 4), or 128 (KB 1) where those
+// would not fill the device twice over; where even these fall short (a short cache,
+// many queries) the rows are split, each split writes its sums and a second kernel
+// adds them in order.
+struct MassPlan {
+    int kb, splits;
+    int64_t tiles;
+};
+
+static MassPlan mass_plan(int64_t rows, int64_t B, int64_t H, int64_t kv_len) {
     const int64_t target = 2LL * device_cus();
-    if (work <= 0 || work >= target) return 1;
-    int64_t sp = target / work;
-    const int64_t cap = rows / (8 * attn::MASS_ROWS);  // at least 8 row tiles each
+    MassPlan pl{4, 1, (kv_len + 511) / 512};
+    if (B * H * pl.tiles >= target) return pl;
+    pl.kb = 1;
+    pl.tiles = (kv_len + 127) / 128;
+    const int64_t work = B * H * pl.tiles;
+    int64_t sp = work > 0 ? target / work : 1;
+    const int64_t cap = rows / (4 * attn::MASS_ROWS);  // at least 4 row tiles each
     if (sp > cap) sp = cap;
-    return sp > 1 ? (int)sp : 1;
+    pl.splits = sp > 1 ? (int)sp : 1;
+    return pl;
 }
 
 extern "C" int64_t hn_attn_key_mass_workspace_size(int64_t Bq, int64_t Lq, int64_t Hq, int64_t B, int64_t H,
                                                    int64_t kv_len) {
     if (Bq <= 0 || Lq <= 0 || B <= 0 || H <= 0 || Hq <= 0 || Hq % H != 0 || Bq % B != 0 || kv_len <= 0) return 0;
-    const int sp = mass_splits(Bq / B * Lq * (Hq / H), B, H, kv_len);
+    const int sp = mass_plan(Bq / B * Lq * (Hq / H), B, H, kv_len).splits;
     return sp > 1 ? (int64_t)sp * B * H * kv_len * (int64_t)sizeof(float) : 0;
 }
 
@@ -763,16 +821,15 @@ extern "C" int hn_attn_key_mass(int fmt, const void* q, const int64_t* qs, int64
     HN_REQUIRE(qs && cs && ss && (prior_len == 0 || ps), HN_E_ARG, "hn_attn_key_mass: null stride array");
     HN_REQUIRE(qs[3] == 1 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0, HN_E_ARG,
                "hn_attn_key_mass: q strides misaligned");
-    HN_REQUIRE(cs[3] == 1 && cs[0] % 8 == 0 && cs[1] % 8 == 0 && cs[2] % 8 == 0, HN_E_ARG,
-               "hn_attn_key_mass: cache strides must be multiples of 8 bytes");
-    HN_REQUIRE(aligned(q, 16) && aligned(kc, 8), HN_E_ARG, "hn_attn_key_mass: misaligned pointer");
+    HN_REQUIRE(cs[3] == 1 && cs[0] % 16 == 0 && cs[1] % 16 == 0 && cs[2] % 16 == 0, HN_E_ARG,
+               "hn_attn_key_mass: cache strides must be multiples of 16 bytes");
+    HN_REQUIRE(aligned(q, 16) && aligned(kc, 16), HN_E_ARG, "hn_attn_key_mass: misaligned pointer");
     if (B == 0 || kv_len == 0) return HN_OK;
     HN_REQUIRE(kc && ks && mass && (prior_len == 0 || prior) && (Bq * Lq == 0 || (q && lse)), HN_E_ARG,
                "hn_attn_key_mass: null pointer");
     const int64_t need = hn_attn_key_mass_workspace_size(Bq, Lq, Hq, B, H, kv_len);
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_attn_key_mass: workspace smaller than hn_attn_key_mass_workspace_size() or misaligned");
-    const int64_t tiles = (kv_len + attn::MASS_KEYS - 1) / attn::MASS_KEYS;
     HN_REQUIRE(B * H <= 65535, HN_E_ARG, "hn_attn_key_mass: too many heads for one launch");
     if (const int rc = require_gfx950("hn_attn_key_mass"); rc != HN_OK) return rc;
     attn::MassParams p = {};
@@ -790,14 +847,24 @@ extern "C" int hn_attn_key_mass(int fmt, const void* q, const int64_t* qs, int64
     p.H = (int)H; p.G = (int)(Hq / H);
     p.rows = (int64_t)p.batches * Lq * p.G;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
-    const int splits = mass_splits(p.rows, B, H, kv_len);
+    const MassPlan pl = mass_plan(p.rows, B, H, kv_len);
+    const int splits = pl.splits;
     p.part = splits > 1 ? (float*)workspace : nullptr;
     const int64_t row_tiles = (p.rows + attn::MASS_ROWS - 1) / attn::MASS_ROWS;
     p.rows_per_split = (row_tiles + splits - 1) / splits * attn::MASS_ROWS;
-    const dim3 grid((unsigned)tiles, (unsigned)(B * H), (unsigned)splits);
+    const int64_t work = B * H * pl.tiles * splits;
+    HN_REQUIRE(work <= 0x3fffffffLL, HN_E_ARG, "hn_attn_key_mass: too much work for one launch");
+    p.B = B; p.tiles = (int)pl.tiles; p.work = (int)work;
+    p.per_xcd = (int)((work + 7) / 8);
+    const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
     hipStream_t st = (hipStream_t)stream;
-    if (fmt == HN_KV_FP8) attn::key_mass_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
-    else attn::key_mass_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
+    if (fmt == HN_KV_FP8) {
+        if (pl.kb == 4) attn::key_mass_kernel<HN_KV_FP8, 4><<<grid, 256, 0, st>>>(p);
+        else attn::key_mass_kernel<HN_KV_FP8, 1><<<grid, 256, 0, st>>>(p);
+    } else {
+        if (pl.kb == 4) attn::key_mass_kernel<HN_KV_INT8, 4><<<grid, 256, 0, st>>>(p);
+        else attn::key_mass_kernel<HN_KV_INT8, 1><<<grid, 256, 0, st>>>(p);
+    }
     const int rc = check_launch("hn_attn_key_mass");
     if (rc != HN_OK || splits == 1) return rc;
     attn::key_mass_sum_kernel<<<dim3((unsigned)((kv_len + 255) / 256), (unsigned)(B * H)), 256, 0, st>>>(p, splits);

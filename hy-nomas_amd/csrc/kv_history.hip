@@ -137,31 +137,54 @@ struct PoolArgs {
     int H, G;
 };
 
+HN_DEVICE void add_pooled(uint32_t x, double (&w)[2], double (&u)[2]) {
+    const float x0 = bf16_lo(x), x1 = bf16_hi(x);
+    w[0] += x0 > 0.0f ? 0.0f : x0;  // (a NaN enters both sums)
+    w[1] += x1 > 0.0f ? 0.0f : x1;
+    u[0] += x0 < 0.0f ? 0.0f : x0;
+    u[1] += x1 < 0.0f ? 0.0f : x1;
+}
+
+// One workgroup per run: 16 threads hold a row (8 channels each), 16 rows at a
+// time, and the 16 partial sums of a channel meet in LDS.
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
-    __shared__ double part[4][256];
+    __shared__ double part[16][257];
     const int64_t unit = blockIdx.x;  // (b * H + h) * runs + run
     const int64_t run = unit % a.runs, h = (unit / a.runs) % a.H, b = unit / (a.runs * a.H);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t = threadIdx.x, l16 = t & 15, g16 = t >> 4;
     const int64_t i0 = run * a.q_block, left = a.Lq - i0;
     const int64_t rows = (left < a.q_block ? left : a.q_block) * a.G;
-    double w0 = 0.0, w1 = 0.0, u0 = 0.0, u1 = 0.0;
-    for (int64_t r = wave; r < rows; r += 4) {
-        const int64_t i = i0 + r / a.G, g = r % a.G;
-        if (a.qvalid && a.qvalid[b * a.qvs + i] == 0) continue;
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(a.q + b * a.qs0 + i * a.qs1 + (h * a.G + g) * a.qs2 + 2 * lane);
-        const float x0 = bf16_lo(x), x1 = bf16_hi(x);
-        w0 += x0 > 0.0f ? 0.0f : x0;  // (a NaN enters both sums)
-        w1 += x1 > 0.0f ? 0.0f : x1;
-        u0 += x0 < 0.0f ? 0.0f : x0;
-        u1 += x1 < 0.0f ? 0.0f : x1;
+    double w[4][2] = {}, u[4][2] = {};
+    const uint16_t* q = a.q + b * a.qs0 + h * a.G * a.qs2 + 8 * l16;
+    for (int64_t r0 = g16; r0 < rows; r0 += 64) {
+        uint4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // four rows' loads in flight
+            const int64_t r = r0 + 16 * e, i = i0 + r / a.G, g = r % a.G;
+            x[e] = make_uint4(0u, 0u, 0u, 0u);  // adds nothing
+            if (r < rows && (!a.qvalid || a.qvalid[b * a.qvs + i] != 0))
+                x[e] = *reinterpret_cast<const uint4*>(q + i * a.qs1 + g * a.qs2);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            add_pooled(x[e].x, w[0], u[0]);
+            add_pooled(x[e].y, w[1], u[1]);
+            add_pooled(x[e].z, w[2], u[2]);
+            add_pooled(x[e].w, w[3], u[3]);
+        }
     }
-    part[wave][2 * lane] = w0;
-    part[wave][2 * lane + 1] = w1;
-    part[wave][D + 2 * lane] = u0;
-    part[wave][D + 2 * lane + 1] = u1;
-    __syncthreads();
-    const int t = threadIdx.x;
-    a.pooled[unit * 256 + t] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
+    double total = 0.0;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[g16][8 * l16 + e] = side ? u[e >> 1][e & 1] : w[e >> 1][e & 1];
+        __syncthreads();
+        if ((t >> 7) == side)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) total += part[e][t & 127];
+        __syncthreads();
+    }
+    a.pooled[unit * 256 + t] = total;
 }
 
 struct ScoreArgs {
@@ -170,6 +193,7 @@ struct ScoreArgs {
     uint32_t* rank;          // [B, H, runs, n]
     int64_t bs0, bs1, bs2, runs, n, first, last;
     int H;
+    PoolArgs pool;           // the queries, where the kernel sums them itself
 };
 
 HN_DEVICE uint32_t block_rank(const ScoreArgs& a, int64_t j, bool empty, double score) {
@@ -178,77 +202,225 @@ HN_DEVICE uint32_t block_rank(const ScoreArgs& a, int64_t j, bool empty, double 
     return rank_of((float)score);
 }
 
-// 16 lanes per block, 16 of the 256 terms each.
-__global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
-    const int l16 = threadIdx.x & 15;
-    const int64_t j = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int64_t bh = blockIdx.y, h = bh % a.H, b = bh / a.H;
-    const bool there = j < a.n;
-    const uint16_t* src = a.bounds + b * a.bs0 + (there ? j : 0) * a.bs1 + h * a.bs2 + l16 * 16;
-    const uint4 x0 = reinterpret_cast<const uint4*>(src)[0], x1 = reinterpret_cast<const uint4*>(src)[1];
-    const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-    const float first = bf16_lo(x0.x);
-    const bool empty = __shfl(first, 0, 16) > __shfl(first, 8, 16);
-    for (int64_t run = 0; run < a.runs; ++run) {
-        const double* p = a.pooled + (bh * a.runs + run) * 256 + l16 * 16;
-        double s = 0.0;
+// Few runs (single tokens): 16 lanes per block, 16 of the 256 terms each, four
+// blocks' loads in flight. The run's sums are staged in LDS once per workgroup;
+// FROM_Q: they are taken from the queries here (few rows), which saves the pooling
+// launch.
+constexpr int SCORE_FEW_RUNS = 4;
+constexpr int SCORE_FEW = 4;  // blocks in flight per lane group
+template <bool FROM_Q>
+__global__ __launch_bounds__(256, 4) void score_few_kernel(ScoreArgs a) {
+    __shared__ __attribute__((aligned(16))) double sums[256];
+    const int t = threadIdx.x, l16 = t & 15;
+    // heads fastest: the bounds of a block's heads lie side by side
+    const int64_t h = blockIdx.x % a.H, b = blockIdx.y, bh = b * a.H + h;
+    uint4 x[SCORE_FEW][2];
+    int64_t j[SCORE_FEW];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            s = __builtin_fma(p[2 * c], (double)bf16_lo(w[c]), s);
-            s = __builtin_fma(p[2 * c + 1], (double)bf16_hi(w[c]), s);
+    for (int e = 0; e < SCORE_FEW; ++e) {
+        j[e] = (int64_t)(blockIdx.x / a.H) * (16 * SCORE_FEW) + 16 * e + (t >> 4);
+        const uint4* src = reinterpret_cast<const uint4*>(a.bounds + b * a.bs0 + (j[e] < a.n ? j[e] : 0) * a.bs1 +
+                                                          h * a.bs2 + l16 * 16);
+        x[e][0] = src[0];
+        x[e][1] = src[1];
+    }
+    for (int64_t run = 0; run < a.runs; ++run) {
+        if constexpr (FROM_Q) {
+            const PoolArgs& pa = a.pool;
+            const int64_t i0 = run * pa.q_block, left = pa.Lq - i0;
+            const int rows = (int)((left < pa.q_block ? left : pa.q_block) * pa.G);
+            const uint16_t* q = pa.q + b * pa.qs0 + i0 * pa.qs1 + h * pa.G * pa.qs2 + (t & 127);
+            double sum = 0.0;
+            for (int r0 = 0; r0 < rows; r0 += 4) {
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // four rows in flight
+                    const int r = r0 + e, i = r / pa.G, g = r % pa.G;
+                    y[e] = 0.0f;  // adds nothing
+                    if (r < rows && (!pa.qvalid || pa.qvalid[b * pa.qvs + i0 + i] != 0))
+                        y[e] = bf16_bits_to_f32(q[i * pa.qs1 + g * pa.qs2]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // threads 0-127 sum min(q, 0), the others max(q, 0); a NaN enters both
+                    sum += (t < 128 ? y[e] > 0.0f : y[e] < 0.0f) ? 0.0f : y[e];
+            }
+            sums[t] = sum;
+        } else {
+            sums[t] = a.pooled[(bh * a.runs + run) * 256 + t];
+        }
+        __syncthreads();
+        // (the bounds' 64-bit forms are made again for each run: held, they would take
+        // four times the registers)
+#pragma unroll
+        for (int e = 0; e < SCORE_FEW; ++e)
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+                asm volatile("" : "+v"(x[e][d].x), "+v"(x[e][d].y), "+v"(x[e][d].z), "+v"(x[e][d].w));
+        double s[SCORE_FEW] = {};
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const double2 p = *reinterpret_cast<const double2*>(sums + 16 * l16 + 2 * d);
+#pragma unroll
+            for (int e = 0; e < SCORE_FEW; ++e) {
+                const uint4& z = x[e][d >> 2];
+                const uint32_t bits = (d & 3) == 0 ? z.x : (d & 3) == 1 ? z.y : (d & 3) == 2 ? z.z : z.w;
+                s[e] = __builtin_fma(p.x, (double)bf16_lo(bits), s[e]);
+                s[e] = __builtin_fma(p.y, (double)bf16_hi(bits), s[e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 16);
-        if (there && l16 == 0) a.rank[(bh * a.runs + run) * a.n + j] = block_rank(a, j, empty, s);
+        for (int e = 0; e < SCORE_FEW; ++e) {
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) s[e] += __shfl_xor(s[e], off, 16);
+            const float first = bf16_lo(x[e][0].x);
+            const bool empty = __shfl(first, 0, 16) > __shfl(first, 8, 16);
+            if (j[e] < a.n && l16 == 0) a.rank[(bh * a.runs + run) * a.n + j[e]] = block_rank(a, j[e], empty, s[e]);
+        }
+        __syncthreads();  // the sums are rewritten for the next run
+    }
+}
+
+// Many runs: [runs x 256] x [256 x blocks] on the 64-bit matrix unit, 16 runs x 16
+// blocks a wave and v_mfma_f64_16x16x4 (lane l: row or column l % 16, term l / 16;
+// result register r: row 4 r + l / 16). Terms are dealt so that lane group g holds
+// terms 64 g .. 64 g + 63: each lane then reads 128 contiguous bytes of its block's
+// bounds. The runs' sums are staged once per workgroup (row pitch 258 doubles:
+// 16-byte reads of 8 rows fall in different banks).
+constexpr int SCORE_TILES = 4;  // 16-block tiles per wave
+__global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
+    constexpr int PITCH = 258;
+    __shared__ __attribute__((aligned(16))) double sums[16 * PITCH];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+    const int64_t bh = blockIdx.z, h = bh % a.H, b = bh / a.H, run0 = (int64_t)blockIdx.y * 16;
+    double in[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r)  // (rows past the last run repeat it; their scores are not written)
+        in[r] = a.pooled[(bh * a.runs + (run0 + r < a.runs ? run0 + r : a.runs - 1)) * 256 + threadIdx.x];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sums[r * PITCH + threadIdx.x] = in[r];
+    __syncthreads();
+    const double* arow = sums + c16 * PITCH + 64 * g;
+    uint4 x[8], y[8];
+    auto fetch = [&](int64_t j0) __attribute__((always_inline)) {
+        const int64_t j = j0 + c16;
+        const uint4* src = reinterpret_cast<const uint4*>(a.bounds + b * a.bs0 + (j < a.n ? j : a.n - 1) * a.bs1 +
+                                                          h * a.bs2 + 64 * g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = src[e];
+    };
+    const int64_t first_j = ((int64_t)blockIdx.x * SCORE_TILES * 4 + wave) * 16;
+    fetch(first_j);
+    for (int tile = 0; tile < SCORE_TILES; ++tile) {
+        const int64_t j0 = first_j + 64 * tile, j = j0 + c16;
+        if (j0 >= a.n) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = y[e];
+        if (tile + 1 < SCORE_TILES) fetch(j0 + 64);  // the next tile's bounds, beside this one's products
+        const float first = bf16_lo(x[0].x);
+        const bool empty = __shfl(first, c16, 64) > __shfl(first, 32 + c16, 64);
+        f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const double2 s = *reinterpret_cast<const double2*>(arow + 8 * e + 2 * d);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(s.x, (double)bf16_lo(w[d]), acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(s.y, (double)bf16_hi(w[d]), acc, 0, 0, 0);
+            }
+        }
+        if (j < a.n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t run = run0 + 4 * r + g;
+                if (run < a.runs) a.rank[(bh * a.runs + run) * a.n + j] = block_rank(a, j, empty, acc[r]);
+            }
     }
 }
 
 // ---------------------------------------------------------------------------
 // The k highest ranks of a row, ties to the lowest index, as ascending indices;
-// -1 behind them where fewer can be chosen. A radix search over the rank's four
-// digits finds the k-th rank T and how many elements equal to T are taken; each
-// wave then writes the chosen indices of its own stretch of the row, from counts
-// of the stretches before it.
+// -1 behind them where fewer can be chosen. One workgroup a row; wave w owns the
+// elements [w stretch, (w + 1) stretch). A radix search over the rank's digits, 8
+// bits at a time from the top, finds the digits of the k-th rank and how many
+// elements that share them are taken; it ends early when all of those are. Each
+// wave then writes the chosen indices of its stretch, from counts of the stretches
+// before it. Scores share their leading bits, so the digit counts are kept in
+// COPIES copies that neighbouring lanes add to. KPT > 0: a thread holds its KPT
+// elements in registers (n <= KPT NT), so that a row is read once; KPT = 0: longer
+// rows are read again in every pass.
+constexpr int COPIES = 8, COPY_PITCH = 260;  // (a copy starts 4 banks after the one before)
+
 template <int NT>
 struct TopShared {
-    uint32_t hist[256];
-    uint32_t prefix, need;
+    uint32_t hist[COPIES * COPY_PITCH];
+    uint32_t prefix, need, count;
     uint32_t above[NT / 64], equal[NT / 64];
 };
 
-template <int NT, class Rank>
-HN_DEVICE void choose_top(TopShared<NT>& sh, Rank rank, int n, int k, int32_t* out) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    constexpr int WAVES = NT / 64;
+// A row's source: load(i) is its raw element (0 past the end: no lane needs a limit),
+// rank(i, raw) that element's rank, RANK_NONE past the end.
+HN_DEVICE __amdgpu_buffer_rsrc_t row_rsrc(const void* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+template <int NT, int KPT, class Row>
+HN_DEVICE void choose_top(TopShared<NT>& sh, const Row& row, int n, int k, int32_t* out) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int WAVES = NT / 64, GROUP = KPT > 0 ? KPT : 8;
+    const int stretch = KPT > 0 ? KPT * 64 : (n + NT * GROUP - 1) / (NT * GROUP) * (64 * GROUP);
+    const int lo = wave * stretch;
     const int kk = k < n ? k : n;
-    uint32_t prefix = 0, need = (uint32_t)kk;
-    for (int shift = 24; shift >= 0 && kk > 0; shift -= 8) {
-        for (int i = tid; i < 256; i += NT) sh.hist[i] = 0;
-        __syncthreads();
-        for (int i0 = 0; i0 < n; i0 += NT) {
-            const int i = i0 + tid;
-            const uint32_t u = i < n ? rank(i) : 0u;
-            bool in = i < n && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8)));
-            const uint32_t digit = (u >> shift) & 255u;
-            if (shift == 24) {
-                // most scores share their leading digit: one add per distinct digit of the wave
-                while (__any(in)) {
-                    const int lead = __builtin_ctzll(__ballot(in));
-                    const uint32_t d = __shfl(digit, lead, 64);
-                    const uint64_t same = __ballot(in && digit == d);
-                    if (lane == lead) atomicAdd(&sh.hist[d], (uint32_t)__builtin_popcountll(same));
-                    in = in && digit != d;
-                }
-            } else if (in) {
-                atomicAdd(&sh.hist[digit], 1u);
+    uint32_t u[GROUP];
+    auto read = [&](int i0) __attribute__((always_inline)) {  // elements i0 + 64 e + lane
+#pragma unroll
+        for (int e = 0; e < GROUP; ++e) u[e] = row.load(i0 + 64 * e + lane);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < GROUP; ++e) {
+            u[e] = row.rank(i0 + 64 * e + lane, u[e]);
+            if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // f(first index, ranks) over the wave's elements, 64 at a time
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (KPT > 0) {
+#pragma unroll
+            for (int e = 0; e < GROUP; ++e) {
+                f(lo + 64 * e, u[e]);
+                if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            for (int i0 = lo; i0 < lo + stretch && i0 < n; i0 += 64 * GROUP) {
+                read(i0);
+#pragma unroll
+                for (int e = 0; e < GROUP; ++e) f(i0 + 64 * e, u[e]);
             }
         }
+    };
+    if constexpr (KPT > 0) read(lo);
+    uint32_t prefix = 0, need = (uint32_t)kk;
+    int shift = 32;  // the digits below it are not fixed yet
+    while (shift > 0 && kk > 0) {
+        shift -= 8;
+        for (int i = tid; i < COPIES * COPY_PITCH; i += NT) sh.hist[i] = 0;
+        __syncthreads();
+        uint32_t* mine = sh.hist + (lane & (COPIES - 1)) * COPY_PITCH;
+        each([&](int i0, uint32_t v) __attribute__((always_inline)) {
+            if (shift == 24 || ((v ^ prefix) >> (shift + 8)) == 0) atomicAdd(&mine[(v >> shift) & 255u], 1u);
+        });
         __syncthreads();
         if (wave == 0) {  // lane l: bins 4 l .. 4 l + 3
-            uint32_t c[4], sum = 0;
+            uint32_t c[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += c[e] = sh.hist[4 * lane + e];
+            for (int e = 0; e < COPIES; ++e) {
+                const uint4 x = *reinterpret_cast<const uint4*>(sh.hist + e * COPY_PITCH + 4 * lane);
+                c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;
+            }
+            const uint32_t sum = c[0] + c[1] + c[2] + c[3];
             uint32_t suffix = sum;  // of this lane's bins and all above
+#pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
                 const uint32_t o = __shfl_down(suffix, off, 64);
                 if (lane + off < 64) suffix += o;
@@ -259,6 +431,7 @@ HN_DEVICE void choose_top(TopShared<NT>& sh, Rank rank, int n, int k, int32_t* o
                 if (over < need && need <= over + c[e]) {
                     sh.prefix = prefix | ((uint32_t)(4 * lane + e) << shift);
                     sh.need = need - over;
+                    sh.count = c[e];
                 }
                 over += c[e];
             }
@@ -266,58 +439,74 @@ HN_DEVICE void choose_top(TopShared<NT>& sh, Rank rank, int n, int k, int32_t* o
         __syncthreads();
         prefix = sh.prefix;
         need = sh.need;
-        __syncthreads();  // hist and the two words are rewritten for the next digit
+        if (sh.count == need) break;  // (every thread reads the same words)
+        __syncthreads();  // hist and the words are rewritten for the next digit
     }
-    if (prefix == RANK_NONE) need = 0;
-    // the wave's stretch of the row
-    const int seg = (((n + WAVES - 1) / WAVES) + 63) / 64 * 64;
-    const int lo = wave * seg, hi = lo + seg < n ? lo + seg : n;
+    // Taken: ranks whose fixed digits are above prefix's, and the first `need` that
+    // equal them (all of them after an early end). RANK_NONE is never taken: it has
+    // to be told from the ranks that share its fixed digits.
+    uint32_t low = prefix > RANK_NONE ? prefix : 1u, high = shift < 32 ? prefix | ((1u << shift) - 1u) : RANK_ALWAYS;
+    uint32_t width = shift < 32 && high >= low ? high - low + 1u : 0u;  // (0: nothing is equal)
+    auto is_above = [&](uint32_t v) { return v > high; };
+    auto is_equal = [&](uint32_t v) { return v - low < width; };
     uint32_t above = 0, equal = 0;
-    for (int i0 = lo; i0 < hi; i0 += 64) {
-        const int i = i0 + lane;
-        const uint32_t u = i < hi ? rank(i) : 0u;
-        above += (uint32_t)__builtin_popcountll(__ballot(i < hi && u > prefix));
-        equal += (uint32_t)__builtin_popcountll(__ballot(i < hi && u == prefix));
+    each([&](int, uint32_t v) __attribute__((always_inline)) {
+        above += is_above(v);
+        equal += is_equal(v);
+        asm volatile("" : "+v"(above), "+v"(equal));
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        above += __shfl_xor(above, off, 64);
+        equal += __shfl_xor(equal, off, 64);
     }
     if (lane == 0) {
         sh.above[wave] = above;
         sh.equal[wave] = equal;
     }
     __syncthreads();
-    uint32_t pos = 0, eq = 0, total = 0, teq = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) {
-            pos += sh.above[w];
-            eq += sh.equal[w];
-        }
-        total += sh.above[w];
-        teq += sh.equal[w];
+    // counts before this wave's stretch, and of the whole row
+    const int w = lane & (WAVES - 1);
+    uint32_t total = sh.above[w], teq = sh.equal[w], pos = w < wave ? total : 0u, eq = w < wave ? teq : 0u;
+#pragma unroll
+    for (int off = WAVES / 2; off > 0; off >>= 1) {
+        total += __shfl_xor(total, off, WAVES);
+        teq += __shfl_xor(teq, off, WAVES);
+        pos += __shfl_xor(pos, off, WAVES);
+        eq += __shfl_xor(eq, off, WAVES);
     }
     pos += eq < need ? eq : need;
     total += teq < need ? teq : need;
     const uint64_t before = (1ull << lane) - 1;
-    if (kk > 0) {
-        for (int i0 = lo; i0 < hi; i0 += 64) {
-            const int i = i0 + lane;
-            const uint32_t u = i < hi ? rank(i) : 0u;
-            const uint64_t eqs = __ballot(i < hi && u == prefix);
-            const bool take = i < hi && (u > prefix || (u == prefix && eq + (uint32_t)__builtin_popcountll(eqs & before) < need));
-            const uint64_t takes = __ballot(take);
-            if (take) out[pos + (uint32_t)__builtin_popcountll(takes & before)] = i;
-            pos += (uint32_t)__builtin_popcountll(takes);
-            eq += (uint32_t)__builtin_popcountll(eqs);
-        }
-    } else {
-        total = 0;
-    }
+    // (the compiler would keep what it knows of every element from the passes before:
+    // comparisons as 64-lane masks and indices, more than there are registers)
+    int me = lane;
+    asm volatile("" : "+v"(low), "+v"(high), "+v"(width), "+v"(me));
+    each([&](int i0, uint32_t v) __attribute__((always_inline)) {
+        const bool same = is_equal(v);
+        const uint64_t eqs = __ballot(same);
+        const bool take = is_above(v) || (same && eq + (uint32_t)__builtin_popcountll(eqs & before) < need);
+        const uint64_t takes = __ballot(take);
+        if (take) out[pos + (uint32_t)__builtin_popcountll(takes & before)] = i0 + me;
+        pos += (uint32_t)__builtin_popcountll(takes);
+        eq += (uint32_t)__builtin_popcountll(eqs);
+        asm volatile("" : "+v"(pos), "+v"(eq));
+    });
     for (int i = (int)total + tid; i < k; i += NT) out[i] = -1;
 }
 
+struct RankRow {  // ranks as score_kernel wrote them
+    __amdgpu_buffer_rsrc_t r;
+    HN_DEVICE uint32_t load(int i) const { return __builtin_amdgcn_raw_buffer_load_b32(r, 4 * i, 0, 0); }
+    HN_DEVICE uint32_t rank(int, uint32_t raw) const { return raw; }
+};
+
+template <int KPT>
 __global__ __launch_bounds__(256) void choose_blocks_kernel(const uint32_t* __restrict__ rank, int n, int k,
                                                             int32_t* __restrict__ idx) {
-    __shared__ TopShared<256> sh;
-    const uint32_t* r = rank + (int64_t)blockIdx.x * n;
-    choose_top<256>(sh, [&](int i) { return r[i]; }, n, k, idx + (int64_t)blockIdx.x * k);
+    __shared__ __attribute__((aligned(16))) TopShared<256> sh;
+    const RankRow row{row_rsrc(rank + (int64_t)blockIdx.x * n, (int64_t)n * 4)};
+    choose_top<256, KPT>(sh, row, n, k, idx + (int64_t)blockIdx.x * k);
 }
 
 struct TokenArgs {
@@ -328,19 +517,30 @@ struct TokenArgs {
     int H, n, keep, first, last;
 };
 
+template <bool MASK>
+struct MassRow {
+    __amdgpu_buffer_rsrc_t m, valid;
+    uint32_t n, first, middle;  // tokens [first, first + middle) are ranked by their mass
+    HN_DEVICE uint32_t load(int i) const { return __builtin_amdgcn_raw_buffer_load_b32(m, 4 * i, 0, 0); }
+    HN_DEVICE uint32_t rank(int i, uint32_t raw) const {
+        uint32_t r = rank_of(__uint_as_float(raw));
+        if ((uint32_t)i - first >= middle) r = RANK_ALWAYS;
+        if (MASK) return __builtin_amdgcn_raw_buffer_load_b8(valid, i, 0, 0) ? r : RANK_NONE;  // (0 past the end)
+        return (uint32_t)i < n ? r : RANK_NONE;
+    }
+};
+
+template <int KPT, bool MASK>
 __global__ __launch_bounds__(1024) void choose_tokens_kernel(TokenArgs a) {
-    __shared__ TopShared<1024> sh;
+    __shared__ __attribute__((aligned(16))) TopShared<1024> sh;
     const int64_t h = blockIdx.x % a.H, b = blockIdx.x / a.H;
-    const float* mass = a.mass + b * a.ms0 + h * a.ms1;
-    const uint8_t* valid = a.valid ? a.valid + b * a.vs : nullptr;
-    choose_top<1024>(
-        sh,
-        [&](int i) {
-            if (valid && valid[i] == 0) return RANK_NONE;
-            if (i < a.first || i >= a.n - a.last) return RANK_ALWAYS;
-            return rank_of(mass[i]);
-        },
-        a.n, a.keep, a.idx + (int64_t)blockIdx.x * a.keep);
+    MassRow<MASK> row;
+    row.m = row_rsrc(a.mass + b * a.ms0 + h * a.ms1, (int64_t)a.n * 4);
+    row.valid = row_rsrc(MASK ? a.valid + b * a.vs : nullptr, MASK ? a.n : 0);
+    row.n = (uint32_t)a.n;
+    row.first = (uint32_t)a.first;
+    row.middle = a.n - a.last > a.first ? (uint32_t)(a.n - a.last - a.first) : 0u;
+    choose_top<1024, KPT>(sh, row, a.n, a.keep, a.idx + (int64_t)blockIdx.x * a.keep);
 }
 
 // ---------------------------------------------------------------------------
@@ -355,13 +555,19 @@ struct MoveArgs {
     const int32_t* idx;
     int64_t cs0, cs1, cs2, ss0, ss1, ss2, ms0, ms1;
     int64_t os0, os1, os2, ts0, ts1, ts2;
-    int64_t keep, tokens, rows;
+    int64_t keep, tokens, rows, per_xcd;
     int H;
 };
 
 __global__ __launch_bounds__(256) void move_tokens_kernel(MoveArgs a) {
+    // Workgroup ids are dealt round-robin to the XCDs: id % 8 picks an eighth of the
+    // rows, so that the lines of scales and indices that neighbouring rows share are
+    // fetched by one L2.
     const int l = threadIdx.x & 7;
-    for (int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); row < a.rows; row += (int64_t)gridDim.x * 32) {
+    const int64_t first = (int64_t)(blockIdx.x & 7) * a.per_xcd, end = first + a.per_xcd;
+    const int64_t step = (int64_t)(gridDim.x >> 3) * 32;
+    for (int64_t row = first + (int64_t)(blockIdx.x >> 3) * 32 + (threadIdx.x >> 3); row < end && row < a.rows;
+         row += step) {
         const int64_t h = row % a.H, i = (row / a.H) % a.keep, b = row / (a.H * a.keep);
         const int64_t at = (b * a.H + h) * a.keep + i;
         const int64_t t = a.idx[at];
@@ -438,47 +644,65 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
     HN_REQUIRE(D == hist::D, HN_E_ARG, "hn_select_kv_blocks: head dim must be 128");
     HN_REQUIRE(B >= 0 && Lq >= 0 && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 65535 && blocks >= 0, HN_E_ARG,
                "hn_select_kv_blocks: invalid shape");
-    HN_REQUIRE(q_block > 0 && top_k > 0 && top_k <= 0x7fffffffLL && blocks <= 0x3fffffffLL, HN_E_ARG,
+    HN_REQUIRE(q_block > 0 && top_k > 0 && top_k <= 0x7fffffffLL && blocks <= 0x1fffffffLL, HN_E_ARG,
                "hn_select_kv_blocks: q_block and top_k must be positive");
     HN_REQUIRE(keep_first >= 0 && keep_last >= 0 && keep_first <= top_k && keep_last <= top_k - keep_first, HN_E_ARG,
                "hn_select_kv_blocks: keep_first + keep_last exceeds top_k");
-    HN_REQUIRE(qs && bs && qs[3] == 1 && qs[0] % 2 == 0 && qs[1] % 2 == 0 && qs[2] % 2 == 0, HN_E_ARG,
-               "hn_select_kv_blocks: q strides");
+    HN_REQUIRE(qs && bs && qs[3] == 1 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0, HN_E_ARG,
+               "hn_select_kv_blocks: q strides must be multiples of 8");
     HN_REQUIRE(bs[0] % 8 == 0 && bs[1] % 8 == 0 && bs[2] % 8 == 0, HN_E_ARG,
                "hn_select_kv_blocks: bounds strides must be multiples of 8");
     HN_REQUIRE(q_valid_stride >= 0, HN_E_ARG, "hn_select_kv_blocks: negative validity stride");
-    HN_REQUIRE(aligned(q, 4) && aligned(bounds, 16) && aligned(idx, 4), HN_E_ARG, "hn_select_kv_blocks: misaligned pointer");
+    HN_REQUIRE(aligned(q, 16) && aligned(bounds, 16) && aligned(idx, 4), HN_E_ARG, "hn_select_kv_blocks: misaligned pointer");
     if (B == 0 || Lq == 0) return HN_OK;
     HN_REQUIRE(q && idx && (bounds || blocks == 0), HN_E_ARG, "hn_select_kv_blocks: null pointer");
     const int64_t runs = (Lq - 1) / q_block + 1;
     const int64_t need = hn_select_kv_blocks_workspace_size(B, H, runs, blocks);
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_select_kv_blocks: workspace smaller than hn_select_kv_blocks_workspace_size() or misaligned");
-    HN_REQUIRE(B * H <= 65535 && B * H * runs <= 0x7fffffffLL, HN_E_ARG, "hn_select_kv_blocks: too much work for one launch");
+    HN_REQUIRE(B * H <= 65535 && B * H * runs <= 0x7fffffffLL && runs <= 16 * 65535LL, HN_E_ARG,
+               "hn_select_kv_blocks: too much work for one launch");
     if (const int rc = require_gfx950("hn_select_kv_blocks"); rc != HN_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
     uint32_t* rank = nullptr;
+    const int64_t rows = B * H * runs, in_run = (q_block < Lq ? q_block : Lq) * (Hq / H);
     if (blocks > 0) {
         hist::PoolArgs pa;
         pa.q = (const uint16_t*)q; pa.qvalid = q_valid; pa.pooled = (double*)workspace;
         pa.qs0 = qs[0]; pa.qs1 = qs[1]; pa.qs2 = qs[2]; pa.qvs = q_valid_stride;
         pa.Lq = Lq; pa.q_block = q_block; pa.runs = runs; pa.H = (int)H; pa.G = (int)(Hq / H);
-        hist::pool_kernel<<<(unsigned)(B * H * runs), 256, 0, st>>>(pa);
         hist::ScoreArgs sa;
-        rank = (uint32_t*)((uint8_t*)workspace + align256(B * H * runs * 256 * 8));
+        rank = (uint32_t*)((uint8_t*)workspace + align256(rows * 256 * 8));
         sa.pooled = pa.pooled; sa.bounds = (const uint16_t*)bounds; sa.rank = rank;
         sa.bs0 = bs[0]; sa.bs1 = bs[1]; sa.bs2 = bs[2];
         sa.runs = runs; sa.n = blocks; sa.first = keep_first; sa.last = keep_last; sa.H = (int)H;
-        hist::score_kernel<<<dim3((unsigned)((blocks + 15) / 16), (unsigned)(B * H)), 256, 0, st>>>(sa);
+        sa.pool = pa;
+        const bool few = runs <= hist::SCORE_FEW_RUNS, from_q = few && in_run <= 16;
+        if (!from_q) hist::pool_kernel<<<(unsigned)rows, 256, 0, st>>>(pa);
+        if (few) {
+            constexpr int64_t per = 16 * hist::SCORE_FEW;
+            const dim3 grid((unsigned)((blocks + per - 1) / per * H), (unsigned)B);
+            if (from_q) hist::score_few_kernel<true><<<grid, 256, 0, st>>>(sa);
+            else hist::score_few_kernel<false><<<grid, 256, 0, st>>>(sa);
+        } else {
+            constexpr int64_t per = 64 * hist::SCORE_TILES;
+            hist::score_kernel<<<dim3((unsigned)((blocks + per - 1) / per), (unsigned)((runs + 15) / 16),
+                                      (unsigned)(B * H)), 256, 0, st>>>(sa);
+        }
     }
-    hist::choose_blocks_kernel<<<(unsigned)(B * H * runs), 256, 0, st>>>(rank, (int)blocks, (int)top_k, idx);
+    if (blocks <= 8 * 256)
+        hist::choose_blocks_kernel<8><<<(unsigned)rows, 256, 0, st>>>(rank, (int)blocks, (int)top_k, idx);
+    else if (blocks <= 32 * 256)
+        hist::choose_blocks_kernel<32><<<(unsigned)rows, 256, 0, st>>>(rank, (int)blocks, (int)top_k, idx);
+    else
+        hist::choose_blocks_kernel<0><<<(unsigned)rows, 256, 0, st>>>(rank, (int)blocks, (int)top_k, idx);
     return check_launch("hn_select_kv_blocks");
 }
 
 extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t B, int64_t H, int64_t kv_len,
                                    const uint8_t* valid, int64_t valid_stride, int64_t keep, int64_t keep_first,
                                    int64_t keep_last, int32_t* idx, void* stream) {
-    HN_REQUIRE(B >= 0 && H > 0 && kv_len >= 0 && kv_len <= 0x3fffffffLL && keep >= 0 && keep <= 0x3fffffffLL, HN_E_ARG,
+    HN_REQUIRE(B >= 0 && H > 0 && kv_len >= 0 && kv_len <= 0x1fffffffLL && keep >= 0 && keep <= 0x1fffffffLL, HN_E_ARG,
                "hn_select_kv_tokens: invalid shape");
     HN_REQUIRE(keep_first >= 0 && keep_last >= 0 && keep_first <= keep && keep_last <= keep - keep_first, HN_E_ARG,
                "hn_select_kv_tokens: keep_first + keep_last exceeds keep");
@@ -493,7 +717,21 @@ extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t
     a.mass = mass; a.valid = valid; a.idx = idx;
     a.ms0 = ms[0]; a.ms1 = ms[1]; a.vs = valid_stride;
     a.H = (int)H; a.n = (int)kv_len; a.keep = (int)keep; a.first = (int)keep_first; a.last = (int)keep_last;
-    hist::choose_tokens_kernel<<<(unsigned)(B * H), 1024, 0, (hipStream_t)stream>>>(a);
+    const unsigned grid = (unsigned)(B * H);
+    hipStream_t st = (hipStream_t)stream;
+    // the smallest register form that holds a row (see choose_top)
+    const int form = kv_len <= 8 * 1024 ? 0 : kv_len <= 32 * 1024 ? 1 : kv_len <= 96 * 1024 ? 2 : 3;
+    if (valid) {
+        if (form == 0) hist::choose_tokens_kernel<8, true><<<grid, 1024, 0, st>>>(a);
+        else if (form == 1) hist::choose_tokens_kernel<32, true><<<grid, 1024, 0, st>>>(a);
+        else if (form == 2) hist::choose_tokens_kernel<96, true><<<grid, 1024, 0, st>>>(a);
+        else hist::choose_tokens_kernel<0, true><<<grid, 1024, 0, st>>>(a);
+    } else {
+        if (form == 0) hist::choose_tokens_kernel<8, false><<<grid, 1024, 0, st>>>(a);
+        else if (form == 1) hist::choose_tokens_kernel<32, false><<<grid, 1024, 0, st>>>(a);
+        else if (form == 2) hist::choose_tokens_kernel<96, false><<<grid, 1024, 0, st>>>(a);
+        else hist::choose_tokens_kernel<0, false><<<grid, 1024, 0, st>>>(a);
+    }
     return check_launch("hn_select_kv_tokens");
 }
 
@@ -522,7 +760,8 @@ extern "C" int hn_move_kv_tokens(const void* k, const void* v, const int64_t* cs
     a.ms0 = ms[0]; a.ms1 = ms[1];
     a.os0 = os[0]; a.os1 = os[1]; a.os2 = os[2]; a.ts0 = ts[0]; a.ts1 = ts[1]; a.ts2 = ts[2];
     a.keep = keep; a.tokens = tokens; a.rows = B * keep * H; a.H = (int)H;
-    const int64_t grid = stream_grid((a.rows + 31) / 32, 16);
+    a.per_xcd = (a.rows + 255) / 256 * 32;  // whole workgroups of 32 rows
+    const int64_t grid = 8 * stream_grid(a.per_xcd / 32, 2);
     hist::move_tokens_kernel<<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("hn_move_kv_tokens");
 }

@@ -845,8 +845,7 @@ def select_kv_blocks(q: torch.Tensor, bounds: torch.Tensor, kv_len: int, top_k: 
         raise ValueError(f"{what}: keep_first + keep_last exceeds top_k")
     if bounds.stride(4) != 1 or bounds.stride(3) != D:
         raise ValueError(f"{what}: the two bounds of a head must be contiguous")
-    if q.stride(3) != 1:
-        q = q.contiguous()
+    q = _head_rows(q)
     if bounds.shape[0] != B:
         bounds = bounds.expand(B, -1, -1, -1, -1)
     vb, vs = _mask_bytes(q_valid, B, Lq, f"{what}: q_valid")
