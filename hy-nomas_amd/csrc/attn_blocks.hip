@@ -162,32 +162,68 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     Run run_{-INFINITY, 0.0f, 0.0f};
     const float c = p.scale_log2;
 
-    // Tile t: segment, first key in it, keys that exist.
-    struct Geom {
-        bool cache;
-        int64_t first;
-        int count;
+    // Loads go through descriptors that span the (b, h) rows of the cache [0, kv_len)
+    // and of the tail: a tile is a 32-bit byte offset in them, and rows past their
+    // ends read as zeros. A span of 2^31 bytes or more is replaced by the tile's own
+    // rows, tile by tile.
+    const bool span_ok = p.kv_len > 0 && (p.kv_len - 1) * p.cs1 + D < ((int64_t)1 << 31) &&
+                         ((p.kv_len - 1) * p.ss1 + 1) * 4 < ((int64_t)1 << 31);
+    const bool tail_ok = (p.cur_len * p.us1 + D) * 2 < ((int64_t)1 << 31);
+    TileBase src = tile_base(p, b, h, 0, span_ok ? (int)p.kv_len : 0);
+    auto tail_rsrc = [&](const uint16_t* base, int64_t first, int64_t rows) __attribute__((always_inline)) {
+        return tile_rsrc(base + b * p.us0 + h * p.us2 + first * p.us1, rows > 0 ? ((rows - 1) * p.us1 + D) * 2 : 0);
     };
-    auto geom = [&](int t) {
-        Geom g;
-        int64_t left;
-        if (t < n_cache) {
-            g.cache = true;
-            const int64_t e = list ? __builtin_amdgcn_readfirstlane(list[t >> p.shift]) : 0;
-            g.first = list ? e * p.block + (int64_t)(t & ((1 << p.shift) - 1)) * BKV : (int64_t)t * BKV;
-            left = p.kv_len - g.first;
-        } else {
-            g.cache = false;
-            g.first = (int64_t)(t - n_cache) * BKV;
-            left = p.cur_len - g.first;
+    const int64_t tail_rows = tail_ok ? p.cur_len : 0;
+    __amdgpu_buffer_rsrc_t tk = tail_rsrc(p.kcur, 0, tail_rows), tv = tail_rsrc(p.vcur, 0, tail_rows);
+
+    // Tile t: keys that exist, and where its loads start: code and scale offsets, its
+    // first key in the validity bytes. Past the last tile, and for a list entry past
+    // the last block: no key, and offsets past every span.
+    struct Place {
+        uint32_t co, so;
+        int count, first;
+    };
+    constexpr uint32_t NOWHERE = 0x80000000u;
+    auto entry = [&](int t) __attribute__((always_inline)) {  // list entry of cache tile t
+        return list && t < n_cache && t < t_end ? __builtin_amdgcn_readfirstlane(list[t >> p.shift]) : 0;
+    };
+    const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len, entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
+    const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1 * 4u, us1 = (uint32_t)p.us1 * 2u;
+    auto cache_place = [&](int t, int e) __attribute__((always_inline)) {
+        Place g;
+        const bool there = t < n_cache && t < t_end && e < entries;
+        g.first = !there ? 0 : list ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : t * BKV;
+        const int left = there ? kv_len - g.first : 0;
+        g.count = left >= BKV ? BKV : left > 0 ? left : 0;
+        g.co = g.count > 0 ? (uint32_t)g.first * cs1 : NOWHERE;
+        g.so = g.count > 0 ? (uint32_t)g.first * ss1 : NOWHERE;
+        if (!span_ok && g.count > 0) {
+            src = tile_base(p, b, h, g.first, g.count);
+            src.mk = p.kvalid ? p.kvalid + b * p.kvs : nullptr;
+            g.co = g.so = 0;
         }
-        g.count = left >= BKV ? BKV : left > 0 ? (int)left : 0;
-        if (left <= 0) g.first = 0;  // an entry past the last block: nothing is read
         return g;
     };
-    // The tile's keys that take part: existing and (MASK) valid.
-    auto word_of = [&](const Geom& g, const uint8_t* st) {
-        const uint64_t all = g.count >= BKV ? ALL_KEYS : (1ull << g.count) - 1;
+    auto tail_count = [&](int t) __attribute__((always_inline)) {
+        const int left = t < t_end ? cur_len - (t - n_cache) * BKV : 0;
+        return left >= BKV ? BKV : left > 0 ? left : 0;
+    };
+    auto tail_place = [&](int t) __attribute__((always_inline)) {
+        Place g;
+        g.first = (t - n_cache) * BKV;
+        g.count = tail_count(t);
+        g.co = g.count > 0 ? (uint32_t)g.first * us1 : NOWHERE;
+        g.so = 0;
+        if (!tail_ok && g.count > 0) {
+            tk = tail_rsrc(p.kcur, g.first, g.count);
+            tv = tail_rsrc(p.vcur, g.first, g.count);
+            g.co = 0;
+        }
+        return g;
+    };
+    // The keys of a tile that take part: existing and (MASK) valid.
+    auto word_of = [&](int count, const uint8_t* st) __attribute__((always_inline)) {
+        const uint64_t all = count >= BKV ? ALL_KEYS : (1ull << count) - 1;
         return tile_mask<MASK>(st) & all;
     };
     const uint32_t ka_off = col * KROW + 16 * half;
@@ -195,80 +231,83 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     CacheRegs<NW> regs;
     regs.s = 0.0f;
     const LaneOffs<NW> lo = lane_offsets<NW>(p);
-
-    auto store_cache_tile = [&](const Geom& g, uint8_t* st, const float* sb) {  // prologue
-        store_mask<NW, MASK>(regs, st);
-        float ks[Shape<NW>::KU];
-        k_scales<NW>(sb, ks);
-        float4 vs = v_scales(sb);
-        if constexpr (MASK) {
-            __syncthreads();
-            const uint64_t word = word_of(g, st);
-            if (word != ALL_KEYS) clear_masked_v(regs, vs, word);
-        }
-        uint32_t kd[4];
-        float vp[Shape<NW>::VD];
-        uint32_t vd[2 * Shape<NW>::VD];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            store_k_part<FMT, NW>(regs, st, i, ks, kd);
-            store_v_part<FMT, NW>(regs.v, st + K_BYTES, i, vs, vp, vd);
-        }
-    };
-    auto copy_tail = [&](const Geom& g, uint8_t* st) {  // prologue and the first tail tile
-        TailRegs<NW> r;
-        load_tail_k<NW, MASK>(p, b, h, g.first, g.count, r);
-        load_tail_v<NW>(p, b, h, g.first, g.count, r);
-        store_tail_k<NW, MASK>(r, st);
-        if constexpr (MASK) {
-            __syncthreads();
-            const uint64_t word = word_of(g, st);
-            if (word != ALL_KEYS) clear_masked_v(r, word);
-        }
-        store_tail_v<NW>(r, st);
+    auto fetch_k = [&](const Place& g) __attribute__((always_inline)) {
+        load_k<NW, MASK>(lo, regs, src, g.count, g.co, g.so, g.first);
     };
 
     if (t_end > t_begin) {
         f32x16 sa, sb;
         float mxa, mxb;
         uint64_t mw;
-        Geom g = geom(t_begin);
-        if (g.cache) {
-            const TileBase tb = tile_base(p, b, h, g.first, g.count);
-            load_k<NW, MASK>(lo, regs, tb, g.count);
-            load_v<NW>(lo, regs, tb);
+        int count, next_count;  // existing keys of tiles t and t + 1
+        TailRegs<NW> tr;
+        const TailOffs<NW> to = tail_offsets<NW>(p);
+        auto fetch_tail_k = [&](const Place& g) __attribute__((always_inline)) {
+            load_tail_span_k<NW, MASK>(p, b, to, tk, g.co, g.first, g.first + g.count, tr);
+        };
+        // ---- prologue: tile t_begin to stage 0, the codes of the next to registers
+        if (t_begin < n_cache) {
+            const Place g = cache_place(t_begin, entry(t_begin));
+            count = g.count;
+            fetch_k(g);
+            load_v<NW>(lo, regs, src, g.co);
             __builtin_amdgcn_s_waitcnt(0);
             if (threadIdx.x < 2 * BKV) sbuf[threadIdx.x] = regs.s;
+            store_mask<NW, MASK>(regs, smem);
             __syncthreads();
-            store_cache_tile(g, smem, sbuf);
+            float ks[Shape<NW>::KU];
+            k_scales<NW>(sbuf, ks);
+            float4 vs = v_scales(sbuf);
+            if constexpr (MASK) {
+                const uint64_t word = word_of(count, smem);
+                if (word != ALL_KEYS) clear_masked_v(regs, vs, word);
+            }
+            uint32_t kd[4];
+            float vp[Shape<NW>::VD];
+            uint32_t vd[2 * Shape<NW>::VD];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                store_k_part<FMT, NW>(regs, smem, i, ks, kd);
+                store_v_part<FMT, NW>(regs.v, smem + K_BYTES, i, vs, vp, vd);
+            }
         } else {
-            copy_tail(g, smem);
+            const Place g = tail_place(t_begin);
+            count = g.count;
+            fetch_tail_k(g);
+            load_tail_span_v<NW>(to, tv, g.co, tr);
+            store_tail_k<NW, MASK>(tr, smem);
+            if constexpr (MASK) {
+                __syncthreads();
+                const uint64_t word = word_of(count, smem);
+                if (word != ALL_KEYS) clear_masked_v(tr, word);
+            }
+            store_tail_v<NW>(tr, smem);
         }
-        Geom gn = geom(t_begin + 1 < t_end ? t_begin + 1 : t_begin);
-        if (t_begin + 1 < t_end && gn.cache) {
-            const TileBase tb = tile_base(p, b, h, gn.first, gn.count);
-            load_k<NW, MASK>(lo, regs, tb, gn.count);
-            load_v<NW>(lo, regs, tb);
+        {
+            const Place g = cache_place(t_begin + 1, entry(t_begin + 1));
+            next_count = t_begin + 1 < n_cache ? g.count : tail_count(t_begin + 1);
+            fetch_k(g);
+            load_v<NW>(lo, regs, src, g.co);
         }
         __builtin_amdgcn_s_waitcnt(0);
         if (threadIdx.x < 2 * BKV) sbuf[SB_FLOATS + threadIdx.x] = regs.s;
         __syncthreads();
-        mw = word_of(g, smem);
+        mw = word_of(count, smem);
         sa = s_block(smem + ka_off, qf);
         mxa = raw_max(sa);
         if ((uint32_t)mw != ~0u) mxa = mask_word(sa, (uint32_t)mw);
         int t = t_begin;
-        // Cache tiles, and the step into the tail.
+        int e2 = entry(t + 2);
+        // ---- cache tiles, and the step into the tail
         for (; t < t_end && t < n_cache; ++t) {
             const int u = t - t_begin;
             const uint8_t* st = smem + (u & 1) * STAGE;
             uint8_t* nst = smem + ((u & 1) ^ 1) * STAGE;
             const float* nsb = sbuf + ((u & 1) ^ 1) * SB_FLOATS;
-            const bool has_next = t + 1 < t_end;
-            const Geom g2 = geom(t + 2 < t_end ? t + 2 : t_end - 1);
-            const int n2 = t + 2 < t_end && g2.cache ? g2.count : 0;  // 0: no fetch (zeros)
+            const Place g2 = cache_place(t + 2, e2);
+            e2 = entry(t + 3);
             f16x8 pf[2];
-            // ---- half 0
+            // half 0
             rebase(mxa, c, run_, o);
             sb = step_a_lse(sa, c, run_.nm, run_.l, pf, st + ka_off + 32 * KROW, qf);
             {
@@ -281,18 +320,16 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
             }
             store_mask<NW, MASK>(regs, nst);
             if ((uint32_t)(mw >> 32) != ~0u) mxb = mask_word(sb, (uint32_t)(mw >> 32));
-            const bool tail_next = has_next && !gn.cache;
-            TailRegs<NW> tr;
-            if (tail_next) {
-                load_tail_k<NW, MASK>(p, b, h, gn.first, gn.count, tr);
+            const bool tail_next = t + 1 < t_end && t + 1 >= n_cache;
+            if (tail_next) {  // once: the tail's first tile, loaded on the spot
+                fetch_tail_k(tail_place(t + 1));
                 store_tail_k<NW, MASK>(tr, nst);
             }
-            const TileBase tb2 = tile_base(p, b, h, g2.first, n2);
-            load_k<NW, MASK>(lo, regs, tb2, n2);
+            fetch_k(g2);
             __syncthreads();
-            // ---- half 1 (on the last tile the S block of "tile t + 1" reads stale
-            // LDS; its result is never used)
-            const uint64_t mwn = word_of(gn, nst);
+            // half 1 (on the last tile the S block of "tile t + 1" reads stale LDS; its
+            // result is never used)
+            const uint64_t mwn = word_of(next_count, nst);
             rebase(mxb, c, run_, o);
             sa = step_a_lse(sb, c, run_.nm, run_.l, pf, nst + ka_off, qf);
             {
@@ -307,54 +344,49 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
             }
             if ((uint32_t)mwn != ~0u) mxa = mask_word(sa, (uint32_t)mwn);
             if (tail_next) {
-                load_tail_v<NW>(p, b, h, gn.first, gn.count, tr);
+                load_tail_span_v<NW>(to, tv, tail_place(t + 1).co, tr);
                 if constexpr (MASK)
                     if (mwn != ALL_KEYS) clear_masked_v(tr, mwn);
                 store_tail_v<NW>(tr, nst);
             }
             if (threadIdx.x < 2 * BKV) sbuf[(u & 1) * SB_FLOATS + threadIdx.x] = regs.s;
-            load_v<NW>(lo, regs, tb2);
+            load_v<NW>(lo, regs, src, g2.co);
             __syncthreads();
-            g = gn;
-            gn = g2;
+            next_count = t + 2 < n_cache ? g2.count : tail_count(t + 2);
             mw = mwn;
         }
-        // Tail tiles.
+        // ---- tail tiles
         if (t < t_end) {
-            TailRegs<NW> tr;
-            auto fetch_k = [&](int tt) {
-                if (tt < t_end) load_tail_k<NW, MASK>(p, b, h, (int64_t)(tt - n_cache) * BKV, geom(tt).count, tr);
-            };
-            auto fetch_v = [&](int tt) {
-                if (tt < t_end) load_tail_v<NW>(p, b, h, (int64_t)(tt - n_cache) * BKV, geom(tt).count, tr);
-            };
-            fetch_k(t + 1);
-            fetch_v(t + 1);
+            {
+                const Place g = tail_place(t + 1);
+                fetch_tail_k(g);
+                load_tail_span_v<NW>(to, tv, g.co, tr);
+            }
             for (; t < t_end; ++t) {
                 const int u = t - t_begin;
                 const uint8_t* st = smem + (u & 1) * STAGE;
                 uint8_t* nst = smem + ((u & 1) ^ 1) * STAGE;
-                const bool has_next = t + 1 < t_end;
                 f16x8 pf[2];
                 rebase(mxa, c, run_, o);
                 sb = step_a_lse(sa, c, run_.nm, run_.l, pf, st + ka_off + 32 * KROW, qf);
                 mxb = step_b_with(pf, st + va_off, 0, o, sb, [&](int i) __attribute__((always_inline)) {
-                    if ((i & 1) && has_next) store_tail_k_part<NW>(tr, nst, i >> 2, (i >> 1) & 1);
+                    if (i & 1) store_tail_k_part<NW>(tr, nst, i >> 2, (i >> 1) & 1);
                 });
-                if (has_next) store_tail_mask<NW, MASK>(tr, nst);
+                store_tail_mask<NW, MASK>(tr, nst);
                 if ((uint32_t)(mw >> 32) != ~0u) mxb = mask_word(sb, (uint32_t)(mw >> 32));
-                fetch_k(t + 2);
+                const Place g2 = tail_place(t + 2);
+                fetch_tail_k(g2);
                 __syncthreads();
-                const uint64_t mwn = word_of(geom(has_next ? t + 1 : t), nst);
+                const uint64_t mwn = word_of(tail_count(t + 1), nst);  // (past the end: unused)
                 if constexpr (MASK)
-                    if (mwn != ALL_KEYS && has_next) clear_masked_v(tr, mwn);
+                    if (mwn != ALL_KEYS) clear_masked_v(tr, mwn);
                 rebase(mxb, c, run_, o);
                 sa = step_a_lse(sb, c, run_.nm, run_.l, pf, nst + ka_off, qf);
                 mxa = step_b_with(pf, st + va_off, 1, o, sa, [&](int i) __attribute__((always_inline)) {
-                    if (has_next) store_tail_v_part<NW>(tr, nst, i);
+                    store_tail_v_part<NW>(tr, nst, i);
                 });
                 if ((uint32_t)mwn != ~0u) mxa = mask_word(sa, (uint32_t)mwn);
-                fetch_v(t + 2);
+                load_tail_span_v<NW>(to, tv, g2.co, tr);
                 __syncthreads();
                 mw = mwn;
             }
@@ -390,32 +422,529 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     if (half == 0) p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Merge of the key splits (as attn_combine_kernel), with the row's log-sum-exp.
+// ---------------------------------------------------------------------------
+// One row a run (single tokens of ungrouped heads). The read of the keys is the whole
+// cost and a matrix tile would hold one row of 32, so the products run on the vector
+// unit, without LDS or barriers in the loop: 8 lanes hold a key (16 dims each, one
+// 16-byte load of K and of V), a wave reads 8 keys per load and has a whole 64-key
+// tile in flight. K^ enters as packed bf16 (v_dot2_f32_bf16 onto fp32), probabilities
+// and V^ as fp32. Each lane group runs an online softmax of its own keys; the 8 groups
+// of a wave, the 4 waves and the splits meet at the end. Against attn_waves_kernel: 8
+// heads x 1000 keys 7.5 against 9.2 us, 64 x 4096 keys 21.2 against 24.2 us, 64 x 32768
+// keys 126 against 127 us (4.4 TB/s); with two rows a run it gained 0-7 %.
+struct RowState {
+    float m, l, o[16];
+};
+
+HN_DEVICE float dpp_add8(float v) {  // sum over the 8 lanes of an aligned group
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));
+    return v;
+}
+
+// bf16(code * s) of a lane's 16 codes, as 8 packed words.
+template <int FMT>
+HN_DEVICE void held16(const uint4& x, float s, uint32_t (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const f32x2 f = codes2_f32<FMT>(word(x, i >> 1), i & 1);
+        w[i] = pack_bf16(f[0] * s, f[1] * s);
+    }
+}
+
+// The group's logit (log2 units) of one key.
+HN_DEVICE float row_logit(const uint32_t (&k)[8], const uint32_t (&q)[8], float c, bool there) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        a = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, k[i]), __builtin_bit_cast(bf16x2, q[i]), a, false);
+    a = dpp_add8(a);
+    return there ? a * c : -INFINITY;
+}
+
+// The running maximum takes in N keys' logits; O and l follow it.
+template <int N>
+HN_DEVICE void row_rebase(const float (&s)[N], RowState& f) {
+    float mx = f.m;
+#pragma unroll
+    for (int e = 0; e < N; ++e) mx = fmaxf(mx, s[e]);
+    const float a = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(f.m - mx);
+    f.m = mx;
+    f.l *= a;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) f.o[d] *= a;
+}
+
+HN_DEVICE void row_add(float s, const uint32_t (&v)[8], bool there, RowState& f) {
+    const float p = there ? __builtin_amdgcn_exp2f(s - f.m) : 0.0f;
+    f.l += p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f.o[2 * i] = __builtin_fmaf(p, bf16_lo(v[i]), f.o[2 * i]);
+        f.o[2 * i + 1] = __builtin_fmaf(p, bf16_hi(v[i]), f.o[2 * i + 1]);
+    }
+}
+
+template <int FMT>
+__global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
+    __shared__ float so[4][D], sml[4][2];
+    const int id = blockIdx.x;
+    const int w = (id & 7) * p.per_xcd + (id >> 3);
+    if (w >= p.work) return;
+    // heads fastest, then the splits of a row
+    const int64_t h = w % p.H;
+    int x = w / (int)p.H;
+    const int split = x % p.splits;
+    x /= p.splits;
+    const int64_t run = x % p.runs, b = x / p.runs, i = run * p.q_block;  // (G = 1: head h, query i)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int piece = lane & 7, grp = lane >> 3;
+    uint32_t q[8];
+    {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.qs0 + i * p.qs1 + h * p.qs2 + 16 * piece);
+        const uint4 y0 = src[0], y1 = src[1];
+        q[0] = y0.x; q[1] = y0.y; q[2] = y0.z; q[3] = y0.w;
+        q[4] = y1.x; q[5] = y1.y; q[6] = y1.z; q[7] = y1.w;
+    }
+    const int32_t* list = p.idx ? p.idx + b * p.is0 + h * p.is1 + run * p.is2 : nullptr;
+    const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len;
+    const int entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
+    const int n_cache = list ? list_length(list, p.top_k) << p.shift : (kv_len + BKV - 1) / BKV;
+    const int n_all = n_cache + (cur_len + BKV - 1) / BKV;
+    const float c = p.scale_log2;
+    RowState f;
+    f.m = -INFINITY;
+    f.l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) f.o[d] = 0.0f;
+    // tiles of 64 keys, dealt to the waves of all splits in turn
+    for (int t = split * 4 + wave; t < n_all; t += 4 * p.splits) {
+        if (t < n_cache) {
+            int first = t * BKV, left = kv_len - first;
+            if (list) {
+                const int e = __builtin_amdgcn_readfirstlane(list[t >> p.shift]);
+                first = e < entries ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : 0;
+                left = e < entries ? kv_len - first : 0;
+            }
+            if (left <= 0) continue;
+            const int64_t base = b * p.cs0 + first * p.cs1 + h * p.cs2 + 16 * piece;
+            uint4 kx[8], vx[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)  // (a key past the end reads the last one)
+                kx[e] = *reinterpret_cast<const uint4*>(p.kc + base + min(8 * e + grp, left - 1) * p.cs1);
+            // this lane's scales and validity: key 8 piece + grp, read by its group in step `piece`
+            const int mine = min(8 * piece + grp, left - 1);
+            const int64_t sa = b * p.ss0 + (first + mine) * p.ss1 + h * p.ss2;
+            const float ks = p.ks[sa], vs = p.vs[sa];
+            int ok = 8 * piece + grp < left;
+            if (p.kvalid) ok &= p.kvalid[b * p.kvs + first + mine] != 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                vx[e] = *reinterpret_cast<const uint4*>(p.vc + base + min(8 * e + grp, left - 1) * p.cs1);
+            float s[8];
+            uint32_t there = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint32_t kw[8];
+                held16<FMT>(kx[e], __shfl(ks, (lane & 56) + e, 64), kw);
+                const bool in = __shfl(ok, (lane & 56) + e, 64) != 0;
+                there |= (uint32_t)in << e;
+                s[e] = row_logit(kw, q, c, in);
+            }
+            row_rebase<8>(s, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool in = (there >> e) & 1u;
+                uint32_t vw[8];
+                // (what a masked key holds must not meet its zero probability)
+                const float sv = __shfl(vs, (lane & 56) + e, 64);
+                held16<FMT>(in ? vx[e] : make_uint4(0u, 0u, 0u, 0u), in ? sv : 0.0f, vw);
+                row_add(s[e], vw, in, f);
+            }
+        } else {
+            const int first = (t - n_cache) * BKV, left = cur_len - first;
+            for (int e = 0; e < 8 && 8 * e < left; ++e) {
+                const int j = first + min(8 * e + grp, left - 1);
+                const bool in = 8 * e + grp < left && (!p.uvalid || p.uvalid[b * p.uvs + j] != 0);
+                const int64_t at = b * p.us0 + j * p.us1 + h * p.us2 + 16 * piece;
+                const uint4 *kp = reinterpret_cast<const uint4*>(p.kcur + at), *vp = reinterpret_cast<const uint4*>(p.vcur + at);
+                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                const uint4 a0 = in ? kp[0] : zero, a1 = in ? kp[1] : zero, b0 = in ? vp[0] : zero, b1 = in ? vp[1] : zero;
+                const uint32_t kw[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+                const uint32_t vw[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                const float s[1] = {row_logit(kw, q, c, in)};
+                row_rebase<1>(s, f);
+                row_add(s[0], vw, in, f);
+            }
+        }
+    }
+    // The 8 groups of the wave: common maximum, then the dims are dealt out while the
+    // groups add up (lane xor 32, 16, 8), each lane ending with two dims.
+    {
+        float m = f.m;
+#pragma unroll
+        for (int off = 8; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        const float a = f.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(f.m - m);
+        float l = f.l * a;
+#pragma unroll
+        for (int off = 8; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
+        float v8[8], v4[4];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const float keep = (grp & 4 ? f.o[8 + d] : f.o[d]) * a, give = (grp & 4 ? f.o[d] : f.o[8 + d]) * a;
+            v8[d] = keep + __shfl_xor(give, 32, 64);
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const float keep = grp & 2 ? v8[4 + d] : v8[d], give = grp & 2 ? v8[d] : v8[4 + d];
+            v4[d] = keep + __shfl_xor(give, 16, 64);
+        }
+        const int d0 = 16 * piece + 8 * (grp >> 2) + 4 * ((grp >> 1) & 1) + 2 * (grp & 1);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const float keep = grp & 1 ? v4[2 + d] : v4[d], give = grp & 1 ? v4[d] : v4[2 + d];
+            so[wave][d0 + d] = keep + __shfl_xor(give, 8, 64);
+        }
+        if (lane == 0) {
+            sml[wave][0] = m;
+            sml[wave][1] = l;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    // the 4 waves, a thread a dim
+    const int d = threadIdx.x;
+    const float m = fmaxf(fmaxf(sml[0][0], sml[1][0]), fmaxf(sml[2][0], sml[3][0]));
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int wv = 0; wv < 4; ++wv) {
+        const float a = __builtin_amdgcn_exp2f(sml[wv][0] - base);
+        l = __builtin_fmaf(sml[wv][1], a, l);
+        v = __builtin_fmaf(so[wv][d], a, v);
+    }
+    const int64_t slot = (b * p.H + h) * p.Lq + i;
+    if (p.splits > 1) {
+        const int64_t part = (int64_t)split * p.B * p.H * p.Lq + slot;
+        p.ws_o[part * D + d] = v;
+        if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, l);
+    } else {
+        p.out[b * p.os0 + i * p.os1 + h * p.os2 + d] = (uint16_t)f32_to_bf16_bits(l > 0.0f ? v / l : 0.0f);
+        if (d == 0) p.lse[slot] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 32 rows a run: one matrix column block holds all of them, so the waves of a
+// workgroup share the keys instead of the rows. Every wave takes 32-key blocks of its
+// own, without barriers: K codes go from global memory to MFMA operands in registers
+// (lane half: 64 contiguous dims, which the Q operand matches), V^ passes through the
+// wave's own LDS tile to be transposed ([dim][key], as attn_tiles.h). While a block is
+// computed the next one's codes are in flight to a second set of registers. The waves
+// and the splits meet at the end.
+constexpr int WV_ROW = 80;                       // V^T row: 32 fp16 keys + 16 B
+constexpr int WV_GROUP = 16 * WV_ROW + 64;       // 16 rows + 64 B (writes of 4 row groups fall in different banks)
+constexpr int WV_BYTES = 8 * WV_GROUP;
+constexpr int WO_PITCH = D + 4;                  // floats
+constexpr int WAVES_SMEM = 4 * 32 * WO_PITCH * 4;  // the partial outputs of 4 waves (over the V^T tiles)
+static_assert(4 * WV_BYTES <= WAVES_SMEM, "V^T tiles fit");
+
+HN_DEVICE int wv_row(int dim) { return (dim >> 4) * WV_GROUP + (dim & 15) * WV_ROW; }
+
+struct WaveRegs {  // codes of a 32-key block
+    uint4 k[4];    // key col, dims 64 half ..
+    uint4 v[4];    // keys quad_key(lane % 8, j), dims 16 (lane / 8) ..
+    float ks, vs;  // of key col
+    uint32_t word; // keys that take part
+};
+
+template <int FMT>
+__global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
+    __shared__ __attribute__((aligned(16))) uint8_t smem[WAVES_SMEM];
+    __shared__ float sml[4][32][2];
+    const int id = blockIdx.x;
+    const int w = (id & 7) * p.per_xcd + (id >> 3);
+    if (w >= p.work) return;
+    // heads fastest, then the splits of a run
+    const int64_t h = w % p.H;
+    int x = w / (int)p.H;
+    const int split = x % p.splits;
+    x /= p.splits;
+    const int64_t run = x % p.runs, b = x / p.runs;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5, qd = lane & 7, dg = lane >> 3;
+    const int64_t i0 = run * p.q_block;
+    const int64_t queries = p.Lq - i0 < p.q_block ? p.Lq - i0 : p.q_block;
+    const int rows = (int)(queries * p.G);  // 1 .. 32
+    uint8_t* const vt = smem + wave * WV_BYTES;
+    bf16x8 qf[8];
+    {
+        const int r = col < rows ? col : rows - 1;
+        const uint16_t* src = p.q + b * p.qs0 + (i0 + r / p.G) * p.qs1 + (h * p.G + r % p.G) * p.qs2 + 64 * half;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) qf[sl] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 8 * sl));
+    }
+    const int32_t* list = p.idx ? p.idx + b * p.is0 + h * p.is1 + run * p.is2 : nullptr;
+    const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len;
+    const int entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
+    const int sh32 = p.shift + 1;  // block = 32 << sh32 tokens
+    const int limit = list ? p.top_k << sh32 : (kv_len + 31) / 32;
+    const int step = 4 * p.splits;
+
+    f32x16 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[i][v] = 0.0f;
+    Run run_{-INFINITY, 0.0f, 0.0f};
+    const float c = p.scale_log2;
+
+    // Codes of cache block t < limit; a block without a key leaves word 0. Keys past the
+    // end read the last one's rows. (The first loads do not wait for the list's length:
+    // what lies past its end is dropped afterwards.)
+    auto load = [&](int t, WaveRegs& r) __attribute__((always_inline)) {
+        r.word = 0;
+        if (t >= limit) return;
+        int first = t * 32, left = kv_len - first;
+        if (list) {
+            const int e = __builtin_amdgcn_readfirstlane(list[t >> sh32]);
+            const bool there = (uint32_t)e < (uint32_t)entries;
+            first = there ? ((e << sh32) + (t & ((1 << sh32) - 1))) * 32 : 0;
+            left = there ? kv_len - first : 0;
+        }
+        if (left <= 0) return;
+        const int mine = min(col, left - 1);
+        const int64_t base = b * p.cs0 + first * p.cs1 + h * p.cs2;
+        const uint4* kp = reinterpret_cast<const uint4*>(p.kc + base + mine * p.cs1 + 64 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.k[e] = kp[e];
+        const int64_t sa = b * p.ss0 + (first + mine) * p.ss1 + h * p.ss2;
+        r.ks = p.ks[sa];
+        r.vs = p.vs[sa];
+        bool ok = col < left;
+        if (p.kvalid) ok = ok && p.kvalid[b * p.kvs + first + mine] != 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            r.v[j] = *reinterpret_cast<const uint4*>(p.vc + base + min(quad_key(qd, j), left - 1) * p.cs1 + 16 * dg);
+        r.word = (uint32_t)__ballot(ok);
+    };
+    // P and PV of a block whose V^T is in the wave's tile.
+    auto finish = [&](f32x16& s, uint32_t word) __attribute__((always_inline)) {
+        const float mx = word != ~0u ? mask_word(s, word) : raw_max(s);
+        rebase(mx, c, run_, o);
+        f16x8 pf[2];
+        uint32_t x8[8];
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, run_.nm));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, run_.nm));
+            x8[i] = pack_f16(p0, p1);
+            l += p0;
+            l += p1;
+        }
+        run_.l += l;
+        pf[0] = __builtin_bit_cast(f16x8, make_uint4(x8[0], x8[1], x8[2], x8[3]));
+        pf[1] = __builtin_bit_cast(f16x8, make_uint4(x8[4], x8[5], x8[6], x8[7]));
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+                o[db] = mfma_f16(ld_f16x8(vt + wv_row(32 * db + col) + 32 * tt + 16 * half), pf[tt], o[db]);
+    };
+    auto block = [&](const WaveRegs& r) __attribute__((always_inline)) {
+        if (r.word == 0) return;
+        // V^: 4 keys x 16 dims to the V^T tile
+        float vs[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[j] = __shfl(r.vs, quad_key(qd, j), 64);
+        uint4 vc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            vc[j] = r.v[j];
+            if (r.word != ~0u && !((r.word >> quad_key(qd, j)) & 1u)) {  // what a masked key holds meets no product
+                vc[j] = make_uint4(0u, 0u, 0u, 0u);
+                vs[j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // dims 16 dg + 2 i, + 1
+            f32x2 f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[j] = codes2_f32<FMT>(word(vc[j], i >> 1), i & 1);
+                f[j][0] *= vs[j];
+                f[j][1] *= vs[j];
+            }
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+                *reinterpret_cast<uint2*>(vt + dg * WV_GROUP + (2 * i + d) * WV_ROW + 8 * qd) =
+                    make_uint2(pack_f16_of_bf16(f[0][d], f[1][d]), pack_f16_of_bf16(f[2][d], f[3][d]));
+        }
+        f32x16 s;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) {
+            uint32_t d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x2 f = codes2_f32<FMT>(word(r.k[sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
+                d[e] = pack_bf16(f[0] * r.ks, f[1] * r.ks);
+            }
+            s = mfma_bf16(__builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3])), qf[sl], s);
+        }
+        finish(s, r.word);
+    };
+    const int dealt = split * 4 + wave;  // blocks dealt, dealt + step, ..
+    {
+        int t = dealt;
+        WaveRegs ra, rb;
+        load(t, ra);
+        load(t + step, rb);
+        const int n_cache = list ? list_length(list, p.top_k) << sh32 : limit;
+        while (t < n_cache) {
+            block(ra);
+            t += step;
+            if (t >= n_cache) break;
+            load(t + step, ra);
+            block(rb);
+            t += step;
+            load(t + step, rb);
+        }
+    }
+    for (int t = step - 1 - dealt; t < (cur_len + 31) / 32; t += step) {  // tail blocks, from the last wave on
+        const int first = t * 32, left = cur_len - first, mine = min(col, left - 1);
+        const bool ok = col < left && (!p.uvalid || p.uvalid[b * p.uvs + first + mine] != 0);
+        const uint32_t word_ = (uint32_t)__ballot(ok);
+        if (word_ == 0) continue;
+        const int64_t base = b * p.us0 + first * p.us1 + h * p.us2;
+        uint4 kx[8], vx[4][2];
+        const uint4* kp = reinterpret_cast<const uint4*>(p.kcur + base + mine * p.us1 + 64 * half);
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) kx[sl] = kp[sl];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int key = quad_key(qd, j);
+            const uint4* vp = reinterpret_cast<const uint4*>(p.vcur + base + min(key, left - 1) * p.us1 + 16 * dg);
+            vx[j][0] = vp[0];
+            vx[j][1] = vp[1];
+            if (!((word_ >> key) & 1u)) vx[j][0] = vx[j][1] = make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = word(vx[j][i >> 2], i & 3);
+            uint8_t* dst = vt + dg * WV_GROUP + 2 * i * WV_ROW + 8 * qd;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[0]), bf16_lo(y[1]))),
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[2]), bf16_lo(y[3]))));
+            *reinterpret_cast<uint2*>(dst + WV_ROW) = make_uint2(
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[0]), bf16_hi(y[1]))),
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[2]), bf16_hi(y[3]))));
+        }
+        f32x16 s;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) s = mfma_bf16(__builtin_bit_cast(bf16x8, kx[sl]), qf[sl], s);
+        finish(s, word_);
+    }
+    // The four waves' partial results meet in LDS (over the V^T tiles).
+    const float l = run_.l + __shfl_xor(run_.l, 32, 64);
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);
+    if (col < rows) {
+        float* dst = so + (wave * 32 + col) * WO_PITCH;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int vq = 0; vq < 4; ++vq)
+                *reinterpret_cast<float4*>(dst + db * 32 + vq * 8 + half * 4) =
+                    make_float4(o[db][vq * 4], o[db][vq * 4 + 1], o[db][vq * 4 + 2], o[db][vq * 4 + 3]);
+        if (half == 0) {
+            sml[wave][col][0] = run_.m;
+            sml[wave][col][1] = l;
+        }
+    }
+    __syncthreads();
+    const int64_t hqs = p.H * p.G;
+    for (int at = threadIdx.x; at < rows * (D / 4); at += 256) {
+        const int r = at / (D / 4), d = (at % (D / 4)) * 4;
+        float m = sml[0][r][0];
+#pragma unroll
+        for (int wv = 1; wv < 4; ++wv) m = fmaxf(m, sml[wv][r][0]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float den = 0.0f;
+        float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int wv = 0; wv < 4; ++wv) {
+            const float a = __builtin_amdgcn_exp2f(sml[wv][r][0] - base);
+            const float4 y = *reinterpret_cast<const float4*>(so + (wv * 32 + r) * WO_PITCH + d);
+            den = __builtin_fmaf(sml[wv][r][1], a, den);
+            num.x = __builtin_fmaf(y.x, a, num.x);
+            num.y = __builtin_fmaf(y.y, a, num.y);
+            num.z = __builtin_fmaf(y.z, a, num.z);
+            num.w = __builtin_fmaf(y.w, a, num.w);
+        }
+        const int64_t i = i0 + r / p.G, hq = h * p.G + r % p.G, slot = (b * hqs + hq) * p.Lq + i;
+        if (p.splits > 1) {
+            const int64_t part = (int64_t)split * p.B * hqs * p.Lq + slot;
+            *reinterpret_cast<float4*>(p.ws_o + part * D + d) = num;
+            if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, den);
+        } else {
+            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+            *reinterpret_cast<uint2*>(p.out + b * p.os0 + i * p.os1 + hq * p.os2 + d) =
+                make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
+            if (d == 0) p.lse[slot] = den > 0.0f ? (m + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+        }
+    }
+}
+
+// Merge of the key splits, with the row's log-sum-exp: with M = max m_s,
+// O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s. 32 threads a row, 4 dims each, eight
+// splits' loads in flight; the order of the sums is that of the splits.
 __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
     const int64_t hqs = p.H * p.G, rows = p.B * hqs * p.Lq;
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // (b * Hq + hq) * Lq + i
     if (r >= rows) return;
     const int d = (threadIdx.x & 31) * 4;
-    float M = -INFINITY;
-    for (int sp = 0; sp < p.splits; ++sp) M = fmaxf(M, p.ws_ml[(sp * rows + r) * 2]);
-    const float base = M == -INFINITY ? 0.0f : M;
-    float den = 0.0f, num[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int sp = 0; sp < p.splits; ++sp) {
-        const int64_t at = sp * rows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + at * 2);
-        const float4 ov = *reinterpret_cast<const float4*>(p.ws_o + at * D + d);
-        const float wgt = __builtin_amdgcn_exp2f(ml.x - base);
-        den = fmaf(wgt, ml.y, den);
-        num[0] = fmaf(wgt, ov.x, num[0]);
-        num[1] = fmaf(wgt, ov.y, num[1]);
-        num[2] = fmaf(wgt, ov.z, num[2]);
-        num[3] = fmaf(wgt, ov.w, num[3]);
+    float M = -INFINITY, den = 0.0f;
+    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+        float2 ml[8];
+        float4 ov[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t at = (int64_t)min(s0 + e, p.splits - 1) * rows + r;
+            ml[e] = *reinterpret_cast<const float2*>(p.ws_ml + at * 2);
+            ov[e] = *reinterpret_cast<const float4*>(p.ws_o + at * D + d);
+            if (s0 + e >= p.splits) ml[e] = make_float2(-INFINITY, 0.0f);  // (the last split again: no weight)
+        }
+        float top = M;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, ml[e].x);
+        const float base = top == -INFINITY ? 0.0f : top, a = __builtin_amdgcn_exp2f(M - base);
+        den *= a;
+        num.x *= a; num.y *= a; num.z *= a; num.w *= a;
+        M = top;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float wgt = __builtin_amdgcn_exp2f(ml[e].x - base);
+            den = fmaf(wgt, ml[e].y, den);
+            num.x = fmaf(wgt, ov[e].x, num.x);
+            num.y = fmaf(wgt, ov[e].y, num.y);
+            num.z = fmaf(wgt, ov[e].z, num.z);
+            num.w = fmaf(wgt, ov[e].w, num.w);
+        }
     }
     const int64_t i = r % p.Lq, hq = (r / p.Lq) % hqs, b = r / (p.Lq * hqs);
     const float inv = den > 0.0f ? 1.0f / den : 0.0f;
     *reinterpret_cast<uint2*>(p.out + b * p.os0 + i * p.os1 + hq * p.os2 + d) =
-        make_uint2(pack_bf16(num[0] * inv, num[1] * inv), pack_bf16(num[2] * inv, num[3] * inv));
-    if (d == 0) p.lse[r] = den > 0.0f ? (base + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+        make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
+    if (d == 0) p.lse[r] = den > 0.0f ? (M + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -639,9 +1168,11 @@ static int blocks_splits(int64_t work, int64_t tiles) {
     return sp > 1 ? (int)sp : 1;
 }
 
+// few: the rows of a run where at most 32 (attn_row_kernel for one, attn_waves_kernel
+// for more), else 0 (attn_blocks_kernel).
 struct BlocksPlan {
     int64_t runs, q_tiles, work;
-    int splits;
+    int splits, few;
 };
 
 static BlocksPlan blocks_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t kv_len, int64_t cur_len,
@@ -649,10 +1180,20 @@ static BlocksPlan blocks_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int6
     BlocksPlan pl;
     pl.runs = (Lq - 1) / q_block + 1;
     const int64_t rows = (q_block < Lq ? q_block : Lq) * (Hq / H);
-    pl.q_tiles = (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
-    pl.work = B * H * pl.runs * pl.q_tiles;
     const int64_t listed = top_k >= 0 ? top_k * (block / attn::BKV) : (kv_len + attn::BKV - 1) / attn::BKV;
-    pl.splits = blocks_splits(pl.work, listed + (cur_len + attn::BKV - 1) / attn::BKV);
+    const int64_t tiles = listed + (cur_len + attn::BKV - 1) / attn::BKV;
+    pl.few = rows <= 32 ? (int)rows : 0;
+    pl.q_tiles = pl.few ? 1 : (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
+    pl.work = B * H * pl.runs * pl.q_tiles;
+    if (pl.few) {
+        // 4 waves a workgroup, a tile each at a time: enough splits for 2 workgroups
+        // per CU, and none without a tile
+        int64_t sp = 2LL * device_cus() / pl.work;
+        if (sp > (tiles + 3) / 4) sp = (tiles + 3) / 4;
+        pl.splits = sp > 1 ? (int)sp : 1;
+    } else {
+        pl.splits = blocks_splits(pl.work, tiles);
+    }
     return pl;
 }
 
@@ -708,8 +1249,9 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     }
     if (cur_len > 0) {
         HN_REQUIRE(kcur && vcur, HN_E_ARG, "hn_attn_kv_blocks: null tail pointer");
-        HN_REQUIRE(curs[3] == 1 && curs[0] % 8 == 0 && curs[1] % 8 == 0 && curs[2] % 8 == 0, HN_E_ARG,
-                   "hn_attn_kv_blocks: tail strides must be multiples of 8");
+        HN_REQUIRE(curs[3] == 1 && curs[0] % 8 == 0 && curs[1] % 8 == 0 && curs[2] % 8 == 0 && curs[0] >= 0 &&
+                       curs[1] >= 0 && curs[1] <= 0xffffffLL && curs[2] >= 0,
+                   HN_E_ARG, "hn_attn_kv_blocks: tail strides must be multiples of 8, below 2^24 per token");
         HN_REQUIRE(aligned(kcur, 16) && aligned(vcur, 16), HN_E_ARG, "hn_attn_kv_blocks: tail misaligned");
     }
     if (B == 0 || Lq == 0) return HN_OK;
@@ -759,7 +1301,15 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
     const bool mask = p.kvalid || p.uvalid;
-    if (fmt == HN_KV_FP8) {
+    if (pl.few) {
+        if (fmt == HN_KV_FP8) {
+            if (pl.few == 1) attn::attn_row_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
+            else attn::attn_waves_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
+        } else {
+            if (pl.few == 1) attn::attn_row_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
+            else attn::attn_waves_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
+        }
+    } else if (fmt == HN_KV_FP8) {
         if (mask) attn::attn_blocks_kernel<HN_KV_FP8, true><<<grid, 256, 0, st>>>(p);
         else attn::attn_blocks_kernel<HN_KV_FP8, false><<<grid, 256, 0, st>>>(p);
     } else {
