@@ -636,7 +636,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to 32 rows a run: one matrix column block holds all of them, so the waves of a
+// Up to 64 rows a run: a matrix column block holds 32 of them, so the waves of a
 // workgroup share the keys instead of the rows. Every wave takes 32-key blocks of its
 // own, without barriers: K codes go from global memory to MFMA operands in registers
 // (lane half: 64 contiguous dims, which the Q operand matches), V^ passes through the
@@ -666,21 +666,40 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     const int id = blockIdx.x;
     const int w = (id & 7) * p.per_xcd + (id >> 3);
     if (w >= p.work) return;
-    // heads fastest, then the splits of a run
-    const int64_t h = w % p.H;
-    int x = w / (int)p.H;
-    const int split = x % p.splits;
-    x /= p.splits;
-    const int64_t run = x % p.runs, b = x / p.runs;
+    // Lists: the row tiles of a run (which read the same blocks), its splits, then the
+    // runs of a head. Whole cache: heads fastest, which share the lines of a key
+    // range's scales.
+    int64_t h, run, b;
+    int split, row0, x = w;
+    if (p.idx) {
+        row0 = 32 * (x % p.q_tiles);
+        x /= p.q_tiles;
+        split = x % p.splits;
+        x /= p.splits;
+        run = x % p.runs;
+        x /= (int)p.runs;
+        h = x % p.H;
+        b = x / p.H;
+    } else {
+        h = x % p.H;
+        x /= (int)p.H;
+        split = x % p.splits;
+        x /= p.splits;
+        row0 = 32 * (x % p.q_tiles);
+        x /= p.q_tiles;
+        run = x % p.runs;
+        b = x / p.runs;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5, qd = lane & 7, dg = lane >> 3;
     const int64_t i0 = run * p.q_block;
     const int64_t queries = p.Lq - i0 < p.q_block ? p.Lq - i0 : p.q_block;
-    const int rows = (int)(queries * p.G);  // 1 .. 32
+    const int rows = min((int)(queries * p.G) - row0, 32);  // rows row0 .. of the run
+    if (rows <= 0) return;  // (the whole workgroup: a last run of fewer rows)
     uint8_t* const vt = smem + wave * WV_BYTES;
     bf16x8 qf[8];
     {
-        const int r = col < rows ? col : rows - 1;
+        const int r = row0 + (col < rows ? col : rows - 1);
         const uint16_t* src = p.q + b * p.qs0 + (i0 + r / p.G) * p.qs1 + (h * p.G + r % p.G) * p.qs2 + 64 * half;
 #pragma unroll
         for (int sl = 0; sl < 8; ++sl) qf[sl] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 8 * sl));
@@ -700,9 +719,20 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     Run run_{-INFINITY, 0.0f, 0.0f};
     const float c = p.scale_log2;
 
-    // Codes of cache block t < limit; a block without a key leaves word 0. Keys past the
-    // end read the last one's rows. (The first loads do not wait for the list's length:
-    // what lies past its end is dropped afterwards.)
+    // Loads through descriptors spanning the (b, h) rows of the cache, at 32-bit offsets
+    // (rows past kv_len read as zeros); a span of 2^31 bytes or more is replaced by the
+    // block's own rows, block by block.
+    const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1 * 4u;
+    const bool span_ok = p.kv_len > 0 && (p.kv_len - 1) * p.cs1 + D < ((int64_t)1 << 31) &&
+                         ((p.kv_len - 1) * p.ss1 + 1) * 4 < ((int64_t)1 << 31);
+    TileBase src = tile_base(p, b, h, 0, span_ok ? kv_len : 0);
+    const uint32_t off_k = (uint32_t)col * cs1 + 64u * half, off_s = (uint32_t)col * ss1;
+    uint32_t off_v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) off_v[j] = (uint32_t)quad_key(qd, j) * cs1 + 16u * dg;
+    // Codes of cache block t < limit; a block without a key leaves word 0. (The first
+    // loads do not wait for the list's length: what lies past its end is dropped
+    // afterwards.)
     auto load = [&](int t, WaveRegs& r) __attribute__((always_inline)) {
         r.word = 0;
         if (t >= limit) return;
@@ -714,74 +744,67 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             left = there ? kv_len - first : 0;
         }
         if (left <= 0) return;
-        const int mine = min(col, left - 1);
-        const int64_t base = b * p.cs0 + first * p.cs1 + h * p.cs2;
-        const uint4* kp = reinterpret_cast<const uint4*>(p.kc + base + mine * p.cs1 + 64 * half);
+        uint32_t co = (uint32_t)first * cs1, so_ = (uint32_t)first * ss1;
+        if (!span_ok) {
+            src = tile_base(p, b, h, first, min(left, 32));
+            co = so_ = 0;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r.k[e] = kp[e];
-        const int64_t sa = b * p.ss0 + (first + mine) * p.ss1 + h * p.ss2;
-        r.ks = p.ks[sa];
-        r.vs = p.vs[sa];
+        for (int e = 0; e < 4; ++e)
+            r.k[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src.k, off_k + co + 16 * e, 0, 0));
+        r.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.ks, off_s + so_, 0, 0));
+        r.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.vs, off_s + so_, 0, 0));
         bool ok = col < left;
-        if (p.kvalid) ok = ok && p.kvalid[b * p.kvs + first + mine] != 0;
+        if (p.kvalid) ok = ok && p.kvalid[b * p.kvs + first + min(col, left - 1)] != 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            r.v[j] = *reinterpret_cast<const uint4*>(p.vc + base + min(quad_key(qd, j), left - 1) * p.cs1 + 16 * dg);
+            r.v[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src.v, off_v[j] + co, 0, 0));
         r.word = (uint32_t)__ballot(ok);
     };
-    // P and PV of a block whose V^T is in the wave's tile.
-    auto finish = [&](f32x16& s, uint32_t word) __attribute__((always_inline)) {
+    // P and PV of a block whose V^T operands are vf (operand 4 tt + db).
+    auto finish = [&](f32x16& s, uint32_t word, const f16x8 (&vf)[8]) __attribute__((always_inline)) {
         const float mx = word != ~0u ? mask_word(s, word) : raw_max(s);
         rebase(mx, c, run_, o);
         f16x8 pf[2];
         uint32_t x8[8];
-        float l = 0.0f;
+        float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, run_.nm));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, run_.nm));
             x8[i] = pack_f16(p0, p1);
-            l += p0;
-            l += p1;
+            l0 += p0;
+            l1 += p1;
         }
-        run_.l += l;
+        run_.l += l0 + l1;
         pf[0] = __builtin_bit_cast(f16x8, make_uint4(x8[0], x8[1], x8[2], x8[3]));
         pf[1] = __builtin_bit_cast(f16x8, make_uint4(x8[4], x8[5], x8[6], x8[7]));
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-                o[db] = mfma_f16(ld_f16x8(vt + wv_row(32 * db + col) + 32 * tt + 16 * half), pf[tt], o[db]);
+        for (int i = 0; i < 8; ++i) o[i & 3] = mfma_f16(vf[i], pf[i >> 2], o[i & 3]);
     };
-    auto block = [&](const WaveRegs& r) __attribute__((always_inline)) {
+    auto read_v = [&](f16x8 (&vf)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vf[i] = ld_f16x8(vt + wv_row(32 * (i & 3) + col) + 32 * (i >> 2) + 16 * half);
+    };
+    auto block = [&](WaveRegs& r) __attribute__((always_inline)) {
         if (r.word == 0) return;
-        // V^: 4 keys x 16 dims to the V^T tile
         float vs[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) vs[j] = __shfl(r.vs, quad_key(qd, j), 64);
-        uint4 vc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            vc[j] = r.v[j];
-            if (r.word != ~0u && !((r.word >> quad_key(qd, j)) & 1u)) {  // what a masked key holds meets no product
-                vc[j] = make_uint4(0u, 0u, 0u, 0u);
-                vs[j] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // dims 16 dg + 2 i, + 1
-            f32x2 f[4];
+        if (r.word != ~0u) {  // what a masked key holds meets no product
+            const uint32_t m = r.word >> quad_key(qd, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f[j] = codes2_f32<FMT>(word(vc[j], i >> 1), i & 1);
-                f[j][0] *= vs[j];
-                f[j][1] *= vs[j];
+                const bool in = (m >> j) & 1u;
+                r.v[j].x = in ? r.v[j].x : 0u;
+                r.v[j].y = in ? r.v[j].y : 0u;
+                r.v[j].z = in ? r.v[j].z : 0u;
+                r.v[j].w = in ? r.v[j].w : 0u;
+                vs[j] = in ? vs[j] : 0.0f;
             }
-#pragma unroll
-            for (int d = 0; d < 2; ++d)
-                *reinterpret_cast<uint2*>(vt + dg * WV_GROUP + (2 * i + d) * WV_ROW + 8 * qd) =
-                    make_uint2(pack_f16_of_bf16(f[0][d], f[1][d]), pack_f16_of_bf16(f[2][d], f[3][d]));
         }
+        // Slot sl: K operand sl and its product, and V^ dims 16 dg + 2 sl, + 1 of the quad's
+        // keys to the V^T tile.
         f32x16 s;
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[v] = 0.0f;
@@ -794,8 +817,22 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
                 d[e] = pack_bf16(f[0] * r.ks, f[1] * r.ks);
             }
             s = mfma_bf16(__builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3])), qf[sl], s);
+            f32x2 f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[j] = codes2_f32<FMT>(word(r.v[j], sl >> 1), sl & 1);
+                f[j][0] *= vs[j];
+                f[j][1] *= vs[j];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint2*>(vt + dg * WV_GROUP + (2 * sl + e) * WV_ROW + 8 * qd) =
+                    make_uint2(pack_f16_of_bf16(f[0][e], f[1][e]), pack_f16_of_bf16(f[2][e], f[3][e]));
+            __builtin_amdgcn_sched_barrier(0);
         }
-        finish(s, r.word);
+        f16x8 vf[8];
+        read_v(vf);
+        finish(s, r.word, vf);
     };
     const int dealt = split * 4 + wave;  // blocks dealt, dealt + step, ..
     {
@@ -814,43 +851,64 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             load(t + step, rb);
         }
     }
-    for (int t = step - 1 - dealt; t < (cur_len + 31) / 32; t += step) {  // tail blocks, from the last wave on
-        const int first = t * 32, left = cur_len - first, mine = min(col, left - 1);
-        const bool ok = col < left && (!p.uvalid || p.uvalid[b * p.uvs + first + mine] != 0);
-        const uint32_t word_ = (uint32_t)__ballot(ok);
-        if (word_ == 0) continue;
-        const int64_t base = b * p.us0 + first * p.us1 + h * p.us2;
+    // Tail blocks, dealt from the last wave on. One set of registers: the next block's V
+    // is fetched once this one's is in LDS, its K once its logits are formed.
+    const int n_tail = (cur_len + 31) / 32;
+    if (step - 1 - dealt < n_tail) {
         uint4 kx[8], vx[4][2];
-        const uint4* kp = reinterpret_cast<const uint4*>(p.kcur + base + mine * p.us1 + 64 * half);
+        bool ok = false;
+        auto fetch_k = [&](int t) __attribute__((always_inline)) {
+            const int first = t * 32, left = cur_len - first;
+            if (left <= 0) return;
+            const int mine = first + min(col, left - 1);
+            const uint4* kp = reinterpret_cast<const uint4*>(p.kcur + b * p.us0 + mine * p.us1 + h * p.us2 + 64 * half);
 #pragma unroll
-        for (int sl = 0; sl < 8; ++sl) kx[sl] = kp[sl];
+            for (int sl = 0; sl < 8; ++sl) kx[sl] = kp[sl];
+            ok = col < left && (!p.uvalid || p.uvalid[b * p.uvs + mine] != 0);
+        };
+        auto fetch_v = [&](int t) __attribute__((always_inline)) {
+            const int first = t * 32, left = cur_len - first;
+            if (left <= 0) return;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int key = quad_key(qd, j);
-            const uint4* vp = reinterpret_cast<const uint4*>(p.vcur + base + min(key, left - 1) * p.us1 + 16 * dg);
-            vx[j][0] = vp[0];
-            vx[j][1] = vp[1];
-            if (!((word_ >> key) & 1u)) vx[j][0] = vx[j][1] = make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < 4; ++j) {
+                const uint4* vp = reinterpret_cast<const uint4*>(
+                    p.vcur + b * p.us0 + (first + min(quad_key(qd, j), left - 1)) * p.us1 + h * p.us2 + 16 * dg);
+                vx[j][0] = vp[0];
+                vx[j][1] = vp[1];
+            }
+        };
+        int t = step - 1 - dealt;
+        fetch_k(t);
+        fetch_v(t);
+        for (; t < n_tail; t += step) {
+            const uint32_t now = (uint32_t)__ballot(ok);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = word(vx[j][i >> 2], i & 3);
+                    if (now != ~0u && !((now >> quad_key(qd, j)) & 1u)) y[j] = 0u;
+                }
+                uint8_t* dst = vt + dg * WV_GROUP + 2 * i * WV_ROW + 8 * qd;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[0]), bf16_lo(y[1]))),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[2]), bf16_lo(y[3]))));
+                *reinterpret_cast<uint2*>(dst + WV_ROW) = make_uint2(
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[0]), bf16_hi(y[1]))),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[2]), bf16_hi(y[3]))));
+            }
+            fetch_v(t + step);
+            f32x16 s;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+            for (int sl = 0; sl < 8; ++sl) s = mfma_bf16(__builtin_bit_cast(bf16x8, kx[sl]), qf[sl], s);
+            fetch_k(t + step);
+            f16x8 vf[8];
+            read_v(vf);
+            if (now != 0) finish(s, now, vf);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint32_t y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = word(vx[j][i >> 2], i & 3);
-            uint8_t* dst = vt + dg * WV_GROUP + 2 * i * WV_ROW + 8 * qd;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[0]), bf16_lo(y[1]))),
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(y[2]), bf16_lo(y[3]))));
-            *reinterpret_cast<uint2*>(dst + WV_ROW) = make_uint2(
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[0]), bf16_hi(y[1]))),
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_hi(y[2]), bf16_hi(y[3]))));
-        }
-        f32x16 s;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
-#pragma unroll
-        for (int sl = 0; sl < 8; ++sl) s = mfma_bf16(__builtin_bit_cast(bf16x8, kx[sl]), qf[sl], s);
-        finish(s, word_);
     }
     // The four waves' partial results meet in LDS (over the V^T tiles).
     const float l = run_.l + __shfl_xor(run_.l, 32, 64);
@@ -889,7 +947,7 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             num.z = __builtin_fmaf(y.z, a, num.z);
             num.w = __builtin_fmaf(y.w, a, num.w);
         }
-        const int64_t i = i0 + r / p.G, hq = h * p.G + r % p.G, slot = (b * hqs + hq) * p.Lq + i;
+        const int64_t i = i0 + (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G, slot = (b * hqs + hq) * p.Lq + i;
         if (p.splits > 1) {
             const int64_t part = (int64_t)split * p.B * hqs * p.Lq + slot;
             *reinterpret_cast<float4*>(p.ws_o + part * D + d) = num;
@@ -1168,8 +1226,12 @@ static int blocks_splits(int64_t work, int64_t tiles) {
     return sp > 1 ? (int)sp : 1;
 }
 
-// few: the rows of a run where at most 32 (attn_row_kernel for one, attn_waves_kernel
-// for more), else 0 (attn_blocks_kernel).
+// few: the rows of a run where at most 64 (attn_row_kernel for one, attn_waves_kernel
+// for more, 32 rows a workgroup), else 0 (attn_blocks_kernel).
+// What a workgroup of the few-row kernels costs beside its tiles, in units of a wave's
+// 64-key tile: the list, the first loads, the meeting of the waves.
+constexpr double FEW_FIXED = 2.0;
+
 struct BlocksPlan {
     int64_t runs, q_tiles, work;
     int splits, few;
@@ -1182,15 +1244,24 @@ static BlocksPlan blocks_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int6
     const int64_t rows = (q_block < Lq ? q_block : Lq) * (Hq / H);
     const int64_t listed = top_k >= 0 ? top_k * (block / attn::BKV) : (kv_len + attn::BKV - 1) / attn::BKV;
     const int64_t tiles = listed + (cur_len + attn::BKV - 1) / attn::BKV;
-    pl.few = rows <= 32 ? (int)rows : 0;
-    pl.q_tiles = pl.few ? 1 : (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
+    pl.few = rows <= 64 ? (int)rows : 0;
+    pl.q_tiles = pl.few ? (rows + 31) / 32 : (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
     pl.work = B * H * pl.runs * pl.q_tiles;
     if (pl.few) {
-        // 4 waves a workgroup, a tile each at a time: enough splits for 2 workgroups
-        // per CU, and none without a tile
-        int64_t sp = 2LL * device_cus() / pl.work;
-        if (sp > (tiles + 3) / 4) sp = (tiles + 3) / 4;
-        pl.splits = sp > 1 ? (int)sp : 1;
+        // 4 waves a workgroup, a tile each at a time, 2 workgroups per CU: splits that
+        // leave no round of workgroups nearly empty (rounds / splits is the time in
+        // units of an unsplit round), each with a tile for every wave
+        const int64_t slots = 2LL * device_cus(), most = (tiles + 3) / 4;
+        double best = 1e30;
+        pl.splits = 1;
+        for (int64_t sp = 1; sp <= most && sp <= 64 && pl.work * sp <= 8 * slots; ++sp) {
+            const double rounds = (double)((pl.work * sp + slots - 1) / slots);
+            const double cost = rounds * (FEW_FIXED + (double)tiles / (double)(4 * sp));
+            if (cost < best) {
+                best = cost;
+                pl.splits = (int)sp;
+            }
+        }
     } else {
         pl.splits = blocks_splits(pl.work, tiles);
     }
