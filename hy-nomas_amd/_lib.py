@@ -71,14 +71,16 @@ SIGNATURES = {
     "hn_attn_key_mass": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _PI64, _I64, _I64, _I64,
                          _I64, _P, _I64, _F, _P, _PI64, _I64, _P, _P, _I64, _P],
     "hn_attn_key_mass_workspace_size": [_I64] * 6,
-    "hn_select_kv_tokens": [_P, _PI64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "hn_select_kv_tokens": [_P, _PI64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P],
+    "hn_select_kv_tokens_workspace_size": [_I64] * 3,
     "hn_move_kv_tokens": [_P, _P, _PI64, _P, _P, _PI64, _P, _PI64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P,
                           _PI64, _P, _P, _PI64, _I64, _P, _P],
     "hn_e4m3_encode_range": [ctypes.c_uint32, _I64, _P, _P],
 }
 RESTYPES = {"hn_last_error": ctypes.c_char_p, "hn_attn_fp8kv_workspace_size": _I64,
             "hn_attn_fp8kv_noalloc_scratch_bytes": _I64, "hn_select_kv_blocks_workspace_size": _I64,
-            "hn_attn_kv_blocks_workspace_size": _I64, "hn_attn_key_mass_workspace_size": _I64}
+            "hn_attn_kv_blocks_workspace_size": _I64, "hn_attn_key_mass_workspace_size": _I64,
+            "hn_select_kv_tokens_workspace_size": _I64}
 
 _lib = None
 _lock = threading.Lock()

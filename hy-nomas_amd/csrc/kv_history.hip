@@ -60,7 +60,7 @@ HN_DEVICE f32x2 decode2(uint32_t w, int hi) {
 template <int FMT>
 __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
     const int lane = threadIdx.x & 63, piece = lane & 7, row = lane >> 3;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (unit >= a.units) return;  // whole waves; no barrier below
     const int64_t h = unit % a.H, jb = unit / a.H, j = a.j0 + jb % a.blocks, b = jb / a.blocks;
     float lo[16], hi[16];
@@ -70,53 +70,70 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
         hi[c] = -INFINITY;
     }
     const int64_t tok0 = j * a.block;
-    const uint8_t* kc = a.kc + b * a.cs0 + h * a.cs2 + piece * 16;
-    const float* ks = a.ks + b * a.ss0 + h * a.ss2;
+    const uint32_t code_off = (uint32_t)row * (uint32_t)a.cs1 + 16u * piece, scale_off = (uint32_t)row * (uint32_t)a.ss1 * 4u;
     for (int64_t t0 = tok0; t0 < tok0 + a.block && t0 < a.end; t0 += 64) {
+        // descriptors of the 64 keys: rows past the end read as zeros
+        const int count = a.end - t0 < 64 ? (int)(a.end - t0) : 64;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(a.kc + b * a.cs0 + t0 * a.cs1 + h * a.cs2), (short)0,
+            (int)((count - 1) * a.cs1 + D), 0x00020000);
+        const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<float*>(a.ks + b * a.ss0 + t0 * a.ss1 + h * a.ss2), (short)0,
+            (int)(((count - 1) * a.ss1 + 1) * 4), 0x00020000);
         uint4 x[8];
         float s[8];
         bool ok[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int64_t t = t0 + 8 * i + row;
-            ok[i] = t < a.end && (!a.valid || a.valid[b * a.vs + t] != 0);
-            if (t < a.end) {
-                x[i] = *reinterpret_cast<const uint4*>(kc + t * a.cs1);
-                s[i] = ks[t * a.ss1];
-            }
+            x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, code_off + 8u * i * (uint32_t)a.cs1, 0, 0));
+            s[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sr, scale_off + 32u * i * (uint32_t)a.ss1, 0, 0));
+            ok[i] = 8 * i + row < count;
+        }
+        if (a.valid) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (ok[i]) ok[i] = a.valid[b * a.vs + t0 + 8 * i + row] != 0;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (!ok[i]) continue;
             const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            // a key that does not count becomes NaN, which minimum and maximum pass over
+            const float si = ok[i] ? s[i] : __builtin_nanf("");
 #pragma unroll
             for (int c = 0; c < 16; c += 2) {
                 const f32x2 f = decode2<FMT>(w[c >> 2], (c >> 1) & 1);
-                lo[c] = fminf(lo[c], f[0] * s[i]);
-                hi[c] = fmaxf(hi[c], f[0] * s[i]);
-                lo[c + 1] = fminf(lo[c + 1], f[1] * s[i]);
-                hi[c + 1] = fmaxf(hi[c + 1], f[1] * s[i]);
+                const float p0 = f[0] * si, p1 = f[1] * si;
+                lo[c] = fminf(lo[c], p0);
+                hi[c] = fmaxf(hi[c], p0);
+                lo[c + 1] = fminf(lo[c + 1], p1);
+                hi[c + 1] = fmaxf(hi[c + 1], p1);
             }
         }
     }
+    // The 8 rows' extremes meet while the channels are dealt out (lane xor 32, 16, 8): each
+    // exchange halves a lane's channels, 28 values a lane cross in all where plain
+    // reductions would move 96.
+    const bool up4 = row & 4, up2 = row & 2, up1 = row & 1;
+    float lo8[8], hi8[8], lo4[4], hi4[4], lo2[2], hi2[2];
 #pragma unroll
-    for (int c = 0; c < 16; ++c)
-#pragma unroll
-        for (int off = 8; off < 64; off <<= 1) {
-            lo[c] = fminf(lo[c], __shfl_xor(lo[c], off, 64));
-            hi[c] = fmaxf(hi[c], __shfl_xor(hi[c], off, 64));
-        }
-    if (row < 2) {  // lanes 0-7 write the lower bounds, lanes 8-15 the upper
-        uint32_t w[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float f0 = row ? hi[2 * c] : lo[2 * c], f1 = row ? hi[2 * c + 1] : lo[2 * c + 1];
-            w[c] = f32_to_bf16_bits(f0) | (f32_to_bf16_bits(f1) << 16);
-        }
-        uint4* dst = reinterpret_cast<uint4*>(a.out + b * a.bs0 + j * a.bs1 + h * a.bs2 + row * D + piece * 16);
-        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    for (int c = 0; c < 8; ++c) {
+        lo8[c] = fminf(up4 ? lo[8 + c] : lo[c], __shfl_xor(up4 ? lo[c] : lo[8 + c], 32, 64));
+        hi8[c] = fmaxf(up4 ? hi[8 + c] : hi[c], __shfl_xor(up4 ? hi[c] : hi[8 + c], 32, 64));
     }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        lo4[c] = fminf(up2 ? lo8[4 + c] : lo8[c], __shfl_xor(up2 ? lo8[c] : lo8[4 + c], 16, 64));
+        hi4[c] = fmaxf(up2 ? hi8[4 + c] : hi8[c], __shfl_xor(up2 ? hi8[c] : hi8[4 + c], 16, 64));
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        lo2[c] = fminf(up1 ? lo4[2 + c] : lo4[c], __shfl_xor(up1 ? lo4[c] : lo4[2 + c], 8, 64));
+        hi2[c] = fmaxf(up1 ? hi4[2 + c] : hi4[c], __shfl_xor(up1 ? hi4[c] : hi4[2 + c], 8, 64));
+    }
+    const int c0 = piece * 16 + (up4 ? 8 : 0) + (up2 ? 4 : 0) + (up1 ? 2 : 0);
+    uint16_t* dst = a.out + b * a.bs0 + j * a.bs1 + h * a.bs2 + c0;
+    *reinterpret_cast<uint32_t*>(dst) = f32_to_bf16_bits(lo2[0]) | (f32_to_bf16_bits(lo2[1]) << 16);
+    *reinterpret_cast<uint32_t*>(dst + D) = f32_to_bf16_bits(hi2[0]) | (f32_to_bf16_bits(hi2[1]) << 16);
 }
 
 // ---------------------------------------------------------------------------
@@ -544,6 +561,178 @@ __global__ __launch_bounds__(1024) void choose_tokens_kernel(TokenArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// Token choice in long rows: one workgroup a row leaves most of the device idle, so a
+// row is dealt to workgroups of PART tokens and each step of the search is a launch:
+// the counts of a digit of the rank (11, 11 and 10 bits) are added to the row's bins
+// (whole numbers: the order does not matter), the next launch reads the digit from
+// them, the last two count the taken tokens of each part and write them.
+constexpr int PART_KPT = 16, PART = 256 * PART_KPT, BINS = 2048;
+
+// Per row in the workspace: bins of the three digits, then {prefix, need} after each,
+// then {above, equal} of every part.
+struct LongRow {
+    uint32_t *bins, *state, *counts;
+};
+
+HN_DEVICE LongRow long_row(uint32_t* ws, int64_t row, int parts) {
+    uint32_t* base = ws + row * (3 * BINS + 8 + 2 * (int64_t)parts);
+    return LongRow{base, base + 3 * BINS, base + 3 * BINS + 8};
+}
+
+__global__ __launch_bounds__(256) void long_clear_kernel(uint32_t* ws, int parts) {
+    const LongRow r = long_row(ws, blockIdx.y, parts);
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < 3 * BINS) r.bins[i] = 0u;
+}
+
+// Digit d of a rank lies at bits SHIFT[d] ..; prefix holds the digits before it.
+HN_DEVICE constexpr int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+HN_DEVICE constexpr int digit_bins(int d) { return d == 2 ? 1024 : 2048; }
+
+// The digit in which the need-th rank (from the top) lies, from the row's bins of digit
+// d: prefix and need move on. Every thread of the 256 gets the same result.
+HN_DEVICE void find_digit(const uint32_t* bins, int d, uint32_t& prefix, uint32_t& need, uint32_t* shared) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = digit_bins(d) / 256;
+    uint32_t c[8], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += c[e] = e < per ? bins[t * per + e] : 0u;
+    uint32_t suffix = sum;  // of this thread's bins and all above, in the wave
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_down(suffix, off, 64);
+        if (lane + off < 64) suffix += o;
+    }
+    if (lane == 0) shared[wave] = suffix;
+    __syncthreads();
+    uint32_t over = suffix - sum;
+    for (int w = wave + 1; w < 4; ++w) over += shared[w];
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+        if (over < need && need <= over + c[e]) {
+            shared[4] = prefix | ((uint32_t)(t * per + e) << digit_shift(d));
+            shared[5] = need - over;
+        }
+        over += c[e];
+    }
+    __syncthreads();
+    prefix = shared[4];
+    need = shared[5];
+}
+
+// Launch `step` of the search over a part: 0, 1, 2 count that digit, 3 counts the part's
+// taken tokens, 4 writes them.
+template <int STEP, bool MASK>
+__global__ __launch_bounds__(256) void long_tokens_kernel(TokenArgs a, uint32_t* ws, int parts) {
+    __shared__ uint32_t hist[STEP < 3 ? 4 * (BINS + 4) : 4], shared[8], wave_counts[4][2];
+    const int64_t rowi = blockIdx.y, h = rowi % a.H, b = rowi / a.H;
+    const int part = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const LongRow lr = long_row(ws, rowi, parts);
+    MassRow<MASK> row;
+    row.m = row_rsrc(a.mass + b * a.ms0 + h * a.ms1, (int64_t)a.n * 4);
+    row.valid = row_rsrc(MASK ? a.valid + b * a.vs : nullptr, MASK ? a.n : 0);
+    row.n = (uint32_t)a.n;
+    row.first = (uint32_t)a.first;
+    row.middle = a.n - a.last > a.first ? (uint32_t)(a.n - a.last - a.first) : 0u;
+    const int i0 = part * PART + wave * (PART / 4);
+    uint32_t u[PART_KPT];
+#pragma unroll
+    for (int e = 0; e < PART_KPT; ++e) u[e] = row.load(i0 + 64 * e + lane);
+    // digits found so far
+    uint32_t prefix = 0, need = (uint32_t)(a.keep < a.n ? a.keep : a.n);
+    if constexpr (STEP == 2 || STEP == 3) {
+        prefix = lr.state[2 * (STEP - 2)];
+        need = lr.state[2 * (STEP - 2) + 1];
+    }
+    if constexpr (STEP >= 1 && STEP <= 3) {
+        find_digit(lr.bins + (STEP - 1) * BINS, STEP - 1, prefix, need, shared);
+        if (part == 0 && t == 0) {
+            lr.state[2 * (STEP - 1)] = prefix;
+            lr.state[2 * (STEP - 1) + 1] = need;
+        }
+    }
+    if constexpr (STEP == 4) {
+        prefix = lr.state[4];
+        need = lr.state[5];
+    }
+#pragma unroll
+    for (int e = 0; e < PART_KPT; ++e) u[e] = row.rank(i0 + 64 * e + lane, u[e]);
+    if constexpr (STEP < 3) {
+        constexpr int shift = digit_shift(STEP);
+        for (int i = t; i < 4 * (BINS + 4); i += 256) hist[i] = 0u;
+        __syncthreads();
+        uint32_t* mine = hist + (lane & 3) * (BINS + 4);
+#pragma unroll
+        for (int e = 0; e < PART_KPT; ++e) {
+            const bool in = STEP == 0 || ((u[e] ^ prefix) >> digit_shift(STEP > 0 ? STEP - 1 : 0)) == 0;
+            if (in) atomicAdd(&mine[(u[e] >> shift) & (uint32_t)(digit_bins(STEP) - 1)], 1u);
+        }
+        __syncthreads();
+        for (int i = t; i < digit_bins(STEP); i += 256) {
+            const uint32_t c = hist[i] + hist[BINS + 4 + i] + hist[2 * (BINS + 4) + i] + hist[3 * (BINS + 4) + i];
+            if (c) atomicAdd(&lr.bins[STEP * BINS + i], c);
+        }
+        return;
+    }
+    // taken: above prefix, and the first `need` equal to it (RANK_NONE, which the bins count
+    // too, is never taken: with fewer candidates than places prefix is RANK_NONE)
+    uint32_t above = 0, equal = 0;
+#pragma unroll
+    for (int e = 0; e < PART_KPT; ++e) {
+        above += u[e] > prefix;
+        equal += u[e] == prefix && u[e] != RANK_NONE;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        above += __shfl_xor(above, off, 64);
+        equal += __shfl_xor(equal, off, 64);
+    }
+    if (lane == 0) {
+        wave_counts[wave][0] = above;
+        wave_counts[wave][1] = equal;
+    }
+    __syncthreads();
+    if constexpr (STEP == 3) {
+        if (t < 2) lr.counts[2 * part + t] = wave_counts[0][t] + wave_counts[1][t] + wave_counts[2][t] + wave_counts[3][t];
+        return;
+    }
+    // counts before this part and of the row, then before this wave
+    uint32_t pa = 0, pe = 0, ta = 0, te = 0;
+    for (int q = lane; q < parts; q += 64) {
+        const uint32_t ca = lr.counts[2 * q], ce = lr.counts[2 * q + 1];
+        ta += ca;
+        te += ce;
+        pa += q < part ? ca : 0u;
+        pe += q < part ? ce : 0u;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        pa += __shfl_xor(pa, off, 64);
+        pe += __shfl_xor(pe, off, 64);
+        ta += __shfl_xor(ta, off, 64);
+        te += __shfl_xor(te, off, 64);
+    }
+    for (int w = 0; w < wave; ++w) {
+        pa += wave_counts[w][0];
+        pe += wave_counts[w][1];
+    }
+    uint32_t pos = pa + (pe < need ? pe : need), eq = pe;
+    const uint32_t total = ta + (te < need ? te : need);
+    int32_t* out = a.idx + rowi * a.keep;
+    const uint64_t before = (1ull << lane) - 1;
+#pragma unroll
+    for (int e = 0; e < PART_KPT; ++e) {
+        const bool same = u[e] == prefix && u[e] != RANK_NONE;
+        const uint64_t eqs = __ballot(same);
+        const bool take = u[e] > prefix || (same && eq + (uint32_t)__builtin_popcountll(eqs & before) < need);
+        const uint64_t takes = __ballot(take);
+        if (take) out[pos + (uint32_t)__builtin_popcountll(takes & before)] = i0 + 64 * e + lane;
+        pos += (uint32_t)__builtin_popcountll(takes);
+        eq += (uint32_t)__builtin_popcountll(eqs);
+    }
+    for (int i = (int)total + part * 256 + t; i < a.keep; i += parts * 256) out[i] = -1;
+}
+
+// ---------------------------------------------------------------------------
 // Move of the chosen tokens: row i of the output cache <- row idx[b, h, i] of
 // the source (codes and scales of K and V, and the mass), head by head. A
 // negative or out-of-range index leaves the row as it is (its mass becomes 0).
@@ -555,22 +744,24 @@ struct MoveArgs {
     const int32_t* idx;
     int64_t cs0, cs1, cs2, ss0, ss1, ss2, ms0, ms1;
     int64_t os0, os1, os2, ts0, ts1, ts2;
-    int64_t keep, tokens, rows, per_xcd;
+    int64_t keep, tokens;
+    uint32_t rows, per_xcd;  // of a batch: keep * H, an eighth of it
     int H;
 };
 
 __global__ __launch_bounds__(256) void move_tokens_kernel(MoveArgs a) {
     // Workgroup ids are dealt round-robin to the XCDs: id % 8 picks an eighth of the
     // rows, so that the lines of scales and indices that neighbouring rows share are
-    // fetched by one L2.
+    // fetched by one L2. (Rows in 32 bits: 64-bit divisions would cost more than the
+    // move itself.)
     const int l = threadIdx.x & 7;
-    const int64_t first = (int64_t)(blockIdx.x & 7) * a.per_xcd, end = first + a.per_xcd;
-    const int64_t step = (int64_t)(gridDim.x >> 3) * 32;
-    for (int64_t row = first + (int64_t)(blockIdx.x >> 3) * 32 + (threadIdx.x >> 3); row < end && row < a.rows;
-         row += step) {
-        const int64_t h = row % a.H, i = (row / a.H) % a.keep, b = row / (a.H * a.keep);
-        const int64_t at = (b * a.H + h) * a.keep + i;
-        const int64_t t = a.idx[at];
+    const int64_t b = blockIdx.y;
+    const uint32_t H = (uint32_t)a.H, first = (blockIdx.x & 7) * a.per_xcd;
+    const uint32_t end = first + a.per_xcd < a.rows ? first + a.per_xcd : a.rows;
+    for (uint32_t row = first + (blockIdx.x >> 3) * 32 + (threadIdx.x >> 3); row < end; row += (gridDim.x >> 3) * 32) {
+        const uint32_t i = row / H, h = row - i * H;
+        const int64_t at = (b * H + h) * a.keep + i;
+        const int32_t t = a.idx[at];
         const bool there = t >= 0 && t < a.tokens;
         if (l == 2) a.omass[at] = there ? a.mass[b * a.ms0 + h * a.ms1 + t] : 0.0f;
         if (!there) continue;
@@ -604,6 +795,8 @@ extern "C" int hn_kv_block_bounds(int fmt, const void* kc, const int64_t* cs, co
     HN_REQUIRE(cs && ss && bs, HN_E_ARG, "hn_kv_block_bounds: null stride array");
     HN_REQUIRE(cs[3] == 1 && cs[0] % 16 == 0 && cs[1] % 16 == 0 && cs[2] % 16 == 0, HN_E_ARG,
                "hn_kv_block_bounds: cache strides must be multiples of 16 bytes");
+    HN_REQUIRE(cs[1] >= 0 && cs[1] <= 0x1ffffffLL && ss[1] >= 0 && ss[1] <= 0x7fffffLL, HN_E_ARG,
+               "hn_kv_block_bounds: invalid cache strides");
     HN_REQUIRE(bs[0] % 8 == 0 && bs[1] % 8 == 0 && bs[2] % 8 == 0, HN_E_ARG,
                "hn_kv_block_bounds: bounds strides must be multiples of 8");
     HN_REQUIRE(valid_stride >= 0, HN_E_ARG, "hn_kv_block_bounds: negative validity stride");
@@ -699,9 +892,21 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
     return check_launch("hn_select_kv_blocks");
 }
 
+// Rows of up to this many tokens go to one workgroup each (which then holds them in
+// registers), longer ones to several.
+constexpr int64_t ONE_GROUP_TOKENS = 32 * 1024;
+
+static int64_t long_parts(int64_t kv_len) { return (kv_len + hist::PART - 1) / hist::PART; }
+
+extern "C" int64_t hn_select_kv_tokens_workspace_size(int64_t B, int64_t H, int64_t kv_len) {
+    if (B <= 0 || H <= 0 || kv_len <= ONE_GROUP_TOKENS) return 0;
+    return B * H * (3 * hist::BINS + 8 + 2 * long_parts(kv_len)) * (int64_t)sizeof(uint32_t);
+}
+
 extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t B, int64_t H, int64_t kv_len,
                                    const uint8_t* valid, int64_t valid_stride, int64_t keep, int64_t keep_first,
-                                   int64_t keep_last, int32_t* idx, void* stream) {
+                                   int64_t keep_last, int32_t* idx, void* workspace, int64_t workspace_bytes,
+                                   void* stream) {
     HN_REQUIRE(B >= 0 && H > 0 && kv_len >= 0 && kv_len <= 0x1fffffffLL && keep >= 0 && keep <= 0x1fffffffLL, HN_E_ARG,
                "hn_select_kv_tokens: invalid shape");
     HN_REQUIRE(keep_first >= 0 && keep_last >= 0 && keep_first <= keep && keep_last <= keep - keep_first, HN_E_ARG,
@@ -711,7 +916,10 @@ extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t
     HN_REQUIRE(aligned(mass, 4) && aligned(idx, 4), HN_E_ARG, "hn_select_kv_tokens: misaligned pointer");
     if (B == 0 || keep == 0) return HN_OK;
     HN_REQUIRE(idx && (mass || kv_len == 0), HN_E_ARG, "hn_select_kv_tokens: null pointer");
-    HN_REQUIRE(B * H <= 0x7fffffffLL, HN_E_ARG, "hn_select_kv_tokens: too many rows");
+    const int64_t need = hn_select_kv_tokens_workspace_size(B, H, kv_len);
+    HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
+               "hn_select_kv_tokens: workspace smaller than hn_select_kv_tokens_workspace_size() or misaligned");
+    HN_REQUIRE(B * H <= 65535, HN_E_ARG, "hn_select_kv_tokens: too many rows");
     if (const int rc = require_gfx950("hn_select_kv_tokens"); rc != HN_OK) return rc;
     hist::TokenArgs a;
     a.mass = mass; a.valid = valid; a.idx = idx;
@@ -719,18 +927,30 @@ extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t
     a.H = (int)H; a.n = (int)kv_len; a.keep = (int)keep; a.first = (int)keep_first; a.last = (int)keep_last;
     const unsigned grid = (unsigned)(B * H);
     hipStream_t st = (hipStream_t)stream;
-    // the smallest register form that holds a row (see choose_top)
-    const int form = kv_len <= 8 * 1024 ? 0 : kv_len <= 32 * 1024 ? 1 : kv_len <= 96 * 1024 ? 2 : 3;
-    if (valid) {
-        if (form == 0) hist::choose_tokens_kernel<8, true><<<grid, 1024, 0, st>>>(a);
-        else if (form == 1) hist::choose_tokens_kernel<32, true><<<grid, 1024, 0, st>>>(a);
-        else if (form == 2) hist::choose_tokens_kernel<96, true><<<grid, 1024, 0, st>>>(a);
-        else hist::choose_tokens_kernel<0, true><<<grid, 1024, 0, st>>>(a);
+    if (kv_len > ONE_GROUP_TOKENS) {
+        const int parts = (int)long_parts(kv_len);
+        uint32_t* ws = (uint32_t*)workspace;
+        const dim3 pg((unsigned)parts, grid);
+        hist::long_clear_kernel<<<dim3((3 * hist::BINS + 255) / 256, grid), 256, 0, st>>>(ws, parts);
+        if (valid) {
+            hist::long_tokens_kernel<0, true><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<1, true><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<2, true><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<3, true><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<4, true><<<pg, 256, 0, st>>>(a, ws, parts);
+        } else {
+            hist::long_tokens_kernel<0, false><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<1, false><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<2, false><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<3, false><<<pg, 256, 0, st>>>(a, ws, parts);
+            hist::long_tokens_kernel<4, false><<<pg, 256, 0, st>>>(a, ws, parts);
+        }
+    } else if (kv_len > 8 * 1024) {
+        if (valid) hist::choose_tokens_kernel<32, true><<<grid, 1024, 0, st>>>(a);
+        else hist::choose_tokens_kernel<32, false><<<grid, 1024, 0, st>>>(a);
     } else {
-        if (form == 0) hist::choose_tokens_kernel<8, false><<<grid, 1024, 0, st>>>(a);
-        else if (form == 1) hist::choose_tokens_kernel<32, false><<<grid, 1024, 0, st>>>(a);
-        else if (form == 2) hist::choose_tokens_kernel<96, false><<<grid, 1024, 0, st>>>(a);
-        else hist::choose_tokens_kernel<0, false><<<grid, 1024, 0, st>>>(a);
+        if (valid) hist::choose_tokens_kernel<8, true><<<grid, 1024, 0, st>>>(a);
+        else hist::choose_tokens_kernel<8, false><<<grid, 1024, 0, st>>>(a);
     }
     return check_launch("hn_select_kv_tokens");
 }
@@ -759,9 +979,10 @@ extern "C" int hn_move_kv_tokens(const void* k, const void* v, const int64_t* cs
     a.cs0 = cs[0]; a.cs1 = cs[1]; a.cs2 = cs[2]; a.ss0 = ss[0]; a.ss1 = ss[1]; a.ss2 = ss[2];
     a.ms0 = ms[0]; a.ms1 = ms[1];
     a.os0 = os[0]; a.os1 = os[1]; a.os2 = os[2]; a.ts0 = ts[0]; a.ts1 = ts[1]; a.ts2 = ts[2];
-    a.keep = keep; a.tokens = tokens; a.rows = B * keep * H; a.H = (int)H;
+    HN_REQUIRE(keep * H <= 0x7fffffffLL && B <= 65535, HN_E_ARG, "hn_move_kv_tokens: too many rows for one launch");
+    a.keep = keep; a.tokens = tokens; a.rows = (uint32_t)(keep * H); a.H = (int)H;
     a.per_xcd = (a.rows + 255) / 256 * 32;  // whole workgroups of 32 rows
     const int64_t grid = 8 * stream_grid(a.per_xcd / 32, 2);
-    hist::move_tokens_kernel<<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(a);
+    hist::move_tokens_kernel<<<dim3((unsigned)grid, (unsigned)B), 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("hn_move_kv_tokens");
 }

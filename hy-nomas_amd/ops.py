@@ -747,12 +747,24 @@ def _check_keys(codes: torch.Tensor, scale: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what}: codes [B, cap, H, D] with fp32 scales [B, cap, H, 1]")
 
 
-def _one_device(what: str, *tensors) -> None:
-    """Every tensor given is on a GPU, and all on the same one."""
-    _gpu(*tensors)
-    first = next(t for t in tensors if t is not None)
-    if any(t is not None and t.device != first.device for t in tensors):
-        raise RuntimeError(f"{what}: tensors are on different devices")
+def _one_device(what: str, first: torch.Tensor, *tensors) -> torch.device:
+    """The device of ``first``, a GPU, on which every other tensor given is too."""
+    _gpu(first, *tensors)
+    device = first.device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{what}: tensors are on different devices")
+    return device
+
+
+@functools.lru_cache(maxsize=1024)
+def _stride_array(strides: tuple):
+    """A C array of strides (read only by the library), one per layout."""
+    return (ctypes.c_int64 * len(strides))(*strides)
+
+
+def _strides(t: torch.Tensor):
+    return _stride_array(t.stride())
 
 
 def _mask_bytes(mask: Optional[torch.Tensor], rows: int, cols: int, what: str):
@@ -805,8 +817,8 @@ def _kv_block_bounds_op(bounds: torch.Tensor, k_codes: torch.Tensor, k_scale: to
     _one_device(what, k_codes, k_scale, bounds, vb)
     with _on(k_codes.device):
         L.check(L.load().hn_kv_block_bounds(
-            fmt, k_codes.data_ptr(), L.strides(k_codes), k_scale.data_ptr(), L.strides(k_scale), B, H, D, cap, start,
-            end, block, L.ptr(vb), vs, bounds.data_ptr(), L.strides(bounds), bounds.shape[1], _stream(k_codes)),
+            fmt, k_codes.data_ptr(), _strides(k_codes), k_scale.data_ptr(), _strides(k_scale), B, H, D, cap, start,
+            end, block, L.ptr(vb), vs, bounds.data_ptr(), _strides(bounds), bounds.shape[1], _stream(k_codes)),
             "hn_kv_block_bounds")
 
 
@@ -857,7 +869,7 @@ def select_kv_blocks(q: torch.Tensor, bounds: torch.Tensor, kv_len: int, top_k: 
         ws_bytes = lib.hn_select_kv_blocks_workspace_size(B, H, runs, blocks)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
         L.check(lib.hn_select_kv_blocks(
-            q.data_ptr(), L.strides(q), B, Lq, Hq, D, L.ptr(vb), vs, bounds.data_ptr(), L.strides(bounds), H, blocks,
+            q.data_ptr(), _strides(q), B, Lq, Hq, D, L.ptr(vb), vs, bounds.data_ptr(), _strides(bounds), H, blocks,
             q_block, top_k, keep_first, keep_last, idx.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)),
             "hn_select_kv_blocks")
     return idx
@@ -891,8 +903,8 @@ def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor
     if q.ndim != 4:
         raise ValueError(f"{what}: q must be [B, Lq, Hq, D]")
     B, Lq, Hq, D = q.shape
-    cap, H = k_codes.shape[1:3]
-    if k_codes.shape[0] not in (B, 1) or k_codes.shape[3] != D or H == 0 or Hq % H:
+    slots, cap, H, Dk = k_codes.shape
+    if slots not in (B, 1) or Dk != D or H == 0 or Hq % H:
         raise ValueError(f"{what}: cache [B or 1, cap, H, D] does not match q")
     if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride()
             or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape
@@ -911,7 +923,7 @@ def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor
         elif block_idx.stride(3) != 1:
             block_idx = block_idx.contiguous()
     scale = _softmax_scale(softmax_scale, D, what)
-    if k_codes.shape[0] != B:  # one history slot read by every query batch
+    if slots != B:  # one history slot read by every query batch
         k_codes, v_codes = k_codes.expand(B, -1, -1, -1), v_codes.expand(B, -1, -1, -1)
         k_scale, v_scale = k_scale.expand(B, -1, -1, -1), v_scale.expand(B, -1, -1, -1)
     cur_len = 0 if k_cur is None else k_cur.shape[1] if k_cur.ndim == 4 else -1
@@ -936,11 +948,11 @@ def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor
         ws_bytes = lib.hn_attn_kv_blocks_workspace_size(B, Lq, Hq, H, kv_len, cur_len, top_k, block, q_block)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
         L.check(lib.hn_attn_kv_blocks(
-            fmt, q.data_ptr(), L.strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), L.strides(k_codes),
-            k_scale.data_ptr(), v_scale.data_ptr(), L.strides(k_scale), H, cap, kv_len, L.ptr(kvb), kvs,
-            L.ptr(block_idx), None if block_idx is None else L.strides(block_idx), max(top_k, 0),
+            fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), _strides(k_codes),
+            k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), H, cap, kv_len, L.ptr(kvb), kvs,
+            L.ptr(block_idx), None if block_idx is None else _strides(block_idx), max(top_k, 0),
             block, q_block, L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
-            L.strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), L.strides(out),
+            _strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), _strides(out),
             lse.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_kv_blocks")
     return out, lse
 
@@ -954,8 +966,9 @@ def _(q, k_codes, v_codes, k_scale, v_scale, kv_len, block_idx=None, block=64, q
 def _head_rows(t: torch.Tensor) -> torch.Tensor:
     """bf16 [B, L, H, D] as the kernels load it: rows of D contiguous values at
     16-byte boundaries (a copy where it is laid out otherwise)."""
-    if t.stride(3) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(2) % 8:
-        return t.contiguous()
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or s0 % 8 or s1 % 8 or s2 % 8:
+        return t.clone(memory_format=torch.contiguous_format)
     return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
 
 
@@ -1000,9 +1013,9 @@ def attn_key_mass(q: torch.Tensor, lse: torch.Tensor, k_codes: torch.Tensor, k_s
         ws_bytes = lib.hn_attn_key_mass_workspace_size(Bq, Lq, Hq, B, H, kv_len)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
         L.check(lib.hn_attn_key_mass(
-            fmt, q.data_ptr(), L.strides(q), Bq, Lq, Hq, D, lse.data_ptr(), k_codes.data_ptr(), L.strides(k_codes),
-            k_scale.data_ptr(), L.strides(k_scale), B, H, cap, kv_len, L.ptr(kvb), kvs, scale,
-            L.ptr(prior) if n_prior else None, L.strides(prior) if n_prior else None, n_prior, mass.data_ptr(),
+            fmt, q.data_ptr(), _strides(q), Bq, Lq, Hq, D, lse.data_ptr(), k_codes.data_ptr(), _strides(k_codes),
+            k_scale.data_ptr(), _strides(k_scale), B, H, cap, kv_len, L.ptr(kvb), kvs, scale,
+            L.ptr(prior) if n_prior else None, _strides(prior) if n_prior else None, n_prior, mass.data_ptr(),
             L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_key_mass")
     return mass
 
@@ -1035,8 +1048,11 @@ def select_kv_tokens(mass: torch.Tensor, kv_len: int, keep: int, keep_first: int
     if H == 0:
         return idx
     with _on(mass.device):
-        L.check(L.load().hn_select_kv_tokens(mass.data_ptr(), L.strides(mass), B, H, kv_len, L.ptr(vb), vs, keep,
-                                             keep_first, keep_last, idx.data_ptr(), _stream(mass)),
+        lib = L.load()
+        ws_bytes = lib.hn_select_kv_tokens_workspace_size(B, H, kv_len)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=mass.device) if ws_bytes else None
+        L.check(lib.hn_select_kv_tokens(mass.data_ptr(), _strides(mass), B, H, kv_len, L.ptr(vb), vs, keep, keep_first,
+                                        keep_last, idx.data_ptr(), L.ptr(ws), ws_bytes, _stream(mass)),
                 "hn_select_kv_tokens")
     return idx
 
@@ -1046,16 +1062,24 @@ def _(mass, kv_len, keep, keep_first=0, keep_last=0, cache_valid=None):
     return mass.new_empty((mass.shape[0], mass.shape[1], keep), dtype=torch.int32)
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges that two tensors span meet."""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The address range that a tensor's elements lie in."""
+    last = 0
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    start = t.data_ptr()
+    return start, start + (last + 1) * t.element_size() if t.numel() else start
 
-    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+
+def _overlaps(outputs, inputs) -> bool:
+    """Whether an output's address range meets an input's."""
+    spans = [_span(t) for t in inputs]
+    for t in outputs:
+        a0, a1 = _span(t)
+        for b0, b1 in spans:
+            if a0 < b1 and b0 < a1:
+                return True
+    return False
 
 
 @eager_op("hy_nomas_amd::move_kv_tokens_", mutates_args=("out_k", "out_v", "out_k_scale", "out_v_scale"))
@@ -1089,9 +1113,8 @@ def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch
     if keep > out_k.shape[1]:
         raise ValueError(f"{what}: {keep} tokens exceed the output cache's capacity {out_k.shape[1]}")
     _one_device(what, k_codes, v_codes, k_scale, v_scale, mass, idx, out_k, out_v, out_k_scale, out_v_scale)
-    for o in (out_k, out_v, out_k_scale, out_v_scale):
-        if any(_overlap(o, t) for t in (k_codes, v_codes, k_scale, v_scale, mass, idx)):
-            raise ValueError(f"{what}: the output cache overlaps the source")
+    if _overlaps((out_k, out_v, out_k_scale, out_v_scale), (k_codes, v_codes, k_scale, v_scale, mass, idx)):
+        raise ValueError(f"{what}: the output cache overlaps the source")
     if mass.stride(2) != 1:
         mass = mass.contiguous()
     idx = idx.contiguous()
@@ -1100,10 +1123,10 @@ def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch
         return moved
     with _on(mass.device):
         L.check(L.load().hn_move_kv_tokens(
-            k_codes.data_ptr(), v_codes.data_ptr(), L.strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(),
-            L.strides(k_scale), mass.data_ptr(), L.strides(mass), B, H, D, mass.shape[2], idx.data_ptr(), keep,
-            out_k.data_ptr(), out_v.data_ptr(), L.strides(out_k), out_k_scale.data_ptr(), out_v_scale.data_ptr(),
-            L.strides(out_k_scale), out_k.shape[1], moved.data_ptr(), _stream(mass)), "hn_move_kv_tokens")
+            k_codes.data_ptr(), v_codes.data_ptr(), _strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(),
+            _strides(k_scale), mass.data_ptr(), _strides(mass), B, H, D, mass.shape[2], idx.data_ptr(), keep,
+            out_k.data_ptr(), out_v.data_ptr(), _strides(out_k), out_k_scale.data_ptr(), out_v_scale.data_ptr(),
+            _strides(out_k_scale), out_k.shape[1], moved.data_ptr(), _stream(mass)), "hn_move_kv_tokens")
     return moved
 
 

@@ -385,10 +385,13 @@ int64_t hn_attn_key_mass_workspace_size(int64_t Bq, int64_t Lq, int64_t Hq, int6
  * keep_last, then those of the largest mass, ties to the lowest index, NaN as -inf;
  * only tokens with valid[b * valid_stride + t] != 0 (NULL: all). idx: int32 [B, H,
  * keep] contiguous, ascending, -1 behind the last. mass: fp32 [B, H, kv_len], strides
- * ms[3] (ms[2] == 1). keep_first + keep_last <= keep. */
+ * ms[3] (ms[2] == 1). keep_first + keep_last <= keep. workspace:
+ * hn_select_kv_tokens_workspace_size() bytes (0 for short rows), 16-byte aligned. */
 int hn_select_kv_tokens(const float *mass, const int64_t *ms, int64_t B, int64_t H, int64_t kv_len,
                         const uint8_t *valid, int64_t valid_stride, int64_t keep, int64_t keep_first,
-                        int64_t keep_last, int32_t *idx, void *stream);
+                        int64_t keep_last, int32_t *idx, void *workspace, int64_t workspace_bytes, void *stream);
+
+int64_t hn_select_kv_tokens_workspace_size(int64_t B, int64_t H, int64_t kv_len);
 
 /* Moves the listed tokens of each head to the front of another cache: row i of the
  * output (codes and scales of K and V) and out_mass[b, h, i] <- token idx[b, h, i].

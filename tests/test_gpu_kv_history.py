@@ -515,6 +515,20 @@ def _evict_reference(mass, kv, keep, first, last, valid):
     return torch.tensor(out, dtype=torch.int32).reshape(B, H, keep)
 
 
+def test_select_tokens_equal_masses(dev):
+    """Rows of one value, and of two: the lowest indices, in short and long rows."""
+    hist = pkg_module("kv_history")
+    for n in (10, 9000, 33001):
+        mass = torch.zeros(1, 2, n, device=dev)
+        mass[0, 1, n // 2:] = 1e-30
+        got = hist.select_tokens(mass, n, n // 2 + 3, keep_last=1).cpu()
+        want = [*range(n // 2 + 2), n - 1]
+        assert got[0, 0].tolist() == want
+        high = list(range(n // 2, n))
+        want = sorted(high + list(range(n // 2 + 3 - len(high))))[:n // 2 + 3]
+        assert got[0, 1].tolist() == want, n
+
+
 @pytest.mark.parametrize("B,H,kv,keep,first,last,fmt,holes,layout", [
     (1, 1, 1, 1, 0, 0, "fp8", 0, "bshd"),
     (2, 3, 1000, 400, 16, 100, "fp8", 0, "bshd"),
@@ -524,6 +538,11 @@ def _evict_reference(mass, kv, keep, first, last, valid):
     (1, 2, 5000, 7, 7, 0, "fp8", 0, "bshd"),              # only the first
     (1, 2, 64, 0, 0, 0, "fp8", 0, "bshd"),
     (1, 3, 0, 5, 0, 0, "fp8", 0, "bshd"),
+    (1, 2, 32769, 20000, 5, 300, "fp8", 0.02, "bshd"),    # past one workgroup a head
+    (2, 1, 70001, 123, 0, 1, "int8", 0, "bshd"),
+    (1, 1, 40000, 39000, 0, 0, "fp8", 0.5, "bshd"),       # long, and fewer valid tokens than places
+    (1, 1, 33000, 40000, 10, 10, "fp8", 0, "bshd"),       # long, and more places than tokens
+    (1, 2, 20000, 9000, 0, 64, "fp8", 0, "bshd"),
 ])
 def test_evict(dev, B, H, kv, keep, first, last, fmt, holes, layout):
     print(f"case evict B={B} H={H} kv={kv} keep={keep} {first}/{last} {fmt} {layout}", flush=True)

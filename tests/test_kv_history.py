@@ -233,10 +233,10 @@ def test_c_abi_refusals():
     assert mass(kv=0, lse=None) == 0
 
     def tokens(kv=100, keep=10, first=0, last=0, m=_A):
-        return lib.hn_select_kv_tokens(m, s3, 1, 2, kv, None, 0, keep, first, last, _A, None)
+        return lib.hn_select_kv_tokens(m, s3, 1, 2, kv, None, 0, keep, first, last, _A, None, 0, None)
 
     for kw, match in ((dict(kv=-1), "shape"), (dict(first=6, last=5), "exceeds"), (dict(m=None), "null"),
-                      (dict(m=_A + 2), "misaligned")):
+                      (dict(m=_A + 2), "misaligned"), (dict(kv=1 << 20), "workspace")):
         assert tokens(**kw) == -1 and match in err(), kw
     assert tokens(keep=0, m=None) == 0
 
@@ -256,6 +256,6 @@ def test_no_gfx950_device_is_refused():
     lib = L.load()
     st = (ctypes.c_int64 * 4)(256, 256, 128, 1)
     s3 = (ctypes.c_int64 * 3)(2, 2, 1)
-    assert lib.hn_select_kv_tokens(_A, s3, 1, 2, 100, None, 0, 10, 0, 0, _A, None) == L.HN_E_DEVICE
+    assert lib.hn_select_kv_tokens(_A, s3, 1, 2, 100, None, 0, 10, 0, 0, _A, None, 0, None) == L.HN_E_DEVICE
     assert lib.hn_kv_block_bounds(0, _A, st, _A, s3, 1, 2, 128, 100, 0, 100, 64, None, 0, _A,
                                   (ctypes.c_int64 * 5)(512, 512, 256, 128, 1), 2, None) == L.HN_E_DEVICE
