@@ -8,6 +8,7 @@ csrc/ for gfx950). Modules mirror the reference surfaces they replace:
   fp8_kv_cache      <- hymm/models/dit/modules/int8_kv_cache.py (KV quantize/decode)
   kv_cache_storage  <- hymm/models/dit/modules/kv_cache_storage.py (format dispatch)
   cache_attention   <- nomas_cpt.causal_attention_with_cache_mp + reactor CacheStaging
+  kv_history        block bounds, block choice, key mass and eviction of a long history
   quantization      <- reactor/hy_nomas_quantization.py (install seam)
   dit_block         <- nomas_compile_prepost.pre/post_attention + the AR chunk loop
   ops               torch custom ops over the C ABI; _lib the ctypes binding

@@ -34,6 +34,7 @@ from . import ops
 from .cache_attention import causal_attention_with_cache_mp, chunk_attention
 from .dit_fp8_linear import FP8StoredLinear, fp8_linear, fp8_linear_codes
 from .fp8_kv_cache import make_fp8_kv_block
+from .kv_history import LayerHistory
 from .metrics import stage
 
 
@@ -201,12 +202,14 @@ class FP8DiTBlock(nn.Module):
 
     def forward(self, img, vec, cos, sin, kv_cache, cache_valid_len: int,
                 update_cache: bool = False, kv_status=None, *, txt=None, vec_txt=None,
-                text_mask=None, cache_mask=None, cache_txt: bool = True):
+                text_mask=None, cache_mask=None, cache_txt: bool = True, history=None):
         """One block at inference. With ``update_cache`` this chunk's rotated K
         and V go into ``kv_cache`` at ``cache_valid_len``. When writes are
         validated and no ``kv_status`` is passed, a non-finite value raises
         ValueError here (one host read of the device flag); with one, the flag
-        is left for the caller to read.
+        is left for the caller to read. ``history`` (a kv_history.LayerHistory of this
+        cache, image-only path) runs the pass's attention: chosen blocks of a long
+        history, the weight its keys draw.
 
         With ``txt`` ([B, L_txt, C], text stream blocks only) the call follows
         the double-stream block (nomas_cpt.py:1293-1459): both streams' Q/K/V,
@@ -219,6 +222,8 @@ class FP8DiTBlock(nn.Module):
         if txt is not None:
             if kv_status is not None:
                 raise ValueError("kv_status applies to the image-only path")
+            if history is not None:
+                raise ValueError("a LayerHistory applies to the image-only path")
             q, k, v, parts = self.pre_attention(img, vec, cos, sin)
             tq, tk, tv, tparts = self.pre_attention_txt(txt, vec_txt)
             img_attn, txt_attn = causal_attention_with_cache_mp(
@@ -234,7 +239,10 @@ class FP8DiTBlock(nn.Module):
         if status is not None and kv_status is None and int(status[0].item()):
             raise ValueError("Cannot quantize non-finite KV values")
         with stage("cache_attention"):
-            attn = chunk_attention(q, kv_cache, cache_valid_len, k_cur=k, v_cur=v)
+            if history is None:
+                attn = chunk_attention(q, kv_cache, cache_valid_len, k_cur=k, v_cur=v)
+            else:
+                attn = history.attend(q, k, v, kv_cache, cache_valid_len, update_cache)
         return self.post_attention(img, attn, parts)
 
 
@@ -248,11 +256,18 @@ class FP8ARModel(nn.Module):
     segment's text tokens [1, text_len, C] beside the image, attends
     [history | img | txt] under ``text_mask`` and the per-layer cache masks,
     and the write pass stores img + txt K/V, so the valid length advances by
-    the image tokens plus ``text_len``."""
+    the image tokens plus ``text_len``.
+
+    A roll-out longer than its cache or its time allows (image-only chunks):
+    ``sparse_top_k`` > 0 lets the denoising passes read that many 64-token blocks of
+    a longer history instead of all of it, and ``evict_keep`` > 0 cuts a full cache
+    to that many tokens of each head, those that the writing passes' queries weighed
+    most (its first latent frame and its newest chunk always, as far as they fit),
+    instead of refusing the chunk."""
 
     def __init__(self, depth: int = 40, hidden: int = 3072, heads: int = 24,
                  latent_shape=(3, 45, 80), max_chunks: int = 17, *, device=None, seed: int = 0,
-                 text_len: int = 0):
+                 text_len: int = 0, sparse_top_k: int = 0, evict_keep: int = 0):
         super().__init__()
         g = torch.Generator(device=device).manual_seed(seed)
         self.text_len = int(text_len)
@@ -274,6 +289,31 @@ class FP8ARModel(nn.Module):
         self.kv_status = torch.zeros(depth, dtype=torch.int32, device=device)
         self.cache_valid_len = 0
         self.frames_done = 0
+        self.evict_keep = int(evict_keep)
+        if self.text_len and (sparse_top_k or evict_keep):
+            raise ValueError("sparse_top_k and evict_keep apply to image-only chunks")
+        if not 0 <= self.evict_keep <= self.capacity - self.write_tokens:
+            raise ValueError(f"evict_keep leaves no room for a chunk's {self.write_tokens} tokens")
+        self.histories = None
+        if sparse_top_k or evict_keep:
+            self.histories = [LayerHistory(c, top_k=int(sparse_top_k), keep_first=min(1, int(sparse_top_k)),
+                                           keep_last=min(2, max(0, int(sparse_top_k) - 1)),
+                                           track_mass=self.evict_keep > 0) for c in self.caches]
+        # the cache that the next layer to be cut moves into
+        self.spare = (make_fp8_kv_block(1, self.capacity, heads, self.head_dim, device=device)
+                      if self.evict_keep else None)
+
+    @torch.no_grad()
+    def evict_history(self) -> None:
+        """Cut every layer's cache to ``evict_keep`` tokens a head: each moves into the
+        spare cache, and its old one is the next layer's spare."""
+        keep = self.evict_keep
+        first = min(math.prod(self.latent_shape[1:]), keep // 4)
+        last = min(self.write_tokens, keep // 2)
+        for i, history in enumerate(self.histories):
+            history.evict(self.caches[i], self.spare, self.cache_valid_len, keep, keep_first=first, keep_last=last)
+            self.caches[i], self.spare = self.spare, self.caches[i]
+        self.cache_valid_len = min(keep, self.cache_valid_len)
 
     @torch.no_grad()
     def forward_chunk(self, img, vec, update_cache: bool, txt=None, vec_txt=None, text_mask=None):
@@ -290,7 +330,8 @@ class FP8ARModel(nn.Module):
             return img
         for i, (block, cache) in enumerate(zip(self.blocks, self.caches)):
             img = block(img, vec, cos, sin, cache, self.cache_valid_len, update_cache,
-                        kv_status=self.kv_status[i:i + 1] if update_cache else None)
+                        kv_status=self.kv_status[i:i + 1] if update_cache else None,
+                        history=None if self.histories is None else self.histories[i])
         return img
 
     @torch.no_grad()
@@ -299,10 +340,12 @@ class FP8ARModel(nn.Module):
         """Euler flow updates over the denoising passes, then the cache write
         at t = 0 and the advance of the valid length (causal_ar.py:2348-2432,
         2624-2645,2852). A chunk that would not fit the cache is refused
-        before any pass runs. In the write pass a layer whose K/V holds a
+        before any pass runs (or, with ``evict_keep``, makes room first). In the write pass a layer whose K/V holds a
         NaN/Inf writes nothing; the valid length then stays where it was (rows
         that other layers wrote past it are never attended) and ValueError
         names the layers (with text: the first such layer raises)."""
+        if self.cache_valid_len + self.write_tokens > self.capacity and getattr(self, "evict_keep", 0):
+            self.evict_history()
         if self.cache_valid_len + self.write_tokens > self.capacity:
             raise ValueError(f"KV cache full: {self.cache_valid_len} + {self.write_tokens} tokens "
                              f"exceed the capacity {self.capacity}")
@@ -314,6 +357,8 @@ class FP8ARModel(nn.Module):
             x = x + (sigmas[i + 1] - sigmas[i]) * v_pred
         self.forward_chunk(x, vec_write, True, txt, vec_txt, text_mask)
         bad = torch.nonzero(self.kv_status).flatten().tolist()
+        for history, cache in zip(self.histories or (), self.caches):
+            history.rollback() if bad else history.commit(cache)
         if bad:
             raise ValueError(f"Cannot quantize non-finite KV values (layers {bad})")
         self.cache_valid_len += self.write_tokens

@@ -18,6 +18,10 @@ both work on the FP8/INT8 cache of fp8_kv_cache.py in place:
       the tokens of largest mass, moved to the front of another cache; keys carry
       their rotation, so a moved token keeps its position
 
+  LayerHistory
+      one layer's bounds and mass, and the attention of its passes over them: what
+      dit_block.FP8ARModel keeps per layer when it reads or cuts a long history
+
 The choices are exact (scores in 64 bits, ties to the lowest index): the same
 inputs give the same blocks and tokens.
 """
@@ -96,3 +100,72 @@ def evict(cache: dict, out: dict, mass: torch.Tensor, kv_len: int, keep: int, *,
     idx = ops.select_kv_tokens(mass, kv_len, keep, keep_first, keep_last, cache_valid)
     moved = ops.move_kv_tokens_(*(out[n] for n in STORAGE_KEYS), *(cache[n] for n in STORAGE_KEYS), mass, idx)
     return idx, moved
+
+
+class LayerHistory:
+    """Bounds and mass of one layer's cache, and its attention over them.
+
+    ``top_k`` > 0: passes that do not write the cache read ``top_k`` blocks of a
+    longer history (the first ``keep_first`` and the last ``keep_last`` of it
+    always) and the current chunk; 0: all of it. ``track_mass``: writing passes,
+    which read everything, add the weight that each cached key drew to ``mass``.
+    A writing pass counts once ``commit`` is called; ``rollback`` forgets it."""
+
+    def __init__(self, cache: dict, *, top_k: int = 0, block: int = 64, q_block: int = 128, keep_first: int = 1,
+                 keep_last: int = 2, track_mass: bool = False):
+        if top_k and keep_first + keep_last > top_k:
+            raise ValueError("keep_first + keep_last exceeds top_k")
+        self.top_k, self.block, self.q_block = top_k, block, q_block
+        self.keep_first, self.keep_last = keep_first, keep_last
+        self.track_mass = track_mass
+        self.bounds = make_block_bounds(cache, block=block) if top_k else None
+        self.mass: Optional[torch.Tensor] = None    # fp32 [B, H, tokens], None: no token yet
+        self._written = None                        # (mass, length) of a pass not committed yet
+
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, kv_len: int,
+               update_cache: bool) -> torch.Tensor:
+        """Attention of one pass over [cache tokens < kv_len | k, v]. On a writing pass
+        k and v are in the cache already, from token kv_len on."""
+        from .cache_attention import chunk_attention, sparse_chunk_attention
+        if update_cache:
+            end = kv_len + k.shape[1]
+            mass = None
+            if self.track_mass:
+                out, lse = sparse_chunk_attention(q, cache, kv_len, None, k_cur=k, v_cur=v)
+                mass = key_mass(q, lse, cache, end, prior=self.mass)
+            else:
+                out = chunk_attention(q, cache, kv_len, k_cur=k, v_cur=v)
+            self._written = (mass, kv_len, end)
+            return out
+        if self.top_k and -(-kv_len // self.block) > self.top_k:
+            idx = select_blocks(q, self.bounds, kv_len, self.top_k, block=self.block, q_block=self.q_block,
+                                keep_first=self.keep_first, keep_last=self.keep_last)
+            return sparse_chunk_attention(q, cache, kv_len, idx, block=self.block, q_block=self.q_block, k_cur=k,
+                                          v_cur=v)[0]
+        return chunk_attention(q, cache, kv_len, k_cur=k, v_cur=v)
+
+    def commit(self, cache: dict) -> None:
+        """The last writing pass stands: its mass, and the bounds of what it wrote."""
+        if self._written is None:
+            return
+        mass, start, end = self._written
+        self._written = None
+        if self.track_mass:
+            self.mass = mass
+        if self.bounds is not None:
+            update_block_bounds(self.bounds, cache, start, end, block=self.block)
+
+    def rollback(self) -> None:
+        """The last writing pass was refused: nothing of it counts."""
+        self._written = None
+
+    def evict(self, cache: dict, out: dict, kv_len: int, keep: int, *, keep_first: int = 0,
+              keep_last: int = 0) -> torch.Tensor:
+        """Keep ``keep`` tokens of every head in ``out`` (kv_history.evict by this layer's
+        mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
+        if not self.track_mass or self.mass is None:
+            raise ValueError("eviction needs the mass of the cached tokens (track_mass)")
+        idx, self.mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
+        if self.bounds is not None:
+            update_block_bounds(self.bounds, out, 0, min(keep, kv_len), block=self.block)
+        return idx

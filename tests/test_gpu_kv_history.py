@@ -677,3 +677,79 @@ def test_compiled_callers_hold_the_ops(dev):
         torch._dynamo.reset()
         compiled = torch.compile(step, backend="aot_eager", fullgraph=True)(q, hist.make_block_bounds(cache))
     assert all(torch.equal(a, b) for a, b in zip(eager, compiled))
+
+
+# --------------------------------------------------------------------------
+# the AR model's long roll-outs
+
+def _model(dev, **kw):
+    dit = pkg_module("dit_block")
+    return dit.FP8ARModel(depth=2, hidden=256, heads=2, latent_shape=(1, 8, 16), max_chunks=4, device=dev, seed=3, **kw)
+
+
+def _chunk(dev, seed):
+    g = _gen(dev, seed)
+    noise = torch.randn(1, 128, 256, device=dev, generator=g).to(BF16)
+    vecs = [torch.randn(1, 256, device=dev, generator=g).to(BF16) for _ in range(3)]
+    return noise, vecs[:2], vecs[2], [1.0, 0.5, 0.0]
+
+
+def test_model_with_enough_blocks_is_the_dense_model(dev):
+    """A history of no more blocks than top_k is read whole: the same outputs, bit for bit."""
+    dense, sparse = _model(dev), _model(dev, sparse_top_k=8)
+    for i in range(4):
+        a, b = dense.generate_chunk(*_chunk(dev, i)), sparse.generate_chunk(*_chunk(dev, i))
+        assert torch.equal(a, b), i
+
+
+def test_model_reads_blocks_and_cuts_a_full_cache(dev):
+    """Denoising passes read the chosen blocks; a full cache is cut to the heaviest
+    tokens and the roll-out goes on; a refused write leaves bounds and mass alone."""
+    hist = pkg_module("kv_history")
+    m = _model(dev, sparse_top_k=3, evict_keep=300)
+    plain = _model(dev)
+    for i in range(4):
+        out = m.generate_chunk(*_chunk(dev, i))
+        assert torch.isfinite(out.float()).all() and m.cache_valid_len == 128 * (i + 1)
+        plain.generate_chunk(*_chunk(dev, i))
+    with pytest.raises(ValueError, match="capacity"):
+        plain.generate_chunk(*_chunk(dev, 9))
+    for h, c in zip(m.histories, m.caches):
+        assert h.mass.shape == (1, 2, 512) and torch.isfinite(h.mass).all() and (h.mass > 0).all()
+        ref = hist.make_block_bounds(c)
+        hist.update_block_bounds(ref, c, 0, 512)
+        assert torch.equal(h.bounds, ref)
+    # a layer's attention over chosen blocks, against the plain form
+    g = _gen(dev, 77)
+    q, k, v = (torch.randn(1, 128, 2, D, device=dev, generator=g).to(BF16) for _ in range(3))
+    h, c = m.histories[0], m.caches[0]
+    idx = hist.select_blocks(q, h.bounds, 512, 3, keep_first=1, keep_last=2)
+    assert (idx == torch.tensor([0, 6, 7], device=dev)).all()   # three places, all spoken for
+    ref = _attend(q, c, 512, idx, 64, 128, k, v, None, None)
+    assert ((h.attend(q, k, v, c, 512, False).to(F64) - ref[0]).abs() <= ref[2]).all()
+    # the fifth chunk cuts the history first
+    before = [{n: t.clone() for n, t in c.items()} for c in m.caches]
+    mass = [h.mass.clone() for h in m.histories]
+    noise, vecs, vec, sigmas = _chunk(dev, 4)
+    out = m.generate_chunk(noise, vecs, vec, sigmas)
+    assert torch.isfinite(out.float()).all() and m.cache_valid_len == 300 + 128
+    for i, c in enumerate(m.caches):
+        kept = _evict_reference(mass[i], 512, 300, 75, 128, None).to(dev).long()
+        for name, t in c.items():
+            want = before[i][name].transpose(1, 2).gather(2, kept[..., None].expand(-1, -1, -1, t.shape[3])) \
+                if t.dtype == torch.float32 else \
+                before[i][name].view(torch.uint8).transpose(1, 2).gather(2, kept[..., None].expand(-1, -1, -1, t.shape[3]))
+            got = t[:, :300].transpose(1, 2)
+            assert torch.equal(got if t.dtype == torch.float32 else got.view(torch.uint8), want), name
+    # a write that is refused: after it (and the cut that made room for it) nothing moves
+    with torch.no_grad():
+        m.blocks[1].qkv.bias[300] = float("nan")
+    with pytest.raises(ValueError, match="non-finite"):
+        m.generate_chunk(noise, [], vec, [1.0])
+    assert m.cache_valid_len == 300
+    bounds, mass = [h.bounds.clone() for h in m.histories], [h.mass.clone() for h in m.histories]
+    with pytest.raises(ValueError, match="non-finite"):
+        m.generate_chunk(noise, [], vec, [1.0])
+    assert m.cache_valid_len == 300
+    for h, b, w in zip(m.histories, bounds, mass):
+        assert torch.equal(h.bounds, b) and torch.equal(h.mass, w) and h.mass.shape == (1, 2, 300)

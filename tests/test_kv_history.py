@@ -259,3 +259,17 @@ def test_no_gfx950_device_is_refused():
     assert lib.hn_select_kv_tokens(_A, s3, 1, 2, 100, None, 0, 10, 0, 0, _A, None, 0, None) == L.HN_E_DEVICE
     assert lib.hn_kv_block_bounds(0, _A, st, _A, s3, 1, 2, 128, 100, 0, 100, 64, None, 0, _A,
                                   (ctypes.c_int64 * 5)(512, 512, 256, 128, 1), 2, None) == L.HN_E_DEVICE
+
+
+def test_model_refusals():
+    dit, hist = pkg_module("dit_block"), pkg_module("kv_history")
+    kvc = pkg_module("fp8_kv_cache")
+    cache = kvc.make_fp8_kv_block(1, 256, 2, 128, device="cpu")
+    with pytest.raises(ValueError, match="exceeds top_k"):
+        hist.LayerHistory(cache, top_k=2, keep_first=1, keep_last=2)
+    h = hist.LayerHistory(cache, top_k=4)
+    with pytest.raises(ValueError, match="mass"):
+        h.evict(cache, cache, 128, 64)
+    block = dit.FP8DiTBlock.__new__(dit.FP8DiTBlock)
+    with pytest.raises(ValueError, match="image-only"):
+        dit.FP8DiTBlock.forward(block, None, None, None, None, cache, 0, txt=1, history=h)
