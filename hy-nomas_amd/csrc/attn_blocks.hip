@@ -41,6 +41,22 @@ HN_DEVICE int list_length(const int32_t* list, int k) {
     return k;
 }
 
+// A list's entries, 64 at a time in a register (lane i: entry 64 chunk + i), so that an
+// entry is a lane read: loaded entry by entry, each would wait for every load issued
+// before it, the prefetched codes among them.
+struct ListReader {
+    const int32_t* list;
+    int k, chunk, held;
+    HN_DEVICE ListReader(const int32_t* l, int top_k) : list(l), k(top_k), chunk(-1), held(0) {}
+    HN_DEVICE int operator()(int i) {  // entry i < k, the same for the whole wave
+        if ((i >> 6) != chunk) {
+            chunk = i >> 6;
+            held = list[min(64 * chunk + (int)(threadIdx.x & 63), k - 1)];
+        }
+        return __builtin_amdgcn_readlane(held, i & 63);
+    }
+};
+
 // Step A with the denominator summed from the fp32 probabilities, so that the
 // row's log-sum-exp carries no rounding of the fp16 ones (their sum would be off
 // by up to 2^-12 relative where one key dominates).
@@ -184,8 +200,9 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
         int count, first;
     };
     constexpr uint32_t NOWHERE = 0x80000000u;
+    ListReader reader(list, p.top_k);
     auto entry = [&](int t) __attribute__((always_inline)) {  // list entry of cache tile t
-        return list && t < n_cache && t < t_end ? __builtin_amdgcn_readfirstlane(list[t >> p.shift]) : 0;
+        return list && t < n_cache && t < t_end ? reader(t >> p.shift) : 0;
     };
     const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len, entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
     const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1 * 4u, us1 = (uint32_t)p.us1 * 2u;
@@ -512,6 +529,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
     const int entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
     const int n_cache = list ? list_length(list, p.top_k) << p.shift : (kv_len + BKV - 1) / BKV;
     const int n_all = n_cache + (cur_len + BKV - 1) / BKV;
+    ListReader reader(list, p.top_k);
     const float c = p.scale_log2;
     RowState f;
     f.m = -INFINITY;
@@ -523,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
         if (t < n_cache) {
             int first = t * BKV, left = kv_len - first;
             if (list) {
-                const int e = __builtin_amdgcn_readfirstlane(list[t >> p.shift]);
+                const int e = reader(t >> p.shift);
                 first = e < entries ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : 0;
                 left = e < entries ? kv_len - first : 0;
             }
@@ -656,7 +674,8 @@ struct WaveRegs {  // codes of a 32-key block
     uint4 k[4];    // key col, dims 64 half ..
     uint4 v[4];    // keys quad_key(lane % 8, j), dims 16 (lane / 8) ..
     float ks, vs;  // of key col
-    uint32_t word; // keys that take part
+    int left;      // keys that exist, from key 0 on (<= 0: none)
+    uint32_t ok;   // of key col: valid
 };
 
 template <int FMT>
@@ -710,6 +729,7 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     const int sh32 = p.shift + 1;  // block = 32 << sh32 tokens
     const int limit = list ? p.top_k << sh32 : (kv_len + 31) / 32;
     const int step = 4 * p.splits;
+    ListReader reader(list, p.top_k);
 
     f32x16 o[4];
 #pragma unroll
@@ -730,15 +750,15 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     uint32_t off_v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) off_v[j] = (uint32_t)quad_key(qd, j) * cs1 + 16u * dg;
-    // Codes of cache block t < limit; a block without a key leaves word 0. (The first
+    // Codes of cache block t < limit; a block without a key leaves `left` 0. (The first
     // loads do not wait for the list's length: what lies past its end is dropped
     // afterwards.)
     auto load = [&](int t, WaveRegs& r) __attribute__((always_inline)) {
-        r.word = 0;
+        r.left = 0;
         if (t >= limit) return;
         int first = t * 32, left = kv_len - first;
         if (list) {
-            const int e = __builtin_amdgcn_readfirstlane(list[t >> sh32]);
+            const int e = reader(t >> sh32);
             const bool there = (uint32_t)e < (uint32_t)entries;
             first = there ? ((e << sh32) + (t & ((1 << sh32) - 1))) * 32 : 0;
             left = there ? kv_len - first : 0;
@@ -754,12 +774,11 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             r.k[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src.k, off_k + co + 16 * e, 0, 0));
         r.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.ks, off_s + so_, 0, 0));
         r.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.vs, off_s + so_, 0, 0));
-        bool ok = col < left;
-        if (p.kvalid) ok = ok && p.kvalid[b * p.kvs + first + min(col, left - 1)] != 0;
+        r.ok = p.kvalid ? (uint32_t)p.kvalid[b * p.kvs + first + min(col, left - 1)] : 1u;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             r.v[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src.v, off_v[j] + co, 0, 0));
-        r.word = (uint32_t)__ballot(ok);
+        r.left = left;
     };
     // P and PV of a block whose V^T operands are vf (operand 4 tt + db).
     auto finish = [&](f32x16& s, uint32_t word, const f16x8 (&vf)[8]) __attribute__((always_inline)) {
@@ -787,12 +806,14 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
         for (int i = 0; i < 8; ++i) vf[i] = ld_f16x8(vt + wv_row(32 * (i & 3) + col) + 32 * (i >> 2) + 16 * half);
     };
     auto block = [&](WaveRegs& r) __attribute__((always_inline)) {
-        if (r.word == 0) return;
+        // the keys that take part (asked for here: at the load it would wait for it)
+        const uint32_t live = (uint32_t)__ballot(col < r.left && r.ok != 0u);
+        if (live == 0) return;
         float vs[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) vs[j] = __shfl(r.vs, quad_key(qd, j), 64);
-        if (r.word != ~0u) {  // what a masked key holds meets no product
-            const uint32_t m = r.word >> quad_key(qd, 0);
+        if (live != ~0u) {  // what a masked key holds meets no product
+            const uint32_t m = live >> quad_key(qd, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bool in = (m >> j) & 1u;
@@ -832,7 +853,7 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
         }
         f16x8 vf[8];
         read_v(vf);
-        finish(s, r.word, vf);
+        finish(s, live, vf);
     };
     const int dealt = split * 4 + wave;  // blocks dealt, dealt + step, ..
     {

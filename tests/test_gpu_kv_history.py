@@ -313,6 +313,9 @@ CASES = [
     (1, 70, 2, 2, 0, 64, 64, 3, 70, "fp8", 0, "bshd", 1),           # no history yet
     (1, 64, 2, 2, 3000, 1024, 64, 2, 0, "fp8", 0.05, "bshd", 1),
     (1, 40, 3, 3, 500, 64, 8, 2, 3, "fp8", 0.97, "bshd", 1),        # masks that leave runs without a key
+    (1, 3, 1, 1, 12800, 64, 1, 150, 0, "fp8", 0, "bshd", 1),        # lists of more than 64 entries: a row,
+    (1, 20, 4, 2, 12800, 64, 16, 150, 33, "int8", 0.1, "bshd", 1),  # up to 64 rows,
+    (1, 150, 1, 1, 12800, 64, 128, 150, 0, "fp8", 0.1, "bshd", 1),  # more
 ]
 
 
