@@ -440,6 +440,314 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
 }
 
 // ---------------------------------------------------------------------------
+// Runs of 33 to 64 rows: two row blocks of 32, and the two 32-key halves of a tile go to
+// different waves (wave w: rows 32 (w % 2) .., keys 32 (w / 2) ..), so that four waves
+// share each tile's dequantization. A wave has one half a tile to compute, so K runs
+// two tiles ahead of its use by the PV product and V one: while tile t's probabilities
+// are formed (beside S of t + 1) and multiplied, V of t + 1 goes to the other stage and
+// K of t + 2 to this one, whose K was last read a tile ago; one barrier a tile. The two
+// halves of a row's keys meet at the end. Scales travel four tiles ahead of V.
+template <int FMT, bool MASK>
+__global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
+    constexpr int NW = 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE + 4 * SB_FLOATS * 4];
+    float* const sbuf = reinterpret_cast<float*>(smem + 2 * STAGE);  // scales of tile t at (t % 4) SB_FLOATS
+    const int id = blockIdx.x;
+    const int w = (id & 7) * p.per_xcd + (id >> 3);
+    if (w >= p.work) return;
+    // the splits of a run, then the runs of a head
+    int x = w;
+    const int split = x % p.splits;
+    x /= p.splits;
+    const int64_t run = x % p.runs;
+    x /= (int)p.runs;
+    const int64_t h = x % p.H, b = x / p.H;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5, kb = wave >> 1;
+    const int64_t i0 = run * p.q_block;
+    const int64_t queries = p.Lq - i0 < p.q_block ? p.Lq - i0 : p.q_block;
+    const int rows = (int)(queries * p.G), row = 32 * (wave & 1) + col;
+    const bool qvalid = row < rows;
+    const int rr = qvalid ? row : rows - 1;
+    const int64_t qi = i0 + rr / p.G, hq = h * p.G + rr % p.G;
+    bf16x8 qf[8];
+    {
+        const uint16_t* src = p.q + b * p.qs0 + qi * p.qs1 + hq * p.qs2 + half * 8;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl)
+            qf[sl] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 16 * sl));
+    }
+    const int32_t* list = p.idx ? p.idx + b * p.is0 + h * p.is1 + run * p.is2 : nullptr;
+    const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len, entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
+    const int n_cache = list ? list_length(list, p.top_k) << p.shift : (kv_len + BKV - 1) / BKV;
+    const int n_all = n_cache + (cur_len + BKV - 1) / BKV;
+    const int t_begin = (int)((int64_t)n_all * split / p.splits), t_end = (int)((int64_t)n_all * (split + 1) / p.splits);
+    f32x16 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[i][v] = 0.0f;
+    Run run_{-INFINITY, 0.0f, 0.0f};
+    const float c = p.scale_log2;
+
+    // Tiles as in attn_blocks_kernel: descriptors over the cache's and the tail's rows,
+    // replaced by a tile's own where a span passes 2^31 bytes.
+    const bool span_ok = p.kv_len > 0 && (p.kv_len - 1) * p.cs1 + D < ((int64_t)1 << 31) &&
+                         ((p.kv_len - 1) * p.ss1 + 1) * 4 < ((int64_t)1 << 31);
+    const bool tail_ok = (p.cur_len * p.us1 + D) * 2 < ((int64_t)1 << 31);
+    auto tail_rsrc = [&](const uint16_t* base, int64_t first, int64_t n) __attribute__((always_inline)) {
+        return tile_rsrc(base + b * p.us0 + h * p.us2 + first * p.us1, n > 0 ? ((n - 1) * p.us1 + D) * 2 : 0);
+    };
+    const TileBase span = tile_base(p, b, h, 0, span_ok ? kv_len : 0);
+    const __amdgpu_buffer_rsrc_t tks = tail_rsrc(p.kcur, 0, tail_ok ? cur_len : 0),
+                                 tvs = tail_rsrc(p.vcur, 0, tail_ok ? cur_len : 0);
+    const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1 * 4u, us1 = (uint32_t)p.us1 * 2u;
+    constexpr uint32_t NOWHERE = 0x80000000u;
+    ListReader reader(list, p.top_k);
+    struct Tile {
+        int first, count;
+    };
+    auto tile_of = [&](int t) __attribute__((always_inline)) {
+        Tile g{0, 0};
+        if (t >= t_end) return g;
+        int left;
+        if (t < n_cache) {
+            const int e = list ? reader(t >> p.shift) : 0;
+            const bool there = e < entries;
+            g.first = !there ? 0 : list ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : t * BKV;
+            left = there ? kv_len - g.first : 0;
+        } else {
+            g.first = (t - n_cache) * BKV;
+            left = cur_len - g.first;
+        }
+        g.count = left >= BKV ? BKV : left > 0 ? left : 0;
+        return g;
+    };
+    auto word_of = [&](int count, const uint8_t* st) __attribute__((always_inline)) {
+        const uint64_t all = count >= BKV ? ALL_KEYS : (1ull << count) - 1;
+        return tile_mask<MASK>(st) & all;
+    };
+    const uint32_t ka_off = (32 * kb + col) * KROW + 16 * half;
+    const uint32_t va_off = K_BYTES + col * VTROW + 16 * half;
+    CacheRegs<NW> regs;
+    regs.s = 0.0f;
+    regs.mk = 0u;
+    TailRegs<NW> tr;
+    tr.mk = 0u;
+    const LaneOffs<NW> lo = lane_offsets<NW>(p);
+    const TailOffs<NW> to = tail_offsets<NW>(p);
+    // K codes and validity of a tile (of the cache or the tail, CT) to registers; V codes;
+    // the scales
+    auto fetch_k = [&](auto ct, const Tile& g) __attribute__((always_inline)) {
+        if constexpr (decltype(ct)::value) {
+            TileBase src = span;
+            uint32_t co = g.count > 0 ? (uint32_t)g.first * cs1 : NOWHERE;
+            if (!span_ok) {
+                src = tile_base(p, b, h, g.first, g.count);
+                co = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                regs.k[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src.k, lo.k[i] + co, 0, 0));
+            if constexpr (MASK)
+                if (wave == 2)
+                    regs.mk = lane < g.count ? (p.kvalid ? (uint32_t)p.kvalid[b * p.kvs + g.first + lane] : 1u) : 0u;
+        } else {
+            const bool own = !tail_ok;
+            load_tail_span_k<NW, MASK>(p, b, to, own ? tail_rsrc(p.kcur, g.first, g.count) : tks,
+                                       own ? 0u : g.count > 0 ? (uint32_t)g.first * us1 : NOWHERE, g.first,
+                                       g.first + g.count, tr);
+        }
+    };
+    auto fetch_v = [&](auto ct, const Tile& g) __attribute__((always_inline)) {
+        if constexpr (decltype(ct)::value) {
+            TileBase src = span;
+            uint32_t co = g.count > 0 ? (uint32_t)g.first * cs1 : NOWHERE;
+            if (!span_ok) {
+                src = tile_base(p, b, h, g.first, g.count);
+                co = 0;
+            }
+            load_v<NW>(lo, regs, src, co);
+        } else {
+            const bool own = !tail_ok;
+            load_tail_span_v<NW>(to, own ? tail_rsrc(p.vcur, g.first, g.count) : tvs,
+                                 own ? 0u : g.count > 0 ? (uint32_t)g.first * us1 : NOWHERE, tr);
+        }
+    };
+    auto fetch_s = [&](const Tile& g, bool cache) __attribute__((always_inline)) {
+        if (wave >= 2 || !cache) return;
+        TileBase src = span;
+        uint32_t so_ = g.count > 0 ? (uint32_t)g.first * ss1 : NOWHERE;
+        if (!span_ok) {
+            src = tile_base(p, b, h, g.first, g.count);
+            so_ = 0;
+        }
+        const __amdgpu_buffer_rsrc_t sr = wave == 0 ? src.ks : src.vs;
+        regs.s = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sr, lo.s + so_, 0, 0));
+    };
+    auto put_s = [&](int t) __attribute__((always_inline)) {
+        if (threadIdx.x < 2 * BKV) sbuf[(t & 3) * SB_FLOATS + threadIdx.x] = regs.s;
+    };
+    auto scales = [&](int t) __attribute__((always_inline)) { return sbuf + (t & 3) * SB_FLOATS; };
+    const auto cache_c = std::integral_constant<bool, true>{};
+    const auto tail_c = std::integral_constant<bool, false>{};
+    auto stage = [&](int t) __attribute__((always_inline)) { return smem + ((t - t_begin) & 1) * STAGE; };
+
+    if (t_end > t_begin) {
+        // ---- prologue: K of t_begin and t_begin + 1 and V of t_begin in LDS, V of t_begin + 1
+        // and K of t_begin + 2 in registers, scales up to t_begin + 3
+        auto store_k_now = [&](auto ct, int t) __attribute__((always_inline)) {
+            uint8_t* st = stage(t);
+            if constexpr (decltype(ct)::value) {
+                store_mask<NW, MASK>(regs, st);
+                float ks[2];
+                k_scales<NW>(scales(t), ks);
+                uint32_t kd[4];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) store_k_part<FMT, NW>(regs, st, i, ks, kd);
+            } else {
+                store_tail_k<NW, MASK>(tr, st);
+            }
+        };
+        Tile g0 = tile_of(t_begin), g1 = tile_of(t_begin + 1), g2 = tile_of(t_begin + 2), g3 = tile_of(t_begin + 3);
+        fetch_s(g0, t_begin < n_cache);
+        put_s(t_begin);
+        fetch_s(g1, t_begin + 1 < n_cache);
+        put_s(t_begin + 1);
+        fetch_s(g2, t_begin + 2 < n_cache);
+        put_s(t_begin + 2);
+        if (t_begin < n_cache) fetch_k(cache_c, g0);
+        else fetch_k(tail_c, g0);
+        __syncthreads();
+        if (t_begin < n_cache) store_k_now(cache_c, t_begin);
+        else store_k_now(tail_c, t_begin);
+        if (t_begin + 1 < n_cache) {
+            fetch_k(cache_c, g1);
+            store_k_now(cache_c, t_begin + 1);
+        } else {
+            fetch_k(tail_c, g1);
+            store_k_now(tail_c, t_begin + 1);
+        }
+        __syncthreads();
+        const uint64_t mw0 = word_of(g0.count, stage(t_begin));
+        if (t_begin < n_cache) {
+            fetch_v(cache_c, g0);
+            float4 vs = v_scales(scales(t_begin));
+            if constexpr (MASK)
+                if (mw0 != ALL_KEYS) clear_masked_v(regs, vs, mw0);
+            float vp[8];
+            uint32_t vd[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) store_v_part<FMT, NW>(regs.v, stage(t_begin) + K_BYTES, i, vs, vp, vd);
+        } else {
+            fetch_v(tail_c, g0);
+            if constexpr (MASK)
+                if (mw0 != ALL_KEYS) clear_masked_v(tr, mw0);
+            store_tail_v<NW>(tr, stage(t_begin));
+        }
+        fetch_s(g3, t_begin + 3 < n_cache);
+        if (t_begin + 1 < n_cache) fetch_v(cache_c, g1);
+        else fetch_v(tail_c, g1);
+        if (t_begin + 2 < n_cache) fetch_k(cache_c, g2);
+        else fetch_k(tail_c, g2);
+        f32x16 s = s_block(stage(t_begin) + ka_off, qf);
+        float mx = raw_max(s);
+        if ((uint32_t)(mw0 >> (32 * kb)) != ~0u) mx = mask_word(s, (uint32_t)(mw0 >> (32 * kb)));
+        __syncthreads();
+        // ---- tile t; KT, VT: K of t + 2, V of t + 1 are the cache's
+        auto iterate = [&](auto kt, auto vt_, int t) __attribute__((always_inline)) {
+            constexpr bool KT = decltype(kt)::value, VT = decltype(vt_)::value;
+            uint8_t* st = stage(t);
+            uint8_t* nst = stage(t + 1);
+            const Tile g4 = tile_of(t + 4);
+            f16x8 pf[2];
+            rebase(mx, c, run_, o);
+            f32x16 sn = step_a_lse(s, c, run_.nm, run_.l, pf, nst + ka_off, qf);
+            const uint64_t mwn = word_of(g1.count, nst);
+            float4 vs = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float ks[2] = {0.0f, 0.0f};
+            if constexpr (VT) vs = v_scales(scales(t + 1));
+            if constexpr (KT) k_scales<NW>(scales(t + 2), ks);
+            if constexpr (MASK)
+                if (mwn != ALL_KEYS) {
+                    if constexpr (VT) clear_masked_v(regs, vs, mwn);
+                    else clear_masked_v(tr, mwn);
+                }
+            uint32_t kd[4], vd[16];
+            float vp[8];
+            mx = step_b_with(pf, st + va_off, kb, o, sn, [&](int i) __attribute__((always_inline)) {
+                if constexpr (VT) store_v_part<FMT, NW>(regs.v, nst + K_BYTES, i, vs, vp, vd);
+                else store_tail_v_part<NW>(tr, nst, i);
+                if constexpr (KT) store_k_part<FMT, NW>(regs, st, i, ks, kd);
+                else if (i & 1) store_tail_k_part<NW>(tr, st, i >> 2, (i >> 1) & 1);
+            });
+            if constexpr (KT) store_mask<NW, MASK>(regs, st);
+            else store_tail_mask<NW, MASK>(tr, st);
+            if ((uint32_t)(mwn >> (32 * kb)) != ~0u) mx = mask_word(sn, (uint32_t)(mwn >> (32 * kb)));
+            s = sn;
+            put_s(t + 3);
+            fetch_s(g4, t + 4 < n_cache);
+            if (t + 2 < n_cache) fetch_v(cache_c, g2);
+            else fetch_v(tail_c, g2);
+            if (t + 3 < n_cache) fetch_k(cache_c, g3);
+            else fetch_k(tail_c, g3);
+            __syncthreads();
+            g1 = g2;
+            g2 = g3;
+            g3 = g4;
+        };
+        int t = t_begin;
+        for (; t < t_end && t + 2 < n_cache; ++t) iterate(cache_c, cache_c, t);
+        for (; t < t_end && t + 1 < n_cache; ++t) iterate(tail_c, cache_c, t);
+        for (; t < t_end; ++t) iterate(tail_c, tail_c, t);
+    }
+    // ---- the two key halves of a row meet: waves 2 and 3 pass theirs through LDS
+    float l = run_.l + __shfl_xor(run_.l, 32, 64), m = run_.m;
+    constexpr int PITCH = D + 4;
+    float* so = reinterpret_cast<float*>(smem);  // [64][PITCH], then [64][2]
+    float* sml = so + 64 * PITCH;
+    __syncthreads();
+    if (kb == 1) {
+        float* dst = so + row * PITCH;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int vq = 0; vq < 4; ++vq)
+                *reinterpret_cast<float4*>(dst + db * 32 + vq * 8 + half * 4) =
+                    make_float4(o[db][vq * 4], o[db][vq * 4 + 1], o[db][vq * 4 + 2], o[db][vq * 4 + 3]);
+        if (half == 0) {
+            sml[2 * row] = m;
+            sml[2 * row + 1] = l;
+        }
+    }
+    __syncthreads();
+    if (kb == 1 || !qvalid) return;
+    const float m1 = sml[2 * row], top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
+    const float a0 = __builtin_amdgcn_exp2f(m - base), a1 = __builtin_amdgcn_exp2f(m1 - base);
+    l = l * a0 + sml[2 * row + 1] * a1;
+    m = top;
+    const int64_t hqs = p.H * p.G, at = (b * hqs + hq) * p.Lq + qi;
+    const int64_t slot = (int64_t)split * p.B * hqs * p.Lq + at;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    uint16_t* dst = p.out + b * p.os0 + qi * p.os1 + hq * p.os2;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) {
+            const int d = db * 32 + vq * 8 + half * 4;
+            const float4 y = *reinterpret_cast<const float4*>(so + row * PITCH + d);
+            const float4 v = make_float4(o[db][vq * 4] * a0 + y.x * a1, o[db][vq * 4 + 1] * a0 + y.y * a1,
+                                         o[db][vq * 4 + 2] * a0 + y.z * a1, o[db][vq * 4 + 3] * a0 + y.w * a1);
+            if (p.splits > 1) *reinterpret_cast<float4*>(p.ws_o + slot * D + d) = v;
+            else *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        }
+    if (half != 0) return;
+    if (p.splits > 1) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
+    else p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------
 // One row a run (single tokens of ungrouped heads). The read of the keys is the whole
 // cost and a matrix tile would hold one row of 32, so the products run on the vector
 // unit, without LDS or barriers in the loop: 8 lanes hold a key (16 dims each, one
@@ -654,7 +962,7 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to 64 rows a run: a matrix column block holds 32 of them, so the waves of a
+// Up to 32 rows a run: one matrix column block holds them all, so the waves of a
 // workgroup share the keys instead of the rows. Every wave takes 32-key blocks of its
 // own, without barriers: K codes go from global memory to MFMA operands in registers
 // (lane half: 64 contiguous dims, which the Q operand matches), V^ passes through the
@@ -685,14 +993,11 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     const int id = blockIdx.x;
     const int w = (id & 7) * p.per_xcd + (id >> 3);
     if (w >= p.work) return;
-    // Lists: the row tiles of a run (which read the same blocks), its splits, then the
-    // runs of a head. Whole cache: heads fastest, which share the lines of a key
-    // range's scales.
+    // Lists: the splits of a run, then the runs of a head. Whole cache: heads fastest,
+    // which share the lines of a key range's scales.
     int64_t h, run, b;
-    int split, row0, x = w;
+    int split, x = w;
     if (p.idx) {
-        row0 = 32 * (x % p.q_tiles);
-        x /= p.q_tiles;
         split = x % p.splits;
         x /= p.splits;
         run = x % p.runs;
@@ -704,8 +1009,6 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
         x /= (int)p.H;
         split = x % p.splits;
         x /= p.splits;
-        row0 = 32 * (x % p.q_tiles);
-        x /= p.q_tiles;
         run = x % p.runs;
         b = x / p.runs;
     }
@@ -713,12 +1016,11 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     const int col = lane & 31, half = lane >> 5, qd = lane & 7, dg = lane >> 3;
     const int64_t i0 = run * p.q_block;
     const int64_t queries = p.Lq - i0 < p.q_block ? p.Lq - i0 : p.q_block;
-    const int rows = min((int)(queries * p.G) - row0, 32);  // rows row0 .. of the run
-    if (rows <= 0) return;  // (the whole workgroup: a last run of fewer rows)
+    const int rows = (int)(queries * p.G);  // 1 .. 32
     uint8_t* const vt = smem + wave * WV_BYTES;
     bf16x8 qf[8];
     {
-        const int r = row0 + (col < rows ? col : rows - 1);
+        const int r = col < rows ? col : rows - 1;
         const uint16_t* src = p.q + b * p.qs0 + (i0 + r / p.G) * p.qs1 + (h * p.G + r % p.G) * p.qs2 + 64 * half;
 #pragma unroll
         for (int sl = 0; sl < 8; ++sl) qf[sl] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 8 * sl));
@@ -968,7 +1270,7 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             num.z = __builtin_fmaf(y.z, a, num.z);
             num.w = __builtin_fmaf(y.w, a, num.w);
         }
-        const int64_t i = i0 + (row0 + r) / p.G, hq = h * p.G + (row0 + r) % p.G, slot = (b * hqs + hq) * p.Lq + i;
+        const int64_t i = i0 + r / p.G, hq = h * p.G + r % p.G, slot = (b * hqs + hq) * p.Lq + i;
         if (p.splits > 1) {
             const int64_t part = (int64_t)split * p.B * hqs * p.Lq + slot;
             *reinterpret_cast<float4*>(p.ws_o + part * D + d) = num;
@@ -1235,58 +1537,59 @@ __global__ __launch_bounds__(256) void key_mass_sum_kernel(MassParams p, int spl
 
 using namespace hn;
 
-// Key splits: a launch wants two workgroups per CU (two fit by LDS and
-// registers); where the runs fall short, each workgroup's tiles are split.
-// Each split keeps at least 4 tiles: a split of fewer costs more in its prologue
-// and in the merge than the wider grid gives.
-static int blocks_splits(int64_t work, int64_t tiles) {
-    const int64_t target = 2LL * device_cus();
-    if (work <= 0 || work >= target) return 1;
-    int64_t sp = target / work;
-    if (sp > tiles / 4) sp = tiles / 4;
-    return sp > 1 ? (int)sp : 1;
-}
-
-// few: the rows of a run where at most 64 (attn_row_kernel for one, attn_waves_kernel
-// for more, 32 rows a workgroup), else 0 (attn_blocks_kernel).
-// What a workgroup of the few-row kernels costs beside its tiles, in units of a wave's
-// 64-key tile: the list, the first loads, the meeting of the waves.
-constexpr double FEW_FIXED = 2.0;
+// Which kernel a run's rows take: one row attn_row_kernel, up to 32 attn_waves_kernel,
+// up to 64 attn_half_kernel, more attn_blocks_kernel.
+enum class BlocksKernel { ROW, WAVES, HALF, TILES };
 
 struct BlocksPlan {
+    BlocksKernel kernel;
     int64_t runs, q_tiles, work;
-    int splits, few;
+    int splits;
 };
 
+// Key splits. Two workgroups fit a CU; with sp splits the launch takes
+// ceil(work sp / 2 CUs) rounds of workgroups, each worth its tiles (64 keys; a
+// workgroup of the first two kernels works on four at a time) and a fixed part (the
+// list, the first loads, the end), and the merge reads and writes every row sp times.
+// In units of a tile of a full round (2.7 us measured in attn_blocks_kernel): the split
+// with the least of it is taken, each keeping at least 4 tiles.
 static BlocksPlan blocks_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t kv_len, int64_t cur_len,
                               int64_t top_k, int64_t block, int64_t q_block) {
+    constexpr double FIXED = 2.0, MERGE = 1e-4;  // per workgroup; per row and split (1 KB at 4 TB/s)
     BlocksPlan pl;
     pl.runs = (Lq - 1) / q_block + 1;
     const int64_t rows = (q_block < Lq ? q_block : Lq) * (Hq / H);
     const int64_t listed = top_k >= 0 ? top_k * (block / attn::BKV) : (kv_len + attn::BKV - 1) / attn::BKV;
     const int64_t tiles = listed + (cur_len + attn::BKV - 1) / attn::BKV;
-    pl.few = rows <= 64 ? (int)rows : 0;
-    pl.q_tiles = pl.few ? (rows + 31) / 32 : (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
+    pl.kernel = rows == 1    ? BlocksKernel::ROW
+                : rows <= 32 ? BlocksKernel::WAVES
+                : rows <= 64 ? BlocksKernel::HALF
+                             : BlocksKernel::TILES;
+    pl.q_tiles = pl.kernel == BlocksKernel::TILES ? (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ : 1;
     pl.work = B * H * pl.runs * pl.q_tiles;
-    if (pl.few) {
-        // 4 waves a workgroup, a tile each at a time, 2 workgroups per CU: splits that
-        // leave no round of workgroups nearly empty (rounds / splits is the time in
-        // units of an unsplit round), each with a tile for every wave
-        const int64_t slots = 2LL * device_cus(), most = (tiles + 3) / 4;
-        double best = 1e30;
-        pl.splits = 1;
-        for (int64_t sp = 1; sp <= most && sp <= 64 && pl.work * sp <= 8 * slots; ++sp) {
-            const double rounds = (double)((pl.work * sp + slots - 1) / slots);
-            const double cost = rounds * (FEW_FIXED + (double)tiles / (double)(4 * sp));
-            if (cost < best) {
-                best = cost;
-                pl.splits = (int)sp;
-            }
+    pl.splits = 1;
+    const int64_t slots = 2LL * device_cus(), at_once = rows <= 32 ? 4 : 1;
+    double best = 1e30;
+    for (int64_t sp = 1; sp <= 64 && (sp == 1 || 4 * sp <= tiles + 3) && (sp == 1 || pl.work * sp <= 8 * slots); ++sp) {
+        const double rounds = (double)((pl.work * sp + slots - 1) / slots);
+        const double cost = rounds * (FIXED + (double)tiles / (double)(at_once * sp)) +
+                            (sp > 1 ? MERGE * (double)sp * (double)(B * Hq * Lq) : 0.0);
+        if (cost < best) {
+            best = cost;
+            pl.splits = (int)sp;
         }
-    } else {
-        pl.splits = blocks_splits(pl.work, tiles);
     }
     return pl;
+}
+
+template <int FMT>
+static void launch_blocks(BlocksKernel kernel, bool mask, const attn::BlockParams& p, dim3 grid, hipStream_t st) {
+    if (kernel == BlocksKernel::ROW) attn::attn_row_kernel<FMT><<<grid, 256, 0, st>>>(p);
+    else if (kernel == BlocksKernel::WAVES) attn::attn_waves_kernel<FMT><<<grid, 256, 0, st>>>(p);
+    else if (kernel == BlocksKernel::HALF && mask) attn::attn_half_kernel<FMT, true><<<grid, 256, 0, st>>>(p);
+    else if (kernel == BlocksKernel::HALF) attn::attn_half_kernel<FMT, false><<<grid, 256, 0, st>>>(p);
+    else if (mask) attn::attn_blocks_kernel<FMT, true><<<grid, 256, 0, st>>>(p);
+    else attn::attn_blocks_kernel<FMT, false><<<grid, 256, 0, st>>>(p);
 }
 
 static bool blocks_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t kv_len, int64_t cur_len,
@@ -1393,21 +1696,8 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
     const bool mask = p.kvalid || p.uvalid;
-    if (pl.few) {
-        if (fmt == HN_KV_FP8) {
-            if (pl.few == 1) attn::attn_row_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
-            else attn::attn_waves_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
-        } else {
-            if (pl.few == 1) attn::attn_row_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
-            else attn::attn_waves_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
-        }
-    } else if (fmt == HN_KV_FP8) {
-        if (mask) attn::attn_blocks_kernel<HN_KV_FP8, true><<<grid, 256, 0, st>>>(p);
-        else attn::attn_blocks_kernel<HN_KV_FP8, false><<<grid, 256, 0, st>>>(p);
-    } else {
-        if (mask) attn::attn_blocks_kernel<HN_KV_INT8, true><<<grid, 256, 0, st>>>(p);
-        else attn::attn_blocks_kernel<HN_KV_INT8, false><<<grid, 256, 0, st>>>(p);
-    }
+    if (fmt == HN_KV_FP8) launch_blocks<HN_KV_FP8>(pl.kernel, mask, p, grid, st);
+    else launch_blocks<HN_KV_INT8>(pl.kernel, mask, p, grid, st);
     const int rc = check_launch("hn_attn_kv_blocks");
     if (rc != HN_OK || pl.splits == 1) return rc;
     attn::blocks_combine_kernel<<<(unsigned)((B * Hq * Lq + 7) / 8), 256, 0, st>>>(p);

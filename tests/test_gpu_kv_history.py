@@ -316,6 +316,11 @@ CASES = [
     (1, 3, 1, 1, 12800, 64, 1, 150, 0, "fp8", 0, "bshd", 1),        # lists of more than 64 entries: a row,
     (1, 20, 4, 2, 12800, 64, 16, 150, 33, "int8", 0.1, "bshd", 1),  # up to 64 rows,
     (1, 150, 1, 1, 12800, 64, 128, 150, 0, "fp8", 0.1, "bshd", 1),  # more
+    (1, 100, 2, 2, 9000, 64, 50, 40, 70, "int8", 0.1, "bshd", 1),   # 50 rows a run: key halves by wave, split
+    (1, 64, 1, 1, 200, 64, 64, 1, 65, "fp8", 0, "bshd", 1),         # one block, two tail tiles
+    (1, 33, 2, 2, 130, 128, 64, 2, 64, "int8", 0, "wide", 1),
+    (2, 11, 8, 2, 5000, 256, 11, 2, 1, "fp8", 0, "bhsd", 2),        # 44 rows of grouped heads
+    (1, 64, 1, 1, 64, 64, 64, 1, 0, "fp8", 0, "bshd", 1),           # one tile in all
 ]
 
 
