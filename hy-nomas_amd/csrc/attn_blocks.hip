@@ -152,8 +152,8 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     const int64_t rows = queries * p.G;  // of this run
     const int64_t row = (int64_t)qt * BQ + wave * QW + col;
     const bool qvalid = row < rows;
-    const int64_t rr = qvalid ? row : rows - 1;
-    const int64_t qi = i0 + rr / p.G, hq = h * p.G + rr % p.G;
+    const uint32_t rr = (uint32_t)(qvalid ? row : rows - 1), G = (uint32_t)p.G;
+    const int64_t qi = i0 + rr / G, hq = h * p.G + rr % G;
 
     bf16x8 qf[8];
     {
@@ -1288,8 +1288,8 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
 // O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s. 32 threads a row, 4 dims each, eight
 // splits' loads in flight; the order of the sums is that of the splits.
 __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
-    const int64_t hqs = p.H * p.G, rows = p.B * hqs * p.Lq;
-    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // (b * Hq + hq) * Lq + i
+    const int64_t hqs = p.H * p.G, rows = p.B * hqs * p.Lq;  // < 2^31
+    const uint32_t r = blockIdx.x * 8 + (threadIdx.x >> 5);   // (b * Hq + hq) * Lq + i
     if (r >= rows) return;
     const int d = (threadIdx.x & 31) * 4;
     float M = -INFINITY, den = 0.0f;
@@ -1321,7 +1321,7 @@ __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
             num.w = fmaf(wgt, ov[e].w, num.w);
         }
     }
-    const int64_t i = r % p.Lq, hq = (r / p.Lq) % hqs, b = r / (p.Lq * hqs);
+    const uint32_t bh = r / (uint32_t)p.Lq, i = r - bh * (uint32_t)p.Lq, b = bh / (uint32_t)hqs, hq = bh - b * (uint32_t)hqs;
     const float inv = den > 0.0f ? 1.0f / den : 0.0f;
     *reinterpret_cast<uint2*>(p.out + b * p.os0 + i * p.os1 + hq * p.os2 + d) =
         make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
@@ -1394,6 +1394,45 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
     const int64_t key0 = ((int64_t)tile * 4 + wave) * (32 * KB);
     const float c = p.scale_log2;
 
+    // This thread's 32 bytes of a query tile: row tid / 8, dims 16 (tid % 8) ..
+    const int tr = tid >> 3, tu = tid & 7;
+    const int64_t row0 = split * p.rows_per_split;
+    const int64_t row1 = row0 + p.rows_per_split < p.rows ? row0 + p.rows_per_split : p.rows;
+    uint4 x0, x1;
+    float lse = INFINITY;
+    // Row r of the next fetch: query head g of the group, query i, batch bb; each fetch
+    // moves 32 rows on (steps dg, di, db with their carries; no division, and the ones
+    // here in 32 bits).
+    const uint32_t G = (uint32_t)p.G, Lq = p.Lq > 0 ? (uint32_t)p.Lq : 1u;
+    int64_t r = row0 + tr;
+    const uint32_t q0 = (uint32_t)r / G;
+    uint32_t g = (uint32_t)r - q0 * G, i = q0 % Lq;
+    int64_t bb = b * p.batches + q0 / Lq;
+    const uint32_t dg = MASS_ROWS % G, di = (MASS_ROWS / G) % Lq, db = MASS_ROWS / G / Lq;
+    auto fetch = [&]() {
+        x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
+        lse = INFINITY;
+        if (r < row1) {  // (the query does not wait for its log-sum-exp)
+            const uint16_t* src = p.q + bb * p.qs0 + i * p.qs1 + (h * p.G + g) * p.qs2 + 16 * tu;
+            x0 = reinterpret_cast<const uint4*>(src)[0];
+            x1 = reinterpret_cast<const uint4*>(src)[1];
+            lse = p.lse[(bb * p.H * p.G + h * p.G + g) * p.Lq + i];
+        }
+        r += MASS_ROWS;
+        g += dg;
+        i += di;
+        bb += db;
+        if (g >= G) {
+            g -= G;
+            ++i;
+        }
+        if (i >= Lq) {
+            i -= Lq;
+            ++bb;
+        }
+    };
+    fetch();
+
     // K fragments: key 32 kb + col, dims 64 half + 8 sl ..: 64 contiguous bytes a lane
     bf16x8 kf[KB][8];
 #pragma unroll
@@ -1421,54 +1460,18 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
         }
     }
 
-    // This thread's 32 bytes of a query tile: row tid / 8, dims 16 (tid % 8) ..
-    const int tr = tid >> 3, tu = tid & 7;
-    const int64_t row0 = split * p.rows_per_split;
-    const int64_t row1 = row0 + p.rows_per_split < p.rows ? row0 + p.rows_per_split : p.rows;
-    uint4 x0, x1;
-    float ln = 0.0f;
-    // Row r0 + tr of the next fetch: query head g of the group, query i, batch bb; each
-    // fetch moves 32 rows on (steps dg, di, db with their carries; no division).
-    int64_t r = row0 + tr;
-    int g = (int)(r % p.G);
-    int64_t i = p.Lq > 0 ? (r / p.G) % p.Lq : 0, bb = b * p.batches + (p.Lq > 0 ? r / (p.G * p.Lq) : 0);
-    const int dg = MASS_ROWS % p.G;
-    const int64_t di = p.Lq > 0 ? (MASS_ROWS / p.G) % p.Lq : 0, db = p.Lq > 0 ? MASS_ROWS / p.G / p.Lq : 0;
-    auto fetch = [&]() {
-        x0 = x1 = make_uint4(0u, 0u, 0u, 0u);
-        ln = -INFINITY;  // a row that adds nothing: exp2(0 - inf) = 0
-        if (r < row1) {
-            const float lse = p.lse[(bb * p.H * p.G + h * p.G + g) * p.Lq + i];
-            if (__builtin_fabsf(lse) != INFINITY) {
-                ln = -lse * 1.4426950408889634f;
-                const uint16_t* src = p.q + bb * p.qs0 + i * p.qs1 + (h * p.G + g) * p.qs2 + 16 * tu;
-                x0 = reinterpret_cast<const uint4*>(src)[0];
-                x1 = reinterpret_cast<const uint4*>(src)[1];
-            }
-        }
-        r += MASS_ROWS;
-        g += dg;
-        i += di;
-        bb += db;
-        if (g >= p.G) {
-            g -= p.G;
-            ++i;
-        }
-        if (i >= p.Lq) {
-            i -= p.Lq;
-            ++bb;
-        }
-    };
     auto put = [&](int buf) {
         uint4* dst = reinterpret_cast<uint4*>(smem + buf * MASS_TILE + tr * KROW + 32 * tu);
-        dst[0] = x0;
-        dst[1] = x1;
-        if (tu == 0) nl[buf][tr] = ln;
+        // a row of infinite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
+        const bool counts = __builtin_fabsf(lse) != INFINITY;
+        const uint32_t keep = counts ? ~0u : 0u;
+        dst[0] = make_uint4(x0.x & keep, x0.y & keep, x0.z & keep, x0.w & keep);
+        dst[1] = make_uint4(x1.x & keep, x1.y & keep, x1.z & keep, x1.w & keep);
+        if (tu == 0) nl[buf][tr] = counts ? -lse * 1.4426950408889634f : -INFINITY;
     };
     float acc[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.0f;
-    fetch();
     put(0);
     __syncthreads();
     int buf = 0;
@@ -1656,7 +1659,7 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_attn_kv_blocks: workspace smaller than hn_attn_kv_blocks_workspace_size() or misaligned");
     const int64_t work = pl.work * pl.splits;
-    HN_REQUIRE(work <= 0x3fffffffLL && pl.runs <= 0x3fffffffLL && B * Hq * Lq <= 0x3ffffffffLL, HN_E_ARG,
+    HN_REQUIRE(work <= 0x3fffffffLL && pl.runs <= 0x3fffffffLL && B * Hq * Lq <= 0x7fffffffLL, HN_E_ARG,
                "hn_attn_kv_blocks: too much work for one launch");
     if (const int rc = require_gfx950("hn_attn_kv_blocks"); rc != HN_OK) return rc;
     attn::BlockParams p = {};
@@ -1704,8 +1707,9 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     return check_launch("hn_attn_kv_blocks (combine)");
 }
 
-// Plan of the key mass: 512 keys per workgroup (KB 4), or 128 (KB 1) where those
-// would not fill the device twice over; where even these fall short (a short cache,
+// Plan of the key mass: 512 keys per workgroup (KB 4: each row tile read from LDS once
+// for four key blocks), or 128 (KB 1: more waves to hide the keys' loads) where the
+// rows fit one tile, or 512 would not fill the device twice over; where even these fall short (a short cache,
 // many queries) the rows are split, each split writes its sums and a second kernel
 // adds them in order.
 struct MassPlan {
@@ -1716,7 +1720,7 @@ struct MassPlan {
 static MassPlan mass_plan(int64_t rows, int64_t B, int64_t H, int64_t kv_len) {
     const int64_t target = 2LL * device_cus();
     MassPlan pl{4, 1, (kv_len + 511) / 512};
-    if (B * H * pl.tiles >= target) return pl;
+    if (B * H * pl.tiles >= target && rows > attn::MASS_ROWS) return pl;
     pl.kb = 1;
     pl.tiles = (kv_len + 127) / 128;
     const int64_t work = B * H * pl.tiles;
@@ -1779,6 +1783,7 @@ extern "C" int hn_attn_key_mass(int fmt, const void* q, const int64_t* qs, int64
     p.H = (int)H; p.G = (int)(Hq / H);
     p.rows = (int64_t)p.batches * Lq * p.G;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
+    HN_REQUIRE(p.rows <= 0x3fffffffLL, HN_E_ARG, "hn_attn_key_mass: too many query rows");
     const MassPlan pl = mass_plan(p.rows, B, H, kv_len);
     const int splits = pl.splits;
     p.part = splits > 1 ? (float*)workspace : nullptr;

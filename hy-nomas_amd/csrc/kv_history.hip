@@ -60,9 +60,10 @@ HN_DEVICE f32x2 decode2(uint32_t w, int hi) {
 template <int FMT>
 __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
     const int lane = threadIdx.x & 63, piece = lane & 7, row = lane >> 3;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // < 2^31
     if (unit >= a.units) return;  // whole waves; no barrier below
-    const int64_t h = unit % a.H, jb = unit / a.H, j = a.j0 + jb % a.blocks, b = jb / a.blocks;
+    const uint32_t blocks = (uint32_t)a.blocks, jb = unit / (uint32_t)a.H;
+    const int64_t h = unit - jb * (uint32_t)a.H, b = jb / blocks, j = a.j0 + (jb - (uint32_t)b * blocks);
     float lo[16], hi[16];
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
@@ -166,21 +167,23 @@ HN_DEVICE void add_pooled(uint32_t x, double (&w)[2], double (&u)[2]) {
 // time, and the 16 partial sums of a channel meet in LDS.
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
     __shared__ double part[16][257];
-    const int64_t unit = blockIdx.x;  // (b * H + h) * runs + run
-    const int64_t run = unit % a.runs, h = (unit / a.runs) % a.H, b = unit / (a.runs * a.H);
+    const uint32_t unit = blockIdx.x;  // (b * H + h) * runs + run
+    const uint32_t runs = (uint32_t)a.runs, bh = unit / runs, H = (uint32_t)a.H, G = (uint32_t)a.G;
+    const int64_t run = unit - bh * runs, b = bh / H, h = bh - (uint32_t)b * H;
     const int t = threadIdx.x, l16 = t & 15, g16 = t >> 4;
     const int64_t i0 = run * a.q_block, left = a.Lq - i0;
-    const int64_t rows = (left < a.q_block ? left : a.q_block) * a.G;
+    const uint32_t rows = (uint32_t)((left < a.q_block ? left : a.q_block) * a.G);  // < 2^31
     double w[4][2] = {}, u[4][2] = {};
-    const uint16_t* q = a.q + b * a.qs0 + h * a.G * a.qs2 + 8 * l16;
-    for (int64_t r0 = g16; r0 < rows; r0 += 64) {
+    const uint16_t* base = a.q + b * a.qs0 + h * a.G * a.qs2 + 8 * l16;
+    for (uint32_t r0 = g16; r0 < rows; r0 += 64) {
         uint4 x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // four rows' loads in flight
-            const int64_t r = r0 + 16 * e, i = i0 + r / a.G, g = r % a.G;
+            const uint32_t r = r0 + 16 * e, q = r / G, g = r - q * G;
+            const int64_t i = i0 + q;
             x[e] = make_uint4(0u, 0u, 0u, 0u);  // adds nothing
             if (r < rows && (!a.qvalid || a.qvalid[b * a.qvs + i] != 0))
-                x[e] = *reinterpret_cast<const uint4*>(q + i * a.qs1 + g * a.qs2);
+                x[e] = *reinterpret_cast<const uint4*>(base + i * a.qs1 + g * a.qs2);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
             for (int e = 0; e < 16; ++e) total += part[e][t & 127];
         __syncthreads();
     }
-    a.pooled[unit * 256 + t] = total;
+    a.pooled[(int64_t)unit * 256 + t] = total;
 }
 
 struct ScoreArgs {
@@ -815,7 +818,7 @@ extern "C" int hn_kv_block_bounds(int fmt, const void* kc, const int64_t* cs, co
     a.end = end; a.H = (int)H; a.block = (int)block;
     a.units = B * a.blocks * H;
     const int64_t grid = (a.units + 3) / 4;
-    HN_REQUIRE(grid <= 0x7fffffffLL, HN_E_ARG, "hn_kv_block_bounds: too many blocks");
+    HN_REQUIRE(a.units <= 0x7fffffffLL, HN_E_ARG, "hn_kv_block_bounds: too many blocks");
     hipStream_t st = (hipStream_t)stream;
     if (fmt == HN_KV_FP8) hist::bounds_kernel<HN_KV_FP8><<<(unsigned)grid, 256, 0, st>>>(a);
     else hist::bounds_kernel<HN_KV_INT8><<<(unsigned)grid, 256, 0, st>>>(a);
@@ -853,7 +856,7 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
     const int64_t need = hn_select_kv_blocks_workspace_size(B, H, runs, blocks);
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_select_kv_blocks: workspace smaller than hn_select_kv_blocks_workspace_size() or misaligned");
-    HN_REQUIRE(B * H <= 65535 && B * H * runs <= 0x7fffffffLL && runs <= 16 * 65535LL, HN_E_ARG,
+    HN_REQUIRE(B * H <= 65535 && B * H * runs <= 0x7fffffffLL && runs <= 16 * 65535LL && Lq <= 0x7fffffffLL / Hq, HN_E_ARG,
                "hn_select_kv_blocks: too much work for one launch");
     if (const int rc = require_gfx950("hn_select_kv_blocks"); rc != HN_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
