@@ -958,6 +958,21 @@ extern "C" int hn_select_kv_tokens(const float* mass, const int64_t* ms, int64_t
     return check_launch("hn_select_kv_tokens");
 }
 
+// The bytes that a tensor of `n` dims spans from its first element.
+struct Span {
+    uintptr_t lo, hi;
+};
+
+static Span span_of(const void* base, const int64_t* shape, const int64_t* strides, int n, int64_t elem) {
+    int64_t last = 0, first = 0;
+    for (int i = 0; i < n; ++i) {
+        if (shape[i] == 0) return Span{0, 0};
+        (strides[i] < 0 ? first : last) += (shape[i] - 1) * strides[i];
+    }
+    const uintptr_t p = (uintptr_t)base;
+    return Span{p + (uintptr_t)(first * elem), p + (uintptr_t)((last + 1) * elem)};
+}
+
 extern "C" int hn_move_kv_tokens(const void* k, const void* v, const int64_t* cs, const float* ks, const float* vs,
                                  const int64_t* ss, const float* mass, const int64_t* ms, int64_t B, int64_t H,
                                  int64_t D, int64_t tokens, const int32_t* idx, int64_t keep, void* out_k, void* out_v,
@@ -975,6 +990,18 @@ extern "C" int hn_move_kv_tokens(const void* k, const void* v, const int64_t* cs
     if (B == 0 || keep == 0) return HN_OK;
     HN_REQUIRE(k && v && ks && vs && mass && idx && out_k && out_v && out_ks && out_vs && out_mass, HN_E_ARG,
                "hn_move_kv_tokens: null pointer");
+    {
+        const int64_t src[4] = {B, tokens, H, D}, dst[4] = {B, keep, H, D}, row[3] = {B, H, tokens};
+        const int64_t ms3[3] = {ms[0], ms[1], 1}, flat = B * H * keep, one = 1;
+        const Span in[6] = {span_of(k, src, cs, 4, 1), span_of(v, src, cs, 4, 1), span_of(ks, src, ss, 3, 4),
+                            span_of(vs, src, ss, 3, 4), span_of(mass, row, ms3, 3, 4), span_of(idx, &flat, &one, 1, 4)};
+        const Span out[5] = {span_of(out_k, dst, os, 4, 1), span_of(out_v, dst, os, 4, 1), span_of(out_ks, dst, ts, 3, 4),
+                             span_of(out_vs, dst, ts, 3, 4), span_of(out_mass, &flat, &one, 1, 4)};
+        for (const Span& o : out)
+            for (const Span& i : in)
+                HN_REQUIRE(!(o.lo < i.hi && i.lo < o.hi), HN_E_ARG,
+                           "hn_move_kv_tokens: the output cache overlaps the source");
+    }
     if (const int rc = require_gfx950("hn_move_kv_tokens"); rc != HN_OK) return rc;
     hist::MoveArgs a;
     a.k = (const uint8_t*)k; a.v = (const uint8_t*)v; a.ks = ks; a.vs = vs; a.mass = mass;

@@ -880,6 +880,12 @@ def _(q, bounds, kv_len, top_k, block=64, q_block=128, keep_first=0, keep_last=0
     return q.new_empty((q.shape[0], bounds.shape[2], -(-q.shape[1] // q_block), top_k), dtype=torch.int32)
 
 
+@functools.lru_cache(maxsize=1024)
+def _blocks_workspace(device: int, *sizes) -> int:
+    """hn_attn_kv_blocks_workspace_size on the current device, ``device``."""
+    return L.load().hn_attn_kv_blocks_workspace_size(*sizes)
+
+
 @eager_op("hy_nomas_amd::attn_kv_blocks", mutates_args=())
 def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
                    v_scale: torch.Tensor, kv_len: int, block_idx: Optional[torch.Tensor] = None, block: int = 64,
@@ -945,7 +951,9 @@ def attn_kv_blocks(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor
     top_k = -1 if block_idx is None else block_idx.shape[3]
     with _on(q.device):
         lib = L.load()
-        ws_bytes = lib.hn_attn_kv_blocks_workspace_size(B, Lq, Hq, H, kv_len, cur_len, top_k, block, q_block)
+        # (with lists the plan does not depend on kv_len, which grows from call to call)
+        ws_bytes = _blocks_workspace(q.device.index, B, Lq, Hq, H, kv_len if top_k < 0 else 0, cur_len, top_k, block,
+                                     q_block)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
         L.check(lib.hn_attn_kv_blocks(
             fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), _strides(k_codes),
@@ -1062,34 +1070,15 @@ def _(mass, kv_len, keep, keep_first=0, keep_last=0, cache_valid=None):
     return mass.new_empty((mass.shape[0], mass.shape[1], keep), dtype=torch.int32)
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """The address range that a tensor's elements lie in."""
-    last = 0
-    for n, s in zip(t.shape, t.stride()):
-        last += (n - 1) * s
-    start = t.data_ptr()
-    return start, start + (last + 1) * t.element_size() if t.numel() else start
-
-
-def _overlaps(outputs, inputs) -> bool:
-    """Whether an output's address range meets an input's."""
-    spans = [_span(t) for t in inputs]
-    for t in outputs:
-        a0, a1 = _span(t)
-        for b0, b1 in spans:
-            if a0 < b1 and b0 < a1:
-                return True
-    return False
-
-
 @eager_op("hy_nomas_amd::move_kv_tokens_", mutates_args=("out_k", "out_v", "out_k_scale", "out_v_scale"))
 def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch.Tensor, out_v_scale: torch.Tensor,
                     k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                     mass: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     """Row i of each head of the output cache <- token idx[b, h, i] of the source, for
     idx int32 [B, H, keep]; returns that token's mass, fp32 [B, H, keep]. An index
-    outside the mass's tokens leaves its row as it is (mass 0). The output cache is
-    another one than the source: [B, >= keep, H, D] of the same dtype."""
+    outside the mass's tokens leaves its row as it is (mass 0). The output cache [B, >=
+    keep, H, D] of the same dtype is another one than the source: the library refuses
+    one whose memory meets it."""
     what = "move_kv_tokens_"
     _kv_fmt(k_codes)
     _check_keys(k_codes, k_scale, what)
@@ -1113,8 +1102,6 @@ def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch
     if keep > out_k.shape[1]:
         raise ValueError(f"{what}: {keep} tokens exceed the output cache's capacity {out_k.shape[1]}")
     _one_device(what, k_codes, v_codes, k_scale, v_scale, mass, idx, out_k, out_v, out_k_scale, out_v_scale)
-    if _overlaps((out_k, out_v, out_k_scale, out_v_scale), (k_codes, v_codes, k_scale, v_scale, mass, idx)):
-        raise ValueError(f"{what}: the output cache overlaps the source")
     if mass.stride(2) != 1:
         mass = mass.contiguous()
     idx = idx.contiguous()

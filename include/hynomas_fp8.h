@@ -395,8 +395,8 @@ int64_t hn_select_kv_tokens_workspace_size(int64_t B, int64_t H, int64_t kv_len)
 
 /* Moves the listed tokens of each head to the front of another cache: row i of the
  * output (codes and scales of K and V) and out_mass[b, h, i] <- token idx[b, h, i].
- * An index outside [0, tokens) leaves the row as it is and its mass 0. The output
- * does not overlap the source.
+ * An index outside [0, tokens) leaves the row as it is and its mass 0. An output whose
+ * address range meets an input's is refused.
  *   cs, ss: strides of the source's codes and scales; os, ts: of the output's;
  *   ms[2]: of the mass [B, H, tokens]; out_mass: fp32 [B, H, keep] contiguous */
 int hn_move_kv_tokens(const void *k, const void *v, const int64_t *cs, const float *ks, const float *vs,

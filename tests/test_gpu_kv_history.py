@@ -589,9 +589,9 @@ def test_evict_refuses_its_own_cache(dev):
     hist = pkg_module("kv_history")
     cache = _cache(dev, 1, 100, 2, "fp8", _gen(dev, 1))
     mass = torch.rand(1, 2, 100, device=dev)
-    with pytest.raises(ValueError, match="overlaps"):
+    with pytest.raises(RuntimeError, match="overlaps"):
         hist.evict(cache, cache, mass, 100, 50)
-    with pytest.raises(ValueError, match="overlaps"):
+    with pytest.raises(RuntimeError, match="overlaps"):
         hist.evict({n: t[:, :60] for n, t in cache.items()}, {n: t[:, 40:] for n, t in cache.items()}, mass[..., :60], 60, 30)
 
 

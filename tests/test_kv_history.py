@@ -240,12 +240,17 @@ def test_c_abi_refusals():
         assert tokens(**kw) == -1 and match in err(), kw
     assert tokens(keep=0, m=None) == 0
 
-    def move(D=128, keep=10, cap=10, os=st, k=_A):
-        return lib.hn_move_kv_tokens(k, _A, st, _A, _A, s3, _A, s3, 1, 2, D, 100, _A, keep, _A, _A, os, _A, _A, s3, cap,
-                                     _A, None)
+    far = _A << 12
+
+    def move(D=128, keep=10, cap=10, os=st, k=_A, out=far, out_scale=far):
+        return lib.hn_move_kv_tokens(k, _A, st, _A, _A, s3, _A, s3, 1, 2, D, 100, _A, keep, out, far, os, out_scale,
+                                     far, s3, cap, far, None)
 
     for kw, match in ((dict(D=64), "head dim"), (dict(keep=11), "capacity"), (dict(k=None), "null"),
-                      (dict(os=(ctypes.c_int64 * 4)(256, 248, 128, 1)), "multiples")):
+                      (dict(os=(ctypes.c_int64 * 4)(256, 248, 128, 1)), "multiples"),
+                      # 100 tokens of 256 bytes and 800 of scales from _A on
+                      (dict(out=_A + 99 * 256), "overlaps"), (dict(out=_A - 10 * 256 + 16), "overlaps"),
+                      (dict(out_scale=_A + 796), "overlaps")):
         assert move(**kw) == -1 and match in err(), kw
     assert move(keep=0, k=None) == 0
 
