@@ -34,6 +34,8 @@ HN_DEVICE uint32_t rank_of(float f) {
 // fp32 products are rounded once at the end. One wave per (batch, block, head):
 // 8 lanes hold a key's 128 codes (16 bytes each) and 8 keys are read per load,
 // all loads of 64 keys in flight; the 8 keys' extremes meet by lane exchanges.
+// Bound by the read of the codes, and for few blocks by the launch: 10800 tokens x 24
+// heads (36 MB) 9.8 us, 3.7 TB/s; one token of 8 batches x 8 heads 4.8 us.
 struct BoundsArgs {
     const uint8_t* kc;
     const float* ks;
@@ -164,7 +166,8 @@ HN_DEVICE void add_pooled(uint32_t x, double (&w)[2], double (&u)[2]) {
 }
 
 // One workgroup per run: 16 threads hold a row (8 channels each), 16 rows at a
-// time, and the 16 partial sums of a channel meet in LDS.
+// time, and the 16 partial sums of a channel meet in LDS. Bound by the read of the
+// queries: 10800 x 24 heads (66 MB) 18.6 us, 3.6 TB/s.
 __global__ __launch_bounds__(256) void pool_kernel(PoolArgs a) {
     __shared__ double part[16][257];
     const uint32_t unit = blockIdx.x;  // (b * H + h) * runs + run
@@ -225,7 +228,8 @@ HN_DEVICE uint32_t block_rank(const ScoreArgs& a, int64_t j, bool empty, double 
 // Few runs (single tokens): 16 lanes per block, 16 of the 256 terms each, four
 // blocks' loads in flight. The run's sums are staged in LDS once per workgroup;
 // FROM_Q: they are taken from the queries here (few rows), which saves the pooling
-// launch.
+// launch. Bound by the read of the bounds: 64 heads x 2048 blocks (67 MB) 20 us, 3.3
+// TB/s.
 constexpr int SCORE_FEW_RUNS = 4;
 constexpr int SCORE_FEW = 4;  // blocks in flight per lane group
 template <bool FROM_Q>
@@ -306,7 +310,11 @@ __global__ __launch_bounds__(256, 4) void score_few_kernel(ScoreArgs a) {
 // result register r: row 4 r + l / 16). Terms are dealt so that lane group g holds
 // terms 64 g .. 64 g + 63: each lane then reads 128 contiguous bytes of its block's
 // bounds. The runs' sums are staged once per workgroup (row pitch 258 doubles:
-// 16-byte reads of 8 rows fall in different banks).
+// 16-byte reads of 8 rows fall in different banks). Bound by the matrix unit's 64
+// cycles a product and by how evenly 864 workgroups fall on 256 CUs: 24 heads x 85 runs
+// x 1350 blocks 48 us (1.4 GFLOP, 20 us at the 71 TFLOP/s of a large 64-bit product);
+// on the vector unit it took 590 us. Two accumulators changed nothing; two tiles a wave
+// took 61 us (twice the staging).
 constexpr int SCORE_TILES = 4;  // 16-block tiles per wave
 __global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
     constexpr int PITCH = 258;
@@ -369,7 +377,9 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
 // before it. Scores share their leading bits, so the digit counts are kept in
 // COPIES copies that neighbouring lanes add to. KPT > 0: a thread holds its KPT
 // elements in registers (n <= KPT NT), so that a row is read once; KPT = 0: longer
-// rows are read again in every pass.
+// rows are read again in every pass. Bound by the passes' barriers and LDS adds, not by
+// bytes: 2040 rows of 1350 13.6 us, 64 rows of 2048 5.9 us, 24 rows of 1001 masses 8.8
+// us, of 32768 23 us.
 constexpr int COPIES = 8, COPY_PITCH = 260;  // (a copy starts 4 banks after the one before)
 
 template <int NT>
@@ -568,7 +578,9 @@ __global__ __launch_bounds__(1024) void choose_tokens_kernel(TokenArgs a) {
 // row is dealt to workgroups of PART tokens and each step of the search is a launch:
 // the counts of a digit of the rank (11, 11 and 10 bits) are added to the row's bins
 // (whole numbers: the order does not matter), the next launch reads the digit from
-// them, the last two count the taken tokens of each part and write them.
+// them, the last two count the taken tokens of each part and write them. Bound by its
+// six launches: 24 heads x 86400 tokens 37 us, where one workgroup a row took 100 us (a
+// row of 32768, the longest that it holds in 74 registers, 23 us).
 constexpr int PART_KPT = 16, PART = 256 * PART_KPT, BINS = 2048;
 
 // Per row in the workspace: bins of the three digits, then {prefix, need} after each,
@@ -738,7 +750,9 @@ __global__ __launch_bounds__(256) void long_tokens_kernel(TokenArgs a, uint32_t*
 // ---------------------------------------------------------------------------
 // Move of the chosen tokens: row i of the output cache <- row idx[b, h, i] of
 // the source (codes and scales of K and V, and the mass), head by head. A
-// negative or out-of-range index leaves the row as it is (its mass becomes 0).
+// negative or out-of-range index leaves the row as it is (its mass becomes 0). 8 lanes
+// move a row. Bound by the scattered 128-byte reads: 43200 of 86400 tokens x 24 heads
+// (568 MB) 136 us, 4.2 TB/s (a plain copy reaches 5.1).
 struct MoveArgs {
     const uint8_t *k, *v;
     const float *ks, *vs, *mass;

@@ -165,7 +165,8 @@ class LayerHistory:
         mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
         if not self.track_mass or self.mass is None:
             raise ValueError("eviction needs the mass of the cached tokens (track_mass)")
-        idx, self.mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
+        idx, mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
+        self.mass = mass[:, :, :min(keep, kv_len)]
         if self.bounds is not None:
             update_block_bounds(self.bounds, out, 0, min(keep, kv_len), block=self.block)
         return idx

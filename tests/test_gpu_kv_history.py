@@ -408,7 +408,7 @@ def test_offsets_past_32_bits(dev):
     ca, hist, kvc = pkg_module("cache_attention"), pkg_module("kv_history"), pkg_module("fp8_kv_cache")
     g = _gen(dev, 5)
     H, n = 24, 300
-    cap = (1 << 32) // (H * D) + 40000                       # tokens of 3072 code bytes... over 2^32 in all
+    cap = (1 << 32) // (H * D) + 40000                       # so many tokens that the codes pass 2^32 bytes
     big = kvc.make_fp8_kv_block(1, cap, H, D, device=dev)
     small = _cache(dev, 1, n, H, "fp8", g)
     start = (cap - n) // 64 * 64
