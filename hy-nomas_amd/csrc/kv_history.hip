@@ -1002,8 +1002,8 @@ extern "C" int hn_move_kv_tokens(const void* k, const void* v, const int64_t* cs
     HN_REQUIRE(aligned(k, 16) && aligned(v, 16) && aligned(out_k, 16) && aligned(out_v, 16), HN_E_ARG,
                "hn_move_kv_tokens: cache misaligned");
     if (B == 0 || keep == 0) return HN_OK;
-    HN_REQUIRE(k && v && ks && vs && mass && idx && out_k && out_v && out_ks && out_vs && out_mass, HN_E_ARG,
-               "hn_move_kv_tokens: null pointer");
+    HN_REQUIRE((tokens == 0 || (k && v && ks && vs && mass)) && idx && out_k && out_v && out_ks && out_vs && out_mass,
+               HN_E_ARG, "hn_move_kv_tokens: null pointer");
     {
         const int64_t src[4] = {B, tokens, H, D}, dst[4] = {B, keep, H, D}, row[3] = {B, H, tokens};
         const int64_t ms3[3] = {ms[0], ms[1], 1}, flat = B * H * keep, one = 1;

@@ -595,6 +595,18 @@ def test_evict_refuses_its_own_cache(dev):
         hist.evict({n: t[:, :60] for n, t in cache.items()}, {n: t[:, 40:] for n, t in cache.items()}, mass[..., :60], 60, 30)
 
 
+def test_evict_of_an_empty_cache(dev):
+    """No token, no mass: every place stays empty and the output as it was."""
+    hist, kvc = pkg_module("kv_history"), pkg_module("fp8_kv_cache")
+    for cap in (0, 20):
+        cache, out = kvc.make_fp8_kv_block(2, cap, 3, D, device=dev), kvc.make_fp8_kv_block(2, 8, 3, D, device=dev)
+        for t in out.values():
+            t.view(torch.uint8).fill_(0x5a)
+        idx, moved = hist.evict(cache, out, torch.empty(2, 3, 0, device=dev), 0, 6)
+        assert idx.shape == (2, 3, 6) and (idx == -1).all() and moved.shape == (2, 3, 6) and (moved == 0).all()
+        assert all((t.view(torch.uint8) == 0x5a).all() for t in out.values())
+
+
 # --------------------------------------------------------------------------
 # together
 
