@@ -854,8 +854,8 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
     HN_REQUIRE(D == hist::D, HN_E_ARG, "hn_select_kv_blocks: head dim must be 128");
     HN_REQUIRE(B >= 0 && Lq >= 0 && H > 0 && Hq > 0 && Hq % H == 0 && Hq <= 65535 && blocks >= 0, HN_E_ARG,
                "hn_select_kv_blocks: invalid shape");
-    HN_REQUIRE(q_block > 0 && top_k > 0 && top_k <= 0x7fffffffLL && blocks <= 0x1fffffffLL, HN_E_ARG,
-               "hn_select_kv_blocks: q_block and top_k must be positive");
+    HN_REQUIRE(q_block > 0 && top_k > 0, HN_E_ARG, "hn_select_kv_blocks: q_block and top_k must be positive");
+    HN_REQUIRE(top_k <= 0x1fffffffLL && blocks <= 0x1fffffffLL, HN_E_ARG, "hn_select_kv_blocks: too many blocks");
     HN_REQUIRE(keep_first >= 0 && keep_last >= 0 && keep_first <= top_k && keep_last <= top_k - keep_first, HN_E_ARG,
                "hn_select_kv_blocks: keep_first + keep_last exceeds top_k");
     HN_REQUIRE(qs && bs && qs[3] == 1 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0, HN_E_ARG,

@@ -204,7 +204,8 @@ def test_c_abi_refusals():
                                        wsb, None)
 
     for kw, match in ((dict(D=96), "head dim"), (dict(Hq=3), "shape"), (dict(q_block=0), "positive"),
-                      (dict(k=0), "positive"), (dict(first=3, last=2), "exceeds"), (dict(last=-1), "exceeds"),
+                      (dict(k=0), "positive"), (dict(k=(1 << 31) - 1), "too many"), (dict(blocks=1 << 30), "too many"),
+                      (dict(first=3, last=2), "exceeds"), (dict(last=-1), "exceeds"),
                       (dict(wsb=64), "workspace"), (dict(ws=_A + 8), "workspace"), (dict(q=None), "null")):
         assert select(**kw) == -1 and match in err(), kw
     assert lib.hn_select_kv_blocks_workspace_size(1, 2, 3, 9) >= 6 * (2048 + 36)
