@@ -308,6 +308,8 @@ class FP8ARModel(nn.Module):
         """Cut every layer's cache to ``evict_keep`` tokens a head: each moves into the
         spare cache, and its old one is the next layer's spare."""
         keep = self.evict_keep
+        if not keep:
+            raise ValueError("evict_history needs evict_keep")
         first = min(math.prod(self.latent_shape[1:]), keep // 4)
         last = min(self.write_tokens, keep // 2)
         for i, history in enumerate(self.histories):

@@ -109,10 +109,15 @@ class LayerHistory:
     longer history (the first ``keep_first`` and the last ``keep_last`` of it
     always) and the current chunk; 0: all of it. ``track_mass``: writing passes,
     which read everything, add the weight that each cached key drew to ``mass``.
-    A writing pass counts once ``commit`` is called; ``rollback`` forgets it."""
+    A writing pass counts once ``commit`` is called; ``rollback`` forgets it. A pass over
+    another number of tokens than ``length``, those accounted for, is refused (bounds and
+    mass would be of other keys); one over none starts anew, and ``reset`` takes a
+    cache's tokens in."""
 
     def __init__(self, cache: dict, *, top_k: int = 0, block: int = 64, q_block: int = 128, keep_first: int = 1,
                  keep_last: int = 2, track_mass: bool = False):
+        if top_k < 0 or keep_first < 0 or keep_last < 0 or q_block < 1:
+            raise ValueError("top_k, keep_first and keep_last must not be negative, q_block must be positive")
         if top_k and keep_first + keep_last > top_k:
             raise ValueError("keep_first + keep_last exceeds top_k")
         self.top_k, self.block, self.q_block = top_k, block, q_block
@@ -120,13 +125,27 @@ class LayerHistory:
         self.track_mass = track_mass
         self.bounds = make_block_bounds(cache, block=block) if top_k else None
         self.mass: Optional[torch.Tensor] = None    # fp32 [B, H, tokens], None: no token yet
-        self._written = None                        # (mass, length) of a pass not committed yet
+        self.length = 0                             # tokens that bounds and mass account for
+        self._written = None                        # (mass, start, end) of a pass not committed yet
+
+    def reset(self, cache: dict, kv_len: int) -> None:
+        """Account for cache tokens [0, kv_len) as they are, without mass so far."""
+        if self.bounds is not None and kv_len:
+            update_block_bounds(self.bounds, cache, 0, kv_len, block=self.block)
+        codes = cache["k"]
+        self.mass = (torch.zeros((codes.shape[0], codes.shape[2], kv_len), device=codes.device)
+                     if self.track_mass and kv_len else None)
+        self.length, self._written = kv_len, None
 
     def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, kv_len: int,
                update_cache: bool) -> torch.Tensor:
         """Attention of one pass over [cache tokens < kv_len | k, v]. On a writing pass
         k and v are in the cache already, from token kv_len on."""
         from .cache_attention import chunk_attention, sparse_chunk_attention
+        if kv_len == 0:  # a new roll-out
+            self.mass, self.length = None, 0
+        elif kv_len != self.length:
+            raise ValueError(f"the history accounts for {self.length} tokens, the pass reads {kv_len} (commit or reset)")
         if update_cache:
             end = kv_len + k.shape[1]
             mass = None
@@ -154,6 +173,7 @@ class LayerHistory:
             self.mass = mass
         if self.bounds is not None:
             update_block_bounds(self.bounds, cache, start, end, block=self.block)
+        self.length = end
 
     def rollback(self) -> None:
         """The last writing pass was refused: nothing of it counts."""
@@ -165,8 +185,11 @@ class LayerHistory:
         mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
         if not self.track_mass or self.mass is None:
             raise ValueError("eviction needs the mass of the cached tokens (track_mass)")
+        if kv_len != self.length:
+            raise ValueError(f"the history accounts for {self.length} tokens, not {kv_len}")
         idx, mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
-        self.mass = mass[:, :, :min(keep, kv_len)]
+        self.length, self._written = min(keep, kv_len), None
+        self.mass = mass[:, :, :self.length]
         if self.bounds is not None:
-            update_block_bounds(self.bounds, out, 0, min(keep, kv_len), block=self.block)
+            update_block_bounds(self.bounds, out, 0, self.length, block=self.block)
         return idx

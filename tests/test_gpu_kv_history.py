@@ -421,6 +421,16 @@ def test_offsets_past_32_bits(dev):
     a = ca.sparse_chunk_attention(q, small, n, near, q_block=2)
     b = ca.sparse_chunk_attention(q, big, kv, near + start // 64, q_block=2)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # the kernels of longer runs and of single rows, with and without holes
+    near_valid = torch.rand(1, n, device=dev, generator=g) >= 0.3
+    far_valid = torch.zeros(1, kv, dtype=torch.bool, device=dev)
+    far_valid[:, start:] = near_valid
+    for L in (1, 50, 100):
+        ql = torch.randn(1, L, H, D, device=dev, generator=g).to(BF16)
+        for nv, fv in ((None, None), (near_valid, far_valid)):
+            c = ca.sparse_chunk_attention(ql, small, n, near, q_block=L, k_cur=ql, v_cur=ql, cache_valid=nv)
+            d = ca.sparse_chunk_attention(ql, big, kv, near + start // 64, q_block=L, k_cur=ql, v_cur=ql, cache_valid=fv)
+            assert all(torch.equal(x, y) for x, y in zip(c, d)), L
     bounds = hist.make_block_bounds(big)
     hist.update_block_bounds(bounds, big, start, kv)
     ref = hist.make_block_bounds(small)
@@ -773,3 +783,34 @@ def test_model_reads_blocks_and_cuts_a_full_cache(dev):
     assert m.cache_valid_len == 300
     for h, b, w in zip(m.histories, bounds, mass):
         assert torch.equal(h.bounds, b) and torch.equal(h.mass, w) and h.mass.shape == (1, 2, 300)
+
+
+def test_model_starts_a_new_roll_out(dev):
+    """A second roll-out over the same caches is the first one again: nothing of the old
+    history's mass or bounds is left; filled caches are taken in by reset."""
+    hist = pkg_module("kv_history")
+    m = _model(dev, sparse_top_k=3, evict_keep=300)
+    first = [m.generate_chunk(*_chunk(dev, i)) for i in range(5)]
+    mass = [h.mass for h in m.histories]
+    m.cache_valid_len = m.frames_done = 0
+    again = [m.generate_chunk(*_chunk(dev, i)) for i in range(5)]
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert all(torch.equal(a, h.mass) for a, h in zip(mass, m.histories))
+    h, c = m.histories[0], m.caches[0]
+    m.cache_valid_len = 100                               # moved by hand: refused until taken in
+    with pytest.raises(ValueError, match="accounts for 428 tokens, the pass reads 100"):
+        m.generate_chunk(*_chunk(dev, 5))
+    for h, c in zip(m.histories, m.caches):
+        h.reset(c, 100)
+        ref = hist.make_block_bounds(c)
+        hist.update_block_bounds(ref, c, 0, 100)
+        assert torch.equal(h.bounds[:, :2], ref[:, :2]) and (h.mass == 0).all() and h.mass.shape == (1, 2, 100)
+    assert torch.isfinite(m.generate_chunk(*_chunk(dev, 5)).float()).all()
+
+
+def test_model_refusals(dev):
+    for kw in (dict(sparse_top_k=-1), dict(evict_keep=-1), dict(evict_keep=385), dict(sparse_top_k=1, text_len=8)):
+        with pytest.raises(ValueError):
+            _model(dev, **kw)
+    with pytest.raises(ValueError, match="evict_keep"):
+        _model(dev).evict_history()

@@ -276,6 +276,23 @@ def test_model_refusals():
     h = hist.LayerHistory(cache, top_k=4)
     with pytest.raises(ValueError, match="mass"):
         h.evict(cache, cache, 128, 64)
+    for kw in (dict(top_k=-1), dict(keep_first=-1), dict(keep_last=-1), dict(q_block=0)):
+        with pytest.raises(ValueError, match="must"):
+            hist.LayerHistory(cache, **{"top_k": 4, **kw})
+    # passes over tokens that bounds and mass do not account for
+    h = hist.LayerHistory(cache, top_k=4, track_mass=True)
+    q = torch.zeros(1, 3, 2, 128, dtype=torch.bfloat16)
+    for update in (False, True):
+        with pytest.raises(ValueError, match="accounts for 0 tokens, the pass reads 64"):
+            h.attend(q, q, q, cache, 64, update)
+    h.mass, h.length = torch.ones(1, 2, 128), 128        # as after a roll-out
+    with pytest.raises(ValueError, match="accounts for 128 tokens, not 100"):
+        h.evict(cache, cache, 100, 64)
+    with pytest.raises(RuntimeError, match="GPU"):       # (a new roll-out: allowed, and on a GPU it would run)
+        h.attend(q, q, q, cache, 0, True)
+    assert h.mass is None and h.length == 0
+    h.reset(cache, 0)
+    assert h.length == 0 and h.mass is None
     block = dit.FP8DiTBlock.__new__(dit.FP8DiTBlock)
     with pytest.raises(ValueError, match="image-only"):
         dit.FP8DiTBlock.forward(block, None, None, None, None, cache, 0, txt=1, history=h)
