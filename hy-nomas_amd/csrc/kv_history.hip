@@ -216,6 +216,7 @@ struct ScoreArgs {
     uint32_t* rank;          // [B, H, runs, n]
     int64_t bs0, bs1, bs2, runs, n, first, last;
     int H;
+    uint32_t run_tiles, stretches, work, per_xcd;  // of score_kernel
     PoolArgs pool;           // the queries, where the kernel sums them itself
 };
 
@@ -312,15 +313,22 @@ __global__ __launch_bounds__(256, 4) void score_few_kernel(ScoreArgs a) {
 // bounds. The runs' sums are staged once per workgroup (row pitch 258 doubles:
 // 16-byte reads of 8 rows fall in different banks). Bound by the matrix unit's 64
 // cycles a product and by how evenly 864 workgroups fall on 256 CUs: 24 heads x 85 runs
-// x 1350 blocks 48 us (1.4 GFLOP, 20 us at the 71 TFLOP/s of a large 64-bit product);
-// on the vector unit it took 590 us. Two accumulators changed nothing; two tiles a wave
-// took 61 us (twice the staging).
+// x 1350 blocks 41 us (1.4 GFLOP, 20 us at the 71 TFLOP/s of a large 64-bit product;
+// 48 us with the runs of a stretch of blocks on different XCDs); on the vector unit it
+// took 590 us. Two accumulators changed nothing; two tiles a wave took 27 % longer (twice
+// the staging).
 constexpr int SCORE_TILES = 4;  // 16-block tiles per wave
 __global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
     constexpr int PITCH = 258;
     __shared__ __attribute__((aligned(16))) double sums[16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
-    const int64_t bh = blockIdx.z, h = bh % a.H, b = bh / a.H, run0 = (int64_t)blockIdx.y * 16;
+    // id % 8 (the XCD) picks a contiguous range of items, the runs of a stretch of blocks
+    // side by side: they share its bounds in one L2
+    const uint32_t w = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+    if (w >= a.work) return;
+    const uint32_t wx = w / a.run_tiles, wz = wx / a.stretches, H = (uint32_t)a.H, wb = wz / H;
+    const int64_t bh = wz, h = wz - wb * H, b = wb, run0 = (int64_t)(w - wx * a.run_tiles) * 16;
+    const int64_t stretch = wx - wz * a.stretches;
     double in[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r)  // (rows past the last run repeat it; their scores are not written)
@@ -337,7 +345,7 @@ __global__ __launch_bounds__(256) void score_kernel(ScoreArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = src[e];
     };
-    const int64_t first_j = ((int64_t)blockIdx.x * SCORE_TILES * 4 + wave) * 16;
+    const int64_t first_j = (stretch * SCORE_TILES * 4 + wave) * 16;
     fetch(first_j);
     for (int tile = 0; tile < SCORE_TILES; ++tile) {
         const int64_t j0 = first_j + 64 * tile, j = j0 + c16;
@@ -881,7 +889,7 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
         pa.q = (const uint16_t*)q; pa.qvalid = q_valid; pa.pooled = (double*)workspace;
         pa.qs0 = qs[0]; pa.qs1 = qs[1]; pa.qs2 = qs[2]; pa.qvs = q_valid_stride;
         pa.Lq = Lq; pa.q_block = q_block; pa.runs = runs; pa.H = (int)H; pa.G = (int)(Hq / H);
-        hist::ScoreArgs sa;
+        hist::ScoreArgs sa = {};
         rank = (uint32_t*)((uint8_t*)workspace + align256(rows * 256 * 8));
         sa.pooled = pa.pooled; sa.bounds = (const uint16_t*)bounds; sa.rank = rank;
         sa.bs0 = bs[0]; sa.bs1 = bs[1]; sa.bs2 = bs[2];
@@ -896,8 +904,13 @@ extern "C" int hn_select_kv_blocks(const void* q, const int64_t* qs, int64_t B, 
             else hist::score_few_kernel<false><<<grid, 256, 0, st>>>(sa);
         } else {
             constexpr int64_t per = 64 * hist::SCORE_TILES;
-            hist::score_kernel<<<dim3((unsigned)((blocks + per - 1) / per), (unsigned)((runs + 15) / 16),
-                                      (unsigned)(B * H)), 256, 0, st>>>(sa);
+            const int64_t work = (blocks + per - 1) / per * ((runs + 15) / 16) * B * H;
+            HN_REQUIRE(work <= 0x3fffffffLL, HN_E_ARG, "hn_select_kv_blocks: too much work for one launch");
+            sa.run_tiles = (uint32_t)((runs + 15) / 16);
+            sa.stretches = (uint32_t)((blocks + per - 1) / per);
+            sa.work = (uint32_t)work;
+            sa.per_xcd = (uint32_t)((work + 7) / 8);
+            hist::score_kernel<<<8 * sa.per_xcd, 256, 0, st>>>(sa);
         }
     }
     if (blocks <= 8 * 256)
