@@ -92,6 +92,28 @@ HN_DEVICE f32x16 step_a_lse(const f32x16& s, float c, float nm, float& l, f16x8 
     return acc;
 }
 
+// rebase (attn_tiles.h) with the running maximum held 2^11 low: probabilities are 2^11 to
+// 2^15 where a row's largest is, so that fp16 holds those down to 2^-25 of it in full
+// (2^-14 with the largest at 1) and what lies below is off by 2^-36 of it. Over a long
+// history many small weights add up to what one large one leaves. (The slack shrinks
+// from 2^8 to 2^4: fp16 ends at 2^16.)
+constexpr float PROB_LOG2 = 11.0f, PROB_TOP = 15.0f;
+
+HN_DEVICE void rebase_high(float mx, float c, Run& run, f32x16 (&o)[4]) {
+    if (!__any(mx * c > run.m + PROB_TOP)) return;
+    const float mnew = fmaxf(run.m, pair_max(mx) * c - PROB_LOG2);
+    const float alpha = run.m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m - mnew);
+    run.m = mnew;
+    run.nm = mnew == -INFINITY ? 0.0f : -mnew;  // m = -inf: every s is -inf (masked)
+    run.l *= alpha;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+}
+
 // The validity bits of this thread's quad keys, as 4 bits.
 HN_DEVICE uint32_t quad_bits(uint64_t w) { return (uint32_t)(w >> quad_key(threadIdx.x & 15, 0)) & 15u; }
 
@@ -329,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
             e2 = entry(t + 3);
             f16x8 pf[2];
             // half 0
-            rebase(mxa, c, run_, o);
+            rebase_high(mxa, c, run_, o);
             sb = step_a_lse(sa, c, run_.nm, run_.l, pf, st + ka_off + 32 * KROW, qf);
             {
                 float ks[Shape<NW>::KU];
@@ -351,7 +373,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
             // half 1 (on the last tile the S block of "tile t + 1" reads stale LDS; its
             // result is never used)
             const uint64_t mwn = word_of(next_count, nst);
-            rebase(mxb, c, run_, o);
+            rebase_high(mxb, c, run_, o);
             sa = step_a_lse(sb, c, run_.nm, run_.l, pf, nst + ka_off, qf);
             {
                 float4 vs = v_scales(nsb);
@@ -388,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
                 const uint8_t* st = smem + (u & 1) * STAGE;
                 uint8_t* nst = smem + ((u & 1) ^ 1) * STAGE;
                 f16x8 pf[2];
-                rebase(mxa, c, run_, o);
+                rebase_high(mxa, c, run_, o);
                 sb = step_a_lse(sa, c, run_.nm, run_.l, pf, st + ka_off + 32 * KROW, qf);
                 mxb = step_b_with(pf, st + va_off, 0, o, sb, [&](int i) __attribute__((always_inline)) {
                     if (i & 1) store_tail_k_part<NW>(tr, nst, i >> 2, (i >> 1) & 1);
@@ -401,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
                 const uint64_t mwn = word_of(tail_count(t + 1), nst);  // (past the end: unused)
                 if constexpr (MASK)
                     if (mwn != ALL_KEYS) clear_masked_v(tr, mwn);
-                rebase(mxb, c, run_, o);
+                rebase_high(mxb, c, run_, o);
                 sa = step_a_lse(sb, c, run_.nm, run_.l, pf, nst + ka_off, qf);
                 mxa = step_b_with(pf, st + va_off, 1, o, sa, [&](int i) __attribute__((always_inline)) {
                     store_tail_v_part<NW>(tr, nst, i);
@@ -669,7 +691,7 @@ __global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
             uint8_t* nst = stage(t + 1);
             const Tile g4 = tile_of(t + 4);
             f16x8 pf[2];
-            rebase(mx, c, run_, o);
+            rebase_high(mx, c, run_, o);
             f32x16 sn = step_a_lse(s, c, run_.nm, run_.l, pf, nst + ka_off, qf);
             const uint64_t mwn = word_of(g1.count, nst);
             float4 vs = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1095,7 +1117,7 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
     // P and PV of a block whose V^T operands are vf (operand 4 tt + db).
     auto finish = [&](f32x16& s, uint32_t word, const f16x8 (&vf)[8]) __attribute__((always_inline)) {
         const float mx = word != ~0u ? mask_word(s, word) : raw_max(s);
-        rebase(mx, c, run_, o);
+        rebase_high(mx, c, run_, o);
         f16x8 pf[2];
         uint32_t x8[8];
         float l0 = 0.0f, l1 = 0.0f;

@@ -343,14 +343,15 @@ int64_t hn_select_kv_blocks_workspace_size(int64_t B, int64_t H, int64_t runs, i
  * over the valid cached tokens t < kv_len of the blocks in idx[b, h, i / q_block]
  * and the valid tail keys. A list ends at its first negative entry; an entry past
  * the last block is ignored; a block that is listed twice counts twice. idx NULL:
- * every cached token (top_k, is unused). A row without a key gets zeros and -inf.
+ * every cached token (`top_k` and `is` are unused). A row without a key gets zeros and -inf.
  * What masked keys and the cache past kv_len hold (Inf and NaN included) does not
  * matter.
  *   idx: int32 [B, H, runs, top_k], runs = ceil(Lq / q_block), strides is[3] of
  *        its first three dims, the last contiguous
  *   lse: fp32 [B, Hq, Lq] contiguous
- * The other arguments, the fp16 rounding of the probabilities and V's range are
- * those of hn_attn_fp8kv. */
+ * Probabilities meet V as fp16 of 2^11 to 2^15 for a row's largest: 2^-11 relative
+ * down to 2^-25 of it, 2^-36 of it below. The other arguments and V's range are those
+ * of hn_attn_fp8kv. */
 int hn_attn_kv_blocks(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
                       const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
                       const int64_t *ss, int64_t H, int64_t cache_cap, int64_t kv_len,

@@ -403,6 +403,40 @@ def test_whole_cache_is_dense_attention(dev, Lq, kv, Lc, fmt):
     assert ((dense.to(F64) - ref[0]).abs() <= 2 * ref[2]).all()
 
 
+@pytest.mark.parametrize("Lq", [1, 20, 50, 100])
+def test_many_small_probabilities_beside_a_large_one(dev, Lq):
+    """One key of every 32 (so one for each wave and split) takes nearly all the weight and
+    holds V = 0; what the others, 2^-26 of it each, add up to is the whole output (_attend's
+    bound is relative to it). A probability below the normal fp16 range is off by up to
+    2^-25, where the largest ones, whose sum divides it, are 2^11 at least: 2^-36 a key
+    over the number of large ones, on top."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 40 + Lq)
+    H, n, gap = 2, 20000, 26 * math.log(2)
+    e4m3 = torch.float8_e4m3fn
+    cache = _cache(dev, 1, n, H, "fp8", g)
+    unit = torch.zeros(D, device=dev)
+    unit[0] = 1
+    cache["k"].copy_((torch.randn(1, n, H, D, device=dev, generator=g) * 0.05).to(e4m3))
+    cache["k"][:, ::32] = (unit * 16).to(e4m3)
+    cache["v"].copy_((torch.rand(1, n, H, D, device=dev, generator=g) + 0.5).to(e4m3))
+    cache["v"][:, ::32] = torch.zeros(D, device=dev).to(e4m3)
+    cache["k_scale"].fill_(1.0)
+    cache["v_scale"].fill_(64.0)
+    # q . K is about 16 * 16 for those keys, near 0 for the others; the scale makes it the gap
+    q = (unit * 16 + torch.randn(1, Lq, H, D, device=dev, generator=g) * 0.05).to(BF16)
+    ref = _attend(q, cache, n, None, 64, Lq, None, None, None, None, scale=gap / 256)
+    vals = _held(cache, "v")[0, :n].abs().sum(0)                       # [H, D]
+    bound = ref[2] + 2.0 ** -36 * vals / (n // 32)
+    blocks = torch.arange(-(-n // 64), dtype=torch.int32, device=dev).expand(1, H, 1, -1)
+    for idx in (None, blocks):
+        out, lse = ca.sparse_chunk_attention(q, cache, n, idx, q_block=Lq, softmax_scale=gap / 256)
+        d = (out.to(F64) - ref[0]).abs() / bound
+        print(f"[small probabilities {Lq}] {d.max().item():.3f} of the bound, output {ref[0].abs().mean():.2e}", flush=True)
+        assert d.max() <= 1
+        assert ((lse.to(F64) - ref[1]).abs() <= ref[3]).all()
+
+
 def test_offsets_past_32_bits(dev):
     """A cache of more than 2^32 bytes a tensor, read, bounded, weighed and moved at its end."""
     ca, hist, kvc = pkg_module("cache_attention"), pkg_module("kv_history"), pkg_module("fp8_kv_cache")
