@@ -1369,10 +1369,9 @@ __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
 // a tile. The MFMAs of one key block run beside the exponentials of the one before.
 // One workgroup sees every row of its keys (or, split, its share of the rows, added
 // in order afterwards), so no two add to one key and the result has one order.
-// Many rows: bound by the exponentials beside the products, 3600 queries x 24 heads over
+// Bound by the exponentials beside the products, 3600 queries x 24 heads over
 // 86400 keys 1.83 ms, 1.05 PFLOP/s (a large bf16 product reaches 1.39; one row per lane
-// column, keys in registers, took 2.64 ms). Few: by the read of the codes, 64 heads x
-// 32768 keys (293 MB), 4 rows each, 81 us, 3.6 TB/s.
+// column, keys in registers, took 2.64 ms).
 struct MassParams {
     const uint16_t* q;
     const float* lse;       // [Bq, Hq, Lq]
@@ -1389,6 +1388,7 @@ struct MassParams {
     int64_t B;
     int batches;            // query batches per cache slot
     int H, G, tiles, work, per_xcd;
+    int keys;               // of a workgroup of key_mass_few_kernel
     float scale_log2;
 };
 
@@ -1557,6 +1557,106 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
         const bool ok = !p.valid || p.valid[b * p.vs + key] != 0;
         const float before = p.prior && key < p.prior_len ? p.prior[b * p.ps0 + h * p.ps1 + key] : 0.0f;
         p.mass[(b * p.H + h) * p.kv_len + key] = ok ? before + s : before;
+    }
+}
+
+// Up to 32 rows (single tokens): they are one MFMA operand, held in registers with their
+// log-sum-exps while the keys stream past, 32 a wave at a time, without LDS or barriers;
+// a block's codes go from global memory to operands while the next block's are in flight
+// to a second set of registers. Bound by the read of the codes: 64
+// heads x 32768 keys (293 MB), 4 rows each, 61 us, 4.8 TB/s (a copy reaches 5.1), where
+// key_mass_kernel, one barrier and one short life a workgroup, took 81.
+struct MassRegs {  // key col of a 32-key block
+    uint4 y[4];    // dims 64 half ..
+    float ks, before;
+    uint32_t ok;   // valid (before: its prior mass)
+};
+
+template <int FMT>
+__global__ __launch_bounds__(256, 4) void key_mass_few_kernel(MassParams p) {
+    const int w = (int)(blockIdx.x & 7) * p.per_xcd + (int)(blockIdx.x >> 3);
+    if (w >= p.work) return;
+    const int64_t h = w % p.H;
+    const int x = w / p.H, tile = x % p.tiles;
+    const int64_t b = x / p.tiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int kv_len = (int)p.kv_len, first = tile * p.keys, last = kv_len - first < p.keys ? kv_len : first + p.keys;
+    const float c = p.scale_log2;
+    const uint8_t* const kc = p.kc + b * p.cs0 + h * p.cs2 + 64 * half;
+    const float* const scales = p.ks + b * p.ss0 + h * p.ss2;
+    const float* const prior = p.prior ? p.prior + b * p.ps0 + h * p.ps1 : nullptr;
+    float* const mass = p.mass + (b * p.H + h) * p.kv_len;
+    auto load = [&](int k0, MassRegs& r) __attribute__((always_inline)) {
+        if (k0 >= last) return;
+        const int64_t key = min(k0 + col, kv_len - 1);
+        const uint4* src = reinterpret_cast<const uint4*>(kc + key * p.cs1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.y[e] = src[e];
+        r.ks = scales[key * p.ss1];
+        r.ok = p.valid ? (uint32_t)p.valid[b * p.vs + key] : 1u;
+        r.before = prior && key < p.prior_len ? prior[key] : 0.0f;
+    };
+    int k0 = first + 32 * wave;
+    MassRegs ra, rb;
+    load(k0, ra);
+    // row col of the query heads of this head's group: its dims 64 half .., its log-sum-exp
+    bf16x8 qf[8];
+    float nl = -INFINITY;
+    {
+        const uint32_t G = (uint32_t)p.G, Lq = p.Lq > 0 ? (uint32_t)p.Lq : 1u, q0 = (uint32_t)col / G, g = col - q0 * G;
+        const uint32_t bb = q0 / Lq, i = q0 - bb * Lq;
+        const int64_t qb = b * p.batches + bb, hq = h * p.G + g;
+        const bool there = col < p.rows;
+        const float lse = there ? p.lse[(qb * p.H * p.G + hq) * p.Lq + i] : INFINITY;
+        // a row of infinite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
+        const bool counts = __builtin_fabsf(lse) != INFINITY;
+        const uint32_t keep = counts ? ~0u : 0u;
+        if (counts) nl = -lse * 1.4426950408889634f;
+        const uint16_t* src = p.q + qb * p.qs0 + i * p.qs1 + hq * p.qs2 + 64 * half;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) {
+            uint4 y = make_uint4(0u, 0u, 0u, 0u);
+            if (there) y = reinterpret_cast<const uint4*>(src)[sl];
+            qf[sl] = __builtin_bit_cast(bf16x8, make_uint4(y.x & keep, y.y & keep, y.z & keep, y.w & keep));
+        }
+    }
+    f32x16 n;  // row 8 (v / 4) + 4 half + v % 4
+#pragma unroll
+    for (int v = 0; v < 16; ++v) n[v] = __shfl(nl, 8 * (v >> 2) + 4 * half + (v & 3), 64);
+    auto block = [&](int k0, MassRegs& r) __attribute__((always_inline)) {
+        f32x16 s;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl) {
+            uint32_t d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x2 f = codes2_f32<FMT>(word(r.y[sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
+                d[e] = pack_bf16(f[0] * r.ks, f[1] * r.ks);
+            }
+            s = mfma_bf16(qf[sl], __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3])), s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            a0 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], c, n[v]));
+            a1 += __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], c, n[v + 1]));
+        }
+        const float half_sum = a0 + a1, sum = half_sum + __shfl_xor(half_sum, 32, 64);
+        // (the column of an invalid key, whatever it holds, is dropped)
+        if (half == 0 && k0 + col < last) mass[k0 + col] = r.ok != 0u ? r.before + sum : r.before;
+    };
+    while (k0 < last) {
+        load(k0 + 128, rb);
+        block(k0, ra);
+        k0 += 128;
+        if (k0 >= last) break;
+        load(k0 + 128, ra);
+        block(k0, rb);
+        k0 += 128;
     }
 }
 
@@ -1744,20 +1844,26 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     return check_launch("hn_attn_kv_blocks (combine)");
 }
 
-// Plan of the key mass: 512 keys per workgroup (KB 4: each row tile read from LDS once
-// for four key blocks), or 128 (KB 1: more waves to hide the keys' loads) where the
-// rows fit one tile, or 512 would not fill the device twice over; where even these fall short (a short cache,
-// many queries) the rows are split, each split writes its sums and a second kernel
-// adds them in order.
+// Plan of the key mass. Up to 32 rows: key_mass_few_kernel (KB 0), with as many keys a
+// workgroup as leave eight workgroups a CU, 128 to 1024. More: 512 keys per workgroup (KB
+// 4: each row tile read from LDS once for four key blocks), or 128 (KB 1) where 512 would
+// not fill the device twice over; where even these fall short (a short cache, many
+// queries) the rows are split, each split writes its sums and a second kernel adds them in
+// order.
 struct MassPlan {
-    int kb, splits;
+    int kb, splits, keys;
     int64_t tiles;
 };
 
 static MassPlan mass_plan(int64_t rows, int64_t B, int64_t H, int64_t kv_len) {
     const int64_t target = 2LL * device_cus();
-    MassPlan pl{4, 1, (kv_len + 511) / 512};
-    if (B * H * pl.tiles >= target && rows > attn::MASS_ROWS) return pl;
+    if (rows <= attn::MASS_ROWS) {
+        const int64_t steps = B * H * ((kv_len + 127) / 128) / (4 * target);
+        const int keys = 128 * (int)(steps < 1 ? 1 : steps > 8 ? 8 : steps);
+        return MassPlan{0, 1, keys, (kv_len + keys - 1) / keys};
+    }
+    MassPlan pl{4, 1, 0, (kv_len + 511) / 512};
+    if (B * H * pl.tiles >= target) return pl;
     pl.kb = 1;
     pl.tiles = (kv_len + 127) / 128;
     const int64_t work = B * H * pl.tiles;
@@ -1828,11 +1934,14 @@ extern "C" int hn_attn_key_mass(int fmt, const void* q, const int64_t* qs, int64
     p.rows_per_split = (row_tiles + splits - 1) / splits * attn::MASS_ROWS;
     const int64_t work = B * H * pl.tiles * splits;
     HN_REQUIRE(work <= 0x3fffffffLL, HN_E_ARG, "hn_attn_key_mass: too much work for one launch");
-    p.B = B; p.tiles = (int)pl.tiles; p.work = (int)work;
+    p.B = B; p.tiles = (int)pl.tiles; p.keys = pl.keys; p.work = (int)work;
     p.per_xcd = (int)((work + 7) / 8);
     const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
     hipStream_t st = (hipStream_t)stream;
-    if (fmt == HN_KV_FP8) {
+    if (pl.kb == 0) {
+        if (fmt == HN_KV_FP8) attn::key_mass_few_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(p);
+        else attn::key_mass_few_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(p);
+    } else if (fmt == HN_KV_FP8) {
         if (pl.kb == 4) attn::key_mass_kernel<HN_KV_FP8, 4><<<grid, 256, 0, st>>>(p);
         else attn::key_mass_kernel<HN_KV_FP8, 1><<<grid, 256, 0, st>>>(p);
     } else {

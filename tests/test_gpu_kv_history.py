@@ -493,6 +493,8 @@ def test_offsets_past_32_bits(dev):
     (1, 1, 33, 3, 3, 257, "fp8", 0.1, "bhsd", 0),
     (1, 1, 2000, 2, 1, 70, "int8", 0.2, "wide", 64),      # few keys, many rows: split rows
     (2, 2, 700, 3, 3, 513, "fp8", 0, "bshd", 1),
+    (1, 1, 3, 16, 8, 70001, "fp8", 0.1, "bshd", 69000),     # few rows, several steps of keys a workgroup
+    (4, 1, 4, 4, 2, 33333, "int8", 0, "bhsd", 0),           # 32 rows of four batches over one slot
     (1, 1, 0, 2, 2, 100, "fp8", 0, "bshd", 60),           # no query: the prior alone
 ])
 def test_key_mass(dev, Bq, slots, Lq, Hq, H, kv, fmt, holes, layout, prior):
