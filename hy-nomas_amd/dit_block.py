@@ -342,8 +342,8 @@ class FP8ARModel(nn.Module):
         """Euler flow updates over the denoising passes, then the cache write
         at t = 0 and the advance of the valid length (causal_ar.py:2348-2432,
         2624-2645,2852). A chunk that would not fit the cache is refused
-        before any pass runs (or, with ``evict_keep``, makes room first). In the write pass a layer whose K/V holds a
-        NaN/Inf writes nothing; the valid length then stays where it was (rows
+        before any pass runs (or, with ``evict_keep``, makes room first). In
+        the write pass a layer whose K/V holds a NaN/Inf writes nothing; the valid length then stays where it was (rows
         that other layers wrote past it are never attended) and ValueError
         names the layers (with text: the first such layer raises)."""
         if self.cache_valid_len + self.write_tokens > self.capacity and getattr(self, "evict_keep", 0):

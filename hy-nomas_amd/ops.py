@@ -837,8 +837,8 @@ def select_kv_blocks(q: torch.Tensor, bounds: torch.Tensor, kv_len: int, top_k: 
     q: bf16 [B, Lq, Hq, D], Hq a multiple of the bounds' H; bounds as
     kv_block_bounds_ writes them, [B or 1, n, H, 2, D]. Chosen are the first
     ``keep_first`` and the last ``keep_last`` blocks and those of the highest score,
-    an upper bound of the run's logits; see hn_select_kv_blocks. q_valid (bool [B or 1, >= Lq]) leaves
-    padded queries out of the score."""
+    an upper bound of the run's logits; see hn_select_kv_blocks. q_valid (bool [B or 1,
+    >= Lq]) leaves padded queries out of the score."""
     what = "select_kv_blocks"
     _check_block(block, what)
     if q.dtype != torch.bfloat16 or bounds.dtype != torch.bfloat16:

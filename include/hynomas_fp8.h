@@ -372,7 +372,8 @@ int64_t hn_attn_kv_blocks_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int6
  * that read slot b. An invalid key draws nothing (its prior stays), and so does a row
  * whose lse is infinite. prior: fp32 [B, H, prior_len <= kv_len] with strides ps[2]
  * (keys past it start at 0) or NULL with prior_len 0; lse: fp32 [Bq, Hq, Lq]
- * contiguous; mass: fp32 [B, H, kv_len] contiguous, not overlapping prior. The sums are in 32 bits, in an order that only the sizes decide.
+ * contiguous; mass: fp32 [B, H, kv_len] contiguous, not overlapping prior. The sums
+ * are in 32 bits, in an order that only the sizes decide.
  * workspace: hn_attn_key_mass_workspace_size() bytes, 16-byte aligned. */
 int hn_attn_key_mass(int fmt, const void *q, const int64_t *qs, int64_t Bq, int64_t Lq, int64_t Hq, int64_t D,
                      const float *lse, const void *kc, const int64_t *cs, const float *ks, const int64_t *ss,

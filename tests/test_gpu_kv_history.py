@@ -745,6 +745,47 @@ def test_compiled_callers_hold_the_ops(dev):
     assert all(torch.equal(a, b) for a, b in zip(eager, compiled))
 
 
+def test_layer_history_of_one_slot(dev):
+    """One history slot read by three query batches of grouped heads: lists of each batch,
+    the weight of all of them on one mass, an eviction, and a pass over what it left."""
+    hist, kvc = pkg_module("kv_history"), pkg_module("fp8_kv_cache")
+    g = _gen(dev, 61)
+    B, H, kv, L = 3, 2, 600, 70
+    cache = _cache(dev, 1, 800, H, "int8", g)
+    out = kvc.make_int8_kv_block(1, 800, H, D, device=dev)
+    h = hist.LayerHistory(cache, top_k=4, q_block=32, keep_first=1, keep_last=1, track_mass=True)
+    h.reset(cache, kv)
+    q = torch.randn(B, L, 2 * H, D, device=dev, generator=g).to(BF16)
+    k, v = (torch.randn(B, L, H, D, device=dev, generator=g).to(BF16) for _ in range(2))
+    idx = hist.select_blocks(q, h.bounds, kv, 4, q_block=32, keep_first=1, keep_last=1)
+    assert torch.equal(idx.cpu(), _select_reference(q, h.bounds, kv, 4, 64, 32, 1, 1, None))
+    ref = _attend(q, cache, kv, idx, 64, 32, k, v, None, None)
+    assert ((h.attend(q, k, v, cache, kv, False).to(F64) - ref[0]).abs() <= ref[2]).all()
+    assert h.length == kv and (h.mass == 0).all()
+    # a writing pass: its tokens are in the cache already; its queries' weight counts once committed
+    ref = _attend(q, cache, kv, None, 64, L, k, v, None, None)
+    assert ((h.attend(q, k, v, cache, kv, True).to(F64) - ref[0]).abs() <= ref[2]).all()
+    assert h.length == kv
+    h.commit(cache)
+    keys = _held(cache, "k")[0, :kv + L]
+    want = torch.zeros(H, kv + L, dtype=F64, device=dev)
+    for b in range(B):
+        for hq in range(2 * H):
+            s = q[b, :, hq].to(F64) @ keys[:, hq // 2].T * SCALE
+            want[hq // 2] += (s - ref[1][b, hq][:, None]).exp().sum(0)
+    # an exponent is off by its logit's fp32 sum, the log-sum-exp's bound and the argument's
+    # rounding; each of the rows' terms adds half a step to its sum
+    worst = (q.to(F64).abs().amax() * keys.abs().sum(-1).amax() * SCALE).item()
+    rel = 128 * 2.0 ** -24 * worst + ref[3].max().item() + 2.0 ** -22 * (1 + worst)
+    assert h.length == kv + L and h.mass.shape == (1, H, kv + L)
+    assert ((h.mass[0].to(F64) - want).abs() <= (rel + 2 * B * L * 2 * 2.0 ** -24) * want).all()
+    kept = h.evict(cache, out, kv + L, 400, keep_first=10, keep_last=L)
+    assert kept.shape == (1, H, 400) and h.length == 400 and h.mass.shape == (1, H, 400)
+    ref = _attend(q, out, 400, hist.select_blocks(q, h.bounds, 400, 4, q_block=32, keep_first=1, keep_last=1), 64, 32,
+                  k, v, None, None)
+    assert ((h.attend(q, k, v, out, 400, False).to(F64) - ref[0]).abs() <= ref[2]).all()
+
+
 # --------------------------------------------------------------------------
 # the AR model's long roll-outs
 
