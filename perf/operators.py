@@ -320,18 +320,8 @@ def _plain_evict(st, c):
     return where.masked_fill(~there, -1).int(), torch.where(there, st["mass"][bi, hi, src], 0.0)
 
 
-_modules = {}
-
-
-def _module(name):
-    """A module of the framework, imported by the first call (a program imports it once)."""
-    if name not in _modules:
-        _modules[name] = importlib.import_module("hy-nomas_amd." + name)
-    return _modules[name]
-
-
 def _own(st, c):
-    hist = _module("kv_history")
+    hist = importlib.import_module("hy-nomas_amd.kv_history")
     if c["kind"] == "bounds":
         hist.update_block_bounds(st["bounds"], st["cache"], c["start"], c["start"] + c["L"], block=c["block"],
                                  cache_valid=st["valid"])
@@ -340,9 +330,10 @@ def _own(st, c):
         return hist.select_blocks(st["q"], st["bounds"], c["kv"], c["top_k"], block=c["block"], q_block=c["q_block"],
                                   keep_first=c["first"], keep_last=c["last"])
     if c["kind"] == "sparse":
-        return _module("cache_attention").sparse_chunk_attention(
-            st["q"], st["cache"], c["kv"], st["idx"], block=c["block"], q_block=c["q_block"], k_cur=st.get("k_cur"),
-            v_cur=st.get("v_cur"), cache_valid=st["valid"], cur_valid=st.get("cur_valid"))
+        ca = importlib.import_module("hy-nomas_amd.cache_attention")
+        return ca.sparse_chunk_attention(st["q"], st["cache"], c["kv"], st["idx"], block=c["block"],
+                                         q_block=c["q_block"], k_cur=st.get("k_cur"), v_cur=st.get("v_cur"),
+                                         cache_valid=st["valid"], cur_valid=st.get("cur_valid"))
     if c["kind"] == "mass":
         return hist.key_mass(st["q"], st["lse"], st["cache"], c["kv"], prior=st["prior"], cache_valid=st["valid"])
     return hist.evict(st["cache"], st["out"], st["mass"], c["kv"], c["keep"], keep_first=c["first"],
