@@ -891,3 +891,102 @@ def test_model_refusals(dev):
             _model(dev, **kw)
     with pytest.raises(ValueError, match="evict_keep"):
         _model(dev).evict_history()
+
+
+# --------------------------------------------------------------------------
+# every kernel of the dispatch, at the sizes that reach it
+
+@pytest.mark.parametrize("B,Lq,Hq,H,kv,block,q_block,K,Lc,fmt,holes,layout,slots", [
+    (1, 1, 3, 3, 700, 64, 1, 5, 40, "int8", 0.3, "bshd", 1),        # one row a run: holes in cache and tail
+    (2, 3, 2, 2, 4097, 128, 1, 20, 70, "fp8", 0.2, "wide", 2),      # split, a ragged last block, two tail tiles
+    (2, 2, 5, 5, 20000, 64, 1, 300, 0, "int8", 0, "bhsd", 1),       # split over many tiles, one slot
+    (1, 9, 2, 2, 300, 64, 1, 3, 1, "int8", 0.95, "bshd", 1),        # hardly a key left
+    (1, 4, 1, 1, 0, 64, 1, 2, 131, "fp8", 0.4, "bshd", 1),          # the tail alone
+])
+def test_attention_of_single_rows(dev, B, Lq, Hq, H, kv, block, q_block, K, Lc, fmt, holes, layout, slots):
+    test_attention_over_listed_blocks(dev, B, Lq, Hq, H, kv, block, q_block, K, Lc, fmt, holes, layout, slots)
+
+
+@pytest.mark.parametrize("Lq,q_block", [(3, 1), (20, 20), (50, 50), (100, 100)])
+def test_attention_over_a_tail_past_31_bits(dev, Lq, q_block):
+    """Tail tokens so far apart that the rows of a head span more than 2^31 bytes: every
+    kernel (by rows a run) gives what it gives for the same tail laid out densely."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 60 + Lq)
+    H, kv, Lc, far = 2, 300, 71, 0xfffff8
+    assert (Lc * far + D) * 2 >= 1 << 31
+    cache = _cache(dev, 1, kv, H, "fp8", g)
+    q = torch.randn(1, Lq, H, D, device=dev, generator=g).to(BF16)
+    buf = torch.full(((Lc - 1) * far + 2 * H * D,), float("nan"), dtype=BF16, device=dev)
+    k_far, v_far = (buf.as_strided((1, Lc, H, D), (Lc * far, far, D, 1), i * H * D) for i in (0, 1))
+    k_far.copy_(torch.randn(1, Lc, H, D, device=dev, generator=g).to(BF16))
+    v_far.copy_(torch.randn(1, Lc, H, D, device=dev, generator=g).to(BF16))
+    k, v = k_far.contiguous(), v_far.contiguous()
+    idx = torch.tensor([4, 0, 1], dtype=torch.int32, device=dev).expand(1, H, -(-Lq // q_block), 3)
+    for u in (None, torch.rand(1, Lc, device=dev, generator=g) >= 0.3):
+        print(f"case far tail Lq={Lq} masked={u is not None}", flush=True)
+        kw = dict(q_block=q_block, cur_valid=u)
+        near = ca.sparse_chunk_attention(q, cache, kv, idx, k_cur=k, v_cur=v, **kw)
+        _check_attention(near, _attend(q, cache, kv, idx, 64, q_block, k, v, None, u), "dense tail")
+        far_ = ca.sparse_chunk_attention(q, cache, kv, idx, k_cur=k_far, v_cur=v_far, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(near, far_))
+
+
+@pytest.mark.parametrize("Lq,q_block", [(3, 1), (20, 20), (50, 50), (100, 100)])
+def test_attention_repeats_itself(dev, Lq, q_block):
+    """Splits are merged in their order: the same call gives the same bits."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 80 + Lq)
+    cache = _cache(dev, 1, 9000, 3, "int8", g)
+    q = torch.randn(1, Lq, 3, D, device=dev, generator=g).to(BF16)
+    valid = torch.rand(1, 9000, device=dev, generator=g) >= 0.1
+    idx = _lists(dev, 1, 3, -(-Lq // q_block), 141, 60, g)
+    first = ca.sparse_chunk_attention(q, cache, 9000, idx, q_block=q_block, k_cur=q, v_cur=q, cache_valid=valid)
+    for _ in range(5):
+        again = ca.sparse_chunk_attention(q, cache, 9000, idx, q_block=q_block, k_cur=q, v_cur=q, cache_valid=valid)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("Lq,Hq,H,n,q_block,top_k,first,last,gone", [
+    (1, 2, 1, 2048, 1, 64, 1, 2, 0.1),        # the last size with 8 elements a thread,
+    (1, 2, 1, 2049, 1, 64, 1, 2, 0.1),        # the first and the last with 32,
+    (2, 2, 2, 8192, 1, 300, 0, 1, 0),
+    (2, 1, 1, 8193, 1, 300, 3, 0, 0.3),       # rows read again in every pass
+    (1, 1, 1, 10001, 1, 9000, 1, 1, 0.2),     # (more places than blocks)
+    (1, 1, 1, 10001, 1, 1, 0, 0, 0),
+    (544, 2, 2, 600, 32, 30, 2, 2, 0.1),      # 17 runs: two run tiles, three stretches of blocks
+    (40, 2, 1, 2049, 8, 100, 1, 1, 0),        # many runs in the longer searches
+    (20, 1, 1, 8193, 4, 77, 0, 2, 0.05),
+])
+@pytest.mark.parametrize("ties", [False, True])
+def test_select_of_many_blocks(dev, Lq, Hq, H, n, q_block, top_k, first, last, gone, ties):
+    """ties: small whole numbers, of which many blocks have the score of the last place."""
+    print(f"case select Lq={Lq} Hq={Hq}/{H} blocks={n} q_block={q_block} k={top_k} ties={ties}", flush=True)
+    hist = pkg_module("kv_history")
+    g = _gen(dev, Lq + n + top_k)
+    if ties:
+        q = torch.randint(-1, 2, (1, Lq, Hq, D), device=dev, generator=g).to(BF16)
+        lo = torch.randint(-1, 1, (1, n, H, 1, D), device=dev, generator=g)
+        bounds = torch.cat([lo, lo + torch.randint(0, 2, (1, n, H, 1, D), device=dev, generator=g)], 3).to(BF16)
+    else:
+        q = torch.randn(1, Lq, Hq, D, device=dev, generator=g).to(BF16)
+        bounds = _random_bounds(dev, 1, n, H, g)
+    if gone:
+        no = torch.rand(1, n, device=dev, generator=g) < gone
+        bounds[:, :, :, 0] = torch.where(no[:, :, None, None], INF, bounds[:, :, :, 0])
+        bounds[:, :, :, 1] = torch.where(no[:, :, None, None], -INF, bounds[:, :, :, 1])
+    got = hist.select_blocks(q, bounds, n * 64 - 9, top_k, q_block=q_block, keep_first=first, keep_last=last)
+    # whole numbers: exact; else a 64-bit sum is off by 2^-44 of its magnitudes at most, which
+    # changes a choice only between two scores at the last place that are as close
+    assert torch.equal(got.cpu(), _select_reference(q, bounds, n * 64 - 9, top_k, 64, q_block, first, last, None))
+
+
+@pytest.mark.parametrize("Bq,slots,Lq,Hq,H,kv,fmt,holes,layout,prior", [
+    (1, 1, 33, 24, 24, 11009, "fp8", 0.1, "bshd", 11009),   # 512 keys a workgroup, a ragged last one
+    (3, 1, 40, 24, 24, 11000, "int8", 0, "bshd", 9001),     # three batches over one slot
+    (2, 2, 17, 48, 24, 5600, "int8", 0.3, "wide", 0),       # grouped heads, rows of two heads
+    (1, 1, 65, 8, 8, 40000, "fp8", 0.97, "bhsd", 700),
+])
+def test_key_mass_of_long_caches(dev, Bq, slots, Lq, Hq, H, kv, fmt, holes, layout, prior):
+    assert slots * H * -(-kv // 512) >= 2 * torch.cuda.get_device_properties(dev).multi_processor_count
+    test_key_mass(dev, Bq, slots, Lq, Hq, H, kv, fmt, holes, layout, prior)
