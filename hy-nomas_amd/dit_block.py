@@ -306,10 +306,13 @@ class FP8ARModel(nn.Module):
     @torch.no_grad()
     def evict_history(self) -> None:
         """Cut every layer's cache to ``evict_keep`` tokens a head: each moves into the
-        spare cache, and its old one is the next layer's spare."""
+        spare cache, and its old one is the next layer's spare. If a layer's history
+        refuses, none is cut."""
         keep = self.evict_keep
         if not keep:
             raise ValueError("evict_history needs evict_keep")
+        for history in self.histories:  # (a move cannot be taken back: its source is the next one's spare)
+            history.check_evict(self.cache_valid_len)
         first = min(math.prod(self.latent_shape[1:]), keep // 4)
         last = min(self.write_tokens, keep // 2)
         for i, history in enumerate(self.histories):

@@ -179,14 +179,19 @@ class LayerHistory:
         """The last writing pass was refused: nothing of it counts."""
         self._written = None
 
-    def evict(self, cache: dict, out: dict, kv_len: int, keep: int, *, keep_first: int = 0,
-              keep_last: int = 0) -> torch.Tensor:
-        """Keep ``keep`` tokens of every head in ``out`` (kv_history.evict by this layer's
-        mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
+    def check_evict(self, kv_len: int) -> None:
+        """ValueError if ``evict`` would refuse these tokens: for a model that cuts all of
+        its layers or none."""
         if not self.track_mass or self.mass is None:
             raise ValueError("eviction needs the mass of the cached tokens (track_mass)")
         if kv_len != self.length:
             raise ValueError(f"the history accounts for {self.length} tokens, not {kv_len}")
+
+    def evict(self, cache: dict, out: dict, kv_len: int, keep: int, *, keep_first: int = 0,
+              keep_last: int = 0) -> torch.Tensor:
+        """Keep ``keep`` tokens of every head in ``out`` (kv_history.evict by this layer's
+        mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
+        self.check_evict(kv_len)
         idx, mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
         self.length, self._written = min(keep, kv_len), None
         self.mass = mass[:, :, :self.length]

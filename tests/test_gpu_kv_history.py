@@ -990,3 +990,28 @@ def test_select_of_many_blocks(dev, Lq, Hq, H, n, q_block, top_k, first, last, g
 def test_key_mass_of_long_caches(dev, Bq, slots, Lq, Hq, H, kv, fmt, holes, layout, prior):
     assert slots * H * -(-kv // 512) >= 2 * torch.cuda.get_device_properties(dev).multi_processor_count
     test_key_mass(dev, Bq, slots, Lq, Hq, H, kv, fmt, holes, layout, prior)
+
+
+def test_model_cuts_every_layer_or_none(dev):
+    """A layer that cannot be cut (its mass is of other tokens, or missing) leaves the
+    layers before it as they were; put right, the roll-out goes on."""
+    m = _model(dev, sparse_top_k=3, evict_keep=300)
+    for i in range(4):
+        m.generate_chunk(*_chunk(dev, i))
+    caches, spare = list(m.caches), m.spare
+    held = [{n: t.clone() for n, t in c.items()} for c in caches]
+    mass, bounds = [h.mass.clone() for h in m.histories], [h.bounds.clone() for h in m.histories]
+    last = m.histories[-1]
+    whole = (last.length, last.mass)
+    for spoiled, message in (((500, last.mass), "accounts for 500 tokens, not 512"), ((512, None), "needs the mass")):
+        last.length, last.mass = spoiled
+        for call in (m.evict_history, lambda: m.generate_chunk(*_chunk(dev, 4))):
+            with pytest.raises(ValueError, match=message):
+                call()
+        last.length, last.mass = whole
+        assert m.cache_valid_len == 512 and m.spare is spare and all(a is b for a, b in zip(m.caches, caches))
+        for c, old in zip(m.caches, held):
+            assert all(torch.equal(c[n].view(torch.uint8), old[n].view(torch.uint8)) for n in old)
+        for h, w, b in zip(m.histories, mass, bounds):
+            assert h.length == 512 and torch.equal(h.mass, w) and torch.equal(h.bounds, b)
+    assert torch.isfinite(m.generate_chunk(*_chunk(dev, 4)).float()).all() and m.cache_valid_len == 300 + 128

@@ -296,3 +296,25 @@ def test_model_refusals():
     block = dit.FP8DiTBlock.__new__(dit.FP8DiTBlock)
     with pytest.raises(ValueError, match="image-only"):
         dit.FP8DiTBlock.forward(block, None, None, None, None, cache, 0, txt=1, history=h)
+
+
+def test_model_looks_at_every_layer_before_it_cuts_one():
+    """(with caches on the CPU, the first move would be refused there)"""
+    dit, hist = pkg_module("dit_block"), pkg_module("kv_history")
+    kvc = pkg_module("fp8_kv_cache")
+    m = dit.FP8ARModel.__new__(dit.FP8ARModel)
+    m.evict_keep, m.latent_shape, m.write_tokens, m.cache_valid_len = 32, (1, 4, 8), 32, 64
+    m.caches = [kvc.make_fp8_kv_block(1, 96, 2, 128, device="cpu") for _ in range(3)]
+    m.spare = kvc.make_fp8_kv_block(1, 96, 2, 128, device="cpu")
+    m.histories = [hist.LayerHistory(c, track_mass=True) for c in m.caches]
+    for h in m.histories:
+        h.mass, h.length = torch.ones(1, 2, 64), 64
+    m.histories[2].length = 60
+    with pytest.raises(ValueError, match="accounts for 60 tokens, not 64"):
+        m.evict_history()
+    m.histories[2].length, m.histories[1].mass = 64, None
+    with pytest.raises(ValueError, match="needs the mass"):
+        m.evict_history()
+    m.histories[1].mass = torch.ones(1, 2, 64)
+    with pytest.raises(RuntimeError, match="GPU"):
+        m.evict_history()
