@@ -345,17 +345,22 @@ class FP8ARModel(nn.Module):
         """Euler flow updates over the denoising passes, then the cache write
         at t = 0 and the advance of the valid length (causal_ar.py:2348-2432,
         2624-2645,2852). A chunk that would not fit the cache is refused
-        before any pass runs (or, with ``evict_keep``, makes room first). In
-        the write pass a layer whose K/V holds a NaN/Inf writes nothing; the valid length then stays where it was (rows
-        that other layers wrote past it are never attended) and ValueError
-        names the layers (with text: the first such layer raises)."""
+        before any pass runs (or, with ``evict_keep``, makes room first, once
+        the schedule and the noise's shape have been looked at). In the write
+        pass a layer whose K/V holds a NaN/Inf writes nothing; the valid length
+        then stays where it was (rows that other layers wrote past it are never
+        attended) and ValueError names the layers (with text: the first such
+        layer raises)."""
+        if len(sigmas) != len(vecs_denoise) + 1:
+            raise ValueError("sigmas must hold one more value than the denoising passes")
         if self.cache_valid_len + self.write_tokens > self.capacity and getattr(self, "evict_keep", 0):
+            want = (1, self.tokens_per_chunk, self.heads * self.head_dim)
+            if tuple(noise.shape) != want:  # (the passes would refuse it, but the history would be cut by then)
+                raise ValueError(f"noise must be {list(want)}, got {list(noise.shape)}")
             self.evict_history()
         if self.cache_valid_len + self.write_tokens > self.capacity:
             raise ValueError(f"KV cache full: {self.cache_valid_len} + {self.write_tokens} tokens "
                              f"exceed the capacity {self.capacity}")
-        if len(sigmas) != len(vecs_denoise) + 1:
-            raise ValueError("sigmas must hold one more value than the denoising passes")
         x = noise
         for i, vec in enumerate(vecs_denoise):
             v_pred = self.forward_chunk(x, vec, False, txt, vec_txt, text_mask)

@@ -1015,3 +1015,20 @@ def test_model_cuts_every_layer_or_none(dev):
         for h, w, b in zip(m.histories, mass, bounds):
             assert h.length == 512 and torch.equal(h.mass, w) and torch.equal(h.bounds, b)
     assert torch.isfinite(m.generate_chunk(*_chunk(dev, 4)).float()).all() and m.cache_valid_len == 300 + 128
+
+
+def test_model_keeps_the_history_of_a_refused_call(dev):
+    """Arguments are looked at before a full cache is cut."""
+    m = _model(dev, evict_keep=300)
+    for i in range(4):
+        m.generate_chunk(*_chunk(dev, i))
+    caches, mass = list(m.caches), [h.mass.clone() for h in m.histories]
+    noise, vecs, vec, sigmas = _chunk(dev, 4)
+    for args, message in (((noise, vecs, vec, sigmas[:-1]), "sigmas"), ((noise[:, :100], vecs, vec, sigmas), "noise"),
+                          ((noise[..., :128], vecs, vec, sigmas), "noise")):
+        with pytest.raises(ValueError, match=message):
+            m.generate_chunk(*args)
+        assert m.cache_valid_len == 512 and all(a is b for a, b in zip(m.caches, caches))
+        assert all(h.length == 512 and torch.equal(h.mass, w) for h, w in zip(m.histories, mass))
+    m.generate_chunk(noise, vecs, vec, sigmas)
+    assert m.cache_valid_len == 300 + 128

@@ -318,3 +318,22 @@ def test_model_looks_at_every_layer_before_it_cuts_one():
     m.histories[1].mass = torch.ones(1, 2, 64)
     with pytest.raises(RuntimeError, match="GPU"):
         m.evict_history()
+
+
+def test_model_looks_at_the_schedule_before_it_cuts():
+    dit = pkg_module("dit_block")
+    m = dit.FP8ARModel.__new__(dit.FP8ARModel)
+    m.cache_valid_len, m.tokens_per_chunk, m.write_tokens, m.capacity, m.evict_keep = 20, 10, 10, 25, 8
+    m.heads, m.head_dim = 2, 128
+    cut = []
+    m.evict_history = lambda: cut.append(1)
+    noise = torch.zeros(1, 10, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="sigmas"):
+        m.generate_chunk(noise, [None], None, [1.0])
+    for bad in (noise[:, :9], noise[..., :128], noise[0], noise.expand(2, -1, -1)):
+        with pytest.raises(ValueError, match="noise"):
+            m.generate_chunk(bad, [], None, [1.0])
+    assert not cut
+    with pytest.raises(ValueError, match="capacity"):     # (this stub makes no room)
+        m.generate_chunk(noise, [], None, [1.0])
+    assert cut == [1]
