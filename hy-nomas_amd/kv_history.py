@@ -190,9 +190,14 @@ class LayerHistory:
     def evict(self, cache: dict, out: dict, kv_len: int, keep: int, *, keep_first: int = 0,
               keep_last: int = 0) -> torch.Tensor:
         """Keep ``keep`` tokens of every head in ``out`` (kv_history.evict by this layer's
-        mass), whose bounds and mass take the old ones' place. Returns the kept tokens."""
+        mass), whose bounds and mass take the old ones' place; ``out`` may be of another
+        capacity. Returns the kept tokens."""
         self.check_evict(kv_len)
+        bounds = self.bounds
+        if bounds is not None and bounds.shape[1] != -(-out["k"].shape[1] // self.block):
+            bounds = make_block_bounds(out, block=self.block)
         idx, mass = evict(cache, out, self.mass, kv_len, keep, keep_first=keep_first, keep_last=keep_last)
+        self.bounds = bounds
         self.length, self._written = min(keep, kv_len), None
         self.mass = mass[:, :, :self.length]
         if self.bounds is not None:

@@ -1032,3 +1032,36 @@ def test_model_keeps_the_history_of_a_refused_call(dev):
         assert all(h.length == 512 and torch.equal(h.mass, w) for h, w in zip(m.histories, mass))
     m.generate_chunk(noise, vecs, vec, sigmas)
     assert m.cache_valid_len == 300 + 128
+
+
+@pytest.mark.parametrize("cap", [140, 2000])
+def test_layer_history_moves_to_a_cache_of_another_size(dev, cap):
+    """After an eviction into a smaller or larger cache the bounds are that cache's: the
+    roll-out goes on to its end."""
+    hist, kvc = pkg_module("kv_history"), pkg_module("fp8_kv_cache")
+    g = _gen(dev, cap)
+    H, L = 2, 100
+    cache, out = kvc.make_fp8_kv_block(1, 300, H, D, device=dev), kvc.make_fp8_kv_block(1, cap, H, D, device=dev)
+    h = hist.LayerHistory(cache, top_k=3, q_block=32, keep_first=1, keep_last=1, track_mass=True)
+
+    def write(c, kv):
+        q, k, v = (torch.randn(1, L, H, D, device=dev, generator=g).to(BF16) for _ in range(3))
+        kvc.quantize_kv_pair_into(c, k, v, kv)
+        h.attend(q, k, v, c, kv, True)
+        h.commit(c)
+
+    for kv in range(0, 300, L):
+        write(cache, kv)
+    h.evict(cache, out, 300, 40)
+    for kv in range(40, cap - L + 1, L):
+        write(out, kv)
+    end = h.length
+    assert end == 40 + (cap - 40) // L * L and h.mass.shape == (1, H, end)
+    ref = hist.make_block_bounds(out)
+    hist.update_block_bounds(ref, out, 0, end)
+    assert torch.equal(h.bounds, ref)
+    q, k, v = (torch.randn(1, L, H, D, device=dev, generator=g).to(BF16) for _ in range(3))
+    idx = hist.select_blocks(q, ref, end, 3, q_block=32, keep_first=1, keep_last=1) if end > 192 else None
+    ref = _attend(q, out, end, idx, 64, 32 if idx is not None else 128, k, v, None, None)
+    # (read whole, the dense attention answers, whose probabilities are fp16 as well)
+    assert ((h.attend(q, k, v, out, end, False).to(F64) - ref[0]).abs() <= 2 * ref[2]).all()
