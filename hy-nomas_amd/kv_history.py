@@ -164,16 +164,16 @@ class LayerHistory:
         return chunk_attention(q, cache, kv_len, k_cur=k, v_cur=v)
 
     def commit(self, cache: dict) -> None:
-        """The last writing pass stands: its mass, and the bounds of what it wrote."""
+        """The last writing pass stands: its mass, and the bounds of what it wrote. If the
+        bounds cannot be made, nothing has changed and the pass still waits."""
         if self._written is None:
             return
         mass, start, end = self._written
-        self._written = None
-        if self.track_mass:
-            self.mass = mass
         if self.bounds is not None:
             update_block_bounds(self.bounds, cache, start, end, block=self.block)
-        self.length = end
+        if self.track_mass:
+            self.mass = mass
+        self.length, self._written = end, None
 
     def rollback(self) -> None:
         """The last writing pass was refused: nothing of it counts."""

@@ -337,3 +337,20 @@ def test_model_looks_at_the_schedule_before_it_cuts():
     with pytest.raises(ValueError, match="capacity"):     # (this stub makes no room)
         m.generate_chunk(noise, [], None, [1.0])
     assert cut == [1]
+
+
+def test_layer_history_commit_counts_all_of_a_pass_or_nothing():
+    """A commit whose bounds cannot be brought up to date (here: of a cache that is not on
+    the GPU) leaves the history as it was, and can be called again."""
+    hist, kvc = pkg_module("kv_history"), pkg_module("fp8_kv_cache")
+    cache = kvc.make_fp8_kv_block(1, 256, 2, 128, device="cpu")
+    h = hist.LayerHistory(cache, top_k=4, track_mass=True)
+    old, new = torch.ones(1, 2, 64), torch.ones(1, 2, 96)
+    h.mass, h.length, h._written = old, 64, (new, 64, 96)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="GPU"):
+            h.commit(cache)
+        assert h.mass is old and h.length == 64 and h._written[0] is new
+    h.rollback()
+    h.commit(cache)
+    assert h.mass is old and h.length == 64
