@@ -133,7 +133,7 @@ class LayerHistory:
         if self.bounds is not None and kv_len:
             update_block_bounds(self.bounds, cache, 0, kv_len, block=self.block)
         codes = cache["k"]
-        self.mass = (torch.zeros((codes.shape[0], codes.shape[2], kv_len), device=codes.device)
+        self.mass = (torch.zeros((codes.shape[0], codes.shape[2], kv_len), dtype=torch.float32, device=codes.device)
                      if self.track_mass and kv_len else None)
         self.length, self._written = kv_len, None
 

@@ -354,3 +354,15 @@ def test_layer_history_commit_counts_all_of_a_pass_or_nothing():
     h.rollback()
     h.commit(cache)
     assert h.mass is old and h.length == 64
+
+
+def test_layer_history_mass_is_fp32_whatever_the_default():
+    hist, kvc = pkg_module("kv_history"), pkg_module("fp8_kv_cache")
+    h = hist.LayerHistory(kvc.make_fp8_kv_block(1, 64, 2, 128, device="cpu"), track_mass=True)
+    for dtype in (torch.bfloat16, torch.float64):
+        torch.set_default_dtype(dtype)
+        try:
+            h.reset(kvc.make_fp8_kv_block(1, 64, 2, 128, device="cpu"), 10)
+        finally:
+            torch.set_default_dtype(torch.float32)
+        assert h.mass.dtype == torch.float32 and h.mass.shape == (1, 2, 10)
