@@ -79,7 +79,7 @@ def sparse_chunk_attention(q: torch.Tensor, kv_cache: dict, kv_len: int, block_i
     ended by the first negative entry; None reads the whole cache. Hq may be a
     multiple of the cache's heads. Every listed key is visible to the run's queries;
     cache_valid and cur_valid are as in chunk_attention. A query without a key gets
-    a zero row and lse -inf.
+    a zero row and lse -inf, one that meets a NaN gets NaN in both.
     """
     if not is_quantized_kv_cache(kv_cache):
         raise TypeError("sparse_chunk_attention reads FP8/INT8 caches")

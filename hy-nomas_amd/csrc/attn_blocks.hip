@@ -20,11 +20,13 @@ namespace attn {
 // head's group. The part of a tile past kv_len, an entry past the last block and
 // invalid keys are masked by the tile's 64-bit word; the V codes and scales of
 // masked keys enter LDS as zeros, so that nothing they hold (an unwritten row, an
-// Inf or NaN) meets a zero probability. Bound by the vector work (dequantization,
-// exponentials) beside the products and by waits at the two barriers a tile: 10800
-// queries x 24 heads, runs of 128, over 128 of 1350 random blocks and a 10800-token tail
-// 3.07-3.2 ms, 0.79-0.82 PFLOP/s; the same list for every run is 10 % faster (L2), the
-// tail alone runs at 0.89, dense attention of 8 waves at 0.95-1.0.
+// Inf or NaN) meets a zero probability. The denominator is 0 only for a row without a
+// key; a NaN that a row meets stays in it, and so in output and log-sum-exp. Bound by
+// the vector work (dequantization, exponentials) beside the products and by waits at
+// the two barriers a tile: 10800 queries x 24 heads, runs of 128, over 128 of 1350
+// random blocks and a 10800-token tail 3.07-3.2 ms, 0.79-0.82 PFLOP/s; the same list
+// for every run is 10 % faster (L2), the tail alone runs at 0.89, dense attention of 8
+// waves at 0.95-1.0.
 struct BlockParams : Params {
     const int32_t* idx;    // null: all blocks
     int64_t is0, is1, is2;
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
         if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
         return;
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     uint16_t* dst = p.out + b * p.os0 + qi * p.os1 + hq * p.os2;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
                 make_uint2(pack_bf16(o[db][vq * 4] * inv, o[db][vq * 4 + 1] * inv),
                            pack_bf16(o[db][vq * 4 + 2] * inv, o[db][vq * 4 + 3] * inv));
         }
-    if (half == 0) p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+    if (half == 0) p.lse[at] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -758,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
     m = top;
     const int64_t hqs = p.H * p.G, at = (b * hqs + hq) * p.Lq + qi;
     const int64_t slot = (int64_t)split * p.B * hqs * p.Lq + at;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     uint16_t* dst = p.out + b * p.os0 + qi * p.os1 + hq * p.os2;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
@@ -773,7 +775,7 @@ __global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
         }
     if (half != 0) return;
     if (p.splits > 1) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
-    else p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+    else p.lse[at] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -985,8 +987,8 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
         p.ws_o[part * D + d] = v;
         if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, l);
     } else {
-        p.out[b * p.os0 + i * p.os1 + h * p.os2 + d] = (uint16_t)f32_to_bf16_bits(l > 0.0f ? v / l : 0.0f);
-        if (d == 0) p.lse[slot] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+        p.out[b * p.os0 + i * p.os1 + h * p.os2 + d] = (uint16_t)f32_to_bf16_bits(l != 0.0f ? v / l : 0.0f);
+        if (d == 0) p.lse[slot] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
     }
 }
 
@@ -1308,10 +1310,10 @@ __global__ __launch_bounds__(256, 2) void attn_waves_kernel(BlockParams p) {
             *reinterpret_cast<float4*>(p.ws_o + part * D + d) = num;
             if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, den);
         } else {
-            const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+            const float inv = den != 0.0f ? 1.0f / den : 0.0f;
             *reinterpret_cast<uint2*>(p.out + b * p.os0 + i * p.os1 + hq * p.os2 + d) =
                 make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
-            if (d == 0) p.lse[slot] = den > 0.0f ? (m + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+            if (d == 0) p.lse[slot] = den != 0.0f ? (m + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
         }
     }
 }
@@ -1355,10 +1357,10 @@ __global__ __launch_bounds__(256) void blocks_combine_kernel(BlockParams p) {
         }
     }
     const uint32_t bh = r / (uint32_t)p.Lq, i = r - bh * (uint32_t)p.Lq, b = bh / (uint32_t)hqs, hq = bh - b * (uint32_t)hqs;
-    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
     *reinterpret_cast<uint2*>(p.out + b * p.os0 + i * p.os1 + hq * p.os2 + d) =
         make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
-    if (d == 0) p.lse[r] = den > 0.0f ? (M + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+    if (d == 0) p.lse[r] = den != 0.0f ? (M + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -1499,8 +1501,8 @@ __global__ __launch_bounds__(256, 2) void key_mass_kernel(MassParams p) {
 
     auto put = [&](int buf) {
         uint4* dst = reinterpret_cast<uint4*>(smem + buf * MASS_TILE + tr * KROW + 32 * tu);
-        // a row of infinite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
-        const bool counts = __builtin_fabsf(lse) != INFINITY;
+        // a row without a finite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
+        const bool counts = __builtin_fabsf(lse) < INFINITY;
         const uint32_t keep = counts ? ~0u : 0u;
         dst[0] = make_uint4(x0.x & keep, x0.y & keep, x0.z & keep, x0.w & keep);
         dst[1] = make_uint4(x1.x & keep, x1.y & keep, x1.z & keep, x1.w & keep);
@@ -1609,8 +1611,8 @@ __global__ __launch_bounds__(256, 4) void key_mass_few_kernel(MassParams p) {
         const int64_t qb = b * p.batches + bb, hq = h * p.G + g;
         const bool there = col < p.rows;
         const float lse = there ? p.lse[(qb * p.H * p.G + hq) * p.Lq + i] : INFINITY;
-        // a row of infinite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
-        const bool counts = __builtin_fabsf(lse) != INFINITY;
+        // a row without a finite log-sum-exp adds nothing, whatever it holds: exp2(0 - inf) = 0
+        const bool counts = __builtin_fabsf(lse) < INFINITY;
         const uint32_t keep = counts ? ~0u : 0u;
         if (counts) nl = -lse * 1.4426950408889634f;
         const uint16_t* src = p.q + qb * p.qs0 + i * p.qs1 + hq * p.qs2 + 64 * half;

@@ -989,7 +989,8 @@ def attn_key_mass(q: torch.Tensor, lse: torch.Tensor, k_codes: torch.Tensor, k_s
     kv_len], keys past it start at 0): a new fp32 [B, H, kv_len].
 
     A cache of one slot (B = 1) collects the weight of every query batch. Invalid
-    keys (cache_valid bool [B or 1, >= kv_len]) and rows of infinite lse add nothing."""
+    keys (cache_valid bool [B or 1, >= kv_len]) draw nothing, rows of infinite or NaN lse
+    give nothing."""
     what = "attn_key_mass"
     if q.dtype != torch.bfloat16 or lse.dtype != torch.float32:
         raise TypeError(f"{what} expects bf16 queries and fp32 log-sum-exps")

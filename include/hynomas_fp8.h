@@ -343,7 +343,8 @@ int64_t hn_select_kv_blocks_workspace_size(int64_t B, int64_t H, int64_t runs, i
  * over the valid cached tokens t < kv_len of the blocks in idx[b, h, i / q_block]
  * and the valid tail keys. A list ends at its first negative entry; an entry past
  * the last block is ignored; a block that is listed twice counts twice. idx NULL:
- * every cached token (`top_k` and `is` are unused). A row without a key gets zeros and -inf.
+ * every cached token (`top_k` and `is` are unused). A row without a key gets zeros and -inf,
+ * a row that meets a NaN gets NaN in both.
  * What masked keys and the cache past kv_len hold (Inf and NaN included) does not
  * matter.
  *   idx: int32 [B, H, runs, top_k], runs = ceil(Lq / q_block), strides is[3] of
@@ -369,10 +370,10 @@ int64_t hn_attn_kv_blocks_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int6
 /* The attention weight that every cached key draws:
  *   mass[b, h, t] = prior[b, h, t] + sum over rows of exp(softmax_scale q . K(t) - lse(row))
  * for t < kv_len, over the Lq queries and G query heads of the Bq / B query batches
- * that read slot b. An invalid key draws nothing (its prior stays), and so does a row
- * whose lse is infinite. prior: fp32 [B, H, prior_len <= kv_len] with strides ps[2]
- * (keys past it start at 0) or NULL with prior_len 0; lse: fp32 [Bq, Hq, Lq]
- * contiguous; mass: fp32 [B, H, kv_len] contiguous, not overlapping prior. The sums
+ * that read slot b. An invalid key draws nothing (its prior stays); a row whose lse is
+ * infinite (no key) or NaN gives nothing. prior: fp32 [B, H, prior_len <= kv_len] with
+ * strides ps[2] (keys past it start at 0) or NULL with prior_len 0; lse: fp32 [Bq, Hq,
+ * Lq] contiguous; mass: fp32 [B, H, kv_len] contiguous, not overlapping prior. The sums
  * are in 32 bits, in an order that only the sizes decide.
  * workspace: hn_attn_key_mass_workspace_size() bytes, 16-byte aligned. */
 int hn_attn_key_mass(int fmt, const void *q, const int64_t *qs, int64_t Bq, int64_t Lq, int64_t Hq, int64_t D,

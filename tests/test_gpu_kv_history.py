@@ -1065,3 +1065,33 @@ def test_layer_history_moves_to_a_cache_of_another_size(dev, cap):
     ref = _attend(q, out, end, idx, 64, 32 if idx is not None else 128, k, v, None, None)
     # (read whole, the dense attention answers, whose probabilities are fp16 as well)
     assert ((h.attend(q, k, v, out, end, False).to(F64) - ref[0]).abs() <= 2 * ref[2]).all()
+
+
+@pytest.mark.parametrize("kv", [500, 20000])               # without and with key splits
+@pytest.mark.parametrize("Lq,q_block", [(4, 1), (20, 20), (50, 50), (100, 100)])
+def test_attention_of_nan_rows(dev, Lq, q_block, kv):
+    """A query row that meets a NaN gets NaN in its output and its log-sum-exp (zeros and
+    -inf say that it had no key); the other rows are what they were."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 90 + Lq)
+    cache = _cache(dev, 1, kv, 2, "fp8", g)
+    q = torch.randn(1, Lq, 2, D, device=dev, generator=g).to(BF16)
+    n = -(-kv // 64)
+    idx = torch.arange(n, dtype=torch.int32, device=dev).expand(1, 2, -(-Lq // q_block), n)
+    ref = _attend(q, cache, kv, idx, 64, q_block, None, None, None, None)
+    bad = q.clone()
+    bad[0, 1, 0, 5] = float("nan")
+    bad[0, 2, 1, 7] = INF                                  # logits of both signs: inf - inf
+    no = torch.zeros(1, 2, Lq, dtype=torch.bool, device=dev)
+    no[0, 0, 1] = no[0, 1, 2] = True
+    for lists in (idx, None):
+        out, lse = ca.sparse_chunk_attention(bad, cache, kv, lists, q_block=q_block)
+        assert torch.equal(torch.isnan(lse), no)
+        assert torch.equal(torch.isnan(out).transpose(1, 2), no[..., None].expand(-1, -1, -1, D))
+        yes = ~no
+        assert ((out.transpose(1, 2)[yes].to(F64) - ref[0].transpose(1, 2)[yes]).abs() <= ref[2].transpose(1, 2)[yes]).all()
+        assert ((lse[yes].to(F64) - ref[1][yes]).abs() <= ref[3][yes]).all()
+        hist = pkg_module("kv_history")                    # such a row adds nothing to a mass
+        gone, without = q.clone(), torch.where(no, -INF, lse)
+        gone[0, 1, 0] = gone[0, 2, 1] = 0
+        assert torch.equal(hist.key_mass(bad, lse, cache, kv), hist.key_mass(gone, without, cache, kv))
