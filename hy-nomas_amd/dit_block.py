@@ -265,6 +265,10 @@ class FP8ARModel(nn.Module):
     most (its first latent frame and its newest chunk always, as far as they fit),
     instead of refusing the chunk."""
 
+    # a model that reads and keeps all of its history
+    evict_keep = 0
+    histories = spare = None
+
     def __init__(self, depth: int = 40, hidden: int = 3072, heads: int = 24,
                  latent_shape=(3, 45, 80), max_chunks: int = 17, *, device=None, seed: int = 0,
                  text_len: int = 0, sparse_top_k: int = 0, evict_keep: int = 0):
@@ -294,14 +298,13 @@ class FP8ARModel(nn.Module):
             raise ValueError("sparse_top_k and evict_keep apply to image-only chunks")
         if not 0 <= self.evict_keep <= self.capacity - self.write_tokens:
             raise ValueError(f"evict_keep leaves no room for a chunk's {self.write_tokens} tokens")
-        self.histories = None
         if sparse_top_k or evict_keep:
             self.histories = [LayerHistory(c, top_k=int(sparse_top_k), keep_first=min(1, int(sparse_top_k)),
                                            keep_last=min(2, max(0, int(sparse_top_k) - 1)),
                                            track_mass=self.evict_keep > 0) for c in self.caches]
         # the cache that the next layer to be cut moves into
-        self.spare = (make_fp8_kv_block(1, self.capacity, heads, self.head_dim, device=device)
-                      if self.evict_keep else None)
+        if self.evict_keep:
+            self.spare = make_fp8_kv_block(1, self.capacity, heads, self.head_dim, device=device)
 
     @torch.no_grad()
     def evict_history(self) -> None:
@@ -353,7 +356,7 @@ class FP8ARModel(nn.Module):
         layer raises)."""
         if len(sigmas) != len(vecs_denoise) + 1:
             raise ValueError("sigmas must hold one more value than the denoising passes")
-        if self.cache_valid_len + self.write_tokens > self.capacity and getattr(self, "evict_keep", 0):
+        if self.cache_valid_len + self.write_tokens > self.capacity and self.evict_keep:
             want = (1, self.tokens_per_chunk, self.heads * self.head_dim)
             if tuple(noise.shape) != want:  # (the passes would refuse it, but the history would be cut by then)
                 raise ValueError(f"noise must be {list(want)}, got {list(noise.shape)}")
