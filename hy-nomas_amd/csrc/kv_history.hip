@@ -3,8 +3,8 @@
 //   * the choice of the blocks that a run of queries reads, by those bounds
 //   * the choice of the tokens that stay when the cache is cut, by their mass
 //   * the move of the kept tokens into another cache
-// All stream their operands once or choose among scores that are exact, so that
-// the chosen indices do not depend on the order of a sum.
+// All stream their operands once; sums have a fixed order, so that the same call gives
+// the same indices.
 #include "hn_capi_internal.h"
 #include "hn_common.h"
 
@@ -144,10 +144,12 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
 // cached head) W_d = sum min(q_d, 0), U_d = sum max(q_d, 0), and
 //   score_j = sum_d W_d lo_jd + U_d hi_jd
 // bounds the sum of the run's logits with any key of block j. Sums and products
-// are in 64 bits: a sum of bf16 values spans far fewer than 53 bits, and so does
-// its product with an 8-bit bound, so the score is exact whatever the order of
-// its terms (as long as the run's values lie within 2^20 or so of one another)
-// and is rounded once, to fp32, to be ranked.
+// are in 64 bits and the score is rounded once, to fp32, to be ranked. Where the
+// queries' sums (from the highest bit of the largest to the lowest bit of any value in
+// them) and the bounds (likewise) span 45 bits together, the 256 products add up exactly,
+// whatever their order (values near 1: about 40). Past that a score is off by up to (rows
+// + 257) 2^-53 of its terms' magnitudes, in an order that is each kernel's own: the
+// kernels for few and for many runs may rank scores apart that differ by no more.
 
 struct PoolArgs {
     const uint16_t* q;

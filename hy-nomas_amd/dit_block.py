@@ -262,8 +262,9 @@ class FP8ARModel(nn.Module):
     ``sparse_top_k`` > 0 lets the denoising passes read that many 64-token blocks of
     a longer history instead of all of it, and ``evict_keep`` > 0 cuts a full cache
     to that many tokens of each head, those that the writing passes' queries weighed
-    most (its first latent frame and its newest chunk always, as far as they fit),
-    instead of refusing the chunk."""
+    most, instead of refusing the chunk. Kept whatever their weight are the first latent
+    frame, up to a quarter of ``evict_keep`` (its first tokens), and the newest chunk, up
+    to half (its last): the rest is always left to the mass."""
 
     # a model that reads and keeps all of its history
     evict_keep = 0

@@ -22,8 +22,8 @@ both work on the FP8/INT8 cache of fp8_kv_cache.py in place:
       one layer's bounds and mass, and the attention of its passes over them: what
       dit_block.FP8ARModel keeps per layer when it reads or cuts a long history
 
-The choices are exact (scores in 64 bits, ties to the lowest index): the same
-inputs give the same blocks and tokens.
+Scores are formed in 64 bits and rounded once to fp32, ties go to the lowest index:
+the same call gives the same blocks and tokens.
 """
 from __future__ import annotations
 

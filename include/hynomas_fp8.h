@@ -216,8 +216,9 @@ int hn_gemm_fp8_blockwise(const void *a, const void *b, const float *sa, const f
  * Range: V (cached values bf16(code * scale) and the bf16 tail) is held as
  * fp16, converted toward zero, so a V value of magnitude above 65504 enters
  * the product as +-65504 (the reference attends the bf16 value); every other
- * bf16 V value is exact in fp16 down to 2^-24. A cached V exceeds 65504 only
- * when the written row held such a value (|bf16(code * s)| <= amax).
+ * bf16 V value is exact in fp16 down to 2^-17 (below, a multiple of 2^-24). A
+ * cached V exceeds 65504 only when the written row held such a value
+ * (|bf16(code * s)| <= amax).
  * workspace: device scratch of at least hn_attn_fp8kv_workspace_size(...)
  *        bytes (16-byte aligned; NULL/0 when that size is 0). It holds per-split
  *        partial results when the key range is split across workgroups to fill
@@ -320,8 +321,8 @@ int hn_kv_block_bounds(int fmt, const void *kc, const int64_t *cs, const float *
  * run's queries (q_valid[b * q_valid_stride + i] != 0; NULL: all) and the G query
  * heads of a cached head, a block's score
  *   sum_d W_d lo_d + U_d hi_d  >=  sum over the run's rows of q . K(t), any t in it,
- * is formed in 64 bits (exact for values of the usual range) and rounded once to
- * fp32. idx[b, h, run, :top_k] (int32, contiguous [B, H, runs, top_k]) are the
+ * is formed in 64 bits (off by at most (rows + 257) 2^-53 of its terms' magnitudes; exact
+ * where the query sums' bits and the bounds' span 45 together) and rounded once to fp32. idx[b, h, run, :top_k] (int32, contiguous [B, H, runs, top_k]) are the
  * blocks < keep_first and >= blocks - keep_last, then those of the highest scores,
  * ties to the lowest index, in ascending order; empty blocks are never chosen,
  * a NaN score ranks as -inf, and -1 fills the entries behind the last.
@@ -352,7 +353,8 @@ int64_t hn_select_kv_blocks_workspace_size(int64_t B, int64_t H, int64_t runs, i
  *   lse: fp32 [B, Hq, Lq] contiguous
  * Probabilities meet V as fp16 of 2^11 to 2^15 for a row's largest: 2^-11 relative
  * down to 2^-25 of it, 2^-36 of it below. The other arguments and V's range are those
- * of hn_attn_fp8kv. */
+ * of hn_attn_fp8kv; where a run is one row (q_block = 1 or Lq = 1, G = 1), probabilities
+ * and V are fp32. */
 int hn_attn_kv_blocks(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
                       const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
                       const int64_t *ss, int64_t H, int64_t cache_cap, int64_t kv_len,

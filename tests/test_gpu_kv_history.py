@@ -1095,3 +1095,22 @@ def test_attention_of_nan_rows(dev, Lq, q_block, kv):
         gone, without = q.clone(), torch.where(no, -INF, lse)
         gone[0, 1, 0] = gone[0, 2, 1] = 0
         assert torch.equal(hist.key_mass(bad, lse, cache, kv), hist.key_mass(gone, without, cache, kv))
+
+
+@pytest.mark.parametrize("Lq,q_block", [(3, 1), (20, 20), (50, 50), (100, 100)])
+def test_attention_of_small_values(dev, Lq, q_block):
+    """V near 2^-20: as fp16 it is a multiple of 2^-24, off by less than one of them toward
+    zero, as _attend's bound on the output allows; a run of one row keeps it in fp32."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 70 + Lq)
+    cache = _cache(dev, 1, 900, 2, "int8", g)
+    cache["v_scale"].mul_(2.0 ** -20)
+    q, k, v = (torch.randn(1, Lq, 2, D, device=dev, generator=g).to(BF16) for _ in range(3))
+    v = (v.float() * 2.0 ** -20).to(BF16)
+    idx = _lists(dev, 1, 2, -(-Lq // q_block), 15, 9, g)
+    ref = _attend(q, cache, 900, idx, 64, q_block, k, v, None, None)
+    got = ca.sparse_chunk_attention(q, cache, 900, idx, q_block=q_block, k_cur=k, v_cur=v)
+    _check_attention(got, ref, "small values")
+    if q_block == 1:
+        bound = ref[2] - 2.0 ** -24                        # without the term for V's last place
+        assert ((got[0].to(F64) - ref[0]).abs() <= bound).all()
