@@ -475,9 +475,15 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
 // are formed (beside S of t + 1) and multiplied, V of t + 1 goes to the other stage and
 // K of t + 2 to this one, whose K was last read a tile ago; one barrier a tile. The two
 // halves of a row's keys meet at the end. Scales travel four tiles ahead of V. Bound by
-// the latency of the codes' loads (a tile is computed in less): 777 queries x 24 heads in
-// runs of 64 over 24 int8 blocks of 128 with holes and a 777-token tail 139 us + 8.6 us
-// of merge; attn_waves_kernel took 169 us, attn_blocks_kernel, half of its waves idle, 203.
+// the latency of the codes' loads (a tile is computed in less). At 254 to 256 VGPRs the
+// registers are full, and the masked forms spill (12 bytes a lane in fp8, 20 in int8).
+// 777 queries x 24 heads in runs of 64 over 24 int8 blocks of 128 with holes and a
+// 777-token tail 139 us + 8.6 us of merge. Calls (merge included) against
+// attn_blocks_kernel, whose waves are half idle: that one 149 against 170 us (fp8 without
+// holes 129 against 136), runs of 48 162 against 190, of 33 240 against 258; a single run
+// of 33 or 64 rows, 64 lists x 4096 keys 37.6 against 37.5 and 40.9 against 40.2, 64 x
+// 32768 200 against 224 and 209 against 228, but 64 x 1024 22.3 against 20.5 and 25.5
+// against 23.6: short lists pay for its longer prologue.
 template <int FMT, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
     constexpr int NW = 4;
@@ -785,9 +791,10 @@ __global__ __launch_bounds__(256, 2) void attn_half_kernel(BlockParams p) {
 // 16-byte load of K and of V), a wave reads 8 keys per load and has a whole 64-key
 // tile in flight. K^ enters as packed bf16 (v_dot2_f32_bf16 onto fp32), probabilities
 // and V^ as fp32. Each lane group runs an online softmax of its own keys; the 8 groups
-// of a wave, the 4 waves and the splits meet at the end. Against attn_waves_kernel: 8
-// heads x 1000 keys 7.5 against 9.2 us, 64 x 4096 keys 21.2 against 24.2 us, 64 x 32768
-// keys 126 against 127 us (4.4 TB/s); with two rows a run it gained 0-7 %.
+// of a wave, the 4 waves and the splits meet at the end. Calls (merge included) against
+// attn_waves_kernel: 64 lists x 1024 keys 10.5 against 13.8 us, x 4096 23.9 against 28.5,
+// x 32768 135 against 153 (4.1 TB/s); 77 runs of 24 heads over 48 blocks and a 77-token
+// tail 318 against 300.
 struct RowState {
     float m, l, o[16];
 };
@@ -1001,8 +1008,10 @@ __global__ __launch_bounds__(256, 2) void attn_row_kernel(BlockParams p) {
 // computed the next one's codes are in flight to a second set of registers. The waves
 // and the splits meet at the end. Bound by the read of the keys and, where each wave has
 // few blocks, by a fixed 8 us (launch, first loads, meeting): 64 lists x 4096 keys, 4
-// rows each (69 MB) 25 us, 64 x 8192 35 us (5.8 TB/s for the second half);
-// attn_blocks_kernel took 36 us for the first.
+// rows each (69 MB) 25 us, 64 x 8192 35 us (5.8 TB/s for the second half). It fills 256
+// VGPRs and spills 10 (44 bytes a lane). Calls (merge included) against attn_half_kernel
+// and attn_blocks_kernel: 4 rows 28.4, 34.6, 35.5 us; 32 rows 31.8, 36.8, 36.8; 777
+// queries x 24 heads in runs of 32 over 48 blocks and the tail 145, 229, 229.
 constexpr int WV_ROW = 80;                       // V^T row: 32 fp16 keys + 16 B
 constexpr int WV_GROUP = 16 * WV_ROW + 64;       // 16 rows + 64 B (writes of 4 row groups fall in different banks)
 constexpr int WV_BYTES = 8 * WV_GROUP;
@@ -1680,7 +1689,8 @@ __global__ __launch_bounds__(256) void key_mass_sum_kernel(MassParams p, int spl
 using namespace hn;
 
 // Which kernel a run's rows take: one row attn_row_kernel, up to 32 attn_waves_kernel,
-// up to 64 attn_half_kernel, more attn_blocks_kernel.
+// up to 64 attn_half_kernel, more attn_blocks_kernel (both sides of each border are
+// measured at the kernels).
 enum class BlocksKernel { ROW, WAVES, HALF, TILES };
 
 struct BlocksPlan {
@@ -1693,8 +1703,9 @@ struct BlocksPlan {
 // ceil(work sp / 2 CUs) rounds of workgroups, each worth its tiles (64 keys; a
 // workgroup of the first two kernels works on four at a time) and a fixed part (the
 // list, the first loads, the end), and the merge reads and writes every row sp times.
-// In units of a tile of a full round (2.7 us measured in attn_blocks_kernel): the split
-// with the least of it is taken, each keeping at least 4 tiles.
+// In units of a tile of a full round (2.7 us measured in attn_blocks_kernel; the other
+// kernels' tiles were not measured apart): the split with the least of it is taken, each
+// keeping at least 4 tiles.
 static BlocksPlan blocks_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t kv_len, int64_t cur_len,
                               int64_t top_k, int64_t block, int64_t q_block) {
     constexpr double FIXED = 2.0, MERGE = 1e-4;  // per workgroup; per row and split (1 KB at 4 TB/s)
@@ -1851,7 +1862,10 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
 // 4: each row tile read from LDS once for four key blocks), or 128 (KB 1) where 512 would
 // not fill the device twice over; where even these fall short (a short cache, many
 // queries) the rows are split, each split writes its sums and a second kernel adds them in
-// order.
+// order. KB 1 against KB 4, 24 heads: 3600 queries over 5500 keys (264 workgroups of 512)
+// 217 against 225 us, 10800 keys (528) 358 against 332, 86400 2493 against 1787; with few
+// rows the border would lie higher, 64 queries over 11000 keys 18.6 against 21.0, 86400
+// 106 against 107.
 struct MassPlan {
     int kb, splits, keys;
     int64_t tiles;

@@ -35,7 +35,7 @@ HN_DEVICE uint32_t rank_of(float f) {
 // 8 lanes hold a key's 128 codes (16 bytes each) and 8 keys are read per load,
 // all loads of 64 keys in flight; the 8 keys' extremes meet by lane exchanges.
 // Bound by the read of the codes, and for few blocks by the launch: 10800 tokens x 24
-// heads (36 MB) 9.8 us, 3.7 TB/s; one token of 8 batches x 8 heads 4.8 us.
+// heads (36 MB) 10.4 us, 3.5 TB/s; one token of 8 batches x 8 heads 4.8 us.
 struct BoundsArgs {
     const uint8_t* kc;
     const float* ks;
