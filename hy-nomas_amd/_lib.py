@@ -29,6 +29,7 @@ _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
 _PI64 = ctypes.POINTER(ctypes.c_int64)
+_PI32 = ctypes.POINTER(ctypes.c_int32)
 
 # name -> argtypes, in the order of include/hynomas_fp8.h
 SIGNATURES = {
@@ -75,12 +76,19 @@ SIGNATURES = {
     "hn_select_kv_tokens_workspace_size": [_I64] * 3,
     "hn_move_kv_tokens": [_P, _P, _PI64, _P, _P, _PI64, _P, _PI64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P,
                           _PI64, _P, _P, _PI64, _I64, _P, _P],
+    "hn_kv_pages_write": [_I, _P, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64,
+                          _P, _I64, _I64, _P, _P, _P, _P],
+    "hn_kv_pages_read": [_I, _P, _PI64, _P, _PI64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "hn_kv_pages_copy": [ctypes.POINTER(_P), _PI64, _PI64, _PI64, _I64, _I64, _PI32, _PI32, _I64, _P],
+    "hn_attn_kv_pages": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64, _I64,
+                         _P, _I64, _I64, _P, _I, _P, _P, _PI64, _I64, _P, _I64, _F, _P, _PI64, _P, _P, _I64, _P],
+    "hn_attn_kv_pages_workspace_size": [_I64] * 6 + [_I],
     "hn_e4m3_encode_range": [ctypes.c_uint32, _I64, _P, _P],
 }
 RESTYPES = {"hn_last_error": ctypes.c_char_p, "hn_attn_fp8kv_workspace_size": _I64,
             "hn_attn_fp8kv_noalloc_scratch_bytes": _I64, "hn_select_kv_blocks_workspace_size": _I64,
             "hn_attn_kv_blocks_workspace_size": _I64, "hn_attn_key_mass_workspace_size": _I64,
-            "hn_select_kv_tokens_workspace_size": _I64}
+            "hn_select_kv_tokens_workspace_size": _I64, "hn_attn_kv_pages_workspace_size": _I64}
 
 _lib = None
 _lock = threading.Lock()

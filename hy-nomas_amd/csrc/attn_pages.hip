@@ -1,0 +1,673 @@
+// Attention over a paged quantized KV cache (gfx950): the queries of every sequence
+// against its own tokens, page by page, then the bf16 tail; O = softmax(Q K^T scale) V
+// and the rows' log-sum-exp. K, V = bf16(code * scale), as in attn_fp8kv.hip.
+#include "attn_tiles.h"
+
+namespace hn {
+namespace attn {
+
+typedef float f32x4_ __attribute__((ext_vector_type(4)));
+
+struct PageParams {
+    const uint16_t* q;
+    const uint8_t* kc;
+    const uint8_t* vc;
+    const float* ks;
+    const float* vs;
+    const uint16_t* kcur;
+    const uint16_t* vcur;
+    const uint8_t* uvalid;   // null: every tail key is valid
+    uint16_t* out;
+    float* lse;              // [B, H G, Lq]
+    const int32_t* table;
+    const int32_t* lens;
+    int64_t ts0, uvs;
+    int64_t qs0, qs1, qs2;
+    int64_t cs0, cs1, cs2;   // page, token, head
+    int64_t ss0, ss1, ss2;
+    int64_t us0, us1, us2;
+    int64_t os0, os1, os2;
+    int64_t Lq;
+    int B, H, G;
+    int rows;                // Lq G: row r of a cached head is query r / G, head r % G of its group
+    int runs;                // ceil(rows / rows of a workgroup)
+    int pages, width, shift; // pool, table row, page = 1 << shift
+    int cur_len;
+    int causal;
+    float scale_log2;
+    int whole;               // a workgroup an item; else the units of all items dealt out evenly
+    int wgs;                 // of the second form
+    int per_xcd;             // ceil(workgroups / 8)
+    int pitch;               // rows of a partial result
+    float* ws_o;             // [workgroup][2][pitch][D] unnormalised
+    float* ws_ml;            // [workgroup][2][pitch][2]
+};
+
+constexpr int UNIT = 128;    // keys a workgroup takes at a time, 32 a wave
+
+// Cached tokens of sequence b that the table can name.
+HN_DEVICE int seq_len(const PageParams& p, int b) {
+    const int n = p.lens[b], most = p.width << p.shift;
+    return n < 0 ? 0 : n < most ? n : most;
+}
+
+// Units of an item: of the cache, of the tail; one at least (a row without keys is written too).
+HN_DEVICE int cache_units(int len) { return (len + UNIT - 1) / UNIT; }
+HN_DEVICE int tail_units(const PageParams& p) { return (p.cur_len + UNIT - 1) / UNIT; }
+HN_DEVICE int item_units(const PageParams& p, int b) {
+    const int n = cache_units(seq_len(p, b)) + tail_units(p);
+    return n > 0 ? n : 1;
+}
+
+HN_DEVICE uint32_t wave_scan(uint32_t v) {  // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(v, off, 64);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+// Where the items lie on the line of all units: sequence after sequence, in each head
+// after head, run after run. `total` units; at(u) finds the item of unit u.
+struct Line {
+    const PageParams& p;
+    uint32_t total;
+    HN_DEVICE explicit Line(const PageParams& pp) : p(pp), total(0) {
+        const int lane = threadIdx.x & 63;
+        uint32_t n = 0;
+        for (int i = lane; i < p.B; i += 64) n += (uint32_t)item_units(p, i);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+        total = n * (uint32_t)(p.H * p.runs);
+    }
+    // The sequence of unit u, its first unit on the line, the units of each of its items.
+    HN_DEVICE void find(uint32_t u, int& b, uint32_t& start, int& n) const {
+        const int lane = threadIdx.x & 63;
+        const uint32_t per = (uint32_t)(p.H * p.runs);
+        uint32_t before = 0;
+        b = 0;
+        start = 0;
+        n = 1;
+        for (int i0 = 0; i0 < p.B; i0 += 64) {
+            const int mine = i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
+            const uint32_t end = wave_scan((uint32_t)mine * per);
+            const uint64_t past = __ballot(before + end > u);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                b = i0 + l;
+                n = __builtin_amdgcn_readlane(mine, l);
+                start = before + __builtin_amdgcn_readlane(end, l) - (uint32_t)n * per;
+                return;
+            }
+            before += __builtin_amdgcn_readlane(end, 63);
+        }
+    }
+    HN_DEVICE uint32_t share() const { return (total + (uint32_t)p.wgs - 1) / (uint32_t)p.wgs; }
+};
+
+HN_DEVICE f32x4_ mfma16_bf16(const bf16x8& a, const bf16x8& b, const f32x4_& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+HN_DEVICE f32x4_ mfma16_f16(const f16x8& a, const f16x8& b, const f32x4_& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Probabilities of 2^11 to 2^15 for a row's largest (attn_blocks.hip: fp16 then holds
+// those down to 2^-25 of it in full).
+constexpr float TOP_LOW = 11.0f, TOP_HIGH = 15.0f;
+
+// ---------------------------------------------------------------------------
+// Few rows against many keys: single tokens, drafted ones, grouped heads. The read of
+// the codes is the cost. A workgroup holds 16 RB rows of one cached head; its four waves
+// take 32-key blocks in turn, each on its own, without LDS or barriers: S^T = K Q^T and
+// O^T += V^T P^T on 16 x 16 x 32 products whose operands are formed in registers from
+// the lane's own loads. With g = lane / 16, r = lane % 16:
+//   K operand of keys 16 t + r: the lane loads dims 16 g .. + 15 and 64 + 16 g .. + 15 of
+//     the key; product s contracts dims 64 (s / 2) + 16 g + 8 (s % 2) + {0..7}, and Q is
+//     loaded the same way.
+//   S^T leaves the lane keys 16 t + 4 g + {0..3} of row r: as they stand they are the P
+//     operand, slots j < 4 being keys 4 g + j and j >= 4 keys 16 + 4 g + j - 4.
+//   V^T operand: for those eight keys the lane loads dims 8 r .. + 7; product db holds dim
+//     8 r + db, so that O^T leaves the lane dims 32 g .. + 31 of row r.
+// The four waves meet in LDS at the end of an item.
+template <int RB>
+struct Rows {
+    f32x4_ o[RB][8];
+    float m[RB], nm[RB], l[RB];
+};
+
+struct PageRegs {  // codes of a 32-key block
+    uint4 k[2][2];
+    uint2 v[8];
+    float ks[2], vs[8];
+    int left;      // keys from the block's first on that the sequence has; 0: none
+    int first;     // its first token
+};
+
+template <int FMT, int RB>
+__global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
+    constexpr int R = 16 * RB, PITCH = D + 4;
+    __shared__ __attribute__((aligned(16))) float so[4][R][PITCH];
+    __shared__ float sml[4][R][2];
+    const int id = blockIdx.x;
+    const int wg = (id & 7) * p.per_xcd + (id >> 3);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int per = p.H * p.runs;
+
+    uint32_t u0, u1, start;   // this workgroup's units; the current sequence's first
+    int b, n;
+    Line line(p);
+    if (p.whole) {
+        if (wg >= p.B * per) return;
+        b = wg / per;
+        n = item_units(p, b);
+        start = 0;
+        u0 = (uint32_t)(wg - b * per) * (uint32_t)n;
+        u1 = u0 + (uint32_t)n;
+    } else {
+        if (wg >= p.wgs) return;
+        const uint32_t share = line.share();
+        u0 = (uint32_t)wg * share;
+        u1 = u0 + share < line.total ? u0 + share : line.total;
+        if (u0 >= u1) return;
+        line.find(u0, b, start, n);
+    }
+    const uint32_t range0 = u0;
+    const float c = p.scale_log2;
+
+    while (u0 < u1) {
+        if (u0 - start >= (uint32_t)n * (uint32_t)per) {  // the next sequence
+            start += (uint32_t)n * (uint32_t)per;
+            ++b;
+            n = item_units(p, b);
+            continue;
+        }
+        const int item = (int)((u0 - start) / (uint32_t)n);   // h runs + run
+        const uint32_t item0 = start + (uint32_t)item * (uint32_t)n;
+        const int lo = (int)(u0 - item0), hi = min(n, (int)(u1 - item0));
+        const int h = item / p.runs, run = item - h * p.runs;
+        const int row0 = run * R, rows = min(R, p.rows - row0);
+        const int len = seq_len(p, b), nc = cache_units(len);
+
+        bf16x8 qf[RB][4];
+        int lim[RB];           // this lane's rows see cached tokens below
+        int lim_all = len;     // all rows do
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int r = row0 + min(16 * rb + r16, rows - 1), qi = r / p.G;
+            const uint16_t* src = p.q + b * p.qs0 + qi * p.qs1 + (int64_t)(h * p.G + r - qi * p.G) * p.qs2 + 16 * g;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                qf[rb][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 64 * (s >> 1) + 8 * (s & 1)));
+            lim[rb] = p.causal ? len - (int)p.Lq + 1 + qi : len;
+        }
+        if (p.causal) lim_all = len - (int)p.Lq + 1 + row0 / p.G;
+        Rows<RB> st;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            st.m[rb] = -INFINITY;
+            st.nm[rb] = 0.0f;
+            st.l[rb] = 0.0f;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) st.o[rb][db] = (f32x4_){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        // Probabilities of a block's logits s[rb][t] (masked ones -inf), as the P operand.
+        auto probs = [&](f32x4_ (&s)[RB][2], f16x8 (&pf)[RB]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rb][t][i]);
+                if (__any(mx * c > st.m[rb] + TOP_HIGH)) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    const float mnew = fmaxf(st.m[rb], mx * c - TOP_LOW);
+                    const float a = st.m[rb] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m[rb] - mnew);
+                    st.m[rb] = mnew;
+                    st.nm[rb] = mnew == -INFINITY ? 0.0f : -mnew;
+                    st.l[rb] *= a;
+#pragma unroll
+                    for (int db = 0; db < 8; ++db) st.o[rb][db] *= a;
+                }
+                uint32_t x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][e >> 1][2 * (e & 1)], c, st.nm[rb]));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][e >> 1][2 * (e & 1) + 1], c, st.nm[rb]));
+                    x[e] = pack_f16(p0, p1);
+                    st.l[rb] += p0 + p1;
+                }
+                pf[rb] = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
+            }
+        };
+
+        // ---- cached keys
+        const int32_t* row_table = p.table + b * p.ts0;
+        int chunk = -1, held = 0;   // 64 table entries, one a lane
+        auto load = [&](int blk, PageRegs& x) __attribute__((always_inline)) {
+            x.first = blk * 32;
+            x.left = len - x.first;
+            if (blk >= 4 * min(hi, nc) || x.left <= 0) {
+                x.left = 0;
+                return;
+            }
+            const int entry = x.first >> p.shift;
+            if ((entry >> 6) != chunk) {
+                chunk = entry >> 6;
+                held = row_table[min(64 * chunk + lane, p.width - 1)];
+            }
+            const int page = __builtin_amdgcn_readlane(held, entry & 63);
+            if ((uint32_t)page >= (uint32_t)p.pages) {  // no such page: no keys
+                x.left = 0;
+                return;
+            }
+            const int64_t slot = x.first & ((1 << p.shift) - 1);
+            const int64_t ca = page * p.cs0 + slot * p.cs1 + h * p.cs2, sa = page * p.ss0 + slot * p.ss1 + h * p.ss2;
+            const uint8_t *kb = p.kc + ca, *vb = p.vc + ca;
+            const float *kss = p.ks + sa, *vss = p.vs + sa;
+            const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t at = (16 * t + r16) * cs1 + 16 * g;
+                x.k[t][0] = *reinterpret_cast<const uint4*>(kb + at);
+                x.k[t][1] = *reinterpret_cast<const uint4*>(kb + at + 64);
+                x.ks[t] = kss[(16 * t + r16) * ss1];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t key = 16 * (j >> 2) + 4 * g + (j & 3);
+                x.v[j] = *reinterpret_cast<const uint2*>(vb + key * cs1 + 8 * r16);
+                x.vs[j] = vss[key * ss1];
+            }
+        };
+        auto block = [&](PageRegs& x) __attribute__((always_inline)) {
+            if (x.left <= 0) return;
+            f32x4_ s[RB][2];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) s[rb][t] = (f32x4_){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int sl = 0; sl < 4; ++sl)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    uint32_t d[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x2 f = codes2_f32<FMT>(word(x.k[t][sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
+                        d[e] = pack_bf16(f[0] * x.ks[t], f[1] * x.ks[t]);
+                    }
+                    const bf16x8 kf = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) s[rb][t] = mfma16_bf16(kf, qf[rb][sl], s[rb][t]);
+                }
+            if (x.first + 32 > lim_all) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (x.first + 16 * t + 4 * g + i >= lim[rb]) s[rb][t][i] = -INFINITY;
+            }
+            if (x.left < 32) {  // what lies behind the sequence's end meets no product
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (16 * (j >> 2) + 4 * g + (j & 3) >= x.left) {
+                        x.v[j] = make_uint2(0u, 0u);
+                        x.vs[j] = 0.0f;
+                    }
+            }
+            f16x8 pf[RB];
+            probs(s, pf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f32x2 f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f[j] = codes2_f32<FMT>(e & 2 ? x.v[j].y : x.v[j].x, e & 1);
+                    f[j][0] *= x.vs[j];
+                    f[j][1] *= x.vs[j];
+                }
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const f16x8 vf = __builtin_bit_cast(
+                        f16x8, make_uint4(pack_f16_of_bf16(f[0][w], f[1][w]), pack_f16_of_bf16(f[2][w], f[3][w]),
+                                          pack_f16_of_bf16(f[4][w], f[5][w]), pack_f16_of_bf16(f[6][w], f[7][w])));
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) st.o[rb][2 * e + w] = mfma16_f16(vf, pf[rb], st.o[rb][2 * e + w]);
+                }
+            }
+        };
+        {
+            const int end = 4 * min(hi, nc);
+            int t = 4 * lo + wave;
+            PageRegs ra, rb_;
+            load(t, ra);
+            load(t + 4, rb_);
+            while (t < end) {
+                block(ra);
+                t += 4;
+                if (t >= end) break;
+                load(t + 4, ra);
+                block(rb_);
+                t += 4;
+                load(t + 4, rb_);
+            }
+        }
+        // ---- the tail
+        for (int u = max(lo, nc); u < hi; ++u) {
+            const int first = (u - nc) * UNIT + 32 * wave, left = p.cur_len - first;
+            if (left <= 0) break;
+            const int64_t at = b * p.us0 + h * p.us2;
+            bool ok = (lane & 31) < left;
+            if (p.uvalid && ok) ok = p.uvalid[b * p.uvs + first + (lane & 31)] != 0;
+            const uint32_t live = (uint32_t)__ballot(ok);
+            if (live == 0) continue;
+            f32x4_ s[RB][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint16_t* kp = p.kcur + at + (int64_t)(first + min(16 * t + r16, left - 1)) * p.us1 + 16 * g;
+                uint4 kx[4];
+#pragma unroll
+                for (int sl = 0; sl < 4; ++sl) kx[sl] = *reinterpret_cast<const uint4*>(kp + 64 * (sl >> 1) + 8 * (sl & 1));
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    s[rb][t] = (f32x4_){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int sl = 0; sl < 4; ++sl)
+                        s[rb][t] = mfma16_bf16(__builtin_bit_cast(bf16x8, kx[sl]), qf[rb][sl], s[rb][t]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!((live >> (16 * t + 4 * g + i)) & 1u)) s[rb][t][i] = -INFINITY;
+                }
+            }
+            uint4 vx[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = 16 * (j >> 2) + 4 * g + (j & 3);
+                vx[j] = make_uint4(0u, 0u, 0u, 0u);
+                if ((live >> key) & 1u)
+                    vx[j] = *reinterpret_cast<const uint4*>(p.vcur + at + (int64_t)(first + key) * p.us1 + 8 * r16);
+            }
+            f16x8 pf[RB];
+            probs(s, pf);
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t a = word(vx[2 * e], db >> 1), z = word(vx[2 * e + 1], db >> 1);
+                    y[e] = __builtin_bit_cast(uint32_t, db & 1 ? __builtin_amdgcn_cvt_pkrtz(bf16_hi(a), bf16_hi(z))
+                                                               : __builtin_amdgcn_cvt_pkrtz(bf16_lo(a), bf16_lo(z)));
+                }
+                const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(y[0], y[1], y[2], y[3]));
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) st.o[rb][db] = mfma16_f16(vf, pf[rb], st.o[rb][db]);
+            }
+        }
+        // ---- the waves meet
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float l = st.l[rb];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            const int r = 16 * rb + r16;
+            if (r < rows) {
+                float* dst = &so[wave][r][32 * g];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float4*>(dst + 8 * i + 4 * e) =
+                            make_float4(st.o[rb][4 * e][i], st.o[rb][4 * e + 1][i], st.o[rb][4 * e + 2][i], st.o[rb][4 * e + 3][i]);
+                if (g == 0) {
+                    sml[wave][r][0] = st.m[rb];
+                    sml[wave][r][1] = l;
+                }
+            }
+        }
+        __syncthreads();
+        const bool done = lo == 0 && hi == n;
+        const int64_t part = (int64_t)wg * 2 + (item0 < range0 ? 0 : 1);
+        for (int at = threadIdx.x; at < rows * (D / 4); at += 256) {
+            const int r = at / (D / 4), d = (at % (D / 4)) * 4;
+            float m = sml[0][r][0];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) m = fmaxf(m, sml[w][r][0]);
+            const float base = m == -INFINITY ? 0.0f : m;
+            float den = 0.0f;
+            float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float a = __builtin_amdgcn_exp2f(sml[w][r][0] - base);
+                const float4 y = *reinterpret_cast<const float4*>(&so[w][r][d]);
+                den = __builtin_fmaf(sml[w][r][1], a, den);
+                num.x = __builtin_fmaf(y.x, a, num.x);
+                num.y = __builtin_fmaf(y.y, a, num.y);
+                num.z = __builtin_fmaf(y.z, a, num.z);
+                num.w = __builtin_fmaf(y.w, a, num.w);
+            }
+            if (done) {
+                const int rr = row0 + r, qi = rr / p.G, hq = h * p.G + rr - qi * p.G;
+                const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+                *reinterpret_cast<uint2*>(p.out + b * p.os0 + qi * p.os1 + hq * p.os2 + d) =
+                    make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
+                if (d == 0)
+                    p.lse[((int64_t)b * p.H * p.G + hq) * p.Lq + qi] =
+                        den != 0.0f ? (m + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+            } else {
+                *reinterpret_cast<float4*>(p.ws_o + (part * p.pitch + r) * D + d) = num;
+                if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + (part * p.pitch + r) * 2) = make_float2(m, den);
+            }
+        }
+        __syncthreads();
+        u0 = item0 + (uint32_t)hi;
+    }
+}
+
+// The parts of items that several workgroups computed, joined in their order: with M =
+// max m, O = sum 2^(m - M) O / sum 2^(m - M) l. 32 threads a row, 4 dims each, eight rows
+// of an item a workgroup.
+__global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
+    const Line line(p);
+    const int per = p.H * p.runs, groups = (min(R, p.rows) + 7) / 8;
+    int x = blockIdx.x;
+    const int grp = x % groups;
+    x /= groups;
+    const int item = x % per, b = x / per;
+    const uint32_t share = line.share();
+    // the sequence's first unit on the line
+    uint32_t before = 0;
+    {
+        const int lane = threadIdx.x & 63;
+        for (int i = lane; i < b; i += 64) before += (uint32_t)item_units(p, i);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+    }
+    const int n = item_units(p, b);
+    const uint32_t i0 = before * (uint32_t)per + (uint32_t)item * (uint32_t)n;
+    const uint32_t w0 = i0 / share, w1 = (i0 + (uint32_t)n - 1) / share;
+    if (w0 == w1) return;  // whole: written already
+    const int h = item / p.runs, run = item - h * p.runs;
+    const int r = grp * 8 + (threadIdx.x >> 5), row = run * R + r, d = (threadIdx.x & 31) * 4;
+    if (r >= R || row >= p.rows) return;
+    float M = -INFINITY, den = 0.0f;
+    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t a0 = w0; a0 <= w1; a0 += 8) {
+        float2 ml[8];
+        float4 ov[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t w = a0 + e < w1 ? a0 + e : w1;
+            const int64_t part = ((int64_t)w * 2 + (i0 < w * share ? 0 : 1)) * p.pitch + r;
+            ml[e] = *reinterpret_cast<const float2*>(p.ws_ml + part * 2);
+            ov[e] = *reinterpret_cast<const float4*>(p.ws_o + part * D + d);
+            if (a0 + e > w1) ml[e] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = M;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, ml[e].x);
+        const float base = top == -INFINITY ? 0.0f : top, a = __builtin_amdgcn_exp2f(M - base);
+        den *= a;
+        num.x *= a; num.y *= a; num.z *= a; num.w *= a;
+        M = top;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float wgt = __builtin_amdgcn_exp2f(ml[e].x - base);
+            den = fmaf(wgt, ml[e].y, den);
+            num.x = fmaf(wgt, ov[e].x, num.x);
+            num.y = fmaf(wgt, ov[e].y, num.y);
+            num.z = fmaf(wgt, ov[e].z, num.z);
+            num.w = fmaf(wgt, ov[e].w, num.w);
+        }
+    }
+    const int qi = row / p.G, hq = h * p.G + row - qi * p.G;
+    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+    *reinterpret_cast<uint2*>(p.out + b * p.os0 + qi * p.os1 + hq * p.os2 + d) =
+        make_uint2(pack_bf16(num.x * inv, num.y * inv), pack_bf16(num.z * inv, num.w * inv));
+    if (d == 0)
+        p.lse[((int64_t)b * p.H * p.G + hq) * p.Lq + qi] =
+            den != 0.0f ? (M + __builtin_amdgcn_logf(den)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace attn
+}  // namespace hn
+
+using namespace hn;
+
+struct PagesPlan {
+    int rb, runs, whole, wgs, pitch;
+    int64_t items;
+};
+
+static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len) {
+    PagesPlan pl;
+    const int64_t rows = Lq * G;
+    pl.rb = rows <= 16 ? 1 : 2;
+    const int64_t R = 16 * pl.rb;
+    pl.runs = (int)((rows + R - 1) / R);
+    pl.items = B * H * pl.runs;
+    pl.pitch = (int)(rows < R ? rows : R);
+    const int64_t units = (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
+    pl.wgs = 2 * device_cus();
+    pl.whole = units <= 2 || pl.items >= 8 * (int64_t)pl.wgs;
+    return pl;
+}
+
+static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
+    return B > 0 && Lq > 0 && H > 0 && Hq > 0 && Hq % H == 0 && max_len >= 0 && cur_len >= 0 && B <= 0x7fffffffLL &&
+           Lq <= 0x7fffffffLL && Hq <= 0x7fffffffLL && max_len <= 0x3fffffffLL && cur_len <= 0x3fffffffLL &&
+           Lq * (Hq / H) <= 0x3fffffffLL;
+}
+
+extern "C" int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
+                                                   int64_t cur_len, int causal) {
+    if (!pages_shape_ok(B, Lq, Hq, H, max_len, cur_len)) return 0;
+    (void)causal;
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
+    return pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+}
+
+extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64_t B, int64_t Lq, int64_t Hq,
+                                int64_t D, const void* kc, const void* vc, const int64_t* cs, const float* ks,
+                                const float* vs, const int64_t* ss, int64_t H, int64_t n_pages, int64_t page,
+                                const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
+                                int causal, const void* kcur, const void* vcur, const int64_t* curs, int64_t cur_len,
+                                const uint8_t* cur_valid, int64_t cur_valid_stride, float softmax_scale, void* out,
+                                const int64_t* os, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    HN_REQUIRE(fmt == HN_KV_FP8 || fmt == HN_KV_INT8, HN_E_ARG, "hn_attn_kv_pages: unknown KV format");
+    HN_REQUIRE(D == attn::D, HN_E_ARG, "hn_attn_kv_pages: head dim must be 128");
+    HN_REQUIRE(page >= 64 && page <= 1024 && (page & (page - 1)) == 0, HN_E_ARG,
+               "hn_attn_kv_pages: page must be 64, 128, 256, 512 or 1024");
+    HN_REQUIRE(B >= 0 && Lq >= 0 && H > 0 && Hq > 0 && Hq % H == 0 && n_pages >= 0 && width >= 0 && cur_len >= 0,
+               HN_E_ARG, "hn_attn_kv_pages: invalid shape");
+    HN_REQUIRE(width <= 0x3fffffffLL / page && n_pages <= 0x7fffffffLL && cur_len <= 0x3fffffffLL, HN_E_ARG,
+               "hn_attn_kv_pages: too many keys");
+    HN_REQUIRE(!causal || cur_len == 0, HN_E_ARG, "hn_attn_kv_pages: a causal call takes no tail");
+    HN_REQUIRE(softmax_scale > 0.0f && softmax_scale <= 3.4028234e38f, HN_E_ARG,
+               "hn_attn_kv_pages: softmax_scale must be finite and positive");
+    HN_REQUIRE(qs && os && cs && ss && (cur_len == 0 || curs), HN_E_ARG, "hn_attn_kv_pages: null stride array");
+    HN_REQUIRE(qs[3] == 1 && os[3] == 1 && cs[3] == 1, HN_E_ARG, "hn_attn_kv_pages: head dim must be contiguous");
+    HN_REQUIRE(qs[0] % 8 == 0 && qs[1] % 8 == 0 && qs[2] % 8 == 0 && os[0] % 4 == 0 && os[1] % 4 == 0 && os[2] % 4 == 0,
+               HN_E_ARG, "hn_attn_kv_pages: q/out strides misaligned");
+    HN_REQUIRE(cs[0] % 16 == 0 && cs[1] % 16 == 0 && cs[2] % 16 == 0 && cs[0] >= 0 && cs[1] >= 0 && cs[2] >= 0 &&
+                   ss[0] >= 0 && ss[1] >= 0 && ss[2] >= 0 && cs[1] <= 0x1ffffffLL && ss[1] <= 0x7fffffLL,
+               HN_E_ARG, "hn_attn_kv_pages: pool strides must be multiples of 16 bytes");
+    HN_REQUIRE(aligned(q, 16) && aligned(out, 8) && aligned(kc, 16) && aligned(vc, 16) && aligned(ks, 4) &&
+                   aligned(vs, 4) && aligned(table, 4) && aligned(lens, 4) && aligned(lse, 4),
+               HN_E_ARG, "hn_attn_kv_pages: misaligned pointer");
+    HN_REQUIRE(table_stride >= 0 && cur_valid_stride >= 0, HN_E_ARG, "hn_attn_kv_pages: negative stride");
+    if (cur_len > 0) {
+        HN_REQUIRE(kcur && vcur, HN_E_ARG, "hn_attn_kv_pages: null tail pointer");
+        HN_REQUIRE(curs[3] == 1 && curs[0] % 8 == 0 && curs[1] % 8 == 0 && curs[2] % 8 == 0 && curs[0] >= 0 &&
+                       curs[1] >= 0 && curs[1] <= 0xffffffLL && curs[2] >= 0,
+                   HN_E_ARG, "hn_attn_kv_pages: tail strides must be multiples of 8, below 2^24 per token");
+        HN_REQUIRE(aligned(kcur, 16) && aligned(vcur, 16), HN_E_ARG, "hn_attn_kv_pages: tail misaligned");
+    }
+    if (B == 0 || Lq == 0) return HN_OK;
+    HN_REQUIRE(q && out && lse && lens, HN_E_ARG, "hn_attn_kv_pages: null pointer");
+    HN_REQUIRE(width == 0 || n_pages == 0 || (table && kc && vc && ks && vs), HN_E_ARG, "hn_attn_kv_pages: null pool pointer");
+    const int64_t max_len = n_pages ? width * page : 0;
+    HN_REQUIRE(pages_shape_ok(B, Lq, Hq, H, max_len, cur_len), HN_E_ARG, "hn_attn_kv_pages: too much work");
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
+    const int64_t units = 1 + (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
+    HN_REQUIRE(pl.items <= 0x3fffffffLL / units, HN_E_ARG, "hn_attn_kv_pages: too much work for one launch");
+    const int64_t need = pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+    HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
+               "hn_attn_kv_pages: workspace smaller than hn_attn_kv_pages_workspace_size() or misaligned");
+    if (const int rc = require_gfx950("hn_attn_kv_pages"); rc != HN_OK) return rc;
+    attn::PageParams p = {};
+    p.q = (const uint16_t*)q; p.out = (uint16_t*)out; p.lse = lse;
+    p.kc = (const uint8_t*)kc; p.vc = (const uint8_t*)vc; p.ks = ks; p.vs = vs;
+    p.kcur = (const uint16_t*)kcur; p.vcur = (const uint16_t*)vcur;
+    p.uvalid = cur_len > 0 ? cur_valid : nullptr;
+    p.uvs = cur_valid_stride;
+    p.table = table; p.lens = lens; p.ts0 = table_stride;
+    p.qs0 = qs[0]; p.qs1 = qs[1]; p.qs2 = qs[2];
+    p.os0 = os[0]; p.os1 = os[1]; p.os2 = os[2];
+    p.cs0 = cs[0]; p.cs1 = cs[1]; p.cs2 = cs[2];
+    p.ss0 = ss[0]; p.ss1 = ss[1]; p.ss2 = ss[2];
+    if (cur_len > 0) {
+        p.us0 = curs[0]; p.us1 = curs[1]; p.us2 = curs[2];
+    }
+    p.Lq = Lq; p.B = (int)B; p.H = (int)H; p.G = (int)(Hq / H);
+    p.rows = (int)(Lq * p.G);
+    p.runs = pl.runs;
+    p.pages = (int)n_pages;
+    p.width = n_pages ? (int)width : 0;
+    p.shift = __builtin_ctzll((unsigned long long)page);
+    p.cur_len = (int)cur_len;
+    p.causal = causal != 0;
+    p.scale_log2 = softmax_scale * 1.4426950408889634f;
+    p.whole = pl.whole;
+    p.wgs = pl.wgs;
+    p.pitch = pl.pitch;
+    if (!pl.whole) {
+        p.ws_o = (float*)workspace;
+        p.ws_ml = (float*)workspace + (int64_t)pl.wgs * 2 * pl.pitch * attn::D;
+    }
+    const int64_t grid = pl.whole ? pl.items : pl.wgs;
+    p.per_xcd = (int)((grid + 7) / 8);
+    const unsigned blocks = 8u * (unsigned)p.per_xcd;
+    const hipStream_t st = (hipStream_t)stream;
+#define HN_PAGES(F, R) attn::attn_pages_kernel<F, R><<<blocks, 256, 0, st>>>(p)
+    if (fmt == HN_KV_FP8) {
+        if (pl.rb == 1) HN_PAGES(HN_KV_FP8, 1);
+        else HN_PAGES(HN_KV_FP8, 2);
+    } else {
+        if (pl.rb == 1) HN_PAGES(HN_KV_INT8, 1);
+        else HN_PAGES(HN_KV_INT8, 2);
+    }
+#undef HN_PAGES
+    if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK || pl.whole) return rc;
+    const int R = 16 * pl.rb, groups = (pl.pitch + 7) / 8;
+    attn::pages_join_kernel<<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
+    return check_launch("hn_attn_kv_pages (join)");
+}

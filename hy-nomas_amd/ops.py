@@ -47,7 +47,7 @@ def _on(device: torch.device):
 
 _TENSOR = (torch.Tensor, torch.nn.Parameter)
 _KINDS = {"Tensor": _TENSOR, "Optional[Tensor]": (*_TENSOR, type(None)), "int": (int,), "float": (float, int),
-          "Optional[float]": (float, int, type(None))}
+          "Optional[float]": (float, int, type(None)), "bool": (bool,), "List[int]": (list, tuple)}
 
 
 try:
@@ -1121,3 +1121,239 @@ def move_kv_tokens_(out_k: torch.Tensor, out_v: torch.Tensor, out_k_scale: torch
 @move_kv_tokens_.register_fake
 def _(out_k, out_v, out_k_scale, out_v_scale, k_codes, v_codes, k_scale, v_scale, mass, idx):
     return mass.new_empty(idx.shape, dtype=torch.float32)
+
+
+# --------------------------------------------------------------------------
+# the cache in pages: write, copy, decode, attention
+
+def _check_pool(codes: torch.Tensor, scale: torch.Tensor, what: str) -> int:
+    """A layer's pool: codes [P, page, H, D] with fp32 scales [P, page, H, 1]. Returns
+    the page's tokens."""
+    if codes.ndim != 4 or scale.dtype != torch.float32 or tuple(scale.shape) != (*codes.shape[:3], 1):
+        raise ValueError(f"{what}: codes [P, page, H, D] with fp32 scales [P, page, H, 1]")
+    if codes.shape[1] not in BLOCK_SIZES:
+        raise ValueError(f"{what}: a page must be of {BLOCK_SIZES} tokens")
+    return codes.shape[1]
+
+
+def _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what: str) -> int:
+    page = _check_pool(k_codes, k_scale, what)
+    if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride()
+            or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape
+            or v_scale.stride() != k_scale.stride()):
+        raise ValueError(f"{what}: K and V must share dtype, shape and strides")
+    return page
+
+
+def _page_table(table: torch.Tensor, B: int, what: str) -> torch.Tensor:
+    """int32 [B, W], the entries of a sequence contiguous."""
+    if table.dtype != torch.int32 or table.ndim != 2 or table.shape[0] != B:
+        raise ValueError(f"{what}: table must be int32 [B, W]")
+    return table if table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
+
+
+def _per_sequence(t: Optional[torch.Tensor], B: int, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+        raise ValueError(f"{what} must be int32 [B]")
+    return t.contiguous()
+
+
+def kv_pages_write_(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts=None, status=None) -> None:
+    """Quantize new tokens into the pages of their sequences (see _kv_pages_write_op)."""
+    _kv_pages_write_op(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status)
+
+
+@eager_op("hy_nomas_amd::kv_pages_write_", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale", "status"))
+def _kv_pages_write_op(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
+                       counts: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
+    """bf16 K/V [B, L, H, D]: token j of sequence b, j < counts[b] (None: L), goes to its
+    token start[b] + j, row (start[b] + j) % page of page table[b, (start[b] + j) // page]
+    of the pool [P, page, H, D]. Tokens whose page is not in the pool are dropped.
+    ``status`` as in _kv_quantize_pair_op; rows past counts do not matter to it."""
+    what = "kv_pages_write_"
+    fmt = _kv_fmt(k_codes)
+    page = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects bf16 values")
+    if k.ndim != 4 or k.shape != v.shape or tuple(k.shape[2:]) != tuple(k_codes.shape[2:]):
+        raise ValueError(f"{what}: k and v must be [B, L, H, D] matching the pool")
+    B, Lt, H, D = k.shape
+    table = _page_table(table, B, what)
+    start, counts = _per_sequence(start, B, f"{what}: start"), _per_sequence(counts, B, f"{what}: counts")
+    sp = _status_ptr(status)
+    k, v = _head_rows(k), _head_rows(v)
+    if k.stride() != v.stride():
+        k, v = k.contiguous(), v.contiguous()
+    _one_device(what, k, v, k_codes, v_codes, k_scale, v_scale, table, start, counts, status)
+    with _on(k.device):
+        L.check(L.load().hn_kv_pages_write(
+            fmt, k.data_ptr(), v.data_ptr(), _strides(k), B, Lt, H, D, k_codes.data_ptr(), v_codes.data_ptr(),
+            _strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), k_codes.shape[0], page,
+            table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), sp, _stream(k)),
+            "hn_kv_pages_write")
+
+
+@_kv_pages_write_op.register_fake
+def _(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status):
+    return None
+
+
+@eager_op("hy_nomas_amd::kv_pages_read", mutates_args=())
+def kv_pages_read(codes: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
+                  max_len: int) -> torch.Tensor:
+    """Tokens [0, max_len) of every sequence decoded: bf16(code * scale) for t <
+    kv_len[b] (int32 [B]), zeros behind: a new [B, max_len, H, D]."""
+    what = "kv_pages_read"
+    fmt = _kv_fmt(codes)
+    page = _check_pool(codes, scale, what)
+    if max_len < 0:
+        raise ValueError(f"{what}: max_len must not be negative")
+    B = table.shape[0] if table.ndim else 0
+    table, kv_len = _page_table(table, B, what), _per_sequence(kv_len, B, f"{what}: kv_len")
+    P, _, H, D = codes.shape
+    _one_device(what, codes, scale, table, kv_len)
+    y = torch.empty((B, max_len, H, D), dtype=torch.bfloat16, device=codes.device)
+    if y.numel() == 0:
+        return y
+    with _on(codes.device):
+        L.check(L.load().hn_kv_pages_read(
+            fmt, codes.data_ptr(), _strides(codes), scale.data_ptr(), _strides(scale), P, page, table.data_ptr(),
+            table.stride(0), table.shape[1], kv_len.data_ptr(), B, max_len, H, D, y.data_ptr(), _stream(codes)),
+            "hn_kv_pages_read")
+    return y
+
+
+@kv_pages_read.register_fake
+def _(codes, scale, table, kv_len, max_len):
+    return codes.new_empty((table.shape[0], max_len, *codes.shape[2:]), dtype=torch.bfloat16)
+
+
+def _page_bytes(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """Bytes from layer to layer, from page to page and of a page of [layers, P, page, H,
+    last], whose pages are runs of bytes each (in any order of the tokens and heads)."""
+    size = t.element_size()
+    run = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape[2:], t.stride()[2:]) if n != 1), key=lambda x: x[1]):
+        if s != run:
+            raise ValueError(f"{what}: a page must be one run of memory")
+        run *= n
+    # (a single page or layer lies nowhere relative to another)
+    step = t.stride(1) if t.shape[1] > 1 else run
+    return (t.stride(0) * size if t.shape[0] > 1 else 0), step * size, run * size
+
+
+@eager_op("hy_nomas_amd::kv_pages_copy_", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale"))
+def kv_pages_copy_(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                   src: list[int], dst: list[int]) -> None:
+    """Page dst[i] <- page src[i] of K and V, codes and scales, in a layer's pool [P, page,
+    H, D] or in all layers of [layers, P, page, H, D]. One src may go to several dst; a
+    dst occurs once, and not as a src."""
+    what = "kv_pages_copy_"
+    _kv_fmt(k_codes)
+    if k_codes.ndim == 4:
+        k_codes, v_codes, k_scale, v_scale = (t.unsqueeze(0) for t in (k_codes, v_codes, k_scale, v_scale))
+    if k_codes.ndim != 5 or k_scale.dtype != torch.float32 or tuple(k_scale.shape) != (*k_codes.shape[:4], 1):
+        raise ValueError(f"{what}: codes [layers, P, page, H, D] with fp32 scales [layers, P, page, H, 1]")
+    if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_scale.dtype != torch.float32
+            or v_scale.shape != k_scale.shape):
+        raise ValueError(f"{what}: K and V must share dtype and shape")
+    layers, P = k_codes.shape[:2]
+    if len(src) != len(dst):
+        raise ValueError(f"{what}: src and dst must be of one length")
+    if not src:
+        return
+    if min(src) < 0 or min(dst) < 0 or max(src) >= P or max(dst) >= P:
+        raise ValueError(f"{what}: pages must lie in [0, {P})")
+    to = set(dst)
+    if len(to) != len(dst) or not to.isdisjoint(src):
+        raise ValueError(f"{what}: a page is written twice, or read and written")
+    arrays = (k_codes, v_codes, k_scale, v_scale)
+    _one_device(what, *arrays)
+    if 0 in k_codes.shape:
+        return
+    sizes = [_page_bytes(t, what) for t in arrays]
+    n = len(src)
+    with _on(k_codes.device):
+        L.check(L.load().hn_kv_pages_copy(
+            (ctypes.c_void_p * 4)(*(t.data_ptr() for t in arrays)), *((ctypes.c_int64 * 4)(*col) for col in zip(*sizes)),
+            layers, P, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, _stream(k_codes)),
+            "hn_kv_pages_copy")
+
+
+@kv_pages_copy_.register_fake
+def _(k_codes, v_codes, k_scale, v_scale, src, dst):
+    return None
+
+
+@functools.lru_cache(maxsize=1024)
+def _pages_workspace(device: int, *sizes) -> int:
+    """hn_attn_kv_pages_workspace_size on the current device, ``device``."""
+    return L.load().hn_attn_kv_pages_workspace_size(*sizes)
+
+
+@eager_op("hy_nomas_amd::attn_kv_pages", mutates_args=())
+def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, causal: bool = False,
+                  k_cur: Optional[torch.Tensor] = None, v_cur: Optional[torch.Tensor] = None,
+                  softmax_scale: Optional[float] = None,
+                  cur_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of q [B, Lq, Hq, D] over each sequence's cached tokens [0, kv_len[b]) in
+    the pages of table [B, W], and the bf16 tail k_cur/v_cur [B, Lc, H, D]: out bf16 [B,
+    Lq, Hq, D] and the rows' log-sum-exp fp32 [B, Hq, Lq].
+
+    The pool is [P, page, H, D], Hq a multiple of H. causal (without a tail): the queries
+    are the sequence's last Lq tokens and each sees what is not behind it. cur_valid (bool
+    [B or 1, >= Lc]) excludes tail keys. See hn_attn_kv_pages."""
+    what = "attn_kv_pages"
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects bf16 queries")
+    fmt = _kv_fmt(k_codes)
+    page = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
+    P, _, H, Dk = k_codes.shape
+    if q.ndim != 4:
+        raise ValueError(f"{what}: q must be [B, Lq, Hq, D]")
+    B, Lq, Hq, D = q.shape
+    if Dk != D or H == 0 or Hq % H:
+        raise ValueError(f"{what}: pool [P, page, H, D] does not match q")
+    table, kv_len = _page_table(table, B, what), _per_sequence(kv_len, B, f"{what}: kv_len")
+    scale = _softmax_scale(softmax_scale, D, what)
+    cur_len = 0 if k_cur is None else k_cur.shape[1] if k_cur.ndim == 4 else -1
+    if k_cur is not None and (k_cur.ndim != 4 or k_cur.shape[0] != B or tuple(k_cur.shape[2:]) != (H, D)):
+        raise ValueError(f"{what}: k_cur must be [B, Lc, H, D] matching the pool")
+    if (k_cur is None) != (v_cur is None) or (k_cur is not None and (
+            v_cur.shape != k_cur.shape or k_cur.dtype != torch.bfloat16 or v_cur.dtype != torch.bfloat16)):
+        raise ValueError(f"{what}: k_cur/v_cur must be matching bf16 tensors")
+    if causal and cur_len:
+        raise ValueError(f"{what}: a causal call takes no tail")
+    q = _head_rows(q)
+    if cur_len:
+        k_cur, v_cur = _head_rows(k_cur), _head_rows(v_cur)
+        if k_cur.stride() != v_cur.stride():
+            k_cur, v_cur = k_cur.contiguous(), v_cur.contiguous()
+    uvb, uvs = _mask_bytes(cur_valid if cur_len else None, B, cur_len, f"{what}: cur_valid")
+    device = _one_device(what, q, k_codes, v_codes, k_scale, v_scale, table, kv_len, k_cur, v_cur, uvb)
+    out = torch.empty((B, Lq, Hq, D), dtype=torch.bfloat16, device=device)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
+    if out.numel() == 0:
+        return out, lse
+    W = table.shape[1]
+    with _on(device):
+        lib = L.load()
+        ws_bytes = _pages_workspace(device.index, B, Lq, Hq, H, W * page if P else 0, cur_len, int(causal))
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes else None
+        L.check(lib.hn_attn_kv_pages(
+            fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), _strides(k_codes),
+            k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), H, P, page, table.data_ptr(), table.stride(0), W,
+            kv_len.data_ptr(), int(causal), L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
+            _strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), _strides(out),
+            lse.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_kv_pages")
+    return out, lse
+
+
+@attn_kv_pages.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, table, kv_len, causal=False, k_cur=None, v_cur=None, softmax_scale=None,
+      cur_valid=None):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)

@@ -410,6 +410,70 @@ int hn_move_kv_tokens(const void *k, const void *v, const int64_t *cs, const flo
                       const int64_t *os, float *out_ks, float *out_vs, const int64_t *ts, int64_t out_cap,
                       float *out_mass, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * The cache in pages: roll-outs that branch from one history, and sessions of
+ * different lengths, share a pool. No counterpart in the reference, whose caches are
+ * one block a roll-out. A layer's pool is n_pages pages of `page` tokens (64, 128, 256,
+ * 512 or 1024): codes [n_pages, page, H, 128] with strides cs[4] (multiples of 16, the
+ * last 1) and fp32 scales with strides ss[3]. Token t of sequence b is row t % page of
+ * page table[b * table_stride + t / page] (int32, `width` entries a sequence, width *
+ * page < 2^31). An entry outside [0, n_pages) names no page: tokens to be written there
+ * are dropped, tokens to be read there are absent. Lengths are int32 on the device, held
+ * to [0, width * page].
+ */
+
+/* Quantizes new tokens into their pages: token j < counts[b] (NULL: L) of sequence b, K
+ * and V bf16 [B, L, H, 128] with strides xs[4] each, becomes its token start[b] + j; codes
+ * and scales are hn_kv_quantize_pair's. Rows past counts[b] are not read. Tokens of a
+ * negative start, or past the table, are dropped. status as in hn_kv_quantize: nothing
+ * is written if a value of a new token is NaN or Inf. Two new tokens of one call at one
+ * place (a page that two of its sequences share) leave either's bytes there. */
+int hn_kv_pages_write(int fmt, const void *k, const void *v, const int64_t *xs, int64_t B, int64_t L,
+                      int64_t H, int64_t D, void *kc, void *vc, const int64_t *cs, float *ks, float *vs,
+                      const int64_t *ss, int64_t n_pages, int64_t page, const int32_t *table,
+                      int64_t table_stride, int64_t width, const int32_t *start, const int32_t *counts,
+                      int32_t *status, void *stream);
+
+/* Decodes tokens [0, L) of every sequence: y[b, t, h, :] = bf16(code * scale) of one of K
+ * and V for t < lens[b], zeros behind and for absent tokens. y: bf16 [B, L, H, 128]
+ * contiguous. */
+int hn_kv_pages_read(int fmt, const void *kc, const int64_t *cs, const float *ks, const int64_t *ss,
+                     int64_t n_pages, int64_t page, const int32_t *table, int64_t table_stride,
+                     int64_t width, const int32_t *lens, int64_t B, int64_t L, int64_t H, int64_t D,
+                     void *y, void *stream);
+
+/* Copies page src[i] to page dst[i] (i < n, host arrays) in four arrays (K and V codes, K
+ * and V scales) of every layer. Array a: layer l's page e is page_bytes[a] bytes at base[a]
+ * + l * layer_stride[a] + e * page_stride[a] (all in bytes, multiples of 16). A dst that
+ * occurs twice, or as a src, leaves either's bytes there. Up to 240 pairs are one launch;
+ * nothing is uploaded. */
+int hn_kv_pages_copy(void *const *base, const int64_t *layer_stride, const int64_t *page_stride,
+                     const int64_t *page_bytes, int64_t layers, int64_t n_pages, const int32_t *src,
+                     const int32_t *dst, int64_t n, void *stream);
+
+/* Attention of q [B, Lq, Hq, 128] over the sequences' cached tokens t < lens[b] and the
+ * bf16 tail, with the rows' log-sum-exp; Hq a multiple of H, query head h G + g reading
+ * cached head h:
+ *   out = softmax(softmax_scale q K^T) V, lse = ln sum exp(softmax_scale q . K).
+ * causal (without a tail): the queries are the sequence's last Lq tokens, query i sees
+ * tokens t <= lens[b] - Lq + i. A row without a key gets zeros and -inf, one that meets a
+ * NaN gets NaN in both. What lies behind a sequence's end does not matter.
+ *   kcur, vcur, cur_valid, out, lse and V's range as in hn_attn_kv_blocks, whose fp16
+ *   probabilities these are.
+ * workspace: hn_attn_kv_pages_workspace_size(.., width * page, ..) bytes, 16-byte aligned. */
+int hn_attn_kv_pages(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
+                     const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
+                     const int64_t *ss, int64_t H, int64_t n_pages, int64_t page, const int32_t *table,
+                     int64_t table_stride, int64_t width, const int32_t *lens, int causal, const void *kcur,
+                     const void *vcur, const int64_t *curs, int64_t cur_len, const uint8_t *cur_valid,
+                     int64_t cur_valid_stride, float softmax_scale, void *out, const int64_t *os, float *lse,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace hn_attn_kv_pages needs for these sizes on the current device (0:
+ * none); max_len = width * page. */
+int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
+                                        int64_t cur_len, int causal);
+
 /* Test support; it replaces no reference interface. Writes to out[i] the e4m3
  * byte that the quantizers' hardware conversion (v_cvt_pk_fp8_f32, round to
  * nearest even) gives for the fp32 value whose bit pattern is first + i, for

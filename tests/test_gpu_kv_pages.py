@@ -1,0 +1,492 @@
+"""The paged KV cache on the GPU: writes against the contiguous cache's codes, attention
+against 64 bits, page copies and decodes against indexing, and a run of them together."""
+import math
+
+import pytest
+import torch
+
+from conftest import pkg_module
+
+pytestmark = pytest.mark.gpu
+
+BF16, F64, I32 = torch.bfloat16, torch.float64, torch.int32
+NAMES = ("k", "v", "k_scale", "v_scale")
+
+
+def _mods():
+    return pkg_module("kv_pages"), pkg_module("cache_attention"), pkg_module("fp8_kv_cache")
+
+
+def _pool(dev, g, pages, page, H, fmt="fp8", layers=None, gain=1.0):
+    """A pool of quantized normal values."""
+    kp, _, kvc = _mods()
+    code = torch.float8_e4m3fn if fmt == "fp8" else torch.int8
+    pool = kp.make_pages(pages, H, page=page, layers=layers, code_dtype=code, device=dev)
+    make = kvc.make_fp8_kv_block if fmt == "fp8" else kvc.make_int8_kv_block
+    for i in range(layers or 1):
+        block = make(pages, page, H, 128, device=dev)
+        k, v = ((torch.randn(pages, page, H, 128, device=dev, generator=g) * gain).to(BF16) for _ in range(2))
+        kvc.quantize_kv_pair_into(block, k, v, 0)
+        for n in NAMES:
+            (pool[n] if layers is None else pool[n][i]).copy_(block[n])
+    return pool
+
+
+def _table(dev, g, lens, page, pages, width=None):
+    """Distinct random pages for every sequence, -1 behind its last."""
+    need = [-(-n // page) for n in lens]
+    t = torch.full((len(lens), width or max(1, *need)), -1, dtype=I32)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(int(g.initial_seed()))).tolist()
+    for b, n in enumerate(need):
+        t[b, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=I32)
+    return t.to(dev)
+
+
+def _i32(dev, values):
+    return torch.tensor(values, dtype=I32, device=dev)
+
+
+def _held(pool, key, table, b, n):
+    """bf16(code * scale) of the first n tokens of a sequence, in 64 bits."""
+    page = pool[key].shape[1]
+    t = torch.arange(n, device=table.device)
+    pg = table[b].long()[t // page]
+    codes = pool[key]
+    x = codes.view(torch.uint8)[pg, t % page].view(codes.dtype).float() * pool[key + "_scale"][pg, t % page]
+    return x.to(BF16).to(F64)
+
+
+def _reference(q, pool, table, lens, causal=False, k_cur=None, v_cur=None, cur_valid=None, scale=None):
+    """out, lse, the rows' sum of p |v| / sum p, and the largest sum of |q k| scale."""
+    B, Lq, Hq, D = q.shape
+    H = pool["k"].shape[2]
+    G, dev = Hq // H, q.device
+    scale = D ** -0.5 if scale is None else scale
+    out, spread = torch.zeros(2, B, Lq, Hq, D, dtype=F64, device=dev).unbind(0)
+    lse = torch.full((B, Hq, Lq), -math.inf, dtype=F64, device=dev)
+    terms = torch.zeros(B, Hq, Lq, dtype=F64, device=dev)
+    for b in range(B):
+        k, v = _held(pool, "k", table, b, lens[b]), _held(pool, "v", table, b, lens[b])
+        seen = torch.ones(Lq, lens[b], dtype=torch.bool, device=dev)
+        if causal:
+            seen = torch.arange(lens[b], device=dev) <= lens[b] - Lq + torch.arange(Lq, device=dev)[:, None]
+        if k_cur is not None:
+            k, v = torch.cat([k, k_cur[b].to(F64)]), torch.cat([v, v_cur[b].to(F64)])
+            ok = torch.ones(k_cur.shape[1], dtype=torch.bool, device=dev) if cur_valid is None else cur_valid[
+                b if cur_valid.shape[0] > 1 else 0, :k_cur.shape[1]].bool()
+            seen = torch.cat([seen, ok.expand(Lq, -1)], 1)
+        v = torch.where(seen.any(0)[:, None, None], v, torch.zeros_like(v)) if len(v) else v
+        for h in range(Hq):
+            if not len(k):
+                continue
+            kh, vh, qh = k[:, h // G], v[:, h // G], q[b, :, h].to(F64)
+            s = (qh @ kh.T * scale).masked_fill(~seen, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - torch.where(top == -math.inf, torch.zeros_like(top), top))
+            total = p.sum(-1, keepdim=True)
+            w = torch.where(total > 0, p / total, torch.zeros_like(p))
+            out[b, :, h], spread[b, :, h] = w @ vh, w @ vh.abs()
+            lse[b, h] = torch.where(total > 0, top + total.log(), -math.inf)[:, 0]
+            terms[b, h] = (qh.abs() @ kh.abs().T * scale).masked_fill(~seen, 0.0).amax(-1)
+    return out, lse, spread, terms
+
+
+def _check(got, want, what=""):
+    """Output: half a step of bf16 at the result, and what moves the probabilities: fp16
+    (2^-11 relative), the logit's fp32 sum of 128 terms (129 2^-24 of the terms), exp2 and
+    the fp32 sums (2^-20). Log-sum-exp: the logit's error, 2^-20, and 2^-22 of itself."""
+    out, lse = got
+    ref, rlse, spread, terms = want
+    assert torch.isfinite(out).all(), what
+    logit = 129 * 2.0 ** -24 * terms
+    rel = (2.0 ** -11 + 2.0 ** -20 + 2 * logit).transpose(1, 2)[..., None]
+    err = rel * spread + 1e-30
+    tol = err + (ref.abs() + err) * 2.0 ** -8
+    worst = ((out.to(F64) - ref).abs() / tol).max().item() if out.numel() else 0.0
+    none = rlse == -math.inf
+    assert torch.equal(lse == -math.inf, none), what
+    assert (out.transpose(1, 2)[none] == 0).all(), what
+    d = (lse.to(F64) - rlse).abs()[~none]
+    ltol = (logit + 2.0 ** -20 + rlse.abs() * 2.0 ** -22)[~none]
+    lworst = (d / ltol).max().item() if d.numel() else 0.0
+    print(f"[pages] {what}: out {worst:.2f} lse {lworst:.2f} of the tolerance", flush=True)
+    assert worst <= 1.0 and lworst <= 1.0, (what, worst, lworst)
+
+
+# --------------------------------------------------------------------------
+# attention
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("H,G", [(8, 4), (3, 1), (1, 16), (2, 17), (1, 40)])
+@pytest.mark.parametrize("lens", [(1,), (700, 0, 64, 65, 63, 1), (129, 128, 127), (4111, 33)])
+def test_one_token(dev, fmt, H, G, lens):
+    _, ca, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(sum(lens) + 7 * H + G)
+    pages = sum(-(-n // 64) for n in lens) + 2
+    pool = _pool(dev, g, pages, 64, H, fmt)
+    table = _table(dev, g, lens, 64, pages)
+    q = torch.randn(len(lens), 1, H * G, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    _check(got, _reference(q, pool, table, lens), f"{fmt} {H}x{G} {lens}")
+
+
+@pytest.mark.parametrize("page", [64, 256, 1024])
+@pytest.mark.parametrize("Lq,G", [(2, 1), (5, 4), (8, 2), (9, 4), (33, 1), (70, 3)])
+def test_causal(dev, page, Lq, G):
+    """Sequences shorter than the queries have rows without a key."""
+    _, ca, _ = _mods()
+    lens = (Lq, 1000, max(1, Lq // 2), 0, 513 + Lq)
+    g = torch.Generator(device=dev).manual_seed(page + Lq)
+    pages = sum(-(-n // page) for n in lens) + 1
+    pool = _pool(dev, g, pages, page, 2)
+    table = _table(dev, g, lens, page, pages)
+    q = torch.randn(len(lens), Lq, 2 * G, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
+    _check(got, _reference(q, pool, table, lens, causal=True), f"page {page} Lq {Lq} G {G}")
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("Lq,G,Lc", [(1, 1, 1), (1, 4, 70), (31, 1, 200), (130, 1, 0), (129, 2, 129), (300, 1, 64), (65, 1, 1)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_queries_and_tail(dev, fmt, Lq, G, Lc, masked):
+    """Any number of queries, with the current chunk's keys behind the history, padded
+    ones among them, and what a masked key holds without effect."""
+    _, ca, _ = _mods()
+    lens, page, H = (0, 777, 64, 1301), 128, 2
+    g = torch.Generator(device=dev).manual_seed(Lq + G + Lc)
+    pages = sum(-(-n // page) for n in lens) + 1
+    pool = _pool(dev, g, pages, page, H, fmt)
+    table = _table(dev, g, lens, page, pages)
+    B = len(lens)
+    q = torch.randn(B, Lq, H * G, 128, device=dev, generator=g).to(BF16)
+    kw = {}
+    if Lc:
+        qkv = torch.randn(B, Lc, 3, H, 128, device=dev, generator=g).to(BF16)
+        kw = dict(k_cur=qkv[:, :, 1], v_cur=qkv[:, :, 2])
+    if masked and Lc:
+        valid = torch.rand(B, Lc, device=dev, generator=g) < 0.7
+        valid[0] = False  # no history either: rows without a key
+        kw["cur_valid"] = valid
+        qkv[:, :, 1:][~valid] = float("nan")
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens), **kw)
+    if masked and Lc:
+        qkv[:, :, 1:][~valid] = 0.0
+    _check(got, _reference(q, pool, table, lens, **kw), f"{fmt} Lq {Lq} G {G} Lc {Lc} masked {masked}")
+
+
+@pytest.mark.parametrize("Lq", [1, 9, 200])
+def test_what_lies_behind_a_sequence_does_not_matter(dev, Lq):
+    """NaN codes and infinite scales behind the end, in unnamed pages and under entries
+    that name none; such entries inside a sequence name no keys."""
+    _, ca, _ = _mods()
+    H, page, lens = 2, 64, (300, 65)
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    pool = _pool(dev, g, 12, page, H)
+    table = _table(dev, g, lens, page, 12, width=9)
+    q = torch.randn(2, Lq, H, 128, device=dev, generator=g).to(BF16)
+    want = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    _check(want, _reference(q, pool, table, lens), "clean")
+    used = torch.zeros(12, page, dtype=torch.bool, device=dev)
+    for b, n in enumerate(lens):
+        t = torch.arange(n, device=dev)
+        used[table[b].long()[t // page], t % page] = True
+    for key in ("k", "v"):
+        pool[key].view(torch.uint8)[~used] = 0x7F
+        pool[key + "_scale"][~used] = float("inf")
+    table[0, 5:], table[1, 2:] = 2 ** 31 - 1, -2 ** 31
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # a hole: its keys are absent, and lengths past the table end with it
+    table[0, 1] = 12
+    got = ca.paged_attention(q, pool, table, _i32(dev, (2 ** 31 - 1, -5)))
+    t = torch.tensor([i for i in range(300) if i // page != 1 and i // page < 5], device=dev)
+    mine = table[0, :5].clone()
+    mine[1] = 0
+    pg = mine.long()[t // page]
+    full = {n: x[pg, t % page][None] for n, x in ((n, pool[n].view(torch.uint8) if n in "kv" else pool[n]) for n in NAMES)}
+    full["k"], full["v"] = full["k"].view(pool["k"].dtype), full["v"].view(pool["v"].dtype)
+    kvc = {n: torch.zeros(1, 1024, *x.shape[2:], dtype=x.dtype, device=dev) for n, x in full.items()}
+    for n in NAMES:
+        a, b = (x.view(torch.uint8) if n in "kv" else x for x in (kvc[n], full[n]))
+        a[:, :len(t)] = b
+    # (the last page is whole here: its tokens behind 300 are NaN, so the length stays 300 in the reference)
+    got = ca.paged_attention(q, pool, table, _i32(dev, (300, -5)))
+    ref = _reference(q[:1], kvc, torch.zeros(1, 1, dtype=I32, device=dev), (len(t),))
+    _check((got[0][:1], got[1][:1]), ref, "hole")
+    assert (got[0][1] == 0).all() and (got[1][1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("Lq", [1, 40, 150])
+def test_nan_and_extreme_logits(dev, Lq):
+    """A row that meets a NaN gets NaN in output and log-sum-exp; rows of other
+    sequences do not. Logits of +-1e4 stay a softmax."""
+    _, ca, _ = _mods()
+    H, page, lens = 2, 64, (200, 200)
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    pool = _pool(dev, g, 8, page, H, gain=30.0)
+    table = _table(dev, g, lens, page, 8)
+    q = (torch.randn(2, Lq, H, 128, device=dev, generator=g) * 30).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    _check(got, _reference(q, pool, table, lens), "large logits")
+    q[0, 0, 0, 5] = float("nan")
+    bad = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    assert torch.isnan(bad[0][0, 0, 0]).all() and torch.isnan(bad[1][0, 0, 0])
+    bad[0][0, 0, 0], bad[1][0, 0, 0] = got[0][0, 0, 0], got[1][0, 0, 0]
+    assert torch.equal(bad[0], got[0]) and torch.equal(bad[1], got[1])
+
+
+def test_strides_scale_and_scratch_of_other_calls(dev):
+    """A pool with token-major scales inside a larger one, a q view, a strided table, a
+    scale of one's own: as the plain layout."""
+    _, ca, _ = _mods()
+    H, page, lens = 4, 64, (515, 1024, 3)
+    g = torch.Generator(device=dev).manual_seed(5)
+    pool = _pool(dev, g, 30, page, H)
+    table = _table(dev, g, lens, page, 30)
+    q = torch.randn(3, 2, H, 128, device=dev, generator=g).to(BF16)
+    want = ca.paged_attention(q, pool, table, _i32(dev, lens), softmax_scale=0.2)
+    _check(want, _reference(q, pool, table, lens, scale=0.2), "plain layout")
+    other = {}
+    for n in NAMES:
+        x = pool[n].contiguous()
+        wide = torch.zeros(30, page, 2 * H, x.shape[3], dtype=x.dtype, device=dev)
+        wide[:, :, H:] = x
+        other[n] = wide[:, :, H:]
+    qkv = torch.randn(3, 2, 3, H, 128, device=dev, generator=g).to(BF16)
+    qkv[:, :, 0] = q
+    t2 = torch.stack([table, table], 2)
+    got = ca.paged_attention(qkv[:, :, 0], other, t2[:, :, 1], _i32(dev, lens), softmax_scale=0.2)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("B,lens", [(70, 130), (300, 40)])
+def test_many_sequences(dev, B, lens):
+    _, ca, _ = _mods()
+    n = [(lens * (b + 1) * 7919) % (3 * lens) for b in range(B)]
+    g = torch.Generator(device=dev).manual_seed(B)
+    pages = sum(-(-x // 64) for x in n) + 1
+    pool = _pool(dev, g, pages, 64, 2)
+    table = _table(dev, g, n, 64, pages)
+    q = torch.randn(B, 1, 4, 128, device=dev, generator=g).to(BF16)
+    _check(ca.paged_attention(q, pool, table, _i32(dev, n)), _reference(q, pool, table, n), f"B {B}")
+
+
+def test_offsets_past_32_bits(dev):
+    """A pool whose codes pass 4 GiB, its last pages read, written and copied."""
+    kp, ca, _ = _mods()
+    H, page = 16, 256
+    pages = (1 << 32) // (page * H * 128) + 40
+    g = torch.Generator(device=dev).manual_seed(3)
+    pool = kp.make_pages(pages, H, page=page, device=dev)
+    n, first = 5 * page - 30, pages - 6
+    table = torch.arange(first, first + 5, dtype=I32, device=dev)[None]
+    k, v = (torch.randn(1, n, H, 128, device=dev, generator=g).to(BF16) for _ in range(2))
+    kp.write_pages(pool, k, v, table, _i32(dev, [0]))
+    q = torch.randn(1, 3, H, 128, device=dev, generator=g).to(BF16)
+    tail = {m: pool[m][first:first + 5] for m in NAMES}
+    at = torch.arange(5, dtype=I32, device=dev)[None]
+    for lq in (1, 3):
+        got = ca.paged_attention(q[:, :lq], pool, table, _i32(dev, [n]))
+        _check(got, _reference(q[:, :lq], tail, at, (n,)), f"far pages Lq {lq}")
+    big = torch.randn(1, 200, H, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(big, pool, table, _i32(dev, [n]))
+    _check(got, _reference(big, tail, at, (n,)), "far pages, 200 queries")
+    assert torch.equal(kp.read_pages(pool, "k", table, _i32(dev, [n]), n), kp.read_pages(tail, "k", at, _i32(dev, [n]), n))
+    kp.copy_pages(pool, [pages - 3], [pages - 1])
+    for m in NAMES:
+        a, b = (pool[m][e].contiguous().view(torch.uint8) for e in (pages - 3, pages - 1))
+        assert torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------
+# write, read, copy
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("layout", ["bshd", "bhsd", "qkv"])
+@pytest.mark.parametrize("L,H", [(1, 1), (1, 8), (1, 70), (3, 24), (64, 5), (129, 24), (1000, 2)])
+def test_write_is_the_contiguous_write(dev, fmt, layout, L, H):
+    """Codes and scales are the contiguous cache's, token for token; nothing else of the
+    pool changes: rows behind the counts, pages of nobody."""
+    kp, _, kvc = _mods()
+    page, starts = 64, (0, 63, 100)
+    counts = (L, max(0, L - 1), L // 2)
+    g = torch.Generator(device=dev).manual_seed(L * H)
+    if layout == "bshd":
+        k, v = (torch.randn(3, L, H, 128, device=dev, generator=g).to(BF16) for _ in range(2))
+    elif layout == "bhsd":
+        k, v = (torch.randn(3, H, L, 128, device=dev, generator=g).to(BF16).transpose(1, 2) for _ in range(2))
+    else:
+        qkv = torch.randn(3, L, 3, H, 128, device=dev, generator=g).to(BF16)
+        k, v = qkv[:, :, 1], qkv[:, :, 2]
+    k[0, 0, 0] = 0.0  # a row of zeros: scale 1
+    if L > 1:
+        k[2, -1] = float("nan")  # behind the counts
+    make = kvc.make_fp8_kv_block if fmt == "fp8" else kvc.make_int8_kv_block
+    flat = make(3, 100 + L, H, 128, device=dev)
+    for b in range(3):
+        one = {n: x[b:b + 1] for n, x in flat.items()}
+        kvc.quantize_kv_pair_into(one, k[b:b + 1, :counts[b]], v[b:b + 1, :counts[b]], starts[b])
+    ends = [s + c for s, c in zip(starts, counts)]
+    pages = sum(-(-e // page) for e in ends) + 2
+    pool = _pool(dev, g, pages, page, H, fmt)
+    before = {n: x.clone() for n, x in pool.items()}
+    table = _table(dev, g, ends, page, pages)
+    status = torch.full((1,), 7, dtype=I32, device=dev)
+    kp.write_pages(pool, k, v, table, _i32(dev, starts), counts=_i32(dev, counts), status=status)
+    assert status.item() == 0
+    for n in NAMES:
+        want, got = before[n], pool[n]
+        raw = (lambda x: x.view(torch.uint8)) if n in "kv" else (lambda x: x)
+        for b in range(3):
+            t = torch.arange(starts[b], ends[b], device=dev)
+            raw(want)[table[b].long()[t // page], t % page] = raw(flat[n])[b, starts[b]:ends[b]]
+        assert torch.equal(raw(want), raw(got)), n
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("B,L", [(2, 3), (3, 700)])
+def test_a_write_of_a_bad_value_writes_nothing(dev, where, value, B, L):
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(1)
+    pages = B * -(-L // 64)
+    pool = _pool(dev, g, pages, 64, 4)
+    before = {n: x.clone() for n, x in pool.items()}
+    table = torch.arange(pages, dtype=I32, device=dev).view(B, -1)
+    kv = {n: torch.randn(B, L, 4, 128, device=dev, generator=g).to(BF16) for n in "kv"}
+    kv[where][B - 1, L - 1, 3, 127] = value
+    start = _i32(dev, [0] * B)
+    status = torch.zeros(1, dtype=I32, device=dev)
+    kp.write_pages(pool, kv["k"], kv["v"], table, start, status=status)
+    assert status.item() == 1
+    with pytest.raises(ValueError, match="non-finite"):
+        kp.write_pages(pool, kv["k"], kv["v"], table, start)
+    for n in NAMES:
+        a, b = (x.view(torch.uint8) if n in "kv" else x for x in (pool[n], before[n]))
+        assert torch.equal(a, b)
+    kv[where][B - 1, L - 1, 3, 127] = 1.0
+    kp.write_pages(pool, kv["k"], kv["v"], table, start, status=status)
+    assert status.item() == 0
+
+
+def test_tokens_without_a_page_are_dropped(dev):
+    """Entries outside the pool, positions past the table, a negative start."""
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(2)
+    pool = _pool(dev, g, 4, 64, 2)
+    before = {n: x.clone() for n, x in pool.items()}
+    table = _i32(dev, [[0, 4], [-1, -7], [2 ** 31 - 1, 1], [2, 3]])
+    k, v = (torch.randn(4, 70, 2, 128, device=dev, generator=g).to(BF16) for _ in range(2))
+    kp.write_pages(pool, k, v, table, _i32(dev, [0, 0, 64, -1]), assume_finite=True)
+    ref = _pool(dev, torch.Generator(device=dev).manual_seed(2), 4, 64, 2)
+    kp.write_pages(ref, k[:1, :64], v[:1, :64], _i32(dev, [[0]]), _i32(dev, [0]))
+    kp.write_pages(ref, k[2:3, :64], v[2:3, :64], _i32(dev, [[1]]), _i32(dev, [0]))
+    for n in NAMES:
+        a, b, c = (x.view(torch.uint8) if n in "kv" else x for x in (pool[n], ref[n], before[n]))
+        assert torch.equal(a, b) and torch.equal(a[2:], c[2:])
+    kp.write_pages(pool, k, v, table, _i32(dev, [2 ** 31 - 1] * 4), assume_finite=True)
+    kp.write_pages(pool, k, v, table[:, :0], _i32(dev, [0] * 4), assume_finite=True)
+    for n in NAMES:
+        a, b = (x.view(torch.uint8) if n in "kv" else x for x in (pool[n], ref[n]))
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("H,page,lens,n", [(3, 64, (0, 1, 200), 200), (8, 256, (700, 9), 1000), (1, 1024, (5,), 3), (2, 64, (64,), 0)])
+def test_read(dev, fmt, H, page, lens, n):
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(n)
+    pages = sum(-(-x // page) for x in lens) + 1
+    pool = _pool(dev, g, pages, page, H, fmt)
+    table = _table(dev, g, lens, page, pages)
+    for key in ("k", "v"):
+        got = kp.read_pages(pool, key, table, _i32(dev, lens), n)
+        assert got.shape == (len(lens), n, H, 128)
+        for b, x in enumerate(lens):
+            m = min(x, n)
+            assert torch.equal(got[b, :m].to(F64), _held(pool, key, table, b, m)) and (got[b, m:] == 0).all()
+
+
+@pytest.mark.parametrize("layers,page,H,pairs", [(None, 64, 3, 1), (3, 64, 24, 5), (2, 1024, 1, 7), (1, 64, 1, 600)])
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_copy(dev, layers, page, H, pairs, fmt):
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(pairs)
+    P = 2 * pairs + 3
+    pool = _pool(dev, g, P, page, H, fmt, layers=layers)
+    before = {n: x.clone() for n, x in pool.items()}
+    order = torch.randperm(P).tolist()
+    dst, src = order[:pairs], [order[pairs + i // 2] for i in range(pairs)]  # (one page to two)
+    kp.copy_pages(pool, src, dst)
+    for n in NAMES:
+        want, got = (x.view(torch.uint8) if n in "kv" else x for x in (before[n], pool[n]))
+        dim = 0 if layers is None else 1
+        want = want.clone().index_copy(dim, torch.tensor(dst, device=dev), want.index_select(dim, torch.tensor(src, device=dev)))
+        assert torch.equal(got, want), n
+
+
+# --------------------------------------------------------------------------
+# streams, graphs
+
+def test_captured_calls_follow_the_tables(dev):
+    """Write and attention captured once, replayed while lengths, tables and values
+    change; two captured graphs beside eager work."""
+    kp, ca, _ = _mods()
+    H, page, B = 4, 64, 3
+    g = torch.Generator(device=dev).manual_seed(9)
+    pool = _pool(dev, g, 60, page, H)
+    table = torch.full((B, 16), -1, dtype=I32, device=dev)
+    start, lens = torch.zeros(2, B, dtype=I32, device=dev).unbind(0)
+    k, v = (torch.zeros(B, 1, H, 128, dtype=BF16, device=dev) for _ in range(2))
+    q = torch.zeros(B, 1, 2 * H, 128, dtype=BF16, device=dev)
+    status = torch.zeros(1, dtype=I32, device=dev)
+
+    def step():
+        kp.write_pages(pool, k, v, table, start, status=status)
+        return ca.paged_attention(q, pool, table, lens)
+
+    step()
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for _ in range(2):
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step())
+        graphs.append(graph)
+    pages = torch.randperm(60)[:48].view(B, 16).to(I32)
+    for i, n in enumerate([(0, 5, 900), (1, 64, 127), (700, 1000, 3), (63, 0, 511)]):
+        now = torch.Generator(device=dev).manual_seed(i)
+        table.copy_(pages.roll(i, 0))
+        start.copy_(_i32(dev, n))
+        lens.copy_(start + 1)
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, device=dev, generator=now).to(BF16))
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        out, lse = (x.clone() for x in outs[i % 2])
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1]) and status.item() == 0
+        _check((out, lse), _reference(q, pool, table, [x + 1 for x in n]), f"replay {i}")
+
+
+def test_calls_on_two_streams(dev):
+    _, ca, _ = _mods()
+    H, page, lens = 2, 64, (3000, 2000)
+    g = torch.Generator(device=dev).manual_seed(4)
+    pages = sum(-(-n // page) for n in lens) + 1
+    pool = _pool(dev, g, pages, page, H)
+    table, n = _table(dev, g, lens, page, pages), _i32(dev, lens)
+    qs = [torch.randn(2, lq, H, 128, device=dev, generator=g).to(BF16) for lq in (1, 1, 40, 150)]
+    want = [ca.paged_attention(q, pool, table, n) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = []
+    for q, s in zip(qs, streams):
+        with torch.cuda.stream(s):
+            got.append([ca.paged_attention(q, pool, table, n) for _ in range(3)])
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        for x in gs:
+            assert torch.equal(x[0], w[0]) and torch.equal(x[1], w[1])
