@@ -7,6 +7,7 @@
 //   hn_attn_key_mass:  mass[t] = sum over query rows of exp(s(row, t) - lse(row)).
 //
 // K, V = bf16(code * scale), as in attn_fp8kv.hip.
+#include "attn_pages.h"
 #include "attn_tiles.h"
 
 namespace hn {
@@ -35,6 +36,8 @@ struct BlockParams : Params {
     int64_t q_block, runs, B;
     int G;                 // query heads per cached head; H counts cached heads
     float* lse;            // [B, H G, Lq]
+    const int32_t* lens;   // of pages: the sequences' tokens
+    int pages;
 };
 
 // Entries of a list before its first negative one. Every wave counts for itself.
@@ -140,7 +143,11 @@ HN_DEVICE void clear_masked_v(TailRegs<4>& r, uint64_t w) {
             for (int d = 0; d < 4; ++d) r.v[j][d] = 0u;
 }
 
-template <int FMT, bool MASK>
+//
+// PAGED: idx is a page table [B, top_k], block a page, and sequence b's tokens are the
+// first lens[b] that its pages hold, in their order; a tile lies in one page and its loads
+// go through descriptors of its own rows. The part of a tile past the length reads as zeros.
+template <int FMT, bool MASK, bool PAGED = false>
 __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     constexpr int NW = 4, BQ = Shape<NW>::BQ;
     __shared__ __attribute__((aligned(16))) uint8_t smem[smem_bytes<NW>()];
@@ -192,7 +199,8 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     }
 
     const int32_t* list = p.idx ? p.idx + b * p.is0 + h * p.is1 + run * p.is2 : nullptr;
-    const int n_cache = list ? list_length(list, p.top_k) << p.shift : (int)((p.kv_len + BKV - 1) / BKV);
+    const int kv_len = PAGED ? __builtin_amdgcn_readfirstlane(seq_len(p.lens, b, p.top_k, p.shift + 6)) : (int)p.kv_len;
+    const int n_cache = list && !PAGED ? list_length(list, p.top_k) << p.shift : (kv_len + BKV - 1) / BKV;
     const int n_tail = (int)((p.cur_len + BKV - 1) / BKV);
     const int n_all = n_cache + n_tail;
     const int t_begin = (int)((int64_t)n_all * split / p.splits);
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     // and of the tail: a tile is a 32-bit byte offset in them, and rows past their
     // ends read as zeros. A span of 2^31 bytes or more is replaced by the tile's own
     // rows, tile by tile.
-    const bool span_ok = p.kv_len > 0 && (p.kv_len - 1) * p.cs1 + D < ((int64_t)1 << 31) &&
+    const bool span_ok = !PAGED && p.kv_len > 0 && (p.kv_len - 1) * p.cs1 + D < ((int64_t)1 << 31) &&
                          ((p.kv_len - 1) * p.ss1 + 1) * 4 < ((int64_t)1 << 31);
     const bool tail_ok = (p.cur_len * p.us1 + D) * 2 < ((int64_t)1 << 31);
     TileBase src = tile_base(p, b, h, 0, span_ok ? (int)p.kv_len : 0);
@@ -230,21 +238,26 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     constexpr uint32_t NOWHERE = 0x80000000u;
     ListReader reader(list, p.top_k);
     auto entry = [&](int t) __attribute__((always_inline)) {  // list entry of cache tile t
+        if constexpr (PAGED) return t < n_cache && t < t_end ? scalar_ints(list)[t >> p.shift] : -1;
         return list && t < n_cache && t < t_end ? reader(t >> p.shift) : 0;
     };
-    const int kv_len = (int)p.kv_len, cur_len = (int)p.cur_len, entries = (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
+    const int cur_len = (int)p.cur_len, entries = PAGED ? p.pages : (kv_len + (BKV << p.shift) - 1) >> (6 + p.shift);
     const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1 * 4u, us1 = (uint32_t)p.us1 * 2u;
     auto cache_place = [&](int t, int e) __attribute__((always_inline)) {
         Place g;
-        const bool there = t < n_cache && t < t_end && e < entries;
-        g.first = !there ? 0 : list ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : t * BKV;
+        const bool there = t < n_cache && t < t_end && (PAGED ? (uint32_t)e < (uint32_t)entries : e < entries);
+        g.first = !there ? 0 : list && !PAGED ? ((e << p.shift) + (t & ((1 << p.shift) - 1))) * BKV : t * BKV;
         const int left = there ? kv_len - g.first : 0;
         g.count = left >= BKV ? BKV : left > 0 ? left : 0;
         g.co = g.count > 0 ? (uint32_t)g.first * cs1 : NOWHERE;
         g.so = g.count > 0 ? (uint32_t)g.first * ss1 : NOWHERE;
         if (!span_ok && g.count > 0) {
-            src = tile_base(p, b, h, g.first, g.count);
-            src.mk = p.kvalid ? p.kvalid + b * p.kvs : nullptr;
+            if constexpr (PAGED) {
+                src = tile_base(p, e, h, (t & ((1 << p.shift) - 1)) * BKV, g.count);
+            } else {
+                src = tile_base(p, b, h, g.first, g.count);
+                src.mk = p.kvalid ? p.kvalid + b * p.kvs : nullptr;
+            }
             g.co = g.so = 0;
         }
         return g;
@@ -1855,6 +1868,69 @@ extern "C" int hn_attn_kv_blocks(int fmt, const void* q, const int64_t* qs, int6
     if (rc != HN_OK || pl.splits == 1) return rc;
     attn::blocks_combine_kernel<<<(unsigned)((B * Hq * Lq + 7) / 8), 256, 0, st>>>(p);
     return check_launch("hn_attn_kv_blocks (combine)");
+}
+
+// Tiles of 128 rows over pages: the plan is that of as many tokens as the table can name.
+static BlocksPlan page_tiles_plan(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
+    // (65 rows at least: the tile kernel whatever their number)
+    const int64_t rows = Lq * (Hq / H), as_rows = rows < 65 ? (65 + Hq / H - 1) / (Hq / H) : Lq;
+    BlocksPlan pl = blocks_plan(B, as_rows, Hq, H, max_len, cur_len, -1, 64, as_rows);
+    pl.q_tiles = (rows + attn::Shape<4>::BQ - 1) / attn::Shape<4>::BQ;
+    pl.work = B * H * pl.q_tiles;
+    return pl;
+}
+
+static int64_t page_tiles_bytes(const BlocksPlan& pl, int64_t rows) {
+    return pl.splits > 1 ? pl.splits * rows * (attn::D + 2) * (int64_t)sizeof(float) : 0;
+}
+
+int64_t hn::page_tiles_workspace(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
+    return page_tiles_bytes(page_tiles_plan(B, Lq, Hq, H, max_len, cur_len), B * Hq * Lq);
+}
+
+int hn::launch_page_tiles(const attn::PageParams& a, int fmt, void* workspace, hipStream_t st) {
+    const int64_t Hq = (int64_t)a.H * a.G, rows = a.B * Hq * a.Lq;
+    const BlocksPlan pl = page_tiles_plan(a.B, a.Lq, Hq, a.H, (int64_t)a.width << a.shift, a.cur_len);
+    const int64_t work = pl.work * pl.splits;
+    HN_REQUIRE(work <= 0x3fffffffLL && rows <= 0x7fffffffLL, HN_E_ARG, "hn_attn_kv_pages: too much work for one launch");
+    attn::BlockParams p = {};
+    p.q = a.q; p.out = a.out; p.lse = a.lse;
+    p.kc = a.kc; p.vc = a.vc; p.ks = a.ks; p.vs = a.vs;
+    p.kcur = a.kcur; p.vcur = a.vcur;
+    p.uvalid = a.uvalid; p.uvs = a.uvs;
+    p.qs0 = a.qs0; p.qs1 = a.qs1; p.qs2 = a.qs2;
+    p.os0 = a.os0; p.os1 = a.os1; p.os2 = a.os2;
+    p.cs0 = a.cs0; p.cs1 = a.cs1; p.cs2 = a.cs2;
+    p.ss0 = a.ss0; p.ss1 = a.ss1; p.ss2 = a.ss2;
+    p.us0 = a.us0; p.us1 = a.us1; p.us2 = a.us2;
+    p.Lq = a.Lq; p.H = a.H; p.G = a.G; p.B = a.B; p.cur_len = a.cur_len;
+    p.scale_log2 = a.scale_log2;
+    p.fmt = fmt;
+    p.idx = a.table; p.is0 = a.ts0;
+    p.top_k = a.width;
+    p.lens = a.lens; p.pages = a.pages;
+    p.block = (int64_t)1 << a.shift;
+    p.shift = a.shift - 6;
+    p.q_block = a.Lq; p.runs = 1;
+    p.q_tiles = (int)pl.q_tiles; p.splits = pl.splits;
+    p.work = (int)work;
+    p.per_xcd = (int)((work + 7) / 8);
+    if (pl.splits > 1) {
+        p.ws_o = (float*)workspace;
+        p.ws_ml = (float*)workspace + pl.splits * rows * attn::D;
+    }
+    const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
+    if (fmt == HN_KV_FP8) {
+        if (p.uvalid) attn::attn_blocks_kernel<HN_KV_FP8, true, true><<<grid, 256, 0, st>>>(p);
+        else attn::attn_blocks_kernel<HN_KV_FP8, false, true><<<grid, 256, 0, st>>>(p);
+    } else {
+        if (p.uvalid) attn::attn_blocks_kernel<HN_KV_INT8, true, true><<<grid, 256, 0, st>>>(p);
+        else attn::attn_blocks_kernel<HN_KV_INT8, false, true><<<grid, 256, 0, st>>>(p);
+    }
+    const int rc = check_launch("hn_attn_kv_pages");
+    if (rc != HN_OK || pl.splits == 1) return rc;
+    attn::blocks_combine_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+    return check_launch("hn_attn_kv_pages (join)");
 }
 
 // Plan of the key mass. Up to 32 rows: key_mass_few_kernel (KB 0), with as many keys a

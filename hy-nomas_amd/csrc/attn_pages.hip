@@ -1,55 +1,19 @@
 // Attention over a paged quantized KV cache (gfx950): the queries of every sequence
 // against its own tokens, page by page, then the bf16 tail; O = softmax(Q K^T scale) V
 // and the rows' log-sum-exp. K, V = bf16(code * scale), as in attn_fp8kv.hip.
-#include "attn_tiles.h"
+#include "attn_pages.h"
 
 namespace hn {
 namespace attn {
 
 typedef float f32x4_ __attribute__((ext_vector_type(4)));
 
-struct PageParams {
-    const uint16_t* q;
-    const uint8_t* kc;
-    const uint8_t* vc;
-    const float* ks;
-    const float* vs;
-    const uint16_t* kcur;
-    const uint16_t* vcur;
-    const uint8_t* uvalid;   // null: every tail key is valid
-    uint16_t* out;
-    float* lse;              // [B, H G, Lq]
-    const int32_t* table;
-    const int32_t* lens;
-    int64_t ts0, uvs;
-    int64_t qs0, qs1, qs2;
-    int64_t cs0, cs1, cs2;   // page, token, head
-    int64_t ss0, ss1, ss2;
-    int64_t us0, us1, us2;
-    int64_t os0, os1, os2;
-    int64_t Lq;
-    int B, H, G;
-    int rows;                // Lq G: row r of a cached head is query r / G, head r % G of its group
-    int runs;                // ceil(rows / rows of a workgroup)
-    int pages, width, shift; // pool, table row, page = 1 << shift
-    int cur_len;
-    int causal;
-    float scale_log2;
-    int whole;               // a workgroup an item; else the units of all items dealt out evenly
-    int wgs;                 // of the second form
-    int per_xcd;             // ceil(workgroups / 8)
-    int pitch;               // rows of a partial result
-    float* ws_o;             // [workgroup][2][pitch][D] unnormalised
-    float* ws_ml;            // [workgroup][2][pitch][2]
-};
+// A value that is the same in every lane, as a scalar.
+HN_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 constexpr int UNIT = 128;    // keys a workgroup takes at a time, 32 a wave
 
-// Cached tokens of sequence b that the table can name.
-HN_DEVICE int seq_len(const PageParams& p, int b) {
-    const int n = p.lens[b], most = p.width << p.shift;
-    return n < 0 ? 0 : n < most ? n : most;
-}
+HN_DEVICE int seq_len(const PageParams& p, int b) { return seq_len(p.lens, b, p.width, p.shift); }
 
 // Units of an item: of the cache, of the tail; one at least (a row without keys is written too).
 HN_DEVICE int cache_units(int len) { return (len + UNIT - 1) / UNIT; }
@@ -80,7 +44,7 @@ struct Line {
         for (int i = lane; i < p.B; i += 64) n += (uint32_t)item_units(p, i);
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-        total = n * (uint32_t)(p.H * p.runs);
+        total = (uint32_t)uniform((int)n) * (uint32_t)(p.H * p.runs);
     }
     // The sequence of unit u, its first unit on the line, the units of each of its items.
     HN_DEVICE void find(uint32_t u, int& b, uint32_t& start, int& n) const {
@@ -138,16 +102,23 @@ struct Rows {
     float m[RB], nm[RB], l[RB];
 };
 
+// Loads go through descriptors of a block's rows in its page: a lane has one offset for
+// its K rows and one for its V rows, what differs between its loads is a scalar. K is
+// asked for again as soon as its operands are formed, V once the product has them, so
+// that one set of registers holds a block and its successor is in flight.
 struct PageRegs {  // codes of a 32-key block
     uint4 k[2][2];
     uint2 v[8];
     float ks[2], vs[8];
-    int left;      // keys from the block's first on that the sequence has; 0: none
-    int first;     // its first token
 };
 
-template <int FMT, int RB>
-__global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
+struct Block {
+    __amdgpu_buffer_rsrc_t k, v, ks, vs;
+    int first, left;  // its first token; keys from there on that the sequence has (<= 0: none)
+};
+
+template <int FMT, int RB, bool SV>
+__global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PageParams p) {
     constexpr int R = 16 * RB, PITCH = D + 4;
     __shared__ __attribute__((aligned(16))) float so[4][R][PITCH];
     __shared__ float sml[4][R][2];
@@ -163,7 +134,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
     if (p.whole) {
         if (wg >= p.B * per) return;
         b = wg / per;
-        n = item_units(p, b);
+        n = uniform(item_units(p, b));
         start = 0;
         u0 = (uint32_t)(wg - b * per) * (uint32_t)n;
         u1 = u0 + (uint32_t)n;
@@ -182,7 +153,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
         if (u0 - start >= (uint32_t)n * (uint32_t)per) {  // the next sequence
             start += (uint32_t)n * (uint32_t)per;
             ++b;
-            n = item_units(p, b);
+            n = uniform(item_units(p, b));
             continue;
         }
         const int item = (int)((u0 - start) / (uint32_t)n);   // h runs + run
@@ -190,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
         const int lo = (int)(u0 - item0), hi = min(n, (int)(u1 - item0));
         const int h = item / p.runs, run = item - h * p.runs;
         const int row0 = run * R, rows = min(R, p.rows - row0);
-        const int len = seq_len(p, b), nc = cache_units(len);
+        const int len = uniform(seq_len(p, b)), nc = cache_units(len);
 
         bf16x8 qf[RB][4];
         int lim[RB];           // this lane's rows see cached tokens below
@@ -248,55 +219,76 @@ __global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
         };
 
         // ---- cached keys
-        const int32_t* row_table = p.table + b * p.ts0;
-        int chunk = -1, held = 0;   // 64 table entries, one a lane
-        auto load = [&](int blk, PageRegs& x) __attribute__((always_inline)) {
+        const ScalarInts row_table = scalar_ints(p.table + b * p.ts0);
+        const int end = 4 * min(hi, nc);
+        // A block's table entry is a scalar load, asked for a block ahead (a vector load's wait
+        // would be for every load before it, the prefetched codes among them).
+        auto entry = [&](int blk) __attribute__((always_inline)) {
+            return row_table[min((32 * blk) >> p.shift, max(p.width - 1, 0))];
+        };
+        const int span_c = 31 * (int)p.cs1 + D, span_s = (31 * (int)p.ss1 + 1) * 4;
+        auto place = [&](int blk, int e) __attribute__((always_inline)) {
+            Block x;
             x.first = blk * 32;
-            x.left = len - x.first;
-            if (blk >= 4 * min(hi, nc) || x.left <= 0) {
-                x.left = 0;
-                return;
-            }
-            const int entry = x.first >> p.shift;
-            if ((entry >> 6) != chunk) {
-                chunk = entry >> 6;
-                held = row_table[min(64 * chunk + lane, p.width - 1)];
-            }
-            const int page = __builtin_amdgcn_readlane(held, entry & 63);
-            if ((uint32_t)page >= (uint32_t)p.pages) {  // no such page: no keys
-                x.left = 0;
-                return;
-            }
+            x.left = blk < end ? len - x.first : 0;
+            if ((uint32_t)e >= (uint32_t)p.pages) x.left = 0;  // no such page: no keys
+            const int page = x.left > 0 ? e : 0;
             const int64_t slot = x.first & ((1 << p.shift) - 1);
             const int64_t ca = page * p.cs0 + slot * p.cs1 + h * p.cs2, sa = page * p.ss0 + slot * p.ss1 + h * p.ss2;
-            const uint8_t *kb = p.kc + ca, *vb = p.vc + ca;
-            const float *kss = p.ks + sa, *vss = p.vs + sa;
-            const uint32_t cs1 = (uint32_t)p.cs1, ss1 = (uint32_t)p.ss1;
+            const int cb = x.left > 0 ? span_c : 0, sb = x.left > 0 ? span_s : 0;
+            x.k = tile_rsrc(p.kc + ca, cb);
+            x.v = tile_rsrc(p.vc + ca, cb);
+            x.ks = tile_rsrc(p.ks + sa, sb);
+            x.vs = tile_rsrc(p.vs + sa, sb);
+            return x;
+        };
+        PageRegs x;
+        const uint32_t cs1 = (uint32_t)p.cs1, ss1 = 4u * (uint32_t)p.ss1;
+        const uint32_t off_k = r16 * cs1 + 16 * g, off_v = 4 * g * cs1 + 8 * r16, off_ks = r16 * ss1, off_vs = 4 * g * ss1;
+        auto load_k = [&](const Block& y, int t) __attribute__((always_inline)) {
+            x.k[t][0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.k, off_k, 16 * t * cs1, 0));
+            x.k[t][1] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.k, off_k + 64, 16 * t * cs1, 0));
+            x.ks[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.ks, off_ks, 16 * t * ss1, 0));
+        };
+        auto load_v = [&](const Block& y) __attribute__((always_inline)) {
+            if constexpr (SV) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t at = (16 * t + r16) * cs1 + 16 * g;
-                x.k[t][0] = *reinterpret_cast<const uint4*>(kb + at);
-                x.k[t][1] = *reinterpret_cast<const uint4*>(kb + at + 64);
-                x.ks[t] = kss[(16 * t + r16) * ss1];
+                for (int t = 0; t < 2; ++t) {
+                    const uint4 w = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.vs, off_vs, 64 * t, 0));
+                    x.vs[4 * t] = __uint_as_float(w.x);
+                    x.vs[4 * t + 1] = __uint_as_float(w.y);
+                    x.vs[4 * t + 2] = __uint_as_float(w.z);
+                    x.vs[4 * t + 3] = __uint_as_float(w.w);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t key = 16 * (j >> 2) + 4 * g + (j & 3);
-                x.v[j] = *reinterpret_cast<const uint2*>(vb + key * cs1 + 8 * r16);
-                x.vs[j] = vss[key * ss1];
+                const uint32_t key = 16 * (j >> 2) + (j & 3);  // + 4 g
+                x.v[j] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(y.v, off_v, key * cs1, 0));
+                if constexpr (!SV)
+                    x.vs[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.vs, off_vs, key * ss1, 0));
             }
         };
-        auto block = [&](PageRegs& x) __attribute__((always_inline)) {
-            if (x.left <= 0) return;
+        int blk = 4 * lo + wave;
+        int e = blk < end ? entry(blk) : 0, e1 = blk + 4 < end ? entry(blk + 4) : 0;
+        Block now = place(blk, e);
+        // (in the loop's order, by which each wait knows its loads)
+        load_k(now, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(now, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(now);
+        __builtin_amdgcn_sched_barrier(0);
+        for (; blk < end; blk += 4) {
+            const Block next = place(blk + 4, e1);
+            e1 = blk + 8 < end ? entry(blk + 8) : 0;
             f32x4_ s[RB][2];
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
+            for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) s[rb][t] = (f32x4_){0.0f, 0.0f, 0.0f, 0.0f};
+                for (int rb = 0; rb < RB; ++rb) s[rb][t] = (f32x4_){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int sl = 0; sl < 4; ++sl)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int sl = 0; sl < 4; ++sl) {
                     uint32_t d[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -306,60 +298,54 @@ __global__ __launch_bounds__(256, 2) void attn_pages_kernel(PageParams p) {
                     const bf16x8 kf = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) s[rb][t] = mfma16_bf16(kf, qf[rb][sl], s[rb][t]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            if (x.first + 32 > lim_all) {
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (x.first + 16 * t + 4 * g + i >= lim[rb]) s[rb][t][i] = -INFINITY;
+                load_k(next, t);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (x.left < 32) {  // what lies behind the sequence's end meets no product
+            if (now.left > 0) {
+                if (now.first + 32 > lim_all) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (16 * (j >> 2) + 4 * g + (j & 3) >= x.left) {
-                        x.v[j] = make_uint2(0u, 0u);
-                        x.vs[j] = 0.0f;
+                    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (now.first + 16 * t + 4 * g + i >= lim[rb]) s[rb][t][i] = -INFINITY;
+                }
+                if (now.left < 32) {  // what lies behind the sequence's end meets no product
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (16 * (j >> 2) + 4 * g + (j & 3) >= now.left) {
+                            x.v[j] = make_uint2(0u, 0u);
+                            x.vs[j] = 0.0f;
+                        }
+                }
+                f16x8 pf[RB];
+                probs(s, pf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f32x2 f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        f[j] = codes2_f32<FMT>(e & 2 ? x.v[j].y : x.v[j].x, e & 1);
+                        f[j][0] *= x.vs[j];
+                        f[j][1] *= x.vs[j];
                     }
-            }
-            f16x8 pf[RB];
-            probs(s, pf);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f32x2 f[8];
+                    for (int w = 0; w < 2; ++w) {
+                        const f16x8 vf = __builtin_bit_cast(
+                            f16x8, make_uint4(pack_f16_of_bf16(f[0][w], f[1][w]), pack_f16_of_bf16(f[2][w], f[3][w]),
+                                              pack_f16_of_bf16(f[4][w], f[5][w]), pack_f16_of_bf16(f[6][w], f[7][w])));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    f[j] = codes2_f32<FMT>(e & 2 ? x.v[j].y : x.v[j].x, e & 1);
-                    f[j][0] *= x.vs[j];
-                    f[j][1] *= x.vs[j];
-                }
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const f16x8 vf = __builtin_bit_cast(
-                        f16x8, make_uint4(pack_f16_of_bf16(f[0][w], f[1][w]), pack_f16_of_bf16(f[2][w], f[3][w]),
-                                          pack_f16_of_bf16(f[4][w], f[5][w]), pack_f16_of_bf16(f[6][w], f[7][w])));
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) st.o[rb][2 * e + w] = mfma16_f16(vf, pf[rb], st.o[rb][2 * e + w]);
+                        for (int rb = 0; rb < RB; ++rb) st.o[rb][2 * e + w] = mfma16_f16(vf, pf[rb], st.o[rb][2 * e + w]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        };
-        {
-            const int end = 4 * min(hi, nc);
-            int t = 4 * lo + wave;
-            PageRegs ra, rb_;
-            load(t, ra);
-            load(t + 4, rb_);
-            while (t < end) {
-                block(ra);
-                t += 4;
-                if (t >= end) break;
-                load(t + 4, ra);
-                block(rb_);
-                t += 4;
-                load(t + 4, rb_);
-            }
+            load_v(next);
+            __builtin_amdgcn_sched_barrier(0);
+            now = next;
         }
         // ---- the tail
         for (int u = max(lo, nc); u < hi; ++u) {
@@ -543,22 +529,33 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
 using namespace hn;
 
 struct PagesPlan {
+    int tiles;   // the tile kernel
     int rb, runs, whole, wgs, pitch;
     int64_t items;
 };
 
-static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len) {
+static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len, int causal) {
     PagesPlan pl;
     const int64_t rows = Lq * G;
+    pl.tiles = !causal && rows > 32;
     pl.rb = rows <= 16 ? 1 : 2;
     const int64_t R = 16 * pl.rb;
     pl.runs = (int)((rows + R - 1) / R);
     pl.items = B * H * pl.runs;
     pl.pitch = (int)(rows < R ? rows : R);
     const int64_t units = (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
-    pl.wgs = 2 * device_cus();
+    pl.wgs = (pl.rb == 1 ? 3 : 2) * device_cus();
     pl.whole = units <= 2 || pl.items >= 8 * (int64_t)pl.wgs;
     return pl;
+}
+
+// SV: the scales of consecutive tokens are consecutive, four to a load.
+template <int FMT>
+static void launch_pages(int rb, bool sv, const attn::PageParams& p, unsigned blocks, hipStream_t st) {
+    if (rb == 1 && sv) attn::attn_pages_kernel<FMT, 1, true><<<blocks, 256, 0, st>>>(p);
+    else if (rb == 1) attn::attn_pages_kernel<FMT, 1, false><<<blocks, 256, 0, st>>>(p);
+    else if (sv) attn::attn_pages_kernel<FMT, 2, true><<<blocks, 256, 0, st>>>(p);
+    else attn::attn_pages_kernel<FMT, 2, false><<<blocks, 256, 0, st>>>(p);
 }
 
 static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
@@ -570,8 +567,8 @@ static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t
 extern "C" int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
                                                    int64_t cur_len, int causal) {
     if (!pages_shape_ok(B, Lq, Hq, H, max_len, cur_len)) return 0;
-    (void)causal;
-    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
+    if (pl.tiles) return page_tiles_workspace(B, Lq, Hq, H, max_len, cur_len);
     return pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
 }
 
@@ -616,10 +613,12 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     HN_REQUIRE(width == 0 || n_pages == 0 || (table && kc && vc && ks && vs), HN_E_ARG, "hn_attn_kv_pages: null pool pointer");
     const int64_t max_len = n_pages ? width * page : 0;
     HN_REQUIRE(pages_shape_ok(B, Lq, Hq, H, max_len, cur_len), HN_E_ARG, "hn_attn_kv_pages: too much work");
-    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
     const int64_t units = 1 + (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
     HN_REQUIRE(pl.items <= 0x3fffffffLL / units, HN_E_ARG, "hn_attn_kv_pages: too much work for one launch");
-    const int64_t need = pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+    const int64_t need = pl.tiles   ? page_tiles_workspace(B, Lq, Hq, H, max_len, cur_len)
+                         : pl.whole ? 0
+                                    : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_attn_kv_pages: workspace smaller than hn_attn_kv_pages_workspace_size() or misaligned");
     if (const int rc = require_gfx950("hn_attn_kv_pages"); rc != HN_OK) return rc;
@@ -646,6 +645,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.cur_len = (int)cur_len;
     p.causal = causal != 0;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
+    if (pl.tiles) return launch_page_tiles(p, fmt, workspace, (hipStream_t)stream);
     p.whole = pl.whole;
     p.wgs = pl.wgs;
     p.pitch = pl.pitch;
@@ -657,15 +657,9 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.per_xcd = (int)((grid + 7) / 8);
     const unsigned blocks = 8u * (unsigned)p.per_xcd;
     const hipStream_t st = (hipStream_t)stream;
-#define HN_PAGES(F, R) attn::attn_pages_kernel<F, R><<<blocks, 256, 0, st>>>(p)
-    if (fmt == HN_KV_FP8) {
-        if (pl.rb == 1) HN_PAGES(HN_KV_FP8, 1);
-        else HN_PAGES(HN_KV_FP8, 2);
-    } else {
-        if (pl.rb == 1) HN_PAGES(HN_KV_INT8, 1);
-        else HN_PAGES(HN_KV_INT8, 2);
-    }
-#undef HN_PAGES
+    const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(vs, 16);
+    if (fmt == HN_KV_FP8) launch_pages<HN_KV_FP8>(pl.rb, sv, p, blocks, st);
+    else launch_pages<HN_KV_INT8>(pl.rb, sv, p, blocks, st);
     if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK || pl.whole) return rc;
     const int R = 16 * pl.rb, groups = (pl.pitch + 7) / 8;
     attn::pages_join_kernel<<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
