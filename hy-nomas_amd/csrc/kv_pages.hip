@@ -19,20 +19,77 @@ struct Pool {  // of one of K, V, or of both (same strides)
     int32_t pages, width, shift;
 };
 
-// The page of token `pos` of sequence b, or -1.
-HN_DEVICE int page_of(const Pool& p, int64_t b, uint32_t pos) {
-    const uint32_t i = pos >> p.shift;
-    if (i >= (uint32_t)p.width) return -1;
-    const int e = p.table[b * p.ts0 + i];
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read by scalar loads: no kernel writes them meanwhile
+
+// ---------------------------------------------------------------------------
+// Rows are (token, head) vectors of 128 values, 8 lanes x 16 values each. A workgroup's
+// tile is 128 rows of one sequence: 2^tsh tokens x 128 / 2^tsh heads, four rows to a lane
+// group, their loads in flight together. A tile's tokens lie in two pages at most, whose
+// numbers are scalars: with 8 values a lane and the rows' places worked out one by one, the
+// instructions were the bound (10800 tokens x 24 heads of two sequences: write 107 us,
+// decode 106).
+constexpr int TILE = 128;
+
+struct Tiles {
+    int32_t L, H, B, tsh;
+    int32_t parts;           // tiles of the same tokens: of their heads (write: of K and V of each)
+    int32_t token_fast;      // rows are enumerated token by token (tokens lie closer than heads)
+};
+
+// A workgroup's tile: the parts of a token range, then the next range, then the next
+// sequence; `back`: from the last one on.
+struct Place {
+    int t0, part;
+};
+
+HN_DEVICE Place tile_place(const Tiles& a, bool back) {
+    const int x = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tt = (uint32_t)x / (uint32_t)a.parts;
+    return {tt << a.tsh, x - tt * a.parts};
+}
+
+struct Row {
+    int t, h;
+    bool there;
+};
+
+// Row g + 32 k of the tile, g = thread / 8.
+HN_DEVICE Row tile_row(const Tiles& a, int t0, int htile, int k, int last) {
+    const int r = (threadIdx.x >> 3) + 32 * k, hsh = 7 - a.tsh;
+    const int tl = a.token_fast ? r & ((1 << a.tsh) - 1) : r >> hsh, hl = a.token_fast ? r >> a.tsh : r & ((1 << hsh) - 1);
+    Row w;
+    w.t = t0 + tl;
+    w.h = (htile << hsh) + hl;
+    w.there = w.t < last && w.h < a.H;
+    return w;
+}
+
+// The pages of a tile whose first token has position `pos`: of its table entry, and of the
+// next one; -1: none.
+struct TilePages {
+    uint32_t entry;
+    int first, next;
+};
+
+HN_DEVICE int page_at(const Pool& p, int64_t b, uint32_t entry) {
+    if (entry >= (uint32_t)p.width) return -1;
+    const int e = ((ScalarInts)(p.table + b * p.ts0))[entry];
     return (uint32_t)e < (uint32_t)p.pages ? e : -1;
 }
 
-// ---------------------------------------------------------------------------
-// Quantize-on-write. A row is one (token, head) vector of 128 values: 16 lanes x 8. A
-// workgroup's unit is 64 rows, 2^tsh tokens x 64 / 2^tsh heads of one sequence, four
-// rows in flight per 16-lane group. HBM bound: 256 bytes read and 132 written a row.
-constexpr int UNIT = 64;
+HN_DEVICE TilePages tile_pages(const Pool& p, int64_t b, uint32_t pos, int tsh) {
+    TilePages t;
+    t.entry = pos >> p.shift;
+    t.first = page_at(p, b, t.entry);
+    t.next = ((pos + (1u << tsh) - 1u) >> p.shift) != t.entry ? page_at(p, b, t.entry + 1) : -1;
+    return t;
+}
 
+HN_DEVICE int page_of(const Pool& p, const TilePages& t, uint32_t pos) {
+    return (pos >> p.shift) == t.entry ? t.first : t.next;
+}
+
+// Quantize-on-write. HBM bound: 256 bytes read and 132 written a row.
 struct WriteArgs {
     const uint16_t* x[2];
     uint8_t* q[2];
@@ -41,148 +98,165 @@ struct WriteArgs {
     int64_t xs0, xs1, xs2;
     const int32_t* start;
     const int32_t* counts;   // null: L new tokens in every sequence
-    int32_t L, H, tsh;
-    int32_t ttiles, htiles, units;
-    int32_t token_fast;      // rows of a unit are enumerated token by token (tokens lie closer than heads)
+    Tiles tiles;
+    float recip;             // not 0: a row's scale is amax times this
     const int32_t* status;
 };
 
-struct Row {
-    int b, t, h;
-    bool there;  // a new token of the sequence
-};
-
-HN_DEVICE Row unit_row(const WriteArgs& a, int unit, int r) {
-    Row w;
-    const int ht = unit % a.htiles, x = unit / a.htiles, tt = x % a.ttiles;
-    w.b = x / a.ttiles;
-    const int hsh = 6 - a.tsh;
-    const int tl = a.token_fast ? r & ((1 << a.tsh) - 1) : r >> hsh, hl = a.token_fast ? r >> a.tsh : r & ((1 << hsh) - 1);
-    w.t = (tt << a.tsh) + tl;
-    w.h = (ht << hsh) + hl;
-    w.there = w.t < a.L && w.h < a.H && (!a.counts || w.t < a.counts[w.b]);
-    return w;
+HN_DEVICE int new_tokens(const WriteArgs& a, int b) {
+    const int n = a.counts ? ((ScalarInts)a.counts)[b] : a.tiles.L;
+    return n < a.tiles.L ? n : a.tiles.L;
 }
 
-HN_DEVICE uint4 row_values(const WriteArgs& a, int sel, const Row& w, int lane16) {
-    return *reinterpret_cast<const uint4*>(a.x[sel] + w.b * a.xs0 + w.t * a.xs1 + w.h * a.xs2 + lane16 * 8);
+struct Values {
+    uint4 a, b;
+};
+
+HN_DEVICE Values row_values(const WriteArgs& a, int sel, int b, const Row& w) {
+    const uint16_t* x = a.x[sel] + b * a.xs0 + w.t * a.xs1 + w.h * a.xs2 + 16 * (threadIdx.x & 7);
+    return {reinterpret_cast<const uint4*>(x)[0], reinterpret_cast<const uint4*>(x)[1]};
+}
+
+HN_DEVICE float max8(float v) {  // over the 8 lanes of an aligned group
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true)));
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true)));
 }
 
 __global__ void pages_clear_kernel(int32_t* status) {
     if (threadIdx.x == 0) *status = 0;
 }
 
-// Sets *status where a new token's value is NaN or Inf (its bf16 exponent is all ones).
+// Sets *status where a new token's value is NaN or Inf: the largest magnitude's bits of
+// either half of the words are then 0x7f80 or more.
 __global__ __launch_bounds__(256) void pages_check_kernel(WriteArgs a, int32_t* status) {
-    const int lane16 = threadIdx.x & 15, g = threadIdx.x >> 4, sel = blockIdx.y;
-    uint32_t bad = 0u;
-    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        uint4 v[4];
+    const Place at = tile_place(a.tiles, false);
+    const int sel = at.part & 1;
+    for (int b = blockIdx.y; b < a.tiles.B; b += gridDim.y) {
+        const int last = new_tokens(a, b);
+        if (at.t0 >= last) continue;
+        Values v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const Row w = unit_row(a, unit, g + 16 * k);
-            v[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (w.there) v[k] = row_values(a, sel, w, lane16);
+            const Row w = tile_row(a.tiles, at.t0, at.part >> 1, k, last);
+            v[k] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+            if (w.there) v[k] = row_values(a, sel, b, w);
         }
+        u16x2 top = {0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+            const uint32_t w[8] = {v[k].a.x, v[k].a.y, v[k].a.z, v[k].a.w, v[k].b.x, v[k].b.y, v[k].b.z, v[k].b.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                bad |= (uint32_t)((w[j] & 0x7f80u) == 0x7f80u) | (uint32_t)((w[j] & 0x7f800000u) == 0x7f800000u);
+            for (int j = 0; j < 8; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
         }
+        if (__any(top[0] >= 0x7f80u || top[1] >= 0x7f80u) && (threadIdx.x & 63) == 0) *status = 1;
     }
-    if (__any(bad != 0u) && (threadIdx.x & 63) == 0) *status = 1;
 }
 
 template <int FMT>
 __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
     if (a.status != nullptr && *a.status != 0) return;  // refused: nothing is written
-    const int lane16 = threadIdx.x & 15, g = threadIdx.x >> 4, sel = blockIdx.y;
-    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        uint4 v[4];
+    // (from the last tile on: what the check has read last may be in a cache yet)
+    const Place at = tile_place(a.tiles, true);
+    const int sel = at.part & 1, t0 = at.t0;
+    for (int b = gridDim.y - 1 - blockIdx.y; b < a.tiles.B; b += gridDim.y) {
+        const int last = new_tokens(a, b);
+        const int first = ((ScalarInts)a.start)[b];
+        if (t0 >= last || first < 0) continue;
+        const uint32_t pos0 = (uint32_t)first + (uint32_t)t0;
+        const TilePages pages = tile_pages(a.pool, b, pos0, a.tiles.tsh);
+        Values v[4];
         Row w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            w[k] = unit_row(a, unit, g + 16 * k);
-            if (w[k].there) v[k] = row_values(a, sel, w[k], lane16);
+            w[k] = tile_row(a.tiles, t0, at.part >> 1, k, last);
+            if (w[k].there) v[k] = row_values(a, sel, b, w[k]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (!w[k].there) continue;
-            const int first = a.start[w[k].b];
-            const uint32_t pos = (uint32_t)first + (uint32_t)w[k].t;
-            const int page = first < 0 ? -1 : page_of(a.pool, w[k].b, pos);
-            const uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-            float f[8];
+            const uint32_t pos = pos0 + (uint32_t)(w[k].t - t0);
+            const int page = page_of(a.pool, pages, pos);
+            if (!w[k].there || page < 0) continue;
+            const uint32_t x[8] = {v[k].a.x, v[k].a.y, v[k].a.z, v[k].a.w, v[k].b.x, v[k].b.y, v[k].b.z, v[k].b.w};
+            float lo[8], hi[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                f[2 * j] = bf16_lo(x[j]);
-                f[2 * j + 1] = bf16_hi(x[j]);
+                lo[2 * j] = bf16_lo(x[j]);
+                lo[2 * j + 1] = bf16_hi(x[j]);
+                hi[2 * j] = bf16_lo(x[4 + j]);
+                hi[2 * j + 1] = bf16_hi(x[4 + j]);
             }
             float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]));
-            amax = group_max<16>(amax);
-            const float s = amax > 0.0f ? amax / (FMT == HN_KV_FP8 ? kE4M3Max : 127.0f) : 1.0f;
-            if (page < 0) continue;
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(fabsf(lo[j]), fabsf(hi[j])));
+            amax = max8(amax);
+            const float quot = a.recip != 0.0f ? amax * a.recip : amax / (FMT == HN_KV_FP8 ? kE4M3Max : 127.0f);
+            const float s = amax > 0.0f ? quot : 1.0f;
+            const Quot d(s);
+            const uint2 c0 = codes8<FMT == HN_KV_FP8>(lo, d), c1 = codes8<FMT == HN_KV_FP8>(hi, d);
             const int64_t slot = pos & ((1u << a.pool.shift) - 1u);
-            *reinterpret_cast<uint2*>(a.q[sel] + page * a.pool.qs0 + slot * a.pool.qs1 + w[k].h * a.pool.qs2 + lane16 * 8) =
-                codes8<FMT == HN_KV_FP8>(f, Quot(s));
-            if (lane16 == 0) a.s[sel][page * a.pool.ss0 + slot * a.pool.ss1 + w[k].h * a.pool.ss2] = s;
+            uint8_t* q = a.q[sel] + page * a.pool.qs0 + slot * a.pool.qs1 + w[k].h * a.pool.qs2 + 16 * (threadIdx.x & 7);
+            *reinterpret_cast<uint4*>(q) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+            if ((threadIdx.x & 7) == 0) a.s[sel][page * a.pool.ss0 + slot * a.pool.ss1 + w[k].h * a.pool.ss2] = s;
         }
     }
 }
 
-// ---------------------------------------------------------------------------
-// A sequence decoded: y[b, t, h] = bf16(code * scale), zeros past its length. 16 lanes a
-// row, four rows in flight. HBM bound: 132 bytes read and 256 written a row.
+// A sequence decoded: y[b, t, h] = bf16(code * scale), zeros past its length. HBM bound:
+// 132 bytes read and 256 written a row.
 struct ReadArgs {
     const uint8_t* q;
     const float* s;
     uint16_t* y;
     Pool pool;
     const int32_t* lens;
-    int32_t L, H;
-    int64_t rows;  // B L H
+    Tiles tiles;
 };
+
+// Two codes (bytes 2 hi, 2 hi + 1 of w) -> bf16(code * s), packed.
+template <int FMT>
+HN_DEVICE uint32_t held2(uint32_t w, bool hi, float s) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if (FMT == HN_KV_FP8) {
+        const f32x2 f = hi ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, true)
+                           : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, false);
+        return f32x2_to_bf16x2(f[0] * s, f[1] * s);
+    }
+    const int sh = hi ? 16 : 0;
+    return f32x2_to_bf16x2((float)(int8_t)(w >> sh) * s, (float)(int8_t)(w >> (sh + 8)) * s);
+}
 
 template <int FMT>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
-    const int lane16 = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const uint32_t per = (uint32_t)a.L * (uint32_t)a.H;
-    for (int64_t r0 = (int64_t)blockIdx.x * UNIT; r0 < a.rows; r0 += (int64_t)gridDim.x * UNIT) {
-        uint2 c[4];
+    const Place at = tile_place(a.tiles, false);
+    const int t0 = at.t0;
+    for (int b = blockIdx.y; b < a.tiles.B; b += gridDim.y) {
+        const int len = ((ScalarInts)a.lens)[b];
+        const TilePages pages = tile_pages(a.pool, b, (uint32_t)t0, a.tiles.tsh);
+        uint4 c[4];
         float s[4];
+        Row w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t row = r0 + 16 * k + g;
-            c[k] = make_uint2(0u, 0u);
+            w[k] = tile_row(a.tiles, t0, at.part, k, a.tiles.L);
+            c[k] = make_uint4(0u, 0u, 0u, 0u);
             s[k] = 0.0f;
-            if (row >= a.rows) continue;
-            const int64_t b = row / per;
-            const uint32_t in = (uint32_t)(row - b * per), t = in / (uint32_t)a.H, h = in - t * (uint32_t)a.H;
-            if ((int)t >= a.lens[b]) continue;
-            const int page = page_of(a.pool, b, t);
-            if (page < 0) continue;
-            const int64_t slot = t & ((1u << a.pool.shift) - 1u);
-            c[k] = *reinterpret_cast<const uint2*>(a.q + page * a.pool.qs0 + slot * a.pool.qs1 + h * a.pool.qs2 + lane16 * 8);
-            s[k] = a.s[page * a.pool.ss0 + slot * a.pool.ss1 + h * a.pool.ss2];
+            const int page = page_of(a.pool, pages, (uint32_t)w[k].t);
+            if (!w[k].there || w[k].t >= len || page < 0) continue;
+            const int64_t slot = w[k].t & ((1 << a.pool.shift) - 1);
+            c[k] = *reinterpret_cast<const uint4*>(a.q + page * a.pool.qs0 + slot * a.pool.qs1 + w[k].h * a.pool.qs2 +
+                                                   16 * (threadIdx.x & 7));
+            s[k] = a.s[page * a.pool.ss0 + slot * a.pool.ss1 + w[k].h * a.pool.ss2];
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t row = r0 + 16 * k + g;
-            if (row >= a.rows) continue;
-            const uint32_t cw[2] = {c[k].x, c[k].y};
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t b0 = (cw[j >> 1] >> (16 * (j & 1))) & 0xffu, b1 = (cw[j >> 1] >> (16 * (j & 1) + 8)) & 0xffu;
-                const float v0 = FMT == HN_KV_FP8 ? e4m3_decode(b0) : (float)(int8_t)b0;
-                const float v1 = FMT == HN_KV_FP8 ? e4m3_decode(b1) : (float)(int8_t)b1;
-                o[j] = f32x2_to_bf16x2(v0 * s[k], v1 * s[k]);
-            }
-            *reinterpret_cast<uint4*>(a.y + row * 128 + lane16 * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+            if (!w[k].there) continue;
+            uint4* y = reinterpret_cast<uint4*>(a.y + (((int64_t)b * a.tiles.L + w[k].t) * a.tiles.H + w[k].h) * 128 +
+                                                16 * (threadIdx.x & 7));
+            y[0] = make_uint4(held2<FMT>(c[k].x, false, s[k]), held2<FMT>(c[k].x, true, s[k]),
+                              held2<FMT>(c[k].y, false, s[k]), held2<FMT>(c[k].y, true, s[k]));
+            y[1] = make_uint4(held2<FMT>(c[k].z, false, s[k]), held2<FMT>(c[k].z, true, s[k]),
+                              held2<FMT>(c[k].w, false, s[k]), held2<FMT>(c[k].w, true, s[k]));
         }
     }
 }
@@ -261,6 +335,20 @@ static int pool_args(const char* who, const int64_t* cs, const int64_t* ss, int6
     return HN_OK;
 }
 
+// Tiles of B x L x H rows of `arrays` arrays: as many tokens as there are, up to 16 (eight
+// heads beside them). False: too many for one launch.
+static bool tiles_of(int64_t B, int64_t L, int64_t H, int arrays, bool token_fast, pages::Tiles& t, dim3& grid) {
+    t.B = (int32_t)B; t.L = (int32_t)L; t.H = (int32_t)H;
+    t.token_fast = token_fast;
+    t.tsh = 0;
+    while (t.tsh < 4 && (1 << t.tsh) < L) ++t.tsh;
+    const int64_t ranges = (L - 1) / (1 << t.tsh) + 1, parts = ((H - 1) / (pages::TILE >> t.tsh) + 1) * arrays;
+    if (parts > 0x7fffffffLL || ranges > 0x7fffffffLL / parts) return false;
+    t.parts = (int32_t)parts;
+    grid = dim3((unsigned)(ranges * parts), (unsigned)(B < 65535 ? B : 65535));
+    return true;
+}
+
 extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const int64_t* xs, int64_t B, int64_t L,
                                  int64_t H, int64_t D, void* kc, void* vc, const int64_t* cs, float* ks, float* vs,
                                  const int64_t* ss, int64_t n_pages, int64_t page, const int32_t* table,
@@ -291,16 +379,9 @@ extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const in
     a.s[0] = ks; a.s[1] = vs;
     a.xs0 = xs[0]; a.xs1 = xs[1]; a.xs2 = xs[2];
     a.start = start; a.counts = counts;
-    a.L = (int32_t)L; a.H = (int32_t)H;
-    a.token_fast = xs[1] < xs[2];
-    a.tsh = 0;
-    while (a.tsh < 4 && (1 << a.tsh) < L) ++a.tsh;
-    a.ttiles = (int32_t)((L - 1) / (1 << a.tsh) + 1);
-    a.htiles = (int32_t)((H - 1) / (pages::UNIT >> a.tsh) + 1);
-    HN_REQUIRE(B * a.ttiles <= 0x7fffffffLL / a.htiles, HN_E_ARG, "hn_kv_pages_write: too many rows");
-    a.units = (int32_t)(B * a.ttiles * a.htiles);
+    dim3 grid;
+    HN_REQUIRE(tiles_of(B, L, H, 2, xs[1] < xs[2], a.tiles, grid), HN_E_ARG, "hn_kv_pages_write: too many rows");
     a.status = status;
-    const dim3 grid((unsigned)stream_grid(a.units, 8), 2);
     if (status) pages::pages_check_kernel<<<grid, 256, 0, st>>>(a, status);
     if (fmt == HN_KV_FP8) pages::pages_write_kernel<HN_KV_FP8><<<grid, 256, 0, st>>>(a);
     else pages::pages_write_kernel<HN_KV_INT8><<<grid, 256, 0, st>>>(a);
@@ -322,13 +403,12 @@ extern "C" int hn_kv_pages_read(int fmt, const void* kc, const int64_t* cs, cons
     if (B == 0 || L == 0) return HN_OK;
     HN_REQUIRE(y && lens && (width == 0 || table) && (n_pages == 0 || (kc && ks)), HN_E_ARG,
                "hn_kv_pages_read: null pointer");
-    HN_REQUIRE(L <= 0x7fffffffLL / H && B <= 0x7fffffffLL, HN_E_ARG, "hn_kv_pages_read: too many rows per sequence");
+    HN_REQUIRE(B <= 0x7fffffffLL && L <= 0x7fffffffLL && H <= 0x7fffffffLL, HN_E_ARG, "hn_kv_pages_read: too many rows");
     if (const int rc = require_gfx950(who); rc != HN_OK) return rc;
     a.q = (const uint8_t*)kc; a.s = ks; a.y = (uint16_t*)y;
     a.lens = lens;
-    a.L = (int32_t)L; a.H = (int32_t)H;
-    a.rows = B * L * H;
-    const unsigned grid = (unsigned)stream_grid((a.rows + pages::UNIT - 1) / pages::UNIT, 16);
+    dim3 grid;
+    HN_REQUIRE(tiles_of(B, L, H, 1, false, a.tiles, grid), HN_E_ARG, "hn_kv_pages_read: too many rows");
     if (fmt == HN_KV_FP8) pages::pages_read_kernel<HN_KV_FP8><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else pages::pages_read_kernel<HN_KV_INT8><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     return check_launch(who);
