@@ -74,13 +74,9 @@ struct Line {
 HN_DEVICE f32x4_ mfma16_bf16(const bf16x8& a, const bf16x8& b, const f32x4_& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-HN_DEVICE f32x4_ mfma16_f16(const f16x8& a, const f16x8& b, const f32x4_& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
 
-// Probabilities of 2^11 to 2^15 for a row's largest (attn_blocks.hip: fp16 then holds
-// those down to 2^-25 of it in full).
-constexpr float TOP_LOW = 11.0f, TOP_HIGH = 15.0f;
+// How far (log2) a logit may pass the point that a row's probabilities refer to.
+constexpr float TOP_HIGH = 8.0f;
 
 // ---------------------------------------------------------------------------
 // Few rows against many keys: single tokens, drafted ones, grouped heads. The read of
@@ -102,15 +98,30 @@ struct Rows {
     float m[RB], nm[RB], l[RB];
 };
 
+// Probabilities are held as the sum of two bf16 (2^-17 relative): V^ is bf16 as it stands,
+// where as fp16 it would take one more instruction a value, and the matrix unit has room
+// for the second product.
 // Loads go through descriptors of a block's rows in its page: a lane has one offset for
 // its K rows and one for its V rows, what differs between its loads is a scalar. K is
 // asked for again as soon as its operands are formed, V once the product has them, so
 // that one set of registers holds a block and its successor is in flight.
+struct Probs {
+    bf16x8 hi, lo;
+};
+
+HN_DEVICE void weigh(const bf16x8& v, const Probs& p, f32x4_& o) {
+    o = mfma16_bf16(v, p.hi, o);
+    o = mfma16_bf16(v, p.lo, o);
+}
+
 struct PageRegs {  // codes of a 32-key block
-    uint4 k[2][2];
+    uint4 k[4];    // load i: dims 16 (lane % 8) .. of key 8 i + lane / 8
     uint2 v[8];
     float ks[2], vs[8];
 };
+
+constexpr int K_TILE = 32 * D;  // bytes of a block's K codes in LDS
+constexpr int ONCE = 2;         // loads that pass the caches by (nt): whole lines that nothing reads again
 
 struct Block {
     __amdgpu_buffer_rsrc_t k, v, ks, vs;
@@ -121,6 +132,7 @@ template <int FMT, int RB, bool SV>
 __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PageParams p) {
     constexpr int R = 16 * RB, PITCH = D + 4;
     __shared__ __attribute__((aligned(16))) float so[4][R][PITCH];
+    static_assert(sizeof(so[0]) >= K_TILE, "a wave's K codes fit where its result goes");
     __shared__ float sml[4][R][2];
     const int id = blockIdx.x;
     const int wg = (id & 7) * p.per_xcd + (id >> 3);
@@ -187,7 +199,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         }
 
         // Probabilities of a block's logits s[rb][t] (masked ones -inf), as the P operand.
-        auto probs = [&](f32x4_ (&s)[RB][2], f16x8 (&pf)[RB]) __attribute__((always_inline)) {
+        auto probs = [&](f32x4_ (&s)[RB][2], Probs (&pf)[RB]) __attribute__((always_inline)) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 float mx = -INFINITY;
@@ -198,7 +210,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                 if (__any(mx * c > st.m[rb] + TOP_HIGH)) {
                     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                    const float mnew = fmaxf(st.m[rb], mx * c - TOP_LOW);
+                    const float mnew = fmaxf(st.m[rb], mx * c);
                     const float a = st.m[rb] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m[rb] - mnew);
                     st.m[rb] = mnew;
                     st.nm[rb] = mnew == -INFINITY ? 0.0f : -mnew;
@@ -206,15 +218,17 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
 #pragma unroll
                     for (int db = 0; db < 8; ++db) st.o[rb][db] *= a;
                 }
-                uint32_t x[4];
+                uint32_t x[4], y[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][e >> 1][2 * (e & 1)], c, st.nm[rb]));
                     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][e >> 1][2 * (e & 1) + 1], c, st.nm[rb]));
-                    x[e] = pack_f16(p0, p1);
+                    x[e] = pack_bf16(p0, p1);
+                    y[e] = pack_bf16(p0 - bf16_lo(x[e]), p1 - bf16_hi(x[e]));
                     st.l[rb] += p0 + p1;
                 }
-                pf[rb] = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
+                pf[rb].hi = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+                pf[rb].lo = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
             }
         };
 
@@ -226,29 +240,37 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         auto entry = [&](int blk) __attribute__((always_inline)) {
             return row_table[min((32 * blk) >> p.shift, max(p.width - 1, 0))];
         };
-        const int span_c = 31 * (int)p.cs1 + D, span_s = (31 * (int)p.ss1 + 1) * 4;
+        const int span_c = 31 * (int)p.cs1 + D, span_s = (31 * (int)p.ss1 + 1) * 4, in_page = (1 << p.shift) - 1;
+        const uint8_t *kh = p.kc + h * p.cs2, *vh = p.vc + h * p.cs2;
+        const float *ksh = p.ks + h * p.ss2, *vsh = p.vs + h * p.ss2;
         auto place = [&](int blk, int e) __attribute__((always_inline)) {
             Block x;
             x.first = blk * 32;
             x.left = blk < end ? len - x.first : 0;
             if ((uint32_t)e >= (uint32_t)p.pages) x.left = 0;  // no such page: no keys
             const int page = x.left > 0 ? e : 0;
-            const int64_t slot = x.first & ((1 << p.shift) - 1);
-            const int64_t ca = page * p.cs0 + slot * p.cs1 + h * p.cs2, sa = page * p.ss0 + slot * p.ss1 + h * p.ss2;
+            const int64_t slot = x.first & in_page;
+            const int64_t ca = page * p.cs0 + slot * p.cs1, sa = page * p.ss0 + slot * p.ss1;
             const int cb = x.left > 0 ? span_c : 0, sb = x.left > 0 ? span_s : 0;
-            x.k = tile_rsrc(p.kc + ca, cb);
-            x.v = tile_rsrc(p.vc + ca, cb);
-            x.ks = tile_rsrc(p.ks + sa, sb);
-            x.vs = tile_rsrc(p.vs + sa, sb);
+            x.k = tile_rsrc(kh + ca, cb);
+            x.v = tile_rsrc(vh + ca, cb);
+            x.ks = tile_rsrc(ksh + sa, sb);
+            x.vs = tile_rsrc(vsh + sa, sb);
             return x;
         };
         PageRegs x;
         const uint32_t cs1 = (uint32_t)p.cs1, ss1 = 4u * (uint32_t)p.ss1;
-        const uint32_t off_k = r16 * cs1 + 16 * g, off_v = 4 * g * cs1 + 8 * r16, off_ks = r16 * ss1, off_vs = 4 * g * ss1;
-        auto load_k = [&](const Block& y, int t) __attribute__((always_inline)) {
-            x.k[t][0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.k, off_k, 16 * t * cs1, 0));
-            x.k[t][1] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.k, off_k + 64, 16 * t * cs1, 0));
-            x.ks[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.ks, off_ks, 16 * t * ss1, 0));
+        const uint32_t off_k = (lane >> 3) * cs1 + 16 * (lane & 7), off_v = 4 * g * cs1 + 8 * r16, off_ks = r16 * ss1,
+                       off_vs = 4 * g * ss1;
+        uint8_t* const kt = reinterpret_cast<uint8_t*>(&so[wave][0][0]);  // (this wave's alone until the waves meet)
+        uint8_t* const kt_in = kt + (lane >> 3) * D + 16 * ((lane & 7) ^ (lane >> 3));
+        auto load_k = [&](const Block& y) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                x.ks[t] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.ks, off_ks, 16 * t * ss1, 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x.k[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(y.k, off_k, 8 * i * cs1, ONCE));
         };
         auto load_v = [&](const Block& y) __attribute__((always_inline)) {
             if constexpr (SV) {
@@ -264,7 +286,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t key = 16 * (j >> 2) + (j & 3);  // + 4 g
-                x.v[j] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(y.v, off_v, key * cs1, 0));
+                x.v[j] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(y.v, off_v, key * cs1, ONCE));
                 if constexpr (!SV)
                     x.vs[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.vs, off_vs, key * ss1, 0));
             }
@@ -273,15 +295,26 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         int e = blk < end ? entry(blk) : 0, e1 = blk + 4 < end ? entry(blk + 4) : 0;
         Block now = place(blk, e);
         // (in the loop's order, by which each wait knows its loads)
-        load_k(now, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(now, 1);
+        load_k(now);
         __builtin_amdgcn_sched_barrier(0);
         load_v(now);
         __builtin_amdgcn_sched_barrier(0);
         for (; blk < end; blk += 4) {
             const Block next = place(blk + 4, e1);
             e1 = blk + 8 < end ? entry(blk + 8) : 0;
+            // K codes through the wave's own LDS tile (chunk c of row r at c ^ r % 8)
+            uint4 kx[2][2];
+            const float ks[2] = {x.ks[0], x.ks[1]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(kt_in + 8 * i * D) = x.k[i];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    kx[t][e] = *reinterpret_cast<const uint4*>(kt + (16 * t + r16) * D + 16 * ((g + 4 * e) ^ (r16 & 7)));
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(next);
+            __builtin_amdgcn_sched_barrier(0);
             f32x4_ s[RB][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -292,16 +325,14 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                     uint32_t d[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const f32x2 f = codes2_f32<FMT>(word(x.k[t][sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
-                        d[e] = pack_bf16(f[0] * x.ks[t], f[1] * x.ks[t]);
+                        const f32x2 f = codes2_f32<FMT>(word(kx[t][sl >> 1], 2 * (sl & 1) + (e >> 1)), e & 1);
+                        d[e] = pack_bf16(f[0] * ks[t], f[1] * ks[t]);
                     }
                     const bf16x8 kf = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) s[rb][t] = mfma16_bf16(kf, qf[rb][sl], s[rb][t]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                load_k(next, t);
-                __builtin_amdgcn_sched_barrier(0);
             }
             if (now.left > 0) {
                 if (now.first + 32 > lim_all) {
@@ -321,7 +352,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                             x.vs[j] = 0.0f;
                         }
                 }
-                f16x8 pf[RB];
+                Probs pf[RB];
                 probs(s, pf);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -334,11 +365,11 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                     }
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const f16x8 vf = __builtin_bit_cast(
-                            f16x8, make_uint4(pack_f16_of_bf16(f[0][w], f[1][w]), pack_f16_of_bf16(f[2][w], f[3][w]),
-                                              pack_f16_of_bf16(f[4][w], f[5][w]), pack_f16_of_bf16(f[6][w], f[7][w])));
+                        const bf16x8 vf = __builtin_bit_cast(
+                            bf16x8, make_uint4(pack_bf16(f[0][w], f[1][w]), pack_bf16(f[2][w], f[3][w]),
+                                               pack_bf16(f[4][w], f[5][w]), pack_bf16(f[6][w], f[7][w])));
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) st.o[rb][2 * e + w] = mfma16_f16(vf, pf[rb], st.o[rb][2 * e + w]);
+                        for (int rb = 0; rb < RB; ++rb) weigh(vf, pf[rb], st.o[rb][2 * e + w]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -382,7 +413,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                 if ((live >> key) & 1u)
                     vx[j] = *reinterpret_cast<const uint4*>(p.vcur + at + (int64_t)(first + key) * p.us1 + 8 * r16);
             }
-            f16x8 pf[RB];
+            Probs pf[RB];
             probs(s, pf);
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
@@ -390,12 +421,11 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t a = word(vx[2 * e], db >> 1), z = word(vx[2 * e + 1], db >> 1);
-                    y[e] = __builtin_bit_cast(uint32_t, db & 1 ? __builtin_amdgcn_cvt_pkrtz(bf16_hi(a), bf16_hi(z))
-                                                               : __builtin_amdgcn_cvt_pkrtz(bf16_lo(a), bf16_lo(z)));
+                    y[e] = __builtin_amdgcn_perm(z, a, db & 1 ? 0x07060302u : 0x05040100u);  // high or low halves
                 }
-                const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(y[0], y[1], y[2], y[3]));
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(y[0], y[1], y[2], y[3]));
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) st.o[rb][db] = mfma16_f16(vf, pf[rb], st.o[rb][db]);
+                for (int rb = 0; rb < RB; ++rb) weigh(vf, pf[rb], st.o[rb][db]);
             }
         }
         // ---- the waves meet
