@@ -33,8 +33,7 @@ struct PageParams {
     int cur_len;
     int causal;
     float scale_log2;
-    int whole;               // a workgroup an item; else the units of all items dealt out evenly
-    int wgs;                 // of the second form
+    int wgs;                 // workgroups that the units of all items are dealt out to
     int per_xcd;             // ceil(workgroups / 8)
     int pitch;               // rows of a partial result
     float* ws_o;             // [workgroup][2][pitch][D] unnormalised

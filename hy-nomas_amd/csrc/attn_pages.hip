@@ -11,62 +11,81 @@ typedef float f32x4_ __attribute__((ext_vector_type(4)));
 // A value that is the same in every lane, as a scalar.
 HN_DEVICE int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-constexpr int UNIT = 128;    // keys a workgroup takes at a time, 32 a wave
+// A workgroup of NW waves takes 32 NW keys at a time, a unit. Items are dealt out in units
+// of four waves.
+constexpr int UNIT = 128;
 
 HN_DEVICE int seq_len(const PageParams& p, int b) { return seq_len(p.lens, b, p.width, p.shift); }
 
 // Units of an item: of the cache, of the tail; one at least (a row without keys is written too).
-HN_DEVICE int cache_units(int len) { return (len + UNIT - 1) / UNIT; }
-HN_DEVICE int tail_units(const PageParams& p) { return (p.cur_len + UNIT - 1) / UNIT; }
-HN_DEVICE int item_units(const PageParams& p, int b) {
-    const int n = cache_units(seq_len(p, b)) + tail_units(p);
+HN_DEVICE int units_of(int keys, int unit) { return (keys + unit - 1) / unit; }
+HN_DEVICE int item_units(const PageParams& p, int b, int unit = UNIT) {
+    const int n = units_of(seq_len(p, b), unit) + units_of(p.cur_len, unit);
     return n > 0 ? n : 1;
 }
 
-HN_DEVICE uint32_t wave_scan(uint32_t v) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(v, off, 64);
-        if (lane >= off) v += o;
-    }
+HN_DEVICE uint32_t wave_scan(uint32_t v) {  // inclusive, over the wave
+#define HN_SCAN(CTRL, ROWS) \
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)
+    HN_SCAN(0x111, 0xf);  // from 1, 2, 4 and 8 lanes before in the row of 16
+    HN_SCAN(0x112, 0xf);
+    HN_SCAN(0x114, 0xf);
+    HN_SCAN(0x118, 0xf);
+    HN_SCAN(0x142, 0xa);  // the row before's last lane
+    HN_SCAN(0x143, 0xc);  // the first half's last lane
+#undef HN_SCAN
     return v;
 }
 
 // Where the items lie on the line of all units: sequence after sequence, in each head
-// after head, run after run. `total` units; at(u) finds the item of unit u.
+// after head, run after run. Up to 64 sequences are held in a register of the wave, a lane
+// each; more are read again where they are needed.
 struct Line {
     const PageParams& p;
-    uint32_t total;
-    HN_DEVICE explicit Line(const PageParams& pp) : p(pp), total(0) {
+    uint32_t per, total;
+    int mine;        // lane's sequence: units of an item
+    uint32_t end;    // and the line's up to its last item
+    HN_DEVICE explicit Line(const PageParams& pp) : p(pp), per((uint32_t)(pp.H * pp.runs)), total(0) {
         const int lane = threadIdx.x & 63;
-        uint32_t n = 0;
-        for (int i = lane; i < p.B; i += 64) n += (uint32_t)item_units(p, i);
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-        total = (uint32_t)uniform((int)n) * (uint32_t)(p.H * p.runs);
+        for (int i0 = 0; i0 < p.B; i0 += 64) {
+            mine = i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
+            end = wave_scan((uint32_t)mine) * per;
+            total += (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+        }
     }
     // The sequence of unit u, its first unit on the line, the units of each of its items.
     HN_DEVICE void find(uint32_t u, int& b, uint32_t& start, int& n) const {
         const int lane = threadIdx.x & 63;
-        const uint32_t per = (uint32_t)(p.H * p.runs);
         uint32_t before = 0;
         b = 0;
         start = 0;
         n = 1;
         for (int i0 = 0; i0 < p.B; i0 += 64) {
-            const int mine = i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
-            const uint32_t end = wave_scan((uint32_t)mine * per);
-            const uint64_t past = __ballot(before + end > u);
+            const int m = p.B <= 64 ? mine : i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
+            const uint32_t e = p.B <= 64 ? end : wave_scan((uint32_t)m) * per;
+            const uint64_t past = __ballot(before + e > u);
             if (past) {
                 const int l = __builtin_ctzll(past);
                 b = i0 + l;
-                n = __builtin_amdgcn_readlane(mine, l);
-                start = before + __builtin_amdgcn_readlane(end, l) - (uint32_t)n * per;
+                n = __builtin_amdgcn_readlane(m, l);
+                start = before + (uint32_t)__builtin_amdgcn_readlane((int)e, l) - (uint32_t)n * per;
                 return;
             }
-            before += __builtin_amdgcn_readlane(end, 63);
+            before += (uint32_t)__builtin_amdgcn_readlane((int)e, 63);
         }
+    }
+    // Of sequence b: its first unit on the line, the units of each of its items.
+    HN_DEVICE void place(int b, uint32_t& start, int& n) const {
+        if (p.B <= 64) {
+            n = __builtin_amdgcn_readlane(mine, b);
+            start = (uint32_t)__builtin_amdgcn_readlane((int)end, b) - (uint32_t)n * per;
+            return;
+        }
+        const int lane = threadIdx.x & 63;
+        uint32_t before = 0;
+        for (int i = lane; i < b; i += 64) before += (uint32_t)item_units(p, i);
+        start = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(before), 63) * per;
+        n = uniform(item_units(p, b));
     }
     HN_DEVICE uint32_t share() const { return (total + (uint32_t)p.wgs - 1) / (uint32_t)p.wgs; }
 };
@@ -128,12 +147,16 @@ struct Block {
     int first, left;  // its first token; keys from there on that the sequence has (<= 0: none)
 };
 
-template <int FMT, int RB, bool SV>
-__global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PageParams p) {
-    constexpr int R = 16 * RB, PITCH = D + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][R][PITCH];
+//
+// NW 4: the units of all items are dealt out evenly, whatever the sequences' lengths, and
+// parts of an item are joined by a second kernel. NW 8 (WHOLE): a workgroup an item.
+template <int FMT, int RB, bool SV, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_pages_kernel(PageParams p) {
+    constexpr int R = 16 * RB, PITCH = D + 4, UNIT = 32 * NW;
+    constexpr bool WHOLE = NW != 4;
+    __shared__ __attribute__((aligned(16))) float so[NW][R][PITCH];
     static_assert(sizeof(so[0]) >= K_TILE, "a wave's K codes fit where its result goes");
-    __shared__ float sml[4][R][2];
+    __shared__ float sml[NW][R][2];
     const int id = blockIdx.x;
     const int wg = (id & 7) * p.per_xcd + (id >> 3);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -142,16 +165,16 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
 
     uint32_t u0, u1, start;   // this workgroup's units; the current sequence's first
     int b, n;
-    Line line(p);
-    if (p.whole) {
+    if constexpr (WHOLE) {
         if (wg >= p.B * per) return;
         b = wg / per;
-        n = uniform(item_units(p, b));
+        n = uniform(item_units(p, b, UNIT));
         start = 0;
         u0 = (uint32_t)(wg - b * per) * (uint32_t)n;
         u1 = u0 + (uint32_t)n;
     } else {
         if (wg >= p.wgs) return;
+        const Line line(p);
         const uint32_t share = line.share();
         u0 = (uint32_t)wg * share;
         u1 = u0 + share < line.total ? u0 + share : line.total;
@@ -165,7 +188,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         if (u0 - start >= (uint32_t)n * (uint32_t)per) {  // the next sequence
             start += (uint32_t)n * (uint32_t)per;
             ++b;
-            n = uniform(item_units(p, b));
+            n = uniform(item_units(p, b, UNIT));
             continue;
         }
         const int item = (int)((u0 - start) / (uint32_t)n);   // h runs + run
@@ -173,7 +196,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         const int lo = (int)(u0 - item0), hi = min(n, (int)(u1 - item0));
         const int h = item / p.runs, run = item - h * p.runs;
         const int row0 = run * R, rows = min(R, p.rows - row0);
-        const int len = uniform(seq_len(p, b)), nc = cache_units(len);
+        const int len = uniform(seq_len(p, b)), nc = units_of(len, UNIT);
 
         bf16x8 qf[RB][4];
         int lim[RB];           // this lane's rows see cached tokens below
@@ -234,7 +257,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
 
         // ---- cached keys
         const ScalarInts row_table = scalar_ints(p.table + b * p.ts0);
-        const int end = 4 * min(hi, nc);
+        const int end = NW * min(hi, nc);
         // A block's table entry is a scalar load, asked for a block ahead (a vector load's wait
         // would be for every load before it, the prefetched codes among them).
         auto entry = [&](int blk) __attribute__((always_inline)) {
@@ -291,17 +314,17 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
                     x.vs[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(y.vs, off_vs, key * ss1, 0));
             }
         };
-        int blk = 4 * lo + wave;
-        int e = blk < end ? entry(blk) : 0, e1 = blk + 4 < end ? entry(blk + 4) : 0;
+        int blk = NW * lo + wave;
+        int e = blk < end ? entry(blk) : 0, e1 = blk + NW < end ? entry(blk + NW) : 0;
         Block now = place(blk, e);
         // (in the loop's order, by which each wait knows its loads)
         load_k(now);
         __builtin_amdgcn_sched_barrier(0);
         load_v(now);
         __builtin_amdgcn_sched_barrier(0);
-        for (; blk < end; blk += 4) {
-            const Block next = place(blk + 4, e1);
-            e1 = blk + 8 < end ? entry(blk + 8) : 0;
+        for (; blk < end; blk += NW) {
+            const Block next = place(blk + NW, e1);
+            e1 = blk + 2 * NW < end ? entry(blk + 2 * NW) : 0;
             // K codes through the wave's own LDS tile (chunk c of row r at c ^ r % 8)
             uint4 kx[2][2];
             const float ks[2] = {x.ks[0], x.ks[1]};
@@ -452,16 +475,16 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void attn_pages_kernel(PagePa
         __syncthreads();
         const bool done = lo == 0 && hi == n;
         const int64_t part = (int64_t)wg * 2 + (item0 < range0 ? 0 : 1);
-        for (int at = threadIdx.x; at < rows * (D / 4); at += 256) {
+        for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * NW) {
             const int r = at / (D / 4), d = (at % (D / 4)) * 4;
             float m = sml[0][r][0];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) m = fmaxf(m, sml[w][r][0]);
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, sml[w][r][0]);
             const float base = m == -INFINITY ? 0.0f : m;
             float den = 0.0f;
             float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float a = __builtin_amdgcn_exp2f(sml[w][r][0] - base);
                 const float4 y = *reinterpret_cast<const float4*>(&so[w][r][d]);
                 den = __builtin_fmaf(sml[w][r][1], a, den);
@@ -499,16 +522,10 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
     x /= groups;
     const int item = x % per, b = x / per;
     const uint32_t share = line.share();
-    // the sequence's first unit on the line
-    uint32_t before = 0;
-    {
-        const int lane = threadIdx.x & 63;
-        for (int i = lane; i < b; i += 64) before += (uint32_t)item_units(p, i);
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
-    }
-    const int n = item_units(p, b);
-    const uint32_t i0 = before * (uint32_t)per + (uint32_t)item * (uint32_t)n;
+    uint32_t start;
+    int n;
+    line.place(b, start, n);
+    const uint32_t i0 = start + (uint32_t)item * (uint32_t)n;
     const uint32_t w0 = i0 / share, w1 = (i0 + (uint32_t)n - 1) / share;
     if (w0 == w1) return;  // whole: written already
     const int h = item / p.runs, run = item - h * p.runs;
@@ -573,19 +590,24 @@ static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t
     pl.runs = (int)((rows + R - 1) / R);
     pl.items = B * H * pl.runs;
     pl.pitch = (int)(rows < R ? rows : R);
-    const int64_t units = (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
+    // A workgroup an item where each has few keys and all are resident at once: calls of
+    // 8 to 256 items of one to four rows, up to 100 keys 6 us against 8.4 to 12.4, 500 8.2 to
+    // 10.6 against 9.1 to 17.1, 1024 11.1 to 16.4 against 11.3 to 24.2, 2048 (eight items) 17.5
+    // against 13.3; twenty rows 500 11.2 against 14.2, 1024 15.3 against 14.6; 1536 items of 100
+    // keys 34.6 against 19.9.
+    const int64_t units = (max_len + 255) / 256 + (cur_len + 255) / 256;
     pl.wgs = (pl.rb == 1 ? 3 : 2) * device_cus();
-    pl.whole = units <= 2 || pl.items >= 8 * (int64_t)pl.wgs;
+    pl.whole = units * pl.rb <= 4 && pl.items <= 2 * (int64_t)device_cus();
     return pl;
 }
 
 // SV: the scales of consecutive tokens are consecutive, four to a load.
-template <int FMT>
+template <int FMT, int NW>
 static void launch_pages(int rb, bool sv, const attn::PageParams& p, unsigned blocks, hipStream_t st) {
-    if (rb == 1 && sv) attn::attn_pages_kernel<FMT, 1, true><<<blocks, 256, 0, st>>>(p);
-    else if (rb == 1) attn::attn_pages_kernel<FMT, 1, false><<<blocks, 256, 0, st>>>(p);
-    else if (sv) attn::attn_pages_kernel<FMT, 2, true><<<blocks, 256, 0, st>>>(p);
-    else attn::attn_pages_kernel<FMT, 2, false><<<blocks, 256, 0, st>>>(p);
+    if (rb == 1 && sv) attn::attn_pages_kernel<FMT, 1, true, NW><<<blocks, 64 * NW, 0, st>>>(p);
+    else if (rb == 1) attn::attn_pages_kernel<FMT, 1, false, NW><<<blocks, 64 * NW, 0, st>>>(p);
+    else if (sv) attn::attn_pages_kernel<FMT, 2, true, NW><<<blocks, 64 * NW, 0, st>>>(p);
+    else attn::attn_pages_kernel<FMT, 2, false, NW><<<blocks, 64 * NW, 0, st>>>(p);
 }
 
 static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
@@ -676,7 +698,6 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.causal = causal != 0;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
     if (pl.tiles) return launch_page_tiles(p, fmt, workspace, (hipStream_t)stream);
-    p.whole = pl.whole;
     p.wgs = pl.wgs;
     p.pitch = pl.pitch;
     if (!pl.whole) {
@@ -688,8 +709,13 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     const unsigned blocks = 8u * (unsigned)p.per_xcd;
     const hipStream_t st = (hipStream_t)stream;
     const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(vs, 16);
-    if (fmt == HN_KV_FP8) launch_pages<HN_KV_FP8>(pl.rb, sv, p, blocks, st);
-    else launch_pages<HN_KV_INT8>(pl.rb, sv, p, blocks, st);
+    if (fmt == HN_KV_FP8) {
+        if (pl.whole) launch_pages<HN_KV_FP8, 8>(pl.rb, sv, p, blocks, st);
+        else launch_pages<HN_KV_FP8, 4>(pl.rb, sv, p, blocks, st);
+    } else {
+        if (pl.whole) launch_pages<HN_KV_INT8, 8>(pl.rb, sv, p, blocks, st);
+        else launch_pages<HN_KV_INT8, 4>(pl.rb, sv, p, blocks, st);
+    }
     if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK || pl.whole) return rc;
     const int R = 16 * pl.rb, groups = (pl.pitch + 7) / 8;
     attn::pages_join_kernel<<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
