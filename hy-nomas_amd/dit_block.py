@@ -35,6 +35,7 @@ from .cache_attention import causal_attention_with_cache_mp, chunk_attention
 from .dit_fp8_linear import FP8StoredLinear, fp8_linear, fp8_linear_codes
 from .fp8_kv_cache import make_fp8_kv_block
 from .kv_history import LayerHistory
+from .kv_pages import PagedKVCache
 from .metrics import stage
 
 
@@ -202,14 +203,17 @@ class FP8DiTBlock(nn.Module):
 
     def forward(self, img, vec, cos, sin, kv_cache, cache_valid_len: int,
                 update_cache: bool = False, kv_status=None, *, txt=None, vec_txt=None,
-                text_mask=None, cache_mask=None, cache_txt: bool = True, history=None):
+                text_mask=None, cache_mask=None, cache_txt: bool = True, history=None, pages=None):
         """One block at inference. With ``update_cache`` this chunk's rotated K
         and V go into ``kv_cache`` at ``cache_valid_len``. When writes are
         validated and no ``kv_status`` is passed, a non-finite value raises
         ValueError here (one host read of the device flag); with one, the flag
         is left for the caller to read. ``history`` (a kv_history.LayerHistory of this
         cache, image-only path) runs the pass's attention: chosen blocks of a long
-        history, the weight its keys draw.
+        history, the weight its keys draw. ``pages`` (a kv_pages.PageBatch and this block's
+        layer in it, image-only path) takes the place of ``kv_cache`` and
+        ``cache_valid_len``: every batch element reads its own sequence and the chunk, and
+        a writing pass adds the chunk to it.
 
         With ``txt`` ([B, L_txt, C], text stream blocks only) the call follows
         the double-stream block (nomas_cpt.py:1293-1459): both streams' Q/K/V,
@@ -224,6 +228,8 @@ class FP8DiTBlock(nn.Module):
                 raise ValueError("kv_status applies to the image-only path")
             if history is not None:
                 raise ValueError("a LayerHistory applies to the image-only path")
+            if pages is not None:
+                raise ValueError("pages apply to the image-only path")
             q, k, v, parts = self.pre_attention(img, vec, cos, sin)
             tq, tk, tv, tparts = self.pre_attention_txt(txt, vec_txt)
             img_attn, txt_attn = causal_attention_with_cache_mp(
@@ -234,12 +240,23 @@ class FP8DiTBlock(nn.Module):
         if update_cache and self.validate_kv_writes:
             status = kv_status if kv_status is not None else torch.empty(
                 1, dtype=torch.int32, device=img.device)
-        q, k, v, parts = self.pre_attention(img, vec, cos, sin, kv_cache if update_cache else None,
-                                            cache_valid_len, status)
+        if pages is not None:
+            if history is not None or kv_cache is not None:
+                raise ValueError("pages take the place of a cache and its history")
+            batch, layer = pages
+            q, k, v, parts = self.pre_attention(img, vec, cos, sin)
+            if update_cache:
+                with stage("fp8_encode"):
+                    batch.write(layer, k, v, assume_finite=status is None, status=status)
+        else:
+            q, k, v, parts = self.pre_attention(img, vec, cos, sin, kv_cache if update_cache else None,
+                                                cache_valid_len, status)
         if status is not None and kv_status is None and int(status[0].item()):
             raise ValueError("Cannot quantize non-finite KV values")
         with stage("cache_attention"):
-            if history is None:
+            if pages is not None:
+                attn, _ = batch.attend(layer, q, k_cur=k, v_cur=v)
+            elif history is None:
                 attn = chunk_attention(q, kv_cache, cache_valid_len, k_cur=k, v_cur=v)
             else:
                 attn = history.attend(q, k, v, kv_cache, cache_valid_len, update_cache)
@@ -264,16 +281,24 @@ class FP8ARModel(nn.Module):
     to that many tokens of each head, those that the writing passes' queries weighed
     most, instead of refusing the chunk. Kept whatever their weight are the first latent
     frame, up to a quarter of ``evict_keep`` (its first tokens), and the newest chunk, up
-    to half (its last): the rest is always left to the mass."""
+    to half (its last): the rest is always left to the mass.
+
+    Roll-outs that branch (image-only chunks): ``pages`` > 0 holds the history in that many
+    pages of ``page`` tokens (kv_pages.PagedKVCache) instead of one cache a layer. A
+    roll-out is then a branch: ``start_branch`` begins one, ``fork_branch`` continues one's
+    history in two without copying it, ``drop_branch`` gives its pages back, and
+    ``generate_chunk`` steps any branches of one length together, a batch element each."""
 
     # a model that reads and keeps all of its history
     evict_keep = 0
-    histories = spare = None
+    histories = spare = paged = None
 
     def __init__(self, depth: int = 40, hidden: int = 3072, heads: int = 24,
                  latent_shape=(3, 45, 80), max_chunks: int = 17, *, device=None, seed: int = 0,
-                 text_len: int = 0, sparse_top_k: int = 0, evict_keep: int = 0):
+                 text_len: int = 0, sparse_top_k: int = 0, evict_keep: int = 0, pages: int = 0, page: int = 64):
         super().__init__()
+        if pages and (text_len or sparse_top_k or evict_keep):
+            raise ValueError("pages apply to image-only chunks without sparse_top_k and evict_keep")
         g = torch.Generator(device=device).manual_seed(seed)
         self.text_len = int(text_len)
         self.blocks = nn.ModuleList(
@@ -286,7 +311,10 @@ class FP8ARModel(nn.Module):
         self.heads, self.head_dim = heads, hidden // heads
         self.device = device
         self.caches = [make_fp8_kv_block(1, self.capacity, heads, self.head_dim, device=device)
-                       for _ in range(depth)]
+                       for _ in range(0 if pages else depth)]
+        if pages:
+            self.paged = PagedKVCache(depth, pages, heads, self.head_dim, page=page, device=device)
+            self.branch_frames = {}
         # history validity per layer (padded text keys stay invalid)
         self.cache_masks = ([torch.zeros(1, self.capacity, dtype=torch.bool, device=device)
                              for _ in range(depth)] if self.text_len else None)
@@ -307,6 +335,28 @@ class FP8ARModel(nn.Module):
         if self.evict_keep:
             self.spare = make_fp8_kv_block(1, self.capacity, heads, self.head_dim, device=device)
 
+    def _branches(self):
+        if self.paged is None:
+            raise ValueError("branches need a model with pages")
+        return self.paged
+
+    def start_branch(self) -> int:
+        """A roll-out without history."""
+        branch = self._branches().new()
+        self.branch_frames[branch] = 0
+        return branch
+
+    def fork_branch(self, branch: int) -> int:
+        """A second roll-out from ``branch``'s history, which both hold from now on."""
+        fork = self._branches().fork(branch)
+        self.branch_frames[fork] = self.branch_frames[branch]
+        return fork
+
+    def drop_branch(self, branch: int) -> None:
+        """Forget a roll-out."""
+        self._branches().free(branch)
+        del self.branch_frames[branch]
+
     @torch.no_grad()
     def evict_history(self) -> None:
         """Cut every layer's cache to ``evict_keep`` tokens a head: each moves into the
@@ -325,9 +375,19 @@ class FP8ARModel(nn.Module):
         self.cache_valid_len = min(keep, self.cache_valid_len)
 
     @torch.no_grad()
-    def forward_chunk(self, img, vec, update_cache: bool, txt=None, vec_txt=None, text_mask=None):
+    def forward_chunk(self, img, vec, update_cache: bool, txt=None, vec_txt=None, text_mask=None, batch=None):
+        """One pass over all blocks. ``batch`` (a kv_pages.PageBatch of this model's
+        branches) is the history of a model with pages."""
+        if (batch is None) != (self.paged is None):
+            raise ValueError("a model with pages, and no other, takes a batch of branches")
         t, h, w = self.latent_shape
-        cos, sin = rope_tables(t, h, w, t_offset=self.frames_done, device=img.device)
+        frames = self.frames_done if batch is None else self._frames_of(batch.seqs)
+        cos, sin = rope_tables(t, h, w, t_offset=frames, device=img.device)
+        if batch is not None:
+            for i, block in enumerate(self.blocks):
+                img = block(img, vec, cos, sin, None, 0, update_cache, pages=(batch, i),
+                            kv_status=self.kv_status[i:i + 1] if update_cache else None)
+            return img
         if self.text_len:
             if txt is None or txt.shape[1] != self.text_len:
                 raise ValueError(f"this model takes {self.text_len} text tokens per chunk")
@@ -343,9 +403,45 @@ class FP8ARModel(nn.Module):
                         history=None if self.histories is None else self.histories[i])
         return img
 
+    def _frames_of(self, branches) -> int:
+        frames = {self.branch_frames[b] for b in branches}
+        if len(frames) != 1:
+            raise ValueError("the branches of a pass must be of one length")
+        return frames.pop()
+
+    @torch.no_grad()
+    def _generate_branches(self, noise, vecs_denoise, vec_write, sigmas, branches):
+        """generate_chunk over pages: the room for the chunk is taken before any pass, and
+        a write that a NaN/Inf refuses leaves the branches as they were."""
+        branches = list(branches)
+        want = (len(branches), self.tokens_per_chunk, self.heads * self.head_dim)
+        if not branches or len(set(branches)) != len(branches):
+            raise ValueError("branches must be distinct, one at least")
+        if tuple(noise.shape) != want:
+            raise ValueError(f"noise must be {list(want)}, got {list(noise.shape)}")
+        for b in branches:
+            self.paged.length(b)
+        self._frames_of(branches)
+        batch = self.paged.open(branches, self.tokens_per_chunk)
+        try:
+            x = noise
+            for i, vec in enumerate(vecs_denoise):
+                x = x + (sigmas[i + 1] - sigmas[i]) * self.forward_chunk(x, vec, False, batch=batch)
+            self.forward_chunk(x, vec_write, True, batch=batch)
+            bad = torch.nonzero(self.kv_status).flatten().tolist()
+            if bad:
+                raise ValueError(f"Cannot quantize non-finite KV values (layers {bad})")
+        except Exception:
+            batch.discard()
+            raise
+        batch.commit()
+        for b in branches:
+            self.branch_frames[b] += self.latent_shape[0]
+        return x
+
     @torch.no_grad()
     def generate_chunk(self, noise, vecs_denoise, vec_write, sigmas, txt=None, vec_txt=None,
-                       text_mask=None):
+                       text_mask=None, branches=None):
         """Euler flow updates over the denoising passes, then the cache write
         at t = 0 and the advance of the valid length (causal_ar.py:2348-2432,
         2624-2645,2852). A chunk that would not fit the cache is refused
@@ -354,9 +450,16 @@ class FP8ARModel(nn.Module):
         pass a layer whose K/V holds a NaN/Inf writes nothing; the valid length
         then stays where it was (rows that other layers wrote past it are never
         attended) and ValueError names the layers (with text: the first such
-        layer raises)."""
+        layer raises). A model with pages steps ``branches``: noise [B, tokens, C] and
+        vectors [B, C], a batch element a branch."""
         if len(sigmas) != len(vecs_denoise) + 1:
             raise ValueError("sigmas must hold one more value than the denoising passes")
+        if (branches is None) != (self.paged is None):
+            raise ValueError("a model with pages, and no other, steps branches")
+        if branches is not None:
+            if txt is not None:
+                raise ValueError("pages apply to image-only chunks")
+            return self._generate_branches(noise, vecs_denoise, vec_write, sigmas, branches)
         if self.cache_valid_len + self.write_tokens > self.capacity and self.evict_keep:
             want = (1, self.tokens_per_chunk, self.heads * self.head_dim)
             if tuple(noise.shape) != want:  # (the passes would refuse it, but the history would be cut by then)

@@ -81,3 +81,210 @@ def read_pages(cache: dict, key: str, table: torch.Tensor, kv_len: torch.Tensor,
     if key not in KV_KEYS:
         raise ValueError(f"Invalid KV key: {key}")
     return ops.kv_pages_read(cache[key], cache[f"{key}_scale"], table, kv_len, max_len)
+
+
+class PagedKVCache:
+    """The pages of all layers, and the sequences that hold them.
+
+    A sequence is an id with a length and a list of pages; page p is the same place in
+    every layer. Sequences share pages: ``fork`` gives a branch the pages of its origin,
+    and a shared page is copied (all layers in one launch) when one of them is about to
+    write it. A pass opens a ``PageBatch`` of its sequences, runs its layers with it and
+    commits it; ``free``, ``truncate`` and ``compact`` run between passes.
+
+    The pages are the host's: numbers and lengths live there, and a batch brings its
+    tables to the GPU in one copy. All work is ordered on the current stream."""
+
+    def __init__(self, layers: int, pages: int, heads: int, dim: int = 128, *, page: int = 64,
+                 code_dtype: torch.dtype = FP8, device: torch.device | str):
+        if layers < 1 or pages < 1:
+            raise ValueError("layers and pages must be positive")
+        self.pool = make_pages(pages, heads, dim, page=page, layers=layers, code_dtype=code_dtype, device=device)
+        self.layers, self.pages, self.page = layers, pages, page
+        self.device = torch.device(device)
+        self._views = [{n: t[i] for n, t in self.pool.items()} for i in range(layers)]
+        self._free = list(range(pages))             # a heap: the lowest number is taken first
+        self._refs = [0] * pages
+        self._table: dict[int, list[int]] = {}      # sequence -> its pages
+        self._length: dict[int, int] = {}
+        self._stamp: dict[int, int] = {}            # changes when a batch's view of the sequence is past
+        self._next = 0
+
+    def layer(self, i: int) -> dict:
+        """Layer i's pool, as write_pages and paged_attention take it."""
+        return self._views[i]
+
+    def length(self, seq: int) -> int:
+        return self._length[self._known(seq)]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _known(self, seq: int) -> int:
+        if seq not in self._table:
+            raise ValueError(f"no sequence {seq}")
+        return seq
+
+    def new(self) -> int:
+        """An empty sequence."""
+        seq, self._next = self._next, self._next + 1
+        self._table[seq], self._length[seq], self._stamp[seq] = [], 0, 0
+        return seq
+
+    def fork(self, seq: int) -> int:
+        """A sequence with the tokens of ``seq``, on its pages: nothing is copied now."""
+        self._known(seq)
+        held = self._table[seq][:-(-self._length[seq] // self.page)]
+        branch = self.new()
+        self._table[branch], self._length[branch] = list(held), self._length[seq]
+        for p in held:
+            self._refs[p] += 1
+        return branch
+
+    def _drop(self, pages: list[int]) -> None:
+        for p in pages:
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def free(self, seq: int) -> None:
+        """Forget a sequence; pages that no other one holds are free again."""
+        self._drop(self._table.pop(self._known(seq)))
+        del self._length[seq], self._stamp[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Keep the first ``length`` tokens (drafted tokens that were refused go)."""
+        if not 0 <= length <= self.length(seq):
+            raise ValueError(f"cannot keep {length} of {self.length(seq)} tokens")
+        held = self._table[seq]
+        keep = -(-length // self.page)
+        self._drop(held[keep:])
+        del held[keep:]
+        self._length[seq] = length
+        self._stamp[seq] += 1
+
+    def open(self, seqs: Sequence[int], tokens: int | Sequence[int] = 0) -> "PageBatch":
+        """A pass of these sequences that adds ``tokens`` tokens to each (a number, or one
+        for every sequence; 0: a pass that only reads). Room for them is taken now, and
+        pages that they would write but share are copied; ValueError, with nothing
+        changed, if the pool has not enough."""
+        seqs = [self._known(s) for s in seqs]
+        adds = [tokens] * len(seqs) if isinstance(tokens, int) else list(tokens)
+        if len(adds) != len(seqs) or min(adds, default=0) < 0:
+            raise ValueError("tokens: a number that is not negative, or one for every sequence")
+        if any(adds) and len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence that grows occurs once in a pass")
+        copies, grown, refs = [], [], {}  # (sequence, place), (sequence, pages), holders that leave a page
+        for s, n in zip(seqs, adds):
+            held, start = self._table[s], self._length[s]
+            for i in range(start // self.page, min(len(held), -(-(start + n) // self.page))) if n else ():
+                p = held[i]
+                left = self._refs[p] - refs.get(p, 0)
+                if left > 1:  # (the last holder writes it in place)
+                    refs[p] = refs.get(p, 0) + 1
+                    copies.append((s, i))
+            grown.append((s, max(0, -(-(start + n) // self.page) - len(held))))
+        if len(copies) + sum(n for _, n in grown) > len(self._free):
+            raise ValueError(f"{len(copies) + sum(n for _, n in grown)} pages are needed, {len(self._free)} are free")
+        src, dst = [], []
+        for s, i in copies:
+            held = self._table[s]
+            src.append(held[i])
+            dst.append(heapq.heappop(self._free))
+            self._refs[held[i]] -= 1
+            self._refs[dst[-1]] = 1
+            held[i] = dst[-1]
+            self._stamp[s] += 1
+        for s, n in grown:
+            for _ in range(n):
+                p = heapq.heappop(self._free)
+                self._refs[p] = 1
+                self._table[s].append(p)
+        if src:
+            copy_pages(self.pool, src, dst)
+        return PageBatch(self, seqs, adds)
+
+    def compact(self) -> int:
+        """Move the pages in use to the lowest numbers (one copy over all layers); returns
+        how many were moved. Batches opened before are of no use afterwards."""
+        used = [p for p in range(self.pages) if self._refs[p]]
+        n = len(used)
+        src = [p for p in used if p >= n]
+        dst = [p for p in range(n) if not self._refs[p]]
+        if src:
+            copy_pages(self.pool, src, dst)
+            to = dict(zip(src, dst))
+            for s, held in self._table.items():
+                held[:] = [to.get(p, p) for p in held]
+                self._stamp[s] += 1
+            for a, b in to.items():
+                self._refs[b], self._refs[a] = self._refs[a], 0
+            self._free = list(range(n, self.pages))
+        return len(src)
+
+
+class PageBatch:
+    """One pass of some sequences of a PagedKVCache: their tables and lengths on the GPU.
+
+    ``write`` puts a layer's new tokens into the pages, ``attend`` runs a layer's
+    attention; ``commit`` makes the new tokens part of the sequences once every layer has
+    written them. A batch that is not committed leaves the sequences as they were. Once
+    one of its sequences is committed, cut, freed or moved, it is refused (ValueError)."""
+
+    def __init__(self, cache: PagedKVCache, seqs: list[int], adds: list[int]):
+        self.cache, self.seqs, self.adds = cache, seqs, adds
+        self.lengths = [cache._length[s] for s in seqs]
+        self._stamps = [cache._stamp[s] for s in seqs]
+        B, tables = len(seqs), [cache._table[s] for s in seqs]
+        width = max((len(t) for t in tables), default=0)
+        flat = self.lengths + [n + a for n, a in zip(self.lengths, adds)] + adds
+        for t in tables:
+            flat += t + [-1] * (width - len(t))
+        host = torch.tensor(flat, dtype=torch.int32)
+        if cache.device.type == "cuda":
+            host = host.pin_memory()
+        flat = host.to(cache.device, non_blocking=True)
+        self.start, self.end, counts = flat[:3 * B].view(3, B).unbind(0)    # tokens before and after the pass
+        self.table = flat[3 * B:].view(B, width)
+        self.counts = None if len(set(adds)) <= 1 else counts
+
+    def _check(self) -> None:
+        stamp = self.cache._stamp
+        if any(stamp.get(s) != n for s, n in zip(self.seqs, self._stamps)):
+            raise ValueError("the batch is past: a sequence was committed, cut, freed or moved since it was opened")
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, assume_finite: bool = False,
+              status: Optional[torch.Tensor] = None) -> None:
+        """Layer ``layer``'s K/V [B, L, H, D] of the new tokens: the first of each
+        sequence's L rows, as many as it adds (write_pages)."""
+        self._check()
+        if k.shape[0] != len(self.seqs) or k.shape[1] < max(self.adds, default=0) or (
+                self.counts is None and k.shape[1] != max(self.adds, default=0)):
+            raise ValueError("k and v must hold the tokens that the batch was opened for")
+        write_pages(self.cache.layer(layer), k, v, self.table, self.start, counts=self.counts,
+                    assume_finite=assume_finite, status=status)
+
+    def attend(self, layer: int, q: torch.Tensor, *, causal: bool = False, k_cur: Optional[torch.Tensor] = None,
+               v_cur: Optional[torch.Tensor] = None, cur_valid: Optional[torch.Tensor] = None,
+               softmax_scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Attention of q [B, Lq, Hq, D]: with k_cur/v_cur over the tokens before the pass
+        and those, without over the tokens written by it too (paged_attention)."""
+        from .cache_attention import paged_attention
+        self._check()
+        return paged_attention(q, self.cache.layer(layer), self.table, self.end if k_cur is None else self.start,
+                               causal=causal, k_cur=k_cur, v_cur=v_cur, cur_valid=cur_valid,
+                               softmax_scale=softmax_scale)
+
+    def commit(self) -> None:
+        """The new tokens stand; the batch is of no use afterwards."""
+        self._check()
+        for s, n, a in zip(self.seqs, self.lengths, self.adds):
+            self.cache._length[s] = n + a
+            self.cache._stamp[s] += 1
+
+    def discard(self) -> None:
+        """Give up the pass: the room that was taken for it is free again."""
+        self._check()
+        for s, n in zip(self.seqs, self.lengths):
+            self.cache.truncate(s, n)

@@ -490,3 +490,144 @@ def test_calls_on_two_streams(dev):
     for w, gs in zip(want, got):
         for x in gs:
             assert torch.equal(x[0], w[0]) and torch.equal(x[1], w[1])
+
+
+# --------------------------------------------------------------------------
+# a run of them together: branches of the AR model
+
+def _model(dev, pages, **kw):
+    db = pkg_module("dit_block")
+    return db.FP8ARModel(2, 256, 2, (2, 5, 9), 4, device=dev, seed=3, pages=pages, **kw)
+
+
+def _inputs(dev, model, B, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    noise = torch.randn(B, model.tokens_per_chunk, 256, device=dev, generator=g).to(BF16)
+    vecs = [torch.randn(B, 256, device=dev, generator=g).to(BF16) for _ in range(3)]
+    return noise, vecs[:2], vecs[2], [1.0, 0.5, 0.0]
+
+
+def _rel(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+def test_a_branch_is_a_roll_out_of_the_contiguous_model(dev):
+    """Chunk after chunk as the model with one cache a layer. The two attend in another
+    order of tiles, so outputs agree to the bf16 steps of a block (2^-8 each, of about ten
+    tensor operations a pass, two passes a chunk), the first layer's cache to the codes of
+    the first chunk."""
+    plain, paged = _model(dev, 0), _model(dev, 9)
+    branch = paged.start_branch()
+    for i in range(3):
+        args = _inputs(dev, plain, 1, i)
+        a, b = plain.generate_chunk(*args), paged.generate_chunk(*args, branches=[branch])
+        assert _rel(b, a) < 20 * 2.0 ** -8
+    assert paged.paged.length(branch) == plain.cache_valid_len == 270
+    kp, _, kvc = _mods()
+    batch = paged.paged.open([branch])
+    for layer in range(2):
+        for key in ("k", "v"):
+            got = kp.read_pages(paged.paged.layer(layer), key, batch.table, batch.start, 270)
+            want = kvc.dequantize_kv(plain.caches[layer], key, 270)
+            assert _rel(got, want) < 0.1
+            if layer == 0:
+                assert _rel(got[:, :90], want[:, :90]) < 20 * 2.0 ** -8
+
+
+def test_forked_branches(dev):
+    """Two branches of one history: equal inputs give equal chunks, other inputs leave the
+    origin as it was, and a branch goes on as its origin would have."""
+    kp, _, _ = _mods()
+    m = _model(dev, 20)
+    a = m.start_branch()
+    noise, vecs, write, sig = _inputs(dev, m, 1, 0)
+    m.generate_chunk(noise, vecs, write, sig, branches=[a])
+    b, c = m.fork_branch(a), m.fork_branch(a)
+    assert m.paged.free_pages == 18  # 90 tokens: two pages
+
+    def held(branch):
+        batch = m.paged.open([branch])
+        return [kp.read_pages(m.paged.layer(i), key, batch.table, batch.start, m.paged.length(branch))
+                for i in range(2) for key in ("k", "v")]
+
+    origin = held(c)
+    two = [torch.cat([x, x]) for x in (noise, *vecs, write)]
+    out = m.generate_chunk(two[0], two[1:3], two[3], sig, branches=[a, b])
+    assert torch.equal(out[0], out[1])
+    assert all(torch.equal(x, y) for x, y in zip(held(a), held(b)))
+    args = _inputs(dev, m, 2, 5)
+    out = m.generate_chunk(*args, branches=[b, a])
+    assert not torch.equal(out[0], out[1])
+    assert all(torch.equal(x, y) for x, y in zip(held(c), origin))
+    with pytest.raises(ValueError, match="of one length"):
+        m.generate_chunk(*_inputs(dev, m, 2, 6), branches=[a, c])
+    m.drop_branch(b)
+    late = m.generate_chunk(noise, vecs, write, sig, branches=[c])
+    again = m.generate_chunk(noise, vecs, write, sig, branches=[m.start_branch()])
+    assert late.shape == again.shape
+    assert all(torch.equal(x[:, :90], y) for x, y in zip(held(c), origin))
+    m.paged.compact()
+    assert all(torch.equal(x[:, :90], y) for x, y in zip(held(c), origin))
+
+
+def test_a_full_pool_and_a_bad_chunk_leave_the_branches(dev):
+    m = _model(dev, 3)
+    a = m.start_branch()
+    args = _inputs(dev, m, 1, 0)
+    m.generate_chunk(*args, branches=[a])
+    fork = m.fork_branch(a)
+    with pytest.raises(ValueError, match="2 pages are needed, 1 are free"):  # (the half page is shared)
+        m.generate_chunk(*args, branches=[fork])
+    m.drop_branch(fork)
+    noise = args[0].clone()
+    noise[0, 3, 7] = float("nan")
+    with pytest.raises(ValueError, match="non-finite"):
+        m.generate_chunk(noise, *args[1:], branches=[a])
+    assert m.paged.length(a) == 90 and m.branch_frames[a] == 2 and m.paged.free_pages == 1
+    with pytest.raises(ValueError, match="noise must"):
+        m.generate_chunk(noise[:, :5], *args[1:], branches=[a])
+    with pytest.raises(ValueError, match="distinct"):
+        m.generate_chunk(torch.cat([noise, noise]), *args[1:], branches=[a, a])
+    with pytest.raises(ValueError, match="no sequence"):
+        m.generate_chunk(noise, *args[1:], branches=[99])
+
+
+def test_drafted_tokens(dev):
+    """Five drafted tokens written and attended causally, two accepted: what follows is as
+    if the others had never been."""
+    kp, ca, _ = _mods()
+    cache = kp.PagedKVCache(1, 40, 4, page=64, device=dev)
+    g = torch.Generator(device=dev).manual_seed(0)
+
+    def tokens(B, L):
+        return torch.randn(B, L, 3, 4, 128, device=dev, generator=g).to(BF16).unbind(2)
+
+    seqs = [cache.new(), cache.new()]
+    batch = cache.open(seqs, [300, 63])
+    _, k, v = tokens(2, 300)
+    batch.write(0, k, v)
+    batch.commit()
+    batch = cache.open(seqs, 5)
+    q, k, v = tokens(2, 5)
+    batch.write(0, k, v)
+    got = batch.attend(0, q, causal=True)
+    _check(got, _reference(q, cache.layer(0), batch.table, (305, 68), causal=True), "drafted")
+    batch.commit()
+    for s, n in zip(seqs, (302, 65)):
+        cache.truncate(s, n)
+    one = cache.open(seqs, 1)
+    q1, k1, v1 = tokens(2, 1)
+    one.write(0, k1, v1)
+    out = one.attend(0, q1)
+    one.commit()
+    fresh = kp.PagedKVCache(1, 40, 4, page=64, device=dev)
+    ids = [fresh.new(), fresh.new()]
+    for b, (s, n) in enumerate(zip(ids, (302, 65))):
+        batch = fresh.open([s], n)
+        mine = [kp.read_pages(cache.layer(0), key, one.table[b:b + 1], _i32(dev, [n]), n) for key in ("k", "v")]
+        batch.write(0, *mine)  # (decoded values: their codes are the same again)
+        batch.commit()
+    batch = fresh.open(ids, 1)
+    batch.write(0, k1, v1)
+    again = batch.attend(0, q1)
+    assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
