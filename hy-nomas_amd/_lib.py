@@ -19,6 +19,7 @@ HN_E_DEVICE = -3
 ABI_VERSION = 4
 HN_SCALE_CLAMP = 0
 HN_SCALE_ZERO_ONE = 1
+HN_SCALE_RECIPROCAL = 2
 HN_KV_FP8 = 0
 HN_KV_INT8 = 1
 HN_ACT_NONE = 0
@@ -77,7 +78,7 @@ SIGNATURES = {
     "hn_move_kv_tokens": [_P, _P, _PI64, _P, _P, _PI64, _P, _PI64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P,
                           _PI64, _P, _P, _PI64, _I64, _P, _P],
     "hn_kv_pages_write": [_I, _P, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64,
-                          _P, _I64, _I64, _P, _P, _P, _P],
+                          _P, _I64, _I64, _P, _P, _I, _P, _P],
     "hn_kv_pages_read": [_I, _P, _PI64, _P, _PI64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
     "hn_kv_pages_copy": [ctypes.POINTER(_P), _PI64, _PI64, _PI64, _I64, _I64, _PI32, _PI32, _I64, _P],
     "hn_attn_kv_pages": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64, _I64,

@@ -405,9 +405,11 @@ extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const in
                                  int64_t H, int64_t D, void* kc, void* vc, const int64_t* cs, float* ks, float* vs,
                                  const int64_t* ss, int64_t n_pages, int64_t page, const int32_t* table,
                                  int64_t table_stride, int64_t width, const int32_t* start, const int32_t* counts,
-                                 int32_t* status, void* stream) {
+                                 int scale_mode, int32_t* status, void* stream) {
     const char* who = "hn_kv_pages_write";
     HN_REQUIRE(fmt == HN_KV_FP8 || fmt == HN_KV_INT8, HN_E_ARG, "hn_kv_pages_write: unknown KV format");
+    HN_REQUIRE(scale_mode == HN_SCALE_ZERO_ONE || scale_mode == HN_SCALE_RECIPROCAL, HN_E_ARG,
+               "hn_kv_pages_write: unknown scale mode");
     HN_REQUIRE(D == 128, HN_E_ARG, "hn_kv_pages_write: head dim must be 128");
     HN_REQUIRE(B >= 0 && L >= 0 && H > 0 && B <= 0x7fffffffLL && L <= 0x7fffffffLL && H <= 0x7fffffffLL, HN_E_ARG,
                "hn_kv_pages_write: invalid shape");
@@ -433,6 +435,7 @@ extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const in
     a.s[0] = ks; a.s[1] = vs;
     a.xs0 = xs[0]; a.xs1 = xs[1]; a.xs2 = xs[2];
     a.start = start; a.counts = counts;
+    if (scale_mode == HN_SCALE_RECIPROCAL) a.recip = 1.0f / (fmt == HN_KV_FP8 ? kE4M3Max : 127.0f);
     dim3 grid;
     HN_REQUIRE(tiles_of(B, L, H, 2, xs[1] < xs[2], a.tiles, grid), HN_E_ARG, "hn_kv_pages_write: too many rows");
     const bool fp8 = fmt == HN_KV_FP8;

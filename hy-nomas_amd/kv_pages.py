@@ -27,6 +27,7 @@ from typing import Optional, Sequence
 
 import torch
 
+from . import _lib as L
 from . import ops
 from .fp8_kv_cache import CODE_DTYPES, FP8, KV_KEYS, STORAGE_KEYS, _raise_if_flagged
 
@@ -49,7 +50,7 @@ def make_pages(pages: int, heads: int, dim: int = 128, *, page: int = 64, layers
 
 def write_pages(cache: dict, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
                 counts: Optional[torch.Tensor] = None, assume_finite: bool = False,
-                status: Optional[torch.Tensor] = None) -> None:
+                status: Optional[torch.Tensor] = None, gpu_scales: bool = False) -> None:
     """Quantize bf16 K/V [B, L, H, D] into a layer's pages: token j of sequence b becomes
     its token start[b] + j (start int32 [B]), for j < counts[b] (int32 [B]; None: all L).
 
@@ -57,13 +58,18 @@ def write_pages(cache: dict, k: torch.Tensor, v: torch.Tensor, table: torch.Tens
     ``assume_finite``, nothing is written if a new token holds a NaN/Inf (ValueError, or
     status[0] = 1 when a status tensor is given). Tokens past the table, and those whose
     page number is not in the pool, are dropped. The sequences of one call must not share
-    the pages that they write."""
+    the pages that they write.
+
+    ``gpu_scales``: a row's scale is amax times the fp32 reciprocal of 448 (127), as torch
+    on a GPU divides a tensor by a number, instead of the rounded quotient: pages that go
+    on from codes a torch program made on the GPU hold what it would have, bit for bit."""
     args = (*(cache[n] for n in STORAGE_KEYS), k, v, table, start, counts)
+    mode = L.HN_SCALE_RECIPROCAL if gpu_scales else L.HN_SCALE_ZERO_ONE
     if assume_finite:
-        ops.kv_pages_write_(*args)
+        ops.kv_pages_write_(*args, None, mode)
         return
     flag = status if status is not None else torch.empty(1, dtype=torch.int32, device=k.device)
-    ops.kv_pages_write_(*args, flag)
+    ops.kv_pages_write_(*args, flag, mode)
     if status is None:
         _raise_if_flagged(flag)
 

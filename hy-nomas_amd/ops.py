@@ -1160,19 +1160,21 @@ def _per_sequence(t: Optional[torch.Tensor], B: int, what: str) -> Optional[torc
     return t.contiguous()
 
 
-def kv_pages_write_(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts=None, status=None) -> None:
+def kv_pages_write_(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts=None, status=None,
+                    scale_mode: int = L.HN_SCALE_ZERO_ONE) -> None:
     """Quantize new tokens into the pages of their sequences (see _kv_pages_write_op)."""
-    _kv_pages_write_op(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status)
+    _kv_pages_write_op(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status, scale_mode)
 
 
 @eager_op("hy_nomas_amd::kv_pages_write_", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale", "status"))
 def _kv_pages_write_op(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                        k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
-                       counts: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
+                       counts: Optional[torch.Tensor], status: Optional[torch.Tensor], scale_mode: int) -> None:
     """bf16 K/V [B, L, H, D]: token j of sequence b, j < counts[b] (None: L), goes to its
     token start[b] + j, row (start[b] + j) % page of page table[b, (start[b] + j) // page]
     of the pool [P, page, H, D]. Tokens whose page is not in the pool are dropped.
-    ``status`` as in _kv_quantize_pair_op; rows past counts do not matter to it."""
+    ``status`` as in _kv_quantize_pair_op; rows past counts do not matter to it.
+    ``scale_mode``: HN_SCALE_ZERO_ONE (the cache's rule) or HN_SCALE_RECIPROCAL."""
     what = "kv_pages_write_"
     fmt = _kv_fmt(k_codes)
     page = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
@@ -1192,12 +1194,12 @@ def _kv_pages_write_op(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: to
         L.check(L.load().hn_kv_pages_write(
             fmt, k.data_ptr(), v.data_ptr(), _strides(k), B, Lt, H, D, k_codes.data_ptr(), v_codes.data_ptr(),
             _strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), k_codes.shape[0], page,
-            table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), sp, _stream(k)),
+            table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), scale_mode, sp, _stream(k)),
             "hn_kv_pages_write")
 
 
 @_kv_pages_write_op.register_fake
-def _(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status):
+def _(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts, status, scale_mode):
     return None
 
 

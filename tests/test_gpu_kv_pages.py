@@ -343,6 +343,37 @@ def test_write_is_the_contiguous_write(dev, fmt, layout, L, H):
         assert torch.equal(raw(want), raw(got)), n
 
 
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("L", [1, 200])
+def test_scales_of_a_torch_program(dev, fmt, L):
+    """gpu_scales: amax / 448.0 (127.0) and the codes of it as torch computes them on the
+    GPU, bit for bit; rows of every magnitude, zeros and the largest values among them."""
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(L)
+    kv = [torch.randn(2, L, 24, 128, device=dev, generator=g) for _ in range(2)]
+    for x in kv:
+        x *= torch.exp2(torch.randint(-126, 126, (2, L, 24, 1), device=dev, generator=g).float())
+        x[0, 0, 0] = 0.0
+        x[1, 0, 1] = torch.finfo(BF16).max
+    kv = [x.to(BF16) for x in kv]
+    pages = 2 * -(-L // 64)
+    pool = _pool(dev, g, pages, 64, 24, fmt)
+    table = torch.arange(pages, dtype=I32, device=dev).view(2, -1)
+    kp.write_pages(pool, *kv, table, _i32(dev, [0, 0]), gpu_scales=True)
+    for key, x in zip("kv", kv):
+        x = x.float()
+        amax = x.abs().amax(-1, keepdim=True)
+        s = torch.where(amax > 0, amax / (448.0 if fmt == "fp8" else 127.0), torch.ones_like(amax))
+        y = x / s
+        codes = y.to(torch.float8_e4m3fn) if fmt == "fp8" else torch.where(
+            y >= 0, torch.floor(y + 0.5), torch.ceil(y - 0.5)).clamp(-127, 127).to(torch.int8)
+        t = torch.arange(L, device=dev)
+        for b in range(2):
+            at = table[b].long()[t // 64], t % 64
+            assert torch.equal(pool[key + "_scale"][at], s[b])
+            assert torch.equal(pool[key].view(torch.uint8)[at], codes[b].view(torch.uint8))
+
+
 @pytest.mark.parametrize("where", ["k", "v"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("B,L", [(2, 3), (3, 700)])

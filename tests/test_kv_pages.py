@@ -161,14 +161,14 @@ def test_c_abi_checks():
     def err():
         return lib.hn_last_error().decode()
 
-    def write(fmt=0, D=128, H=2, B=1, xs=st, cs=st, page=64, width=2, k=P, start=P):
+    def write(fmt=0, D=128, H=2, B=1, xs=st, cs=st, page=64, width=2, k=P, start=P, mode=1):
         return lib.hn_kv_pages_write(fmt, k, P, xs, B, 5, H, D, P, P, cs, P, P, st, 6, page, P, 2, width, start, None,
-                                     None, None)
+                                     mode, None, None)
 
     for kw, match in ((dict(fmt=3), "format"), (dict(D=64), "head dim"), (dict(H=0), "shape"), (dict(page=32), "page"),
                       (dict(page=96), "page"), (dict(width=-1), "table"), (dict(width=2 ** 31), "table"),
                       (dict(cs=odd), "multiples of 16"), (dict(xs=(ctypes.c_int64 * 4)(9, 9, 9, 1)), "multiples of 8"),
-                      (dict(k=ctypes.c_void_p(8)), "misaligned"), (dict(start=None), "null")):
+                      (dict(k=ctypes.c_void_p(8)), "misaligned"), (dict(start=None), "null"), (dict(mode=0), "scale mode")):
         assert write(**kw) == L.HN_E_ARG and match in err(), kw
     assert write(B=0) == 0
 
