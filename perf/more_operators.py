@@ -282,7 +282,7 @@ def _own(st, c):
     pages = importlib.import_module("hy-nomas_amd.kv_pages")
     if c["kind"] == "write":
         pages.write_pages(st["cache"], st["k"], st["v"], st["table"], st["start"], counts=st["counts"],
-                          status=st["status"])
+                          status=st["status"], gpu_scales=True)
         return st["status"]
     if c["kind"] == "copy":
         return pages.copy_pages(st["cache"], st["src"], st["dst"])
