@@ -19,7 +19,7 @@ HN_DEVICE int seq_len(const PageParams& p, int b) { return seq_len(p.lens, b, p.
 
 // Units of an item: of the cache, of the tail; one at least (a row without keys is written too).
 HN_DEVICE int units_of(int keys, int unit) { return (keys + unit - 1) / unit; }
-HN_DEVICE int item_units(const PageParams& p, int b, int unit = UNIT) {
+HN_DEVICE int item_units(const PageParams& p, int b, int unit) {
     const int n = units_of(seq_len(p, b), unit) + units_of(p.cur_len, unit);
     return n > 0 ? n : 1;
 }
@@ -40,6 +40,7 @@ HN_DEVICE uint32_t wave_scan(uint32_t v) {  // inclusive, over the wave
 // Where the items lie on the line of all units: sequence after sequence, in each head
 // after head, run after run. Up to 64 sequences are held in a register of the wave, a lane
 // each; more are read again where they are needed.
+template <int U>
 struct Line {
     const PageParams& p;
     uint32_t per, total;
@@ -48,7 +49,7 @@ struct Line {
     HN_DEVICE explicit Line(const PageParams& pp) : p(pp), per((uint32_t)(pp.H * pp.runs)), total(0) {
         const int lane = threadIdx.x & 63;
         for (int i0 = 0; i0 < p.B; i0 += 64) {
-            mine = i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
+            mine = i0 + lane < p.B ? item_units(p, i0 + lane, U) : 0;
             end = wave_scan((uint32_t)mine) * per;
             total += (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
         }
@@ -61,7 +62,7 @@ struct Line {
         start = 0;
         n = 1;
         for (int i0 = 0; i0 < p.B; i0 += 64) {
-            const int m = p.B <= 64 ? mine : i0 + lane < p.B ? item_units(p, i0 + lane) : 0;
+            const int m = p.B <= 64 ? mine : i0 + lane < p.B ? item_units(p, i0 + lane, U) : 0;
             const uint32_t e = p.B <= 64 ? end : wave_scan((uint32_t)m) * per;
             const uint64_t past = __ballot(before + e > u);
             if (past) {
@@ -83,9 +84,9 @@ struct Line {
         }
         const int lane = threadIdx.x & 63;
         uint32_t before = 0;
-        for (int i = lane; i < b; i += 64) before += (uint32_t)item_units(p, i);
+        for (int i = lane; i < b; i += 64) before += (uint32_t)item_units(p, i, U);
         start = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(before), 63) * per;
-        n = uniform(item_units(p, b));
+        n = uniform(item_units(p, b, U));
     }
     HN_DEVICE uint32_t share() const { return (total + (uint32_t)p.wgs - 1) / (uint32_t)p.wgs; }
 };
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
         u1 = u0 + (uint32_t)n;
     } else {
         if (wg >= p.wgs) return;
-        const Line line(p);
+        const Line<UNIT> line(p);
         const uint32_t share = line.share();
         u0 = (uint32_t)wg * share;
         u1 = u0 + share < line.total ? u0 + share : line.total;
@@ -511,23 +512,325 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: the 8-wave, three-stage half-tile loop of attn_fp8kv.hip (256 rows a
+// workgroup, one barrier a tile), its cache tiles from the pages through descriptors of
+// their own rows, its denominator from the fp32 probabilities. The tiles of all items are
+// dealt out evenly to as many workgroups as there are CUs, so that neither the sequences'
+// lengths nor a last round of workgroups leaves any idle; parts meet in
+// pages_join_kernel. The part of a tile past a length or a tail, and a page that is none,
+// read as zeros and are masked by the tile's 64-bit word.
+constexpr int TILE_WAVES = 8;
+constexpr int TILE_ROWS = Shape<TILE_WAVES>::BQ;
+
+template <int FMT, bool MASK, bool CAUSAL>
+__global__ __launch_bounds__(64 * TILE_WAVES, 1) void attn_page_tiles_kernel(PageParams p, Params t_) {
+    constexpr int NW = TILE_WAVES, NS = 3;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[NS * STAGE + 2 * SB_FLOATS * 4];
+    float* const sbuf = reinterpret_cast<float*>(smem + NS * STAGE);  // [2][128]
+    const int id = blockIdx.x;
+    const int wg = (id & 7) * p.per_xcd + (id >> 3);
+    if (wg >= p.wgs) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5, qd = threadIdx.x & 15;
+    const int per = p.H * p.runs;
+    uint32_t u0, u1, start;
+    int b, n;
+    {
+        const Line<BKV> line(p);
+        const uint32_t share = line.share();
+        u0 = (uint32_t)wg * share;
+        u1 = u0 + share < line.total ? u0 + share : line.total;
+        if (u0 >= u1) return;
+        line.find(u0, b, start, n);
+    }
+    const uint32_t range0 = u0;
+    const float c = p.scale_log2;
+    const int cur_len = p.cur_len;
+    const LaneOffs<NW> lo = lane_offsets<NW>(t_);
+    const TailOffs<NW> to = tail_offsets<NW>(t_);
+    const bool tail_ok = ((int64_t)cur_len * p.us1 + D) * 2 < ((int64_t)1 << 31);
+    const uint32_t ka_off = col * KROW + 16 * half, va_off = K_BYTES + col * VTROW + 16 * half;
+
+    while (u0 < u1) {
+        if (u0 - start >= (uint32_t)n * (uint32_t)per) {  // the next sequence
+            start += (uint32_t)n * (uint32_t)per;
+            ++b;
+            n = uniform(item_units(p, b, BKV));
+            continue;
+        }
+        const int item = (int)((u0 - start) / (uint32_t)n);  // h runs + run
+        const uint32_t item0 = start + (uint32_t)item * (uint32_t)n;
+        const int h = item / p.runs, run = item - h * p.runs;
+        const int t_begin = (int)(u0 - item0), hi = min(n, (int)(u1 - item0));
+        const int len = uniform(seq_len(p, b)), nc = units_of(len, BKV), n_all = nc + units_of(cur_len, BKV);
+        const int row = run * TILE_ROWS + wave * QW + col;
+        const bool qvalid = row < p.rows;
+        const int rr = qvalid ? row : p.rows - 1, qi = rr / p.G, hq = h * p.G + rr - qi * p.G;
+        // CAUSAL: this lane's row sees tokens below lim, every row those below lim_all, and
+        // none those from lim_end on.
+        int lim = 0, lim_all = 0, t_end = min(hi, n_all);  // (an item without a key has a unit, but no tile)
+        if constexpr (CAUSAL) {
+            const int before = len - (int)p.Lq + 1;
+            lim = before + qi;
+            lim_all = before + run * TILE_ROWS / p.G;
+            const int lim_end = before + min(run * TILE_ROWS + TILE_ROWS - 1, p.rows - 1) / p.G;
+            t_end = min(t_end, units_of(max(lim_end, 0), BKV));
+        }
+        bf16x8 qf[8];
+        {
+            const uint16_t* src = p.q + b * p.qs0 + qi * p.qs1 + hq * p.qs2 + half * 8;
+#pragma unroll
+            for (int sl = 0; sl < 8; ++sl)
+                qf[sl] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 16 * sl));
+        }
+        f32x16 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[i][v] = 0.0f;
+        Run run_{-INFINITY, 0.0f, 0.0f};
+
+        // Keys of tile t, and where its loads start.
+        struct Place {
+            TileBase src;
+            int count;
+        };
+        const ScalarInts row_table = scalar_ints(p.table + b * p.ts0);
+        const int in_page = (1 << p.shift) - 1;
+        auto cache_tile = [&](int t) __attribute__((always_inline)) {
+            Place g;
+            const int first = t * BKV;
+            int page = -1;
+            if (t < nc && t < t_end) page = row_table[first >> p.shift];
+            const bool there = (uint32_t)page < (uint32_t)p.pages;
+            g.count = there ? min(BKV, len - first) : 0;
+            g.src = tile_base(t_, there ? page : 0, h, first & in_page, g.count);
+            return g;
+        };
+        auto tail_keys = [&](int t) __attribute__((always_inline)) {
+            const int left = t < t_end ? cur_len - (t - nc) * BKV : 0;
+            return left >= BKV ? BKV : left > 0 ? left : 0;
+        };
+        auto tail_rsrc = [&](const uint16_t* base, int64_t first, int64_t rows) __attribute__((always_inline)) {
+            return tile_rsrc(base + b * p.us0 + h * p.us2 + first * p.us1, rows > 0 ? ((rows - 1) * p.us1 + D) * 2 : 0);
+        };
+        __amdgpu_buffer_rsrc_t tk = tail_rsrc(p.kcur, 0, tail_ok ? cur_len : 0),
+                               tv = tail_rsrc(p.vcur, 0, tail_ok ? cur_len : 0);
+        CacheRegs<NW> regs;
+        regs.s = 0.0f;
+        TailRegs<NW> tr;
+        uint32_t vbits = 0xffffffffu;  // MASK: validity bytes of this thread's four V keys
+        auto fetch_cache_k = [&](const Place& g) __attribute__((always_inline)) { load_k<NW, false>(lo, regs, g.src, g.count); };
+        auto fetch_tail = [&](int t) __attribute__((always_inline)) {
+            const int count = tail_keys(t);
+            const int64_t first = (int64_t)(t - nc) * BKV;
+            uint32_t co = count > 0 ? (uint32_t)(first * p.us1 * 2) : 0x80000000u;
+            if (!tail_ok && count > 0) {
+                tk = tail_rsrc(p.kcur, first, count);
+                tv = tail_rsrc(p.vcur, first, count);
+                co = 0;
+            }
+            load_tail_span_k<NW, MASK>(t_, b, to, tk, co, first, first + count, tr);
+            load_tail_span_v<NW>(to, tv, co, tr);
+            if constexpr (MASK) {
+                vbits = 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = quad_key(qd, j);
+                    if (key < count && (!p.uvalid || p.uvalid[b * p.uvs + first + key] != 0)) vbits |= 0xffu << (8 * j);
+                }
+            }
+        };
+        // What a masked key's V holds meets no product.
+        auto clear_tail_v = [&]() __attribute__((always_inline)) {
+            if constexpr (MASK)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!((vbits >> (8 * j)) & 1u)) tr.v[j][0] = tr.v[j][1] = 0u;
+        };
+        // The keys of tile t that take part, in the stage that holds it.
+        auto word_of = [&](int t, int count, const uint8_t* st) __attribute__((always_inline)) {
+            const uint64_t all = count >= BKV ? ALL_KEYS : (1ull << count) - 1;
+            if constexpr (MASK)
+                if (t >= nc) return tile_mask<true>(st) & all;
+            return all;
+        };
+
+        if (t_end > t_begin) {
+            // ---- prologue: tiles t_begin, + 1 in stages 0, 1, the next one's codes in registers
+            int c0 = 0, c1 = 0, c2 = 0;  // keys of tiles t, t + 1, t + 2
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int t = t_begin + k;
+                int count = 0;
+                if (t < nc) {
+                    const Place g = cache_tile(t);
+                    count = g.count;
+                    fetch_cache_k(g);
+                    load_v<NW>(lo, regs, g.src);
+                    __builtin_amdgcn_s_waitcnt(0);
+                    if (threadIdx.x < 2 * BKV) sbuf[(k & 1) * SB_FLOATS + threadIdx.x] = regs.s;
+                    __syncthreads();
+                    store_tile<FMT, NW, false>(regs, smem + k * STAGE, sbuf + (k & 1) * SB_FLOATS);
+                } else {
+                    count = tail_keys(t);
+                    fetch_tail(t);
+                    store_tail_k<NW, MASK>(tr, smem + k * STAGE);
+                    clear_tail_v();
+                    store_tail_v<NW>(tr, smem + k * STAGE);
+                }
+                if (k == 0) c0 = count;
+                else c1 = count;
+            }
+            {
+                const Place g = cache_tile(t_begin + 2);
+                fetch_cache_k(g);
+                load_v<NW>(lo, regs, g.src);
+                c2 = g.count;
+                if (t_begin + 2 >= nc) {
+                    c2 = tail_keys(t_begin + 2);
+                    fetch_tail(t_begin + 2);
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0);
+            // (before a tail tile no barrier has ended the reads of tile t_begin's scales)
+            if (t_begin + 2 < nc && threadIdx.x < 2 * BKV) sbuf[threadIdx.x] = regs.s;
+            __syncthreads();
+            uint64_t mw = word_of(t_begin, c0, smem);
+            f32x16 sa = s_block(smem + ka_off, qf), sb;
+            float mxa = raw_max(sa), mxb;
+            // Masks half kb of tile t, whose largest logit was mx.
+            auto masked = [&](f32x16& x, int t, int kb, uint64_t word, float mx) __attribute__((always_inline)) {
+                if constexpr (CAUSAL)
+                    if ((t + 1) * BKV > lim_all) return mask_raw(x, kb, half, lim - t * BKV, word);
+                const uint32_t w = (uint32_t)(word >> (32 * kb));
+                return w == ~0u ? mx : mask_word(x, w);
+            };
+            mxa = masked(sa, t_begin, 0, mw, mxa);
+            int t = t_begin, s0 = 0;  // s0: stage of tile t
+
+            // Tile t: S of t + 1 and the write of t + 2 beside its products; KC, FC: tile t + 2
+            // (written), t + 3 (asked for) are the cache's.
+            auto tile = [&](auto kc, auto fc) __attribute__((always_inline)) {
+                constexpr bool KC = decltype(kc)::value, FC = decltype(fc)::value;
+                const int u = t - t_begin;
+                const int s1 = s0 == NS - 1 ? 0 : s0 + 1, sw = s0 == 0 ? NS - 1 : s0 - 1;
+                const uint8_t* st = smem + s0 * STAGE;
+                const uint8_t* st1 = smem + s1 * STAGE;
+                uint8_t* wst = smem + sw * STAGE;
+                const float* wsb = sbuf + (u & 1) * SB_FLOATS;
+                Place g3;
+                if constexpr (FC) g3 = cache_tile(t + 3);
+                const int c3 = FC ? g3.count : tail_keys(t + 3);
+                f16x8 pf[2];
+                const uint64_t mwn = word_of(t + 1, c1, st1);
+                // half 0
+                rebase_high(mxa, c, run_, o);
+                sb = step_a_lse(sa, c, run_.nm, run_.l, pf, st + ka_off + 32 * KROW, qf);
+                if constexpr (KC) {
+                    mxb = step_b<FMT, NW, 1>(pf, st + va_off, 0, o, sb, regs, wst, wsb);
+                } else {
+                    mxb = step_b_with(pf, st + va_off, 0, o, sb, [&](int i) __attribute__((always_inline)) {
+                        if (i == 3 || i == 6) store_tail_k_part<NW>(tr, wst, 0, i == 6);
+                    });
+                    store_tail_mask<NW, MASK>(tr, wst);
+                }
+                mxb = masked(sb, t, 1, mw, mxb);
+                if constexpr (FC) fetch_cache_k(g3);
+                // half 1 (on the last tile the S block of "tile t + 1" reads stale LDS; its
+                // result is never used)
+                rebase_high(mxb, c, run_, o);
+                sa = step_a_lse(sb, c, run_.nm, run_.l, pf, st1 + ka_off, qf);
+                if constexpr (KC) {
+                    mxa = step_b<FMT, NW, 2>(pf, st + va_off, 1, o, sa, regs, wst, wsb);
+                } else {
+                    clear_tail_v();
+                    mxa = step_b_with(pf, st + va_off, 1, o, sa, [&](int i) __attribute__((always_inline)) {
+                        if (i & 1) store_tail_v_part<NW>(tr, wst, i >> 1);
+                    });
+                }
+                mxa = masked(sa, t + 1, 0, mwn, mxa);
+                if constexpr (FC) {
+                    if (threadIdx.x < 2 * BKV) sbuf[((u + 1) & 1) * SB_FLOATS + threadIdx.x] = regs.s;
+                    load_v<NW>(lo, regs, g3.src);
+                } else {
+                    fetch_tail(t + 3);
+                }
+                __syncthreads();
+                s0 = s1;
+                mw = mwn;
+                c0 = c1;
+                c1 = c2;
+                c2 = c3;
+            };
+            const auto yes = std::integral_constant<bool, true>{};
+            const auto no = std::integral_constant<bool, false>{};
+            // (past the end of the range both kinds are empty: cache_tile and tail_keys say so)
+            for (; t < t_end && t + 3 < nc; ++t) tile(yes, yes);
+            for (; t < t_end && t + 2 < nc; ++t) tile(yes, no);
+            for (; t < t_end; ++t) tile(no, no);
+        }
+        const float l = run_.l + __shfl_xor(run_.l, 32, 64), m = run_.m;
+        if (qvalid) {
+            if (t_begin == 0 && hi == n) {
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                uint16_t* dst = p.out + b * p.os0 + qi * p.os1 + hq * p.os2;
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+#pragma unroll
+                    for (int vq = 0; vq < 4; ++vq)
+                        *reinterpret_cast<uint2*>(dst + db * 32 + vq * 8 + half * 4) =
+                            make_uint2(pack_bf16(o[db][vq * 4] * inv, o[db][vq * 4 + 1] * inv),
+                                       pack_bf16(o[db][vq * 4 + 2] * inv, o[db][vq * 4 + 3] * inv));
+                if (half == 0)
+                    p.lse[((int64_t)b * p.H * p.G + hq) * p.Lq + qi] =
+                        l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+            } else {
+                const int64_t at = ((int64_t)wg * 2 + (item0 < range0 ? 0 : 1)) * p.pitch + wave * QW + col;
+                float* dst = p.ws_o + at * D;
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+#pragma unroll
+                    for (int vq = 0; vq < 4; ++vq)
+                        *reinterpret_cast<float4*>(dst + db * 32 + vq * 8 + half * 4) =
+                            make_float4(o[db][vq * 4], o[db][vq * 4 + 1], o[db][vq * 4 + 2], o[db][vq * 4 + 3]);
+                if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + at * 2) = make_float2(m, l);
+            }
+        }
+        __syncthreads();  // (the stages are the next item's)
+        u0 = item0 + (uint32_t)hi;
+    }
+}
+
 // The parts of items that several workgroups computed, joined in their order: with M =
 // max m, O = sum 2^(m - M) O / sum 2^(m - M) l. 32 threads a row, 4 dims each, eight rows
-// of an item a workgroup.
+// of an item a workgroup. Workgroups stand for the items, or (SEAMS) for the borders
+// between two workgroups' shares, whichever are fewer: an item is its first border's
+// (two branches' frames, 720 items of 256 rows: 40 us by items, 27 by borders).
+template <int U, bool SEAMS>
 __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
-    const Line line(p);
+    const Line<U> line(p);
     const int per = p.H * p.runs, groups = (min(R, p.rows) + 7) / 8;
     int x = blockIdx.x;
     const int grp = x % groups;
     x /= groups;
-    const int item = x % per, b = x / per;
     const uint32_t share = line.share();
     uint32_t start;
-    int n;
-    line.place(b, start, n);
+    int n, b, item;
+    if constexpr (SEAMS) {
+        const uint32_t seam = (uint32_t)(x + 1) * share;
+        if (seam >= line.total) return;
+        line.find(seam, b, start, n);
+        item = (int)((seam - start) / (uint32_t)n);
+    } else {
+        item = x % per;
+        b = x / per;
+        line.place(b, start, n);
+    }
     const uint32_t i0 = start + (uint32_t)item * (uint32_t)n;
     const uint32_t w0 = i0 / share, w1 = (i0 + (uint32_t)n - 1) / share;
-    if (w0 == w1) return;  // whole: written already
+    if (w0 == w1 || (SEAMS && (uint32_t)x != w0)) return;  // whole (written already), or another border's
     const int h = item / p.runs, run = item - h * p.runs;
     const int r = grp * 8 + (threadIdx.x >> 5), row = run * R + r, d = (threadIdx.x & 31) * 4;
     if (r >= R || row >= p.rows) return;
@@ -576,7 +879,7 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
 using namespace hn;
 
 struct PagesPlan {
-    int tiles;   // the tile kernel
+    int tiles;   // 0: attn_pages_kernel, 4 and 8: the tile kernels of as many waves
     int rb, runs, whole, wgs, pitch;
     int64_t items;
 };
@@ -584,7 +887,19 @@ struct PagesPlan {
 static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len, int causal) {
     PagesPlan pl;
     const int64_t rows = Lq * G;
-    pl.tiles = !causal && rows > 32;
+    // Two sequences x 24 heads x 20000 keys (calls, us): 32 rows 59 in attn_pages_kernel and 95 in
+    // the 4-wave tiles, 64 rows 101 and 99, 128 rows 182 and 107, there 147 in the 8-wave ones; 129
+    // rows 179 against 148, 300 264 and 277, 777 583 and 539, 3600 2293 and 1951; with 3000 keys
+    // 128 rows 38 against 47, 256 48 and 57, 512 81 and 78. Causal rows have no 4-wave tiles.
+    pl.tiles = rows <= 32 ? 0 : rows > 128 ? attn::TILE_WAVES : causal ? 0 : 4;
+    if (pl.tiles == attn::TILE_WAVES) {
+        pl.runs = (int)((rows + attn::TILE_ROWS - 1) / attn::TILE_ROWS);
+        pl.items = B * H * pl.runs;
+        pl.pitch = (int)(rows < attn::TILE_ROWS ? rows : attn::TILE_ROWS);
+        pl.wgs = device_cus();
+        pl.whole = 0;
+        return pl;
+    }
     pl.rb = rows <= 16 ? 1 : 2;
     const int64_t R = 16 * pl.rb;
     pl.runs = (int)((rows + R - 1) / R);
@@ -610,18 +925,39 @@ static void launch_pages(int rb, bool sv, const attn::PageParams& p, unsigned bl
     else attn::attn_pages_kernel<FMT, 2, false, NW><<<blocks, 64 * NW, 0, st>>>(p);
 }
 
+template <int FMT>
+static void launch_tiles(const attn::PageParams& p, const attn::Params& t, unsigned blocks, hipStream_t st) {
+    constexpr int threads = 64 * attn::TILE_WAVES;
+    if (p.causal) attn::attn_page_tiles_kernel<FMT, false, true><<<blocks, threads, 0, st>>>(p, t);
+    else if (p.uvalid) attn::attn_page_tiles_kernel<FMT, true, false><<<blocks, threads, 0, st>>>(p, t);
+    else attn::attn_page_tiles_kernel<FMT, false, false><<<blocks, threads, 0, st>>>(p, t);
+}
+
 static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len, int64_t cur_len) {
     return B > 0 && Lq > 0 && H > 0 && Hq > 0 && Hq % H == 0 && max_len >= 0 && cur_len >= 0 && B <= 0x7fffffffLL &&
            Lq <= 0x7fffffffLL && Hq <= 0x7fffffffLL && max_len <= 0x3fffffffLL && cur_len <= 0x3fffffffLL &&
            Lq * (Hq / H) <= 0x3fffffffLL;
 }
 
+template <int U>
+static int join_pages(const PagesPlan& pl, const attn::PageParams& p, int R, hipStream_t st) {
+    const int64_t groups = (pl.pitch + 7) / 8;
+    if (pl.items < pl.wgs) attn::pages_join_kernel<U, false><<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
+    else attn::pages_join_kernel<U, true><<<(unsigned)((pl.wgs - 1) * groups), 256, 0, st>>>(p, R);
+    return check_launch("hn_attn_kv_pages (join)");
+}
+
+static int64_t plan_bytes(const PagesPlan& pl, int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
+                          int64_t cur_len) {
+    if (pl.tiles == 4) return page_tiles_workspace(B, Lq, Hq, H, max_len, cur_len);
+    return pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+}
+
 extern "C" int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
                                                    int64_t cur_len, int causal) {
     if (!pages_shape_ok(B, Lq, Hq, H, max_len, cur_len)) return 0;
     const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
-    if (pl.tiles) return page_tiles_workspace(B, Lq, Hq, H, max_len, cur_len);
-    return pl.whole ? 0 : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+    return plan_bytes(pl, B, Lq, Hq, H, max_len, cur_len);
 }
 
 extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64_t B, int64_t Lq, int64_t Hq,
@@ -666,11 +1002,9 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     const int64_t max_len = n_pages ? width * page : 0;
     HN_REQUIRE(pages_shape_ok(B, Lq, Hq, H, max_len, cur_len), HN_E_ARG, "hn_attn_kv_pages: too much work");
     const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
-    const int64_t units = 1 + (max_len + attn::UNIT - 1) / attn::UNIT + (cur_len + attn::UNIT - 1) / attn::UNIT;
+    const int64_t units = 1 + (max_len + attn::BKV - 1) / attn::BKV + (cur_len + attn::BKV - 1) / attn::BKV;
     HN_REQUIRE(pl.items <= 0x3fffffffLL / units, HN_E_ARG, "hn_attn_kv_pages: too much work for one launch");
-    const int64_t need = pl.tiles   ? page_tiles_workspace(B, Lq, Hq, H, max_len, cur_len)
-                         : pl.whole ? 0
-                                    : (int64_t)pl.wgs * 2 * pl.pitch * (attn::D + 2) * (int64_t)sizeof(float);
+    const int64_t need = plan_bytes(pl, B, Lq, Hq, H, max_len, cur_len);
     HN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))), HN_E_ARG,
                "hn_attn_kv_pages: workspace smaller than hn_attn_kv_pages_workspace_size() or misaligned");
     if (const int rc = require_gfx950("hn_attn_kv_pages"); rc != HN_OK) return rc;
@@ -697,7 +1031,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.cur_len = (int)cur_len;
     p.causal = causal != 0;
     p.scale_log2 = softmax_scale * 1.4426950408889634f;
-    if (pl.tiles) return launch_page_tiles(p, fmt, workspace, (hipStream_t)stream);
+    if (pl.tiles == 4) return launch_page_tiles(p, fmt, workspace, (hipStream_t)stream);
     p.wgs = pl.wgs;
     p.pitch = pl.pitch;
     if (!pl.whole) {
@@ -708,6 +1042,17 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.per_xcd = (int)((grid + 7) / 8);
     const unsigned blocks = 8u * (unsigned)p.per_xcd;
     const hipStream_t st = (hipStream_t)stream;
+    if (pl.tiles) {
+        attn::Params t = {};
+        t.kc = p.kc; t.vc = p.vc; t.ks = p.ks; t.vs = p.vs;
+        t.cs0 = p.cs0; t.cs1 = p.cs1; t.cs2 = p.cs2;
+        t.ss0 = p.ss0; t.ss1 = p.ss1; t.ss2 = p.ss2;
+        t.uvalid = p.uvalid; t.uvs = p.uvs; t.us1 = p.us1;
+        if (fmt == HN_KV_FP8) launch_tiles<HN_KV_FP8>(p, t, blocks, st);
+        else launch_tiles<HN_KV_INT8>(p, t, blocks, st);
+        if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK) return rc;
+        return join_pages<attn::BKV>(pl, p, attn::TILE_ROWS, st);
+    }
     const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(vs, 16);
     if (fmt == HN_KV_FP8) {
         if (pl.whole) launch_pages<HN_KV_FP8, 8>(pl.rb, sv, p, blocks, st);
@@ -717,7 +1062,5 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
         else launch_pages<HN_KV_INT8, 4>(pl.rb, sv, p, blocks, st);
     }
     if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK || pl.whole) return rc;
-    const int R = 16 * pl.rb, groups = (pl.pitch + 7) / 8;
-    attn::pages_join_kernel<<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
-    return check_launch("hn_attn_kv_pages (join)");
+    return join_pages<attn::UNIT>(pl, p, 16 * pl.rb, st);
 }

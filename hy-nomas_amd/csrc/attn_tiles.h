@@ -768,5 +768,61 @@ HN_DEVICE float step_b(const f16x8 (&pf)[2], const uint8_t* va, int kb, f32x16 (
     });
 }
 
+// ---------------------------------------------------------------------------
+// The steps of the kernels that return a row's log-sum-exp.
+
+// Step A with the denominator summed from the fp32 probabilities, so that the
+// row's log-sum-exp carries no rounding of the fp16 ones (their sum would be off
+// by up to 2^-12 relative where one key dominates).
+HN_DEVICE f32x16 step_a_lse(const f32x16& s, float c, float nm, float& l, f16x8 (&pf)[2], const uint8_t* ka,
+                            const bf16x8 (&qf)[8]) {
+    bf16x8 kf[8];
+    kf[0] = ld_bf16x8(ka);
+    kf[1] = ld_bf16x8(ka + 32);
+    f32x16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.0f;
+    float ls = 0.0f;
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i + 2 < 8) kf[i + 2] = ld_bf16x8(ka + 32 * (i + 2));
+        acc = mfma_bf16(kf[i], qf[i], acc);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], c, nm));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], c, nm));
+        x[i] = pack_f16(p0, p1);
+        ls += p0;
+        ls += p1;
+        pin(x[i], ls);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    l += ls;
+    pf[0] = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
+    pf[1] = __builtin_bit_cast(f16x8, make_uint4(x[4], x[5], x[6], x[7]));
+    return acc;
+}
+
+// rebase with the running maximum held 2^11 low: probabilities are 2^11 to
+// 2^15 where a row's largest is, so that fp16 holds those down to 2^-25 of it in full
+// (2^-14 with the largest at 1) and what lies below is off by 2^-36 of it. Over a long
+// history many small weights add up to what one large one leaves. (The slack shrinks
+// from 2^8 to 2^4: fp16 ends at 2^16.)
+constexpr float PROB_LOG2 = 11.0f, PROB_TOP = 15.0f;
+
+HN_DEVICE void rebase_high(float mx, float c, Run& run, f32x16 (&o)[4]) {
+    if (!__any(mx * c > run.m + PROB_TOP)) return;
+    const float mnew = fmaxf(run.m, pair_max(mx) * c - PROB_LOG2);
+    const float alpha = run.m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m - mnew);
+    run.m = mnew;
+    run.nm = mnew == -INFINITY ? 0.0f : -mnew;  // m = -inf: every s is -inf (masked)
+    run.l *= alpha;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+    }
+}
+
 }  // namespace attn
 }  // namespace hn

@@ -131,7 +131,7 @@ def test_one_token(dev, fmt, H, G, lens):
 
 
 @pytest.mark.parametrize("page", [64, 256, 1024])
-@pytest.mark.parametrize("Lq,G", [(2, 1), (5, 4), (8, 2), (9, 4), (33, 1), (70, 3)])
+@pytest.mark.parametrize("Lq,G", [(2, 1), (5, 4), (8, 2), (9, 4), (33, 1), (70, 3), (129, 1), (300, 1), (101, 5)])
 def test_causal(dev, page, Lq, G):
     """Sequences shorter than the queries have rows without a key."""
     _, ca, _ = _mods()
