@@ -204,18 +204,17 @@ __global__ __launch_bounds__(ALONE ? 1024 : 256) void pages_write_kernel(WriteAr
         const bool ok = all_finite(a);
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.flag = !ok;
         if (!ok) return;
-    } else {
-        if (a.status != nullptr && *a.status != 0) return;  // refused: nothing is written
     }
+    // (asked for here, looked at before the first store: the values' loads do not wait for it)
+    int32_t refused = 0;
+    if (!ALONE && a.status) refused = *(ScalarInts)a.status;
     // (from the last tile on: what the check has read last may be in a cache yet)
     const Place at = tile_place(a.tiles, true);
     const int sel = at.part & 1, t0 = at.t0;
     for (int b = gridDim.y - 1 - blockIdx.y; b < a.tiles.B; b += gridDim.y) {
         const int last = new_tokens(a, b);
         const int first = ((ScalarInts)a.start)[b];
-        if (t0 >= last || first < 0) continue;
-        const uint32_t pos0 = (uint32_t)first + (uint32_t)t0;
-        const TilePages pages = tile_pages(a.pool, b, pos0, a.tiles.tsh);
+        if (t0 >= last) continue;
         Values v[NK];
         Row w[NK];
 #pragma unroll
@@ -223,6 +222,10 @@ __global__ __launch_bounds__(ALONE ? 1024 : 256) void pages_write_kernel(WriteAr
             w[k] = tile_row(a.tiles, t0, at.part >> 1, k, last);
             if (w[k].there) v[k] = row_values(a, sel, b, w[k]);
         }
+        const uint32_t pos0 = (uint32_t)first + (uint32_t)t0;
+        const TilePages pages = tile_pages(a.pool, b, pos0, a.tiles.tsh);
+        if (refused != 0) return;  // nothing is written
+        if (first < 0) continue;
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
             const uint32_t pos = pos0 + (uint32_t)(w[k].t - t0);
@@ -508,7 +511,7 @@ extern "C" int hn_kv_pages_copy(void* const* base, const int64_t* layer_stride, 
                    "hn_kv_pages_copy: a page outside the pool");
     if (const int rc = require_gfx950(who); rc != HN_OK) return rc;
     const int64_t per_pair = (int64_t)a.piece0[4] * layers;
-    int64_t most = 0x7fffffffLL / per_pair;
+    int64_t most = 0xffffffLL / per_pair;  // (a grid has fewer than 2^32 threads)
     HN_REQUIRE(most > 0, HN_E_ARG, "hn_kv_pages_copy: a page of all layers is too large");
     most = most < pages::MAX_PAIRS ? most : pages::MAX_PAIRS;
     for (int64_t i0 = 0; i0 < n; i0 += most) {

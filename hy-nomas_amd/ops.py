@@ -1126,23 +1126,25 @@ def _(out_k, out_v, out_k_scale, out_v_scale, k_codes, v_codes, k_scale, v_scale
 # --------------------------------------------------------------------------
 # the cache in pages: write, copy, decode, attention
 
-def _check_pool(codes: torch.Tensor, scale: torch.Tensor, what: str) -> int:
-    """A layer's pool: codes [P, page, H, D] with fp32 scales [P, page, H, 1]. Returns
-    the page's tokens."""
-    if codes.ndim != 4 or scale.dtype != torch.float32 or tuple(scale.shape) != (*codes.shape[:3], 1):
+def _check_pool(codes: torch.Tensor, scale: torch.Tensor, what: str) -> tuple:
+    """A layer's pool: codes [P, page, H, D] with fp32 scales [P, page, H, 1]. Returns the
+    codes' shape."""
+    shape = codes.shape
+    if len(shape) != 4 or scale.dtype != torch.float32 or scale.shape != (*shape[:3], 1):
         raise ValueError(f"{what}: codes [P, page, H, D] with fp32 scales [P, page, H, 1]")
-    if codes.shape[1] not in BLOCK_SIZES:
+    if shape[1] not in BLOCK_SIZES:
         raise ValueError(f"{what}: a page must be of {BLOCK_SIZES} tokens")
-    return codes.shape[1]
+    return shape
 
 
-def _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what: str) -> int:
-    page = _check_pool(k_codes, k_scale, what)
-    if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride()
-            or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape
-            or v_scale.stride() != k_scale.stride()):
+def _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what: str) -> tuple:
+    """Both pools of a layer: their shape, and the strides of codes and scales as C arrays."""
+    shape = _check_pool(k_codes, k_scale, what)
+    cs, ss = k_codes.stride(), k_scale.stride()
+    if (v_codes.dtype != k_codes.dtype or v_codes.shape != shape or v_codes.stride() != cs
+            or v_scale.dtype != torch.float32 or v_scale.shape != k_scale.shape or v_scale.stride() != ss):
         raise ValueError(f"{what}: K and V must share dtype, shape and strides")
-    return page
+    return shape, _stride_array(cs), _stride_array(ss)
 
 
 def _page_table(table: torch.Tensor, B: int, what: str) -> torch.Tensor:
@@ -1155,9 +1157,9 @@ def _page_table(table: torch.Tensor, B: int, what: str) -> torch.Tensor:
 def _per_sequence(t: Optional[torch.Tensor], B: int, what: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+    if t.dtype != torch.int32 or t.shape != (B,):
         raise ValueError(f"{what} must be int32 [B]")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def kv_pages_write_(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts=None, status=None,
@@ -1177,23 +1179,26 @@ def _kv_pages_write_op(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: to
     ``scale_mode``: HN_SCALE_ZERO_ONE (the cache's rule) or HN_SCALE_RECIPROCAL."""
     what = "kv_pages_write_"
     fmt = _kv_fmt(k_codes)
-    page = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
+    (P, page, *row), cs, ss = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise TypeError(f"{what} expects bf16 values")
-    if k.ndim != 4 or k.shape != v.shape or tuple(k.shape[2:]) != tuple(k_codes.shape[2:]):
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or list(shape[2:]) != row:
         raise ValueError(f"{what}: k and v must be [B, L, H, D] matching the pool")
-    B, Lt, H, D = k.shape
+    B, Lt, H, D = shape
     table = _page_table(table, B, what)
     start, counts = _per_sequence(start, B, f"{what}: start"), _per_sequence(counts, B, f"{what}: counts")
     sp = _status_ptr(status)
     k, v = _head_rows(k), _head_rows(v)
-    if k.stride() != v.stride():
+    xs = k.stride()
+    if v.stride() != xs:
         k, v = k.contiguous(), v.contiguous()
-    _one_device(what, k, v, k_codes, v_codes, k_scale, v_scale, table, start, counts, status)
-    with _on(k.device):
+        xs = k.stride()
+    device = _one_device(what, k, v, k_codes, v_codes, k_scale, v_scale, table, start, counts, status)
+    with _on(device):
         L.check(L.load().hn_kv_pages_write(
-            fmt, k.data_ptr(), v.data_ptr(), _strides(k), B, Lt, H, D, k_codes.data_ptr(), v_codes.data_ptr(),
-            _strides(k_codes), k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), k_codes.shape[0], page,
+            fmt, k.data_ptr(), v.data_ptr(), _stride_array(xs), B, Lt, H, D, k_codes.data_ptr(), v_codes.data_ptr(),
+            cs, k_scale.data_ptr(), v_scale.data_ptr(), ss, P, page,
             table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), scale_mode, sp, _stream(k)),
             "hn_kv_pages_write")
 
@@ -1210,12 +1215,11 @@ def kv_pages_read(codes: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
     kv_len[b] (int32 [B]), zeros behind: a new [B, max_len, H, D]."""
     what = "kv_pages_read"
     fmt = _kv_fmt(codes)
-    page = _check_pool(codes, scale, what)
+    P, page, H, D = _check_pool(codes, scale, what)
     if max_len < 0:
         raise ValueError(f"{what}: max_len must not be negative")
     B = table.shape[0] if table.ndim else 0
     table, kv_len = _page_table(table, B, what), _per_sequence(kv_len, B, f"{what}: kv_len")
-    P, _, H, D = codes.shape
     _one_device(what, codes, scale, table, kv_len)
     y = torch.empty((B, max_len, H, D), dtype=torch.bfloat16, device=codes.device)
     if y.numel() == 0:
@@ -1313,33 +1317,35 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
     if q.dtype != torch.bfloat16:
         raise TypeError(f"{what} expects bf16 queries")
     fmt = _kv_fmt(k_codes)
-    page = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
-    P, _, H, Dk = k_codes.shape
-    if q.ndim != 4:
+    (P, page, H, Dk), cs, ss = _check_pool_pair(k_codes, v_codes, k_scale, v_scale, what)
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"{what}: q must be [B, Lq, Hq, D]")
-    B, Lq, Hq, D = q.shape
+    B, Lq, Hq, D = shape
     if Dk != D or H == 0 or Hq % H:
         raise ValueError(f"{what}: pool [P, page, H, D] does not match q")
     table, kv_len = _page_table(table, B, what), _per_sequence(kv_len, B, f"{what}: kv_len")
     scale = _softmax_scale(softmax_scale, D, what)
-    cur_len = 0 if k_cur is None else k_cur.shape[1] if k_cur.ndim == 4 else -1
-    if k_cur is not None and (k_cur.ndim != 4 or k_cur.shape[0] != B or tuple(k_cur.shape[2:]) != (H, D)):
-        raise ValueError(f"{what}: k_cur must be [B, Lc, H, D] matching the pool")
-    if (k_cur is None) != (v_cur is None) or (k_cur is not None and (
-            v_cur.shape != k_cur.shape or k_cur.dtype != torch.bfloat16 or v_cur.dtype != torch.bfloat16)):
-        raise ValueError(f"{what}: k_cur/v_cur must be matching bf16 tensors")
-    if causal and cur_len:
-        raise ValueError(f"{what}: a causal call takes no tail")
+    cur_len, uvb, uvs = 0, None, 0
+    if k_cur is not None or v_cur is not None:
+        if k_cur is not None and (k_cur.ndim != 4 or k_cur.shape[0] != B or tuple(k_cur.shape[2:]) != (H, D)):
+            raise ValueError(f"{what}: k_cur must be [B, Lc, H, D] matching the pool")
+        if k_cur is None or v_cur is None or (
+                v_cur.shape != k_cur.shape or k_cur.dtype != torch.bfloat16 or v_cur.dtype != torch.bfloat16):
+            raise ValueError(f"{what}: k_cur/v_cur must be matching bf16 tensors")
+        cur_len = k_cur.shape[1]
+        if causal and cur_len:
+            raise ValueError(f"{what}: a causal call takes no tail")
+        if cur_len:
+            k_cur, v_cur = _head_rows(k_cur), _head_rows(v_cur)
+            if k_cur.stride() != v_cur.stride():
+                k_cur, v_cur = k_cur.contiguous(), v_cur.contiguous()
+            uvb, uvs = _mask_bytes(cur_valid, B, cur_len, f"{what}: cur_valid")
     q = _head_rows(q)
-    if cur_len:
-        k_cur, v_cur = _head_rows(k_cur), _head_rows(v_cur)
-        if k_cur.stride() != v_cur.stride():
-            k_cur, v_cur = k_cur.contiguous(), v_cur.contiguous()
-    uvb, uvs = _mask_bytes(cur_valid if cur_len else None, B, cur_len, f"{what}: cur_valid")
     device = _one_device(what, q, k_codes, v_codes, k_scale, v_scale, table, kv_len, k_cur, v_cur, uvb)
-    out = torch.empty((B, Lq, Hq, D), dtype=torch.bfloat16, device=device)
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
-    if out.numel() == 0:
+    if B == 0 or Lq == 0 or Hq == 0:
         return out, lse
     W = table.shape[1]
     with _on(device):
@@ -1347,8 +1353,8 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
         ws_bytes = _pages_workspace(device.index, B, Lq, Hq, H, W * page if P else 0, cur_len, int(causal))
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes else None
         L.check(lib.hn_attn_kv_pages(
-            fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), _strides(k_codes),
-            k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale), H, P, page, table.data_ptr(), table.stride(0), W,
+            fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), cs,
+            k_scale.data_ptr(), v_scale.data_ptr(), ss, H, P, page, table.data_ptr(), table.stride(0), W,
             kv_len.data_ptr(), int(causal), L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
             _strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), _strides(out),
             lse.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_kv_pages")
