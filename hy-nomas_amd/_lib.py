@@ -82,7 +82,7 @@ SIGNATURES = {
     "hn_kv_pages_read": [_I, _P, _PI64, _P, _PI64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
     "hn_kv_pages_copy": [ctypes.POINTER(_P), _PI64, _PI64, _PI64, _I64, _I64, _PI32, _PI32, _I64, _P],
     "hn_attn_kv_pages": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64, _I64,
-                         _P, _I64, _I64, _P, _I, _P, _P, _PI64, _I64, _P, _I64, _F, _P, _PI64, _P, _P, _I64, _P],
+                         _P, _I64, _I64, _P, _I, _P, _P, _P, _PI64, _I64, _P, _I64, _F, _P, _PI64, _P, _P, _I64, _P],
     "hn_attn_kv_pages_workspace_size": [_I64] * 6 + [_I],
     "hn_e4m3_encode_range": [ctypes.c_uint32, _I64, _P, _P],
 }

@@ -92,8 +92,8 @@ def sparse_chunk_attention(q: torch.Tensor, kv_cache: dict, kv_len: int, block_i
 
 def paged_attention(q: torch.Tensor, cache: dict, table: torch.Tensor, kv_len: torch.Tensor, *,
                     causal: bool = False, k_cur: Optional[torch.Tensor] = None, v_cur: Optional[torch.Tensor] = None,
-                    softmax_scale: Optional[float] = None,
-                    cur_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+                    softmax_scale: Optional[float] = None, cur_valid: Optional[torch.Tensor] = None,
+                    q_start: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """softmax(q K^T * scale) V over every sequence's own tokens in a pool of pages, then
     k_cur/v_cur, and the rows' log-sum-exp: (out [B, Lq, Hq, D], lse fp32 [B, Hq, Lq]).
 
@@ -101,15 +101,15 @@ def paged_attention(q: torch.Tensor, cache: dict, table: torch.Tensor, kv_len: t
     table int32 [B, W] names the pages of each sequence, kv_len int32 [B] its tokens, both
     on the GPU: they may change between replays of a captured call. Hq may be a multiple
     of the pool's heads. Without ``causal`` every query sees its sequence's tokens and the
-    valid tail (cur_valid bool [B or 1, >= Lc]); with it the queries are the sequence's
-    last Lq tokens, written already, and each sees those up to itself. A query without a
-    key gets a zero row and lse -inf, one that meets a NaN gets NaN in both. Entries of
+    valid tail (cur_valid bool [B or 1, >= Lc]); with it query i is the sequence's token
+    q_start[b] + i, written already (int32 [B]; None: the queries are its last Lq tokens),
+    and sees those up to itself. A query without a key gets a zero row and lse -inf, one that meets a NaN gets NaN in both. Entries of
     the table outside the pool name no keys.
     """
     if not is_quantized_kv_cache(cache):
         raise TypeError("paged_attention reads FP8/INT8 caches")
     return ops.attn_kv_pages(q, cache["k"], cache["v"], cache["k_scale"], cache["v_scale"], table, kv_len, bool(causal),
-                             k_cur, v_cur, None if softmax_scale is None else float(softmax_scale), cur_valid)
+                             k_cur, v_cur, None if softmax_scale is None else float(softmax_scale), cur_valid, q_start)
 
 
 def _dense_sparse_context(sparse_context, kv_cache, update_cache):

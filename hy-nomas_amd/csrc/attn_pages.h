@@ -19,6 +19,7 @@ struct PageParams {
     float* lse;              // [B, H G, Lq]
     const int32_t* table;
     const int32_t* lens;
+    const int32_t* q_start;  // causal: each sequence's first query's token; null: its last Lq tokens are the queries
     int64_t ts0, uvs;
     int64_t qs0, qs1, qs2;
     int64_t cs0, cs1, cs2;   // page, token, head
@@ -49,6 +50,12 @@ HN_DEVICE ScalarInts scalar_ints(const int32_t* p) { return (ScalarInts)p; }
 HN_DEVICE int seq_len(const int32_t* lens, int64_t b, int width, int shift) {
     const int n = lens[b], most = width << shift;
     return n < 0 ? 0 : n < most ? n : most;
+}
+
+// Causal rows: query i sees tokens below seen_before + i, and below the sequence's length.
+HN_DEVICE int seen_before(const PageParams& p, int b, int len) {
+    const int first = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : len - (int)p.Lq;
+    return (first < len ? first : len) + 1;
 }
 
 }  // namespace attn

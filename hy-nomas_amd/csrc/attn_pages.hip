@@ -202,6 +202,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
         bf16x8 qf[RB][4];
         int lim[RB];           // this lane's rows see cached tokens below
         int lim_all = len;     // all rows do
+        const int before = p.causal ? seen_before(p, b, len) : len;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int r = row0 + min(16 * rb + r16, rows - 1), qi = r / p.G;
@@ -209,9 +210,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
 #pragma unroll
             for (int s = 0; s < 4; ++s)
                 qf[rb][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 64 * (s >> 1) + 8 * (s & 1)));
-            lim[rb] = p.causal ? len - (int)p.Lq + 1 + qi : len;
+            lim[rb] = p.causal ? min(before + qi, len) : len;
         }
-        if (p.causal) lim_all = len - (int)p.Lq + 1 + row0 / p.G;
+        if (p.causal) lim_all = min(before + row0 / p.G, len);
         Rows<RB> st;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -571,9 +572,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES, 1) void attn_page_tiles_kernel(Pag
         // none those from lim_end on.
         int lim = 0, lim_all = 0, t_end = min(hi, n_all);  // (an item without a key has a unit, but no tile)
         if constexpr (CAUSAL) {
-            const int before = len - (int)p.Lq + 1;
-            lim = before + qi;
-            lim_all = before + run * TILE_ROWS / p.G;
+            const int before = seen_before(p, b, len);
+            lim = min(before + qi, len);
+            lim_all = min(before + run * TILE_ROWS / p.G, len);
             const int lim_end = before + min(run * TILE_ROWS + TILE_ROWS - 1, p.rows - 1) / p.G;
             t_end = min(t_end, units_of(max(lim_end, 0), BKV));
         }
@@ -964,7 +965,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
                                 int64_t D, const void* kc, const void* vc, const int64_t* cs, const float* ks,
                                 const float* vs, const int64_t* ss, int64_t H, int64_t n_pages, int64_t page,
                                 const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
-                                int causal, const void* kcur, const void* vcur, const int64_t* curs, int64_t cur_len,
+                                int causal, const int32_t* q_start, const void* kcur, const void* vcur, const int64_t* curs, int64_t cur_len,
                                 const uint8_t* cur_valid, int64_t cur_valid_stride, float softmax_scale, void* out,
                                 const int64_t* os, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
     HN_REQUIRE(fmt == HN_KV_FP8 || fmt == HN_KV_INT8, HN_E_ARG, "hn_attn_kv_pages: unknown KV format");
@@ -976,6 +977,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     HN_REQUIRE(width <= 0x3fffffffLL / page && n_pages <= 0x7fffffffLL && cur_len <= 0x3fffffffLL, HN_E_ARG,
                "hn_attn_kv_pages: too many keys");
     HN_REQUIRE(!causal || cur_len == 0, HN_E_ARG, "hn_attn_kv_pages: a causal call takes no tail");
+    HN_REQUIRE(causal || !q_start, HN_E_ARG, "hn_attn_kv_pages: q_start is a causal call's");
     HN_REQUIRE(softmax_scale > 0.0f && softmax_scale <= 3.4028234e38f, HN_E_ARG,
                "hn_attn_kv_pages: softmax_scale must be finite and positive");
     HN_REQUIRE(qs && os && cs && ss && (cur_len == 0 || curs), HN_E_ARG, "hn_attn_kv_pages: null stride array");
@@ -986,7 +988,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
                    ss[0] >= 0 && ss[1] >= 0 && ss[2] >= 0 && cs[1] <= 0x1ffffffLL && ss[1] <= 0x7fffffLL,
                HN_E_ARG, "hn_attn_kv_pages: pool strides must be multiples of 16 bytes");
     HN_REQUIRE(aligned(q, 16) && aligned(out, 8) && aligned(kc, 16) && aligned(vc, 16) && aligned(ks, 4) &&
-                   aligned(vs, 4) && aligned(table, 4) && aligned(lens, 4) && aligned(lse, 4),
+                   aligned(vs, 4) && aligned(table, 4) && aligned(lens, 4) && aligned(q_start, 4) && aligned(lse, 4),
                HN_E_ARG, "hn_attn_kv_pages: misaligned pointer");
     HN_REQUIRE(table_stride >= 0 && cur_valid_stride >= 0, HN_E_ARG, "hn_attn_kv_pages: negative stride");
     if (cur_len > 0) {
@@ -1014,11 +1016,16 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     p.kcur = (const uint16_t*)kcur; p.vcur = (const uint16_t*)vcur;
     p.uvalid = cur_len > 0 ? cur_valid : nullptr;
     p.uvs = cur_valid_stride;
-    p.table = table; p.lens = lens; p.ts0 = table_stride;
+    p.table = table; p.lens = lens; p.q_start = q_start; p.ts0 = table_stride;
     p.qs0 = qs[0]; p.qs1 = qs[1]; p.qs2 = qs[2];
     p.os0 = os[0]; p.os1 = os[1]; p.os2 = os[2];
     p.cs0 = cs[0]; p.cs1 = cs[1]; p.cs2 = cs[2];
     p.ss0 = ss[0]; p.ss1 = ss[1]; p.ss2 = ss[2];
+    if (max_len == 0) {  // no pool: what the kernels' empty loads are based on is a query's first 256 bytes
+        p.kc = p.vc = (const uint8_t*)q;
+        p.ks = p.vs = (const float*)q;
+        p.cs0 = p.cs1 = p.cs2 = p.ss0 = p.ss1 = p.ss2 = 0;
+    }
     if (cur_len > 0) {
         p.us0 = curs[0]; p.us1 = curs[1]; p.us2 = curs[2];
     }
@@ -1053,7 +1060,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
         if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK) return rc;
         return join_pages<attn::BKV>(pl, p, attn::TILE_ROWS, st);
     }
-    const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(vs, 16);
+    const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(p.vs, 16);
     if (fmt == HN_KV_FP8) {
         if (pl.whole) launch_pages<HN_KV_FP8, 8>(pl.rb, sv, p, blocks, st);
         else launch_pages<HN_KV_FP8, 4>(pl.rb, sv, p, blocks, st);

@@ -1304,15 +1304,16 @@ def _pages_workspace(device: int, *sizes) -> int:
 def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, causal: bool = False,
                   k_cur: Optional[torch.Tensor] = None, v_cur: Optional[torch.Tensor] = None,
-                  softmax_scale: Optional[float] = None,
-                  cur_valid: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  softmax_scale: Optional[float] = None, cur_valid: Optional[torch.Tensor] = None,
+                  q_start: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of q [B, Lq, Hq, D] over each sequence's cached tokens [0, kv_len[b]) in
     the pages of table [B, W], and the bf16 tail k_cur/v_cur [B, Lc, H, D]: out bf16 [B,
     Lq, Hq, D] and the rows' log-sum-exp fp32 [B, Hq, Lq].
 
-    The pool is [P, page, H, D], Hq a multiple of H. causal (without a tail): the queries
-    are the sequence's last Lq tokens and each sees what is not behind it. cur_valid (bool
-    [B or 1, >= Lc]) excludes tail keys. See hn_attn_kv_pages."""
+    The pool is [P, page, H, D], Hq a multiple of H. causal (without a tail): query i is
+    the sequence's token q_start[b] + i (int32 [B]; None: its last Lq tokens are the
+    queries) and sees what is not behind it. cur_valid (bool [B or 1, >= Lc]) excludes tail
+    keys. See hn_attn_kv_pages."""
     what = "attn_kv_pages"
     if q.dtype != torch.bfloat16:
         raise TypeError(f"{what} expects bf16 queries")
@@ -1326,6 +1327,9 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
         raise ValueError(f"{what}: pool [P, page, H, D] does not match q")
     table, kv_len = _page_table(table, B, what), _per_sequence(kv_len, B, f"{what}: kv_len")
     scale = _softmax_scale(softmax_scale, D, what)
+    q_start = _per_sequence(q_start, B, f"{what}: q_start")
+    if q_start is not None and not causal:
+        raise ValueError(f"{what}: q_start is a causal call's")
     cur_len, uvb, uvs = 0, None, 0
     if k_cur is not None or v_cur is not None:
         if k_cur is not None and (k_cur.ndim != 4 or k_cur.shape[0] != B or tuple(k_cur.shape[2:]) != (H, D)):
@@ -1342,7 +1346,7 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
                 k_cur, v_cur = k_cur.contiguous(), v_cur.contiguous()
             uvb, uvs = _mask_bytes(cur_valid, B, cur_len, f"{what}: cur_valid")
     q = _head_rows(q)
-    device = _one_device(what, q, k_codes, v_codes, k_scale, v_scale, table, kv_len, k_cur, v_cur, uvb)
+    device = _one_device(what, q, k_codes, v_codes, k_scale, v_scale, table, kv_len, k_cur, v_cur, uvb, q_start)
     out = torch.empty(shape, dtype=torch.bfloat16, device=device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
     if B == 0 or Lq == 0 or Hq == 0:
@@ -1355,7 +1359,7 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
         L.check(lib.hn_attn_kv_pages(
             fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), cs,
             k_scale.data_ptr(), v_scale.data_ptr(), ss, H, P, page, table.data_ptr(), table.stride(0), W,
-            kv_len.data_ptr(), int(causal), L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
+            kv_len.data_ptr(), int(causal), L.ptr(q_start), L.ptr(k_cur) if cur_len else None, L.ptr(v_cur) if cur_len else None,
             _strides(k_cur) if cur_len else None, cur_len, L.ptr(uvb), uvs, scale, out.data_ptr(), _strides(out),
             lse.data_ptr(), L.ptr(ws), ws_bytes, _stream(q)), "hn_attn_kv_pages")
     return out, lse
@@ -1363,5 +1367,5 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
 
 @attn_kv_pages.register_fake
 def _(q, k_codes, v_codes, k_scale, v_scale, table, kv_len, causal=False, k_cur=None, v_cur=None, softmax_scale=None,
-      cur_valid=None):
+      cur_valid=None, q_start=None):
     return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)

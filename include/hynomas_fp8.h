@@ -461,17 +461,20 @@ int hn_kv_pages_copy(void *const *base, const int64_t *layer_stride, const int64
  * bf16 tail, with the rows' log-sum-exp; Hq a multiple of H, query head h G + g reading
  * cached head h:
  *   out = softmax(softmax_scale q K^T) V, lse = ln sum exp(softmax_scale q . K).
- * causal (without a tail): the queries are the sequence's last Lq tokens, query i sees
- * tokens t <= lens[b] - Lq + i. A row without a key gets zeros and -inf, one that meets a
- * NaN gets NaN in both. What lies behind a sequence's end does not matter.
- *   kcur, vcur, cur_valid, out, lse and V's range as in hn_attn_kv_blocks, whose fp16
- *   probabilities these are.
+ * causal (without a tail): query i sees tokens t <= q_start[b] + i (int32 [B]) of the
+ * sequence; with q_start null the queries are its last Lq tokens, q_start[b] = lens[b] -
+ * Lq. A row without a key gets zeros and -inf, one that meets a NaN gets NaN in both. What
+ * lies behind a sequence's end does not matter.
+ *   kcur, vcur, cur_valid, out and lse as in hn_attn_kv_blocks. Probabilities are held to
+ *   2^-17 of themselves (the sum of two bf16) where a cached head has up to 32 rows, Lq Hq
+ *   / H of them, or up to 128 causal ones, and V is bf16 there; else probabilities and V
+ *   are fp16 as in hn_attn_kv_blocks.
  * workspace: hn_attn_kv_pages_workspace_size(.., width * page, ..) bytes, 16-byte aligned. */
 int hn_attn_kv_pages(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
                      const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
                      const int64_t *ss, int64_t H, int64_t n_pages, int64_t page, const int32_t *table,
-                     int64_t table_stride, int64_t width, const int32_t *lens, int causal, const void *kcur,
-                     const void *vcur, const int64_t *curs, int64_t cur_len, const uint8_t *cur_valid,
+                     int64_t table_stride, int64_t width, const int32_t *lens, int causal, const int32_t *q_start,
+                     const void *kcur, const void *vcur, const int64_t *curs, int64_t cur_len, const uint8_t *cur_valid,
                      int64_t cur_valid_stride, float softmax_scale, void *out, const int64_t *os, float *lse,
                      void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -56,7 +56,8 @@ def _held(pool, key, table, b, n):
     return x.to(BF16).to(F64)
 
 
-def _reference(q, pool, table, lens, causal=False, k_cur=None, v_cur=None, cur_valid=None, scale=None):
+def _reference(q, pool, table, lens, causal=False, k_cur=None, v_cur=None, cur_valid=None, scale=None,
+               first=None):
     """out, lse, the rows' sum of p |v| / sum p, and the largest sum of |q k| scale."""
     B, Lq, Hq, D = q.shape
     H = pool["k"].shape[2]
@@ -69,7 +70,8 @@ def _reference(q, pool, table, lens, causal=False, k_cur=None, v_cur=None, cur_v
         k, v = _held(pool, "k", table, b, lens[b]), _held(pool, "v", table, b, lens[b])
         seen = torch.ones(Lq, lens[b], dtype=torch.bool, device=dev)
         if causal:
-            seen = torch.arange(lens[b], device=dev) <= lens[b] - Lq + torch.arange(Lq, device=dev)[:, None]
+            start = lens[b] - Lq if first is None else first[b]
+            seen = torch.arange(lens[b], device=dev) <= start + torch.arange(Lq, device=dev)[:, None]
         if k_cur is not None:
             k, v = torch.cat([k, k_cur[b].to(F64)]), torch.cat([v, v_cur[b].to(F64)])
             ok = torch.ones(k_cur.shape[1], dtype=torch.bool, device=dev) if cur_valid is None else cur_valid[
@@ -143,6 +145,71 @@ def test_causal(dev, page, Lq, G):
     q = torch.randn(len(lens), Lq, 2 * G, 128, device=dev, generator=g).to(BF16)
     got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
     _check(got, _reference(q, pool, table, lens, causal=True), f"page {page} Lq {Lq} G {G}")
+
+
+@pytest.mark.parametrize("Lq,G", [(1, 1), (7, 2), (40, 1), (200, 2)])
+def test_causal_queries_of_their_own_places(dev, Lq, G):
+    """Prompts of different lengths: rows before a sequence's first token see none, rows
+    past its last see all of it."""
+    _, ca, _ = _mods()
+    H, page, lens, first = 2, 64, (700, 230, 64, 5, 0), (700 - Lq // 2, 230 - Lq, 3, -3, 0)
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    pool = _pool(dev, g, 30, page, H)
+    table = _table(dev, g, lens, page, 30)
+    q = torch.randn(len(lens), Lq, H * G, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True, q_start=_i32(dev, first))
+    _check(got, _reference(q, pool, table, lens, causal=True, first=first), f"{Lq} rows")
+    last = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
+    same = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True, q_start=_i32(dev, [n - Lq for n in lens]))
+    assert torch.equal(last[0], same[0]) and torch.equal(last[1], same[1])
+    far = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True, q_start=_i32(dev, [2 ** 31 - 1] * 5))
+    _check(far, _reference(q, pool, table, lens), "queries past the end")
+    none = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True, q_start=_i32(dev, [-2 ** 31] * 5))
+    assert (none[0] == 0).all() and (none[1] == -math.inf).all()
+
+
+def test_prompts_of_one_batch(dev):
+    """Prompts of different lengths written and attended in one pass: as each alone."""
+    kp, _, _ = _mods()
+    H, adds = 2, (70, 1, 0, 33)
+    g = torch.Generator(device=dev).manual_seed(2)
+    cache = kp.PagedKVCache(1, 20, H, page=64, device=dev)
+    cache.pool["k"].view(torch.uint8).fill_(0x7f)  # (NaN codes: what no token was written to)
+    cache.pool["v"].view(torch.uint8).fill_(0x7f)
+    old = torch.randn(4, 100, 2, H, 128, device=dev, generator=g).to(BF16)
+    seqs = [cache.new() for _ in adds]
+    batch = cache.open(seqs, [100, 64, 3, 0])
+    batch.write(0, old[:, :, 0], old[:, :, 1])
+    batch.commit()
+    q, k, v = torch.randn(4, 70, 3, H, 128, device=dev, generator=g).to(BF16).unbind(2)
+    batch = cache.open(seqs, adds)
+    batch.write(0, k, v)
+    out, lse = batch.attend(0, q, causal=True)
+    batch.commit()
+    for b, (s, n) in enumerate(zip(seqs, adds)):
+        if n:
+            one = cache.open([s])
+            want = _reference(q[b:b + 1, :n], cache.layer(0), one.table, (cache.length(s),), causal=True)
+            _check((out[b:b + 1, :n], lse[b:b + 1, :, :n]), want, f"prompt {b}")
+
+
+@pytest.mark.parametrize("Lq", [1, 40, 200])
+def test_a_pool_without_pages(dev, Lq):
+    """No key but the tail's, or none at all."""
+    kp, ca, _ = _mods()
+    pool = kp.make_pages(0, 2, device=dev)
+    table, n = torch.zeros(3, 0, dtype=I32, device=dev), _i32(dev, (0, 5, 70))
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    q = torch.randn(3, Lq, 2, 128, device=dev, generator=g).to(BF16)
+    out, lse = ca.paged_attention(q, pool, table, n)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    k, v = torch.randn(3, 67, 2, 2, 128, device=dev, generator=g).to(BF16).unbind(2)
+    got = ca.paged_attention(q, pool, table, n, k_cur=k, v_cur=v)
+    _check(got, _reference(q, pool, table, (0, 0, 0), k_cur=k, v_cur=v), "tail alone")
+    wide = ca.paged_attention(q, pool, torch.zeros(3, 4, dtype=I32, device=dev), n, k_cur=k, v_cur=v)
+    assert torch.equal(wide[0], got[0]) and torch.equal(wide[1], got[1])
+    kp.write_pages(pool, k, v, table, n)
+    assert kp.read_pages(pool, "k", table, n, 5).abs().sum().item() == 0
 
 
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])

@@ -172,13 +172,15 @@ def test_c_abi_checks():
         assert write(**kw) == L.HN_E_ARG and match in err(), kw
     assert write(B=0) == 0
 
-    def attend(page=64, D=128, Hq=4, causal=0, cur=0, scale=0.1, q=P, cs=st, ws=None, nbytes=0, width=2, Lq=1):
-        return lib.hn_attn_kv_pages(0, q, st, 1, Lq, Hq, D, P, P, cs, P, P, st, 2, 6, page, P, 2, width, P, causal,
+    def attend(page=64, D=128, Hq=4, causal=0, cur=0, scale=0.1, q=P, cs=st, ws=None, nbytes=0, width=2, Lq=1,
+               first=None):
+        return lib.hn_attn_kv_pages(0, q, st, 1, Lq, Hq, D, P, P, cs, P, P, st, 2, 6, page, P, 2, width, P, causal, first,
                                     P if cur else None, P if cur else None, st if cur else None, cur, None, 0, scale, P,
                                     st, P, ws, nbytes, None)
 
     for kw, match in ((dict(page=48), "page"), (dict(D=96), "head dim"), (dict(Hq=3), "shape"),
-                      (dict(causal=1, cur=3), "no tail"), (dict(scale=0.0), "softmax_scale"),
+                      (dict(causal=1, cur=3), "no tail"), (dict(first=P), "q_start"),
+                      (dict(causal=1, first=ctypes.c_void_p(2)), "misaligned"), (dict(scale=0.0), "softmax_scale"),
                       (dict(scale=float("nan")), "softmax_scale"), (dict(q=ctypes.c_void_p(8)), "misaligned"),
                       (dict(cs=odd), "multiples of 16"), (dict(width=2 ** 28), "too many keys"), (dict(q=None), "null"),
                       (dict(width=300), "workspace")):
