@@ -78,7 +78,8 @@ SIGNATURES = {
     "hn_move_kv_tokens": [_P, _P, _PI64, _P, _P, _PI64, _P, _PI64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P,
                           _PI64, _P, _P, _PI64, _I64, _P, _P],
     "hn_kv_pages_write": [_I, _P, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64,
-                          _P, _I64, _I64, _P, _P, _I, _P, _P],
+                          _P, _I64, _I64, _P, _P, _I, _P, _P, _I64, _P],
+    "hn_kv_pages_write_workspace_size": [_I64] * 3,
     "hn_kv_pages_read": [_I, _P, _PI64, _P, _PI64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P],
     "hn_kv_pages_copy": [ctypes.POINTER(_P), _PI64, _PI64, _PI64, _I64, _I64, _PI32, _PI32, _I64, _P],
     "hn_attn_kv_pages": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64, _I64,
@@ -89,7 +90,8 @@ SIGNATURES = {
 RESTYPES = {"hn_last_error": ctypes.c_char_p, "hn_attn_fp8kv_workspace_size": _I64,
             "hn_attn_fp8kv_noalloc_scratch_bytes": _I64, "hn_select_kv_blocks_workspace_size": _I64,
             "hn_attn_kv_blocks_workspace_size": _I64, "hn_attn_key_mass_workspace_size": _I64,
-            "hn_select_kv_tokens_workspace_size": _I64, "hn_attn_kv_pages_workspace_size": _I64}
+            "hn_select_kv_tokens_workspace_size": _I64, "hn_attn_kv_pages_workspace_size": _I64,
+            "hn_kv_pages_write_workspace_size": _I64}
 
 _lib = None
 _lock = threading.Lock()

@@ -101,7 +101,10 @@ HN_DEVICE int page_of(const Pool& p, const TilePages& t, uint32_t pos) {
     return (pos >> p.shift) == t.entry ? t.first : t.next;
 }
 
-// Quantize-on-write. HBM bound: 256 bytes read and 132 written a row.
+// Quantize-on-write: s = amax |x| / 448 (127), code = round(x / s). HBM bound: 256 bytes
+// read and 132 written a row, and the values a second time by the check that comes before
+// (nothing is written where one is not finite). Two sequences of 10800 tokens x 24 heads
+// (265 MB of values, 137 MB written): check 45 us (5.9 TB/s), write 68 (5.9).
 struct WriteArgs {
     const uint16_t* x[2];
     uint8_t* q[2];
@@ -112,8 +115,8 @@ struct WriteArgs {
     const int32_t* counts;   // null: L new tokens in every sequence
     Tiles tiles;
     float recip;             // not 0: a row's scale is amax times this
-    const int32_t* status;   // set by the check: nothing is written; null: unchecked
-    int32_t* flag;           // small writes: the status to be set
+    int32_t* status;         // not null: the values are checked, and nothing is written where one is not finite
+    uint8_t* flags;          // workspace: a byte of every workgroup of the check
 };
 
 HN_DEVICE int new_tokens(const WriteArgs& a, int b) {
@@ -148,11 +151,21 @@ __global__ void pages_clear_kernel(int32_t* status) {
     if (threadIdx.x == 0) *status = 0;
 }
 
-// Sets *status where a new token's value is NaN or Inf: the largest magnitude's bits of
-// either half of the words are then 0x7f80 or more.
-__global__ __launch_bounds__(256) void pages_check_kernel(WriteArgs a, int32_t* status) {
+// Where the check's verdict lies. Up to FLAGS workgroups leave a byte each, which all
+// workgroups of the write look at, 16 to a thread; more of them set the status, which a
+// launch of its own has cleared (three sequences of up to 777 tokens x 24 heads, 882
+// workgroups: kernels 4.7 + 5.3 + 10.7 us by the status, 6.0 + 9.7 by flags; calls 25.7 us
+// and 24.3).
+enum Check { NONE, ALONE, BY_FLAGS, BY_STATUS };
+constexpr int FLAGS = 4096;
+
+// Looks for a new token's value that is NaN or Inf: the largest magnitude's bits of either
+// half of the words are then 0x7f80 or more.
+template <Check CHECK>
+__global__ __launch_bounds__(256) void pages_check_kernel(WriteArgs a) {
     const Place at = tile_place(a.tiles, false);
     const int sel = at.part & 1;
+    bool bad = false;
     for (int b = blockIdx.y; b < a.tiles.B; b += gridDim.y) {
         const int last = new_tokens(a, b);
         if (at.t0 >= last) continue;
@@ -166,7 +179,15 @@ __global__ __launch_bounds__(256) void pages_check_kernel(WriteArgs a, int32_t* 
         u16x2 top = {0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = largest(top, v[k]);
-        if (__any(top[0] >= 0x7f80u || top[1] >= 0x7f80u) && (threadIdx.x & 63) == 0) *status = 1;
+        bad |= top[0] >= 0x7f80u || top[1] >= 0x7f80u;
+    }
+    if constexpr (CHECK == BY_STATUS) {
+        if (__any(bad) && (threadIdx.x & 63) == 0) *a.status = 1;
+    } else {
+        const bool any = __syncthreads_or(bad);
+        const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, n = gridDim.x * gridDim.y;
+        if (threadIdx.x == 0) a.flags[id] = any;
+        if (id == n - 1 && threadIdx.x > 0 && threadIdx.x <= (-n & 15u)) a.flags[id + threadIdx.x] = 0;  // to whole 16
     }
 }
 
@@ -192,29 +213,42 @@ HN_DEVICE bool all_finite(const WriteArgs& a) {
     return !__syncthreads_or(top[0] >= 0x7f80u || top[1] >= 0x7f80u);
 }
 
-// ALONE: small writes (up to SMALL bytes of values) are one launch, in which every
-// workgroup, 1024 threads then, looks at all values : 64 tokens x 8 heads 7.4 us, where three kernels take
-// 7.7 and two launches more (the call 32 -> 26).
+// CHECK ALONE: small writes (up to SMALL bytes of values) are one launch, in which every
+// workgroup, 1024 threads then, looks at all values: 64 tokens x 8 heads 7.4 us, where
+// three kernels take 7.7 and two launches more (the call 32 us against 26).
 constexpr int64_t SMALL = 1 << 18;
 
-template <int FMT, bool ALONE>
-__global__ __launch_bounds__(ALONE ? 1024 : 256) void pages_write_kernel(WriteArgs a) {
-    constexpr int NK = ALONE ? 1 : 4;  // rows of the tile to a lane group
-    if constexpr (ALONE) {
+template <int FMT, Check CHECK>
+__global__ __launch_bounds__(CHECK == ALONE ? 1024 : 256) void pages_write_kernel(WriteArgs a) {
+    constexpr int NK = CHECK == ALONE ? 1 : 4;  // rows of the tile to a lane group
+    const bool first_wg = blockIdx.x == 0 && blockIdx.y == 0;
+    if constexpr (CHECK == ALONE) {
         const bool ok = all_finite(a);
-        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.flag = !ok;
+        if (first_wg && threadIdx.x == 0) *a.status = !ok;
         if (!ok) return;
     }
     // (asked for here, looked at before the first store: the values' loads do not wait for it)
     int32_t refused = 0;
-    if (!ALONE && a.status) refused = *(ScalarInts)a.status;
+    uint4 flags = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (CHECK == BY_STATUS) refused = *(ScalarInts)a.status;
+    if constexpr (CHECK == BY_FLAGS)
+        if (16 * threadIdx.x < gridDim.x * gridDim.y) flags = reinterpret_cast<const uint4*>(a.flags)[threadIdx.x];
+    auto verdict = [&]() {
+        if constexpr (CHECK != BY_FLAGS) return refused != 0;
+        const bool bad = __syncthreads_or((flags.x | flags.y | flags.z | flags.w) != 0u);
+        if (first_wg && threadIdx.x == 0) *a.status = bad;
+        return bad;
+    };
     // (from the last tile on: what the check has read last may be in a cache yet)
     const Place at = tile_place(a.tiles, true);
     const int sel = at.part & 1, t0 = at.t0;
     for (int b = gridDim.y - 1 - blockIdx.y; b < a.tiles.B; b += gridDim.y) {
         const int last = new_tokens(a, b);
         const int first = ((ScalarInts)a.start)[b];
-        if (t0 >= last) continue;
+        if (t0 >= last) {
+            if (CHECK == BY_FLAGS && first_wg) verdict();  // (for the status)
+            continue;
+        }
         Values v[NK];
         Row w[NK];
 #pragma unroll
@@ -224,7 +258,7 @@ __global__ __launch_bounds__(ALONE ? 1024 : 256) void pages_write_kernel(WriteAr
         }
         const uint32_t pos0 = (uint32_t)first + (uint32_t)t0;
         const TilePages pages = tile_pages(a.pool, b, pos0, a.tiles.tsh);
-        if (refused != 0) return;  // nothing is written
+        if (verdict()) return;  // nothing is written
         if (first < 0) continue;
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
@@ -257,7 +291,7 @@ __global__ __launch_bounds__(ALONE ? 1024 : 256) void pages_write_kernel(WriteAr
 }
 
 // A sequence decoded: y[b, t, h] = bf16(code * scale), zeros past its length. HBM bound:
-// 132 bytes read and 256 written a row.
+// 132 bytes read and 256 written a row (1.03 million rows, 401 MB, 69 us: 5.8 TB/s).
 struct ReadArgs {
     const uint8_t* q;
     const float* s;
@@ -320,7 +354,8 @@ __global__ __launch_bounds__(256) void pages_read_kernel(ReadArgs a) {
 // Pages copied, every layer in one launch. The pairs travel in the kernel's arguments,
 // so that a copy needs no upload and can be captured; longer lists take several
 // launches. A page is one run of bytes in each of the four arrays, moved in pieces of
-// 16 KB a workgroup. HBM bound.
+// 16 KB a workgroup, all loads of a thread in flight. HBM bound: 260 MB in 48 us, 1.3 GB in
+// 237 (5.4 to 5.5 TB/s, where torch's copy of 2 GiB reaches 4.95).
 constexpr int MAX_PAIRS = 240;
 constexpr int PIECE = 16384;
 
@@ -404,18 +439,55 @@ static bool tiles_of(int64_t B, int64_t L, int64_t H, int arrays, bool token_fas
     return true;
 }
 
+static pages::Check check_of(const int32_t* status, int64_t B, int64_t L, int64_t H, dim3 grid) {
+    if (!status) return pages::NONE;
+    if (L * H <= pages::SMALL / (4 * 128) / B) return pages::ALONE;
+    return (int64_t)grid.x * grid.y <= pages::FLAGS ? pages::BY_FLAGS : pages::BY_STATUS;
+}
+
+static int64_t flag_bytes(dim3 grid) { return ((int64_t)grid.x * grid.y + 15) / 16 * 16; }
+
+template <int FMT>
+static void launch_write(pages::Check check, const pages::WriteArgs& a, dim3 grid, hipStream_t st) {
+    using namespace pages;
+    if (check == ALONE) {
+        pages_write_kernel<FMT, ALONE><<<grid, 1024, 0, st>>>(a);
+    } else if (check == NONE) {
+        pages_write_kernel<FMT, NONE><<<grid, 256, 0, st>>>(a);
+    } else if (check == BY_FLAGS) {
+        pages_check_kernel<BY_FLAGS><<<grid, 256, 0, st>>>(a);
+        pages_write_kernel<FMT, BY_FLAGS><<<grid, 256, 0, st>>>(a);
+    } else {
+        pages_clear_kernel<<<1, 64, 0, st>>>(a.status);
+        pages_check_kernel<BY_STATUS><<<grid, 256, 0, st>>>(a);
+        pages_write_kernel<FMT, BY_STATUS><<<grid, 256, 0, st>>>(a);
+    }
+}
+
+static bool write_shape_ok(int64_t B, int64_t L, int64_t H) {
+    return B >= 0 && L >= 0 && H > 0 && B <= 0x7fffffffLL && L <= 0x7fffffffLL && H <= 0x7fffffffLL;
+}
+
+extern "C" int64_t hn_kv_pages_write_workspace_size(int64_t B, int64_t L, int64_t H) {
+    pages::Tiles tiles;
+    dim3 grid;
+    if (!write_shape_ok(B, L, H) || B == 0 || L == 0 || !tiles_of(B, L, H, 2, false, tiles, grid)) return 0;
+    const int32_t checked = 0;
+    return check_of(&checked, B, L, H, grid) == pages::BY_FLAGS ? flag_bytes(grid) : 0;
+}
+
 extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const int64_t* xs, int64_t B, int64_t L,
                                  int64_t H, int64_t D, void* kc, void* vc, const int64_t* cs, float* ks, float* vs,
                                  const int64_t* ss, int64_t n_pages, int64_t page, const int32_t* table,
                                  int64_t table_stride, int64_t width, const int32_t* start, const int32_t* counts,
-                                 int scale_mode, int32_t* status, void* stream) {
+                                 int scale_mode, int32_t* status, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
     const char* who = "hn_kv_pages_write";
     HN_REQUIRE(fmt == HN_KV_FP8 || fmt == HN_KV_INT8, HN_E_ARG, "hn_kv_pages_write: unknown KV format");
     HN_REQUIRE(scale_mode == HN_SCALE_ZERO_ONE || scale_mode == HN_SCALE_RECIPROCAL, HN_E_ARG,
                "hn_kv_pages_write: unknown scale mode");
     HN_REQUIRE(D == 128, HN_E_ARG, "hn_kv_pages_write: head dim must be 128");
-    HN_REQUIRE(B >= 0 && L >= 0 && H > 0 && B <= 0x7fffffffLL && L <= 0x7fffffffLL && H <= 0x7fffffffLL, HN_E_ARG,
-               "hn_kv_pages_write: invalid shape");
+    HN_REQUIRE(write_shape_ok(B, L, H), HN_E_ARG, "hn_kv_pages_write: invalid shape");
     pages::WriteArgs a = {};
     if (const int rc = pool_args(who, cs, ss, n_pages, page, table, table_stride, width, a.pool); rc != HN_OK) return rc;
     HN_REQUIRE(xs && xs[3] == 1 && xs[0] % 8 == 0 && xs[1] % 8 == 0 && xs[2] % 8 == 0, HN_E_ARG,
@@ -427,10 +499,9 @@ extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const in
     if (none && !status) return HN_OK;
     HN_REQUIRE(none || (k && v && start && (n_pages == 0 || (kc && vc && ks && vs)) && (width == 0 || table)), HN_E_ARG,
                "hn_kv_pages_write: null pointer");
-    if (const int rc = require_gfx950(who); rc != HN_OK) return rc;
-    const hipStream_t st = (hipStream_t)stream;
     if (none) {
-        pages::pages_clear_kernel<<<1, 64, 0, st>>>(status);
+        if (const int rc = require_gfx950(who); rc != HN_OK) return rc;
+        pages::pages_clear_kernel<<<1, 64, 0, (hipStream_t)stream>>>(status);
         return check_launch(who);
     }
     a.x[0] = (const uint16_t*)k; a.x[1] = (const uint16_t*)v;
@@ -441,20 +512,14 @@ extern "C" int hn_kv_pages_write(int fmt, const void* k, const void* v, const in
     if (scale_mode == HN_SCALE_RECIPROCAL) a.recip = 1.0f / (fmt == HN_KV_FP8 ? kE4M3Max : 127.0f);
     dim3 grid;
     HN_REQUIRE(tiles_of(B, L, H, 2, xs[1] < xs[2], a.tiles, grid), HN_E_ARG, "hn_kv_pages_write: too many rows");
-    const bool fp8 = fmt == HN_KV_FP8;
-    if (status && L * H <= pages::SMALL / (4 * D) / B) {
-        a.flag = status;
-        if (fp8) pages::pages_write_kernel<HN_KV_FP8, true><<<grid, 1024, 0, st>>>(a);
-        else pages::pages_write_kernel<HN_KV_INT8, true><<<grid, 1024, 0, st>>>(a);
-        return check_launch(who);
-    }
     a.status = status;
-    if (status) {
-        pages::pages_clear_kernel<<<1, 64, 0, st>>>(status);
-        pages::pages_check_kernel<<<grid, 256, 0, st>>>(a, status);
-    }
-    if (fp8) pages::pages_write_kernel<HN_KV_FP8, false><<<grid, 256, 0, st>>>(a);
-    else pages::pages_write_kernel<HN_KV_INT8, false><<<grid, 256, 0, st>>>(a);
+    a.flags = (uint8_t*)workspace;
+    const pages::Check check = check_of(status, B, L, H, grid);
+    HN_REQUIRE(check != pages::BY_FLAGS || (workspace && aligned(workspace, 16) && workspace_bytes >= flag_bytes(grid)),
+               HN_E_ARG, "hn_kv_pages_write: workspace smaller than hn_kv_pages_write_workspace_size() or misaligned");
+    if (const int rc = require_gfx950(who); rc != HN_OK) return rc;
+    if (fmt == HN_KV_FP8) launch_write<HN_KV_FP8>(check, a, grid, (hipStream_t)stream);
+    else launch_write<HN_KV_INT8>(check, a, grid, (hipStream_t)stream);
     return check_launch(who);
 }
 

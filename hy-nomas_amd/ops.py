@@ -1162,6 +1162,11 @@ def _per_sequence(t: Optional[torch.Tensor], B: int, what: str) -> Optional[torc
     return t if t.is_contiguous() else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
+def _write_workspace(*sizes) -> int:
+    return L.load().hn_kv_pages_write_workspace_size(*sizes)
+
+
 def kv_pages_write_(k_codes, v_codes, k_scale, v_scale, k, v, table, start, counts=None, status=None,
                     scale_mode: int = L.HN_SCALE_ZERO_ONE) -> None:
     """Quantize new tokens into the pages of their sequences (see _kv_pages_write_op)."""
@@ -1196,10 +1201,14 @@ def _kv_pages_write_op(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: to
         xs = k.stride()
     device = _one_device(what, k, v, k_codes, v_codes, k_scale, v_scale, table, start, counts, status)
     with _on(device):
-        L.check(L.load().hn_kv_pages_write(
+        lib = L.load()
+        ws_bytes = _write_workspace(B, Lt, H) if sp else 0
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes else None
+        L.check(lib.hn_kv_pages_write(
             fmt, k.data_ptr(), v.data_ptr(), _stride_array(xs), B, Lt, H, D, k_codes.data_ptr(), v_codes.data_ptr(),
             cs, k_scale.data_ptr(), v_scale.data_ptr(), ss, P, page,
-            table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), scale_mode, sp, _stream(k)),
+            table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), L.ptr(counts), scale_mode, sp, L.ptr(ws),
+            ws_bytes, _stream(k)),
             "hn_kv_pages_write")
 
 

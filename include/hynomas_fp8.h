@@ -430,15 +430,21 @@ int hn_move_kv_tokens(const void *k, const void *v, const int64_t *cs, const flo
 /* Quantizes new tokens into their pages: token j < counts[b] (NULL: L) of sequence b, K
  * and V bf16 [B, L, H, 128] with strides xs[4] each, becomes its token start[b] + j. With
  * scale_mode HN_SCALE_ZERO_ONE codes and scales are hn_kv_quantize_pair's; the other is
- * HN_SCALE_RECIPROCAL. Codes are those of x / s either way. Rows past counts[b] are not read. Tokens of a
- * negative start, or past the table, are dropped. status as in hn_kv_quantize: nothing
- * is written if a value of a new token is NaN or Inf. Two new tokens of one call at one
- * place (a page that two of its sequences share) leave either's bytes there. */
+ * HN_SCALE_RECIPROCAL. Codes are those of x / s either way. Rows past counts[b] are not
+ * read. Tokens of a negative start, or past the table, are dropped. status as in
+ * hn_kv_quantize: nothing is written if a value of a new token is NaN or Inf. Two new
+ * tokens of one call at one place (a page that two of its sequences share) leave either's
+ * bytes there.
+ * workspace: with a status hn_kv_pages_write_workspace_size(B, L, H) bytes, 16-byte
+ * aligned. */
 int hn_kv_pages_write(int fmt, const void *k, const void *v, const int64_t *xs, int64_t B, int64_t L,
                       int64_t H, int64_t D, void *kc, void *vc, const int64_t *cs, float *ks, float *vs,
                       const int64_t *ss, int64_t n_pages, int64_t page, const int32_t *table,
                       int64_t table_stride, int64_t width, const int32_t *start, const int32_t *counts,
-                      int scale_mode, int32_t *status, void *stream);
+                      int scale_mode, int32_t *status, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Bytes of workspace hn_kv_pages_write needs for these sizes with a status (0: none). */
+int64_t hn_kv_pages_write_workspace_size(int64_t B, int64_t L, int64_t H);
 
 /* Decodes tokens [0, L) of every sequence: y[b, t, h, :] = bf16(code * scale) of one of K
  * and V for t < lens[b], zeros behind and for absent tokens. y: bf16 [B, L, H, 128]

@@ -443,7 +443,7 @@ def test_scales_of_a_torch_program(dev, fmt, L):
 
 @pytest.mark.parametrize("where", ["k", "v"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-@pytest.mark.parametrize("B,L", [(2, 3), (3, 700)])
+@pytest.mark.parametrize("B,L", [(2, 3), (3, 700), (1, 33000)])
 def test_a_write_of_a_bad_value_writes_nothing(dev, where, value, B, L):
     kp, _, _ = _mods()
     g = torch.Generator(device=dev).manual_seed(1)
@@ -465,6 +465,31 @@ def test_a_write_of_a_bad_value_writes_nothing(dev, where, value, B, L):
     kv[where][B - 1, L - 1, 3, 127] = 1.0
     kp.write_pages(pool, kv["k"], kv["v"], table, start, status=status)
     assert status.item() == 0
+
+
+@pytest.mark.parametrize("counts", [(300, 0), (0, 300), (0, 0), (1, 300)])
+def test_the_status_of_padded_writes(dev, counts):
+    """The status stands for the rows that count, whichever those are, after any before it."""
+    kp, _, _ = _mods()
+    g = torch.Generator(device=dev).manual_seed(3)
+    pool = _pool(dev, g, 10, 64, 4)
+    table = torch.arange(10, dtype=I32, device=dev).view(2, 5)
+    k, v = (torch.randn(2, 300, 4, 128, device=dev, generator=g).to(BF16) for _ in range(2))
+    n, start = _i32(dev, counts), _i32(dev, (0, 0))
+    for b, c in enumerate(counts):
+        k[b, c:], v[b, c:] = float("nan"), float("inf")
+    for was in (0, 1, 7):
+        status = _i32(dev, [was])
+        kp.write_pages(pool, k, v, table, start, counts=n, status=status)
+        assert status.item() == 0
+    held = kp.read_pages(pool, "k", table, n, 300)
+    for b, c in enumerate(counts):
+        assert ((held[b, :c].float() - k[b, :c].float()).abs() <= k[b, :c].float().abs().amax(-1, keepdim=True) / 16).all()
+        if c:
+            bad = k.clone()
+            bad[b, c - 1, 0, 0] = float("inf")
+            kp.write_pages(pool, bad, v, table, start, counts=n, status=status)
+            assert status.item() == 1
 
 
 def test_tokens_without_a_page_are_dropped(dev):

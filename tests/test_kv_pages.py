@@ -161,9 +161,10 @@ def test_c_abi_checks():
     def err():
         return lib.hn_last_error().decode()
 
-    def write(fmt=0, D=128, H=2, B=1, xs=st, cs=st, page=64, width=2, k=P, start=P, mode=1):
-        return lib.hn_kv_pages_write(fmt, k, P, xs, B, 5, H, D, P, P, cs, P, P, st, 6, page, P, 2, width, start, None,
-                                     mode, None, None)
+    def write(fmt=0, D=128, H=2, B=1, xs=st, cs=st, page=64, width=2, k=P, start=P, mode=1, n=5,
+              status=None, ws=None, nbytes=0):
+        return lib.hn_kv_pages_write(fmt, k, P, xs, B, n, H, D, P, P, cs, P, P, st, 6, page, P, 2, width, start, None,
+                                     mode, status, ws, nbytes, None)
 
     for kw, match in ((dict(fmt=3), "format"), (dict(D=64), "head dim"), (dict(H=0), "shape"), (dict(page=32), "page"),
                       (dict(page=96), "page"), (dict(width=-1), "table"), (dict(width=2 ** 31), "table"),
@@ -171,6 +172,10 @@ def test_c_abi_checks():
                       (dict(k=ctypes.c_void_p(8)), "misaligned"), (dict(start=None), "null"), (dict(mode=0), "scale mode")):
         assert write(**kw) == L.HN_E_ARG and match in err(), kw
     assert write(B=0) == 0
+    size = lib.hn_kv_pages_write_workspace_size
+    assert size(1, 256, 2) == 0 and size(1, 257, 2) == 48 and size(1, 2 ** 20, 2) == 0 and size(0, 9, 9) == 0
+    for kw in (dict(ws=None, nbytes=48), dict(ws=P, nbytes=47), dict(ws=ctypes.c_void_p(8), nbytes=48)):
+        assert write(n=257, status=P, **kw) == L.HN_E_ARG and "workspace" in err(), kw
 
     def attend(page=64, D=128, Hq=4, causal=0, cur=0, scale=0.1, q=P, cs=st, ws=None, nbytes=0, width=2, Lq=1,
                first=None):
