@@ -805,21 +805,27 @@ __global__ __launch_bounds__(64 * TILE_WAVES, 1) void attn_page_tiles_kernel(Pag
 }
 
 // The parts of items that several workgroups computed, joined in their order: with M =
-// max m, O = sum 2^(m - M) O / sum 2^(m - M) l. 32 threads a row, 4 dims each, eight rows
-// of an item a workgroup. Workgroups stand for the items, or (SEAMS) for the borders
-// between two workgroups' shares, whichever are fewer: an item is its first border's
-// (two branches' frames, 720 items of 256 rows: 40 us by items, 27 by borders).
-template <int U, bool SEAMS>
+// max m, O = sum 2^(m - M) O / sum 2^(m - M) l. 32 threads a row, 4 dims each, eight parts
+// in flight, eight rows of an item a workgroup. Workgroups stand for the items, or (SEAMS)
+// for the borders between two workgroups' shares, whichever are fewer: an item is its first
+// border's (two branches' frames, 720 items of 256 rows: 40 us by items, 27 by borders). Where
+// an item has many parts (ROWS) a workgroup has one row, whose parts its eight groups of
+// threads take in turn (one sequence of 100000 keys, 96 parts: 4.4 us, by eight rows 10.2;
+// four parts of twenty rows 8.0, by eight rows 4.7).
+enum Join { ITEMS, SEAMS, ROWS };
+constexpr int MANY_PARTS = 16;
+
+template <int U, Join JOIN>
 __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
     const Line<U> line(p);
-    const int per = p.H * p.runs, groups = (min(R, p.rows) + 7) / 8;
+    const int per = p.H * p.runs, groups = JOIN == ROWS ? p.pitch : (p.pitch + 7) / 8;
     int x = blockIdx.x;
     const int grp = x % groups;
     x /= groups;
     const uint32_t share = line.share();
     uint32_t start;
     int n, b, item;
-    if constexpr (SEAMS) {
+    if constexpr (JOIN == SEAMS) {
         const uint32_t seam = (uint32_t)(x + 1) * share;
         if (seam >= line.total) return;
         line.find(seam, b, start, n);
@@ -831,22 +837,23 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
     }
     const uint32_t i0 = start + (uint32_t)item * (uint32_t)n;
     const uint32_t w0 = i0 / share, w1 = (i0 + (uint32_t)n - 1) / share;
-    if (w0 == w1 || (SEAMS && (uint32_t)x != w0)) return;  // whole (written already), or another border's
+    if (w0 == w1 || (JOIN == SEAMS && (uint32_t)x != w0)) return;  // whole (written already), or another border's
     const int h = item / p.runs, run = item - h * p.runs;
-    const int r = grp * 8 + (threadIdx.x >> 5), row = run * R + r, d = (threadIdx.x & 31) * 4;
-    if (r >= R || row >= p.rows) return;
+    constexpr uint32_t STEP = JOIN == ROWS ? 8 : 1;
+    const int tg = threadIdx.x >> 5, r = JOIN == ROWS ? grp : grp * 8 + tg, row = run * R + r, d = (threadIdx.x & 31) * 4;
+    if (r >= p.pitch || row >= p.rows) return;
     float M = -INFINITY, den = 0.0f;
     float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t a0 = w0; a0 <= w1; a0 += 8) {
+    for (uint32_t a0 = w0 + (JOIN == ROWS ? tg : 0); a0 <= w1; a0 += 8 * STEP) {
         float2 ml[8];
         float4 ov[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t w = a0 + e < w1 ? a0 + e : w1;
+            const uint32_t w = min(a0 + e * STEP, w1);
             const int64_t part = ((int64_t)w * 2 + (i0 < w * share ? 0 : 1)) * p.pitch + r;
             ml[e] = *reinterpret_cast<const float2*>(p.ws_ml + part * 2);
             ov[e] = *reinterpret_cast<const float4*>(p.ws_o + part * D + d);
-            if (a0 + e > w1) ml[e] = make_float2(-INFINITY, 0.0f);
+            if (a0 + e * STEP > w1) ml[e] = make_float2(-INFINITY, 0.0f);
         }
         float top = M;
 #pragma unroll
@@ -863,6 +870,29 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
             num.y = fmaf(wgt, ov[e].y, num.y);
             num.z = fmaf(wgt, ov[e].z, num.z);
             num.w = fmaf(wgt, ov[e].w, num.w);
+        }
+    }
+    if constexpr (JOIN == ROWS) {
+        __shared__ __attribute__((aligned(16))) float4 so[8][D / 4];
+        __shared__ float2 sml[8];
+        so[tg][d / 4] = num;
+        if (d == 0) sml[tg] = make_float2(M, den);
+        __syncthreads();
+        if (tg > 0) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) M = fmaxf(M, sml[e].x);
+        const float base = M == -INFINITY ? 0.0f : M;
+        den = 0.0f;
+        num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float wgt = __builtin_amdgcn_exp2f(sml[e].x - base);
+            const float4 y = so[e][d / 4];
+            den = fmaf(wgt, sml[e].y, den);
+            num.x = fmaf(wgt, y.x, num.x);
+            num.y = fmaf(wgt, y.y, num.y);
+            num.z = fmaf(wgt, y.z, num.z);
+            num.w = fmaf(wgt, y.w, num.w);
         }
     }
     const int qi = row / p.G, hq = h * p.G + row - qi * p.G;
@@ -943,8 +973,11 @@ static bool pages_shape_ok(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t
 template <int U>
 static int join_pages(const PagesPlan& pl, const attn::PageParams& p, int R, hipStream_t st) {
     const int64_t groups = (pl.pitch + 7) / 8;
-    if (pl.items < pl.wgs) attn::pages_join_kernel<U, false><<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
-    else attn::pages_join_kernel<U, true><<<(unsigned)((pl.wgs - 1) * groups), 256, 0, st>>>(p, R);
+    if (pl.items * attn::MANY_PARTS <= pl.wgs)
+        attn::pages_join_kernel<U, attn::ROWS><<<(unsigned)(pl.items * pl.pitch), 256, 0, st>>>(p, R);
+    else if (pl.items < pl.wgs)
+        attn::pages_join_kernel<U, attn::ITEMS><<<(unsigned)(pl.items * groups), 256, 0, st>>>(p, R);
+    else attn::pages_join_kernel<U, attn::SEAMS><<<(unsigned)((pl.wgs - 1) * groups), 256, 0, st>>>(p, R);
     return check_launch("hn_attn_kv_pages (join)");
 }
 

@@ -338,6 +338,19 @@ def test_many_sequences(dev, B, lens):
     _check(ca.paged_attention(q, pool, table, _i32(dev, n)), _reference(q, pool, table, n), f"B {B}")
 
 
+@pytest.mark.parametrize("Lq", [1, 5, 150])
+def test_one_long_sequence(dev, Lq):
+    """Every workgroup holds a part of the same few items."""
+    _, ca, _ = _mods()
+    page, lens = 1024, (100_001,)
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    pool = _pool(dev, g, 99, page, 1)
+    table = _table(dev, g, lens, page, 99)
+    q = torch.randn(1, Lq, 3, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
+    _check(got, _reference(q, pool, table, lens, causal=True), f"{Lq} rows")
+
+
 def test_offsets_past_32_bits(dev):
     """A pool whose codes pass 4 GiB, its last pages read, written and copied."""
     kp, ca, _ = _mods()
