@@ -94,6 +94,7 @@ HN_DEVICE void clear_masked_v(TailRegs<4>& r, uint64_t w) {
 // PAGED: idx is a page table [B, top_k], block a page, and sequence b's tokens are the
 // first lens[b] that its pages hold, in their order; a tile lies in one page and its loads
 // go through descriptors of its own rows. The part of a tile past the length reads as zeros.
+// It serves runs of 33 to 128 rows (where, and what the others take: pages_plan).
 template <int FMT, bool MASK, bool PAGED = false>
 __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     constexpr int NW = 4, BQ = Shape<NW>::BQ;
