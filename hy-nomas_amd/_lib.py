@@ -84,7 +84,7 @@ SIGNATURES = {
     "hn_kv_pages_copy": [ctypes.POINTER(_P), _PI64, _PI64, _PI64, _I64, _I64, _PI32, _PI32, _I64, _P],
     "hn_attn_kv_pages": [_I, _P, _PI64, _I64, _I64, _I64, _I64, _P, _P, _PI64, _P, _P, _PI64, _I64, _I64, _I64,
                          _P, _I64, _I64, _P, _I, _P, _P, _P, _PI64, _I64, _P, _I64, _F, _P, _PI64, _P, _P, _I64, _P],
-    "hn_attn_kv_pages_workspace_size": [_I64] * 6 + [_I],
+    "hn_attn_kv_pages_workspace_size": [_I64] * 6,
     "hn_e4m3_encode_range": [ctypes.c_uint32, _I64, _P, _P],
 }
 RESTYPES = {"hn_last_error": ctypes.c_char_p, "hn_attn_fp8kv_workspace_size": _I64,

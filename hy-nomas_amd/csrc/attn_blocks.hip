@@ -37,6 +37,7 @@ struct BlockParams : Params {
     int G;                 // query heads per cached head; H counts cached heads
     float* lse;            // [B, H G, Lq]
     const int32_t* lens;   // of pages: the sequences' tokens
+    const int32_t* q_start;  // as in PageParams
     int pages;
 };
 
@@ -94,8 +95,9 @@ HN_DEVICE void clear_masked_v(TailRegs<4>& r, uint64_t w) {
 // PAGED: idx is a page table [B, top_k], block a page, and sequence b's tokens are the
 // first lens[b] that its pages hold, in their order; a tile lies in one page and its loads
 // go through descriptors of its own rows. The part of a tile past the length reads as zeros.
-// It serves runs of 33 to 128 rows (where, and what the others take: pages_plan).
-template <int FMT, bool MASK, bool PAGED = false>
+// It serves 33 to 128 rows, and more over short sequences (where, and what the others take:
+// pages_plan). CAUSAL: no tail, and query i sees tokens below seen_before + i.
+template <int FMT, bool MASK, bool PAGED = false, bool CAUSAL = false>
 __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
     constexpr int NW = 4, BQ = Shape<NW>::BQ;
     __shared__ __attribute__((aligned(16))) uint8_t smem[smem_bytes<NW>()];
@@ -148,7 +150,14 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
 
     const int32_t* list = p.idx ? p.idx + b * p.is0 + h * p.is1 + run * p.is2 : nullptr;
     const int kv_len = PAGED ? __builtin_amdgcn_readfirstlane(seq_len(p.lens, b, p.top_k, p.shift + 6)) : (int)p.kv_len;
-    const int n_cache = list && !PAGED ? list_length(list, p.top_k) << p.shift : (kv_len + BKV - 1) / BKV;
+    int lim = 0, lim_all = 0, lim_end = kv_len;  // CAUSAL: tokens that this row, every row and any row sees
+    if constexpr (CAUSAL) {
+        const int before = seen_before(p, b, kv_len), last = (int)rows - 1;
+        lim = min(before + (int)qi, kv_len);
+        lim_all = min(before + qt * BQ / p.G, kv_len);
+        lim_end = max(min(before + min(qt * BQ + BQ - 1, last) / p.G, kv_len), 0);
+    }
+    const int n_cache = list && !PAGED ? list_length(list, p.top_k) << p.shift : (lim_end + BKV - 1) / BKV;
     const int n_tail = (int)((p.cur_len + BKV - 1) / BKV);
     const int n_all = n_cache + n_tail;
     const int t_begin = (int)((int64_t)n_all * split / p.splits);
@@ -232,6 +241,13 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
         const uint64_t all = count >= BKV ? ALL_KEYS : (1ull << count) - 1;
         return tile_mask<MASK>(st) & all;
     };
+    // Half kb of cache tile t, its keys' word and largest logit: without those that take no part.
+    auto masked = [&](f32x16& x, int t, int kb, uint64_t word, float mx) __attribute__((always_inline)) {
+        if constexpr (CAUSAL)
+            if ((t + 1) * BKV > lim_all) return mask_raw(x, kb, half, lim - t * BKV, word);
+        const uint32_t w = (uint32_t)(word >> (32 * kb));
+        return w == ~0u ? mx : mask_word(x, w);
+    };
     const uint32_t ka_off = col * KROW + 16 * half;
     const uint32_t va_off = K_BYTES + col * VTROW + 16 * half;
     CacheRegs<NW> regs;
@@ -300,8 +316,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
         __syncthreads();
         mw = word_of(count, smem);
         sa = s_block(smem + ka_off, qf);
-        mxa = raw_max(sa);
-        if ((uint32_t)mw != ~0u) mxa = mask_word(sa, (uint32_t)mw);
+        mxa = masked(sa, t_begin, 0, mw, raw_max(sa));
         int t = t_begin;
         int e2 = entry(t + 2);
         // ---- cache tiles, and the step into the tail
@@ -325,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
                 });
             }
             store_mask<NW, MASK>(regs, nst);
-            if ((uint32_t)(mw >> 32) != ~0u) mxb = mask_word(sb, (uint32_t)(mw >> 32));
+            mxb = masked(sb, t, 1, mw, mxb);
             const bool tail_next = t + 1 < t_end && t + 1 >= n_cache;
             if (tail_next) {  // once: the tail's first tile, loaded on the spot
                 fetch_tail_k(tail_place(t + 1));
@@ -348,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void attn_blocks_kernel(BlockParams p) {
                     store_v_part<FMT, NW>(regs.v, nst + K_BYTES, i, vs, vp, vd);
                 });
             }
-            if ((uint32_t)mwn != ~0u) mxa = mask_word(sa, (uint32_t)mwn);
+            mxa = masked(sa, t + 1, 0, mwn, mxa);
             if (tail_next) {
                 load_tail_span_v<NW>(to, tv, tail_place(t + 1).co, tr);
                 if constexpr (MASK)
@@ -1856,7 +1871,7 @@ int hn::launch_page_tiles(const attn::PageParams& a, int fmt, void* workspace, h
     p.fmt = fmt;
     p.idx = a.table; p.is0 = a.ts0;
     p.top_k = a.width;
-    p.lens = a.lens; p.pages = a.pages;
+    p.lens = a.lens; p.q_start = a.q_start; p.pages = a.pages;
     p.block = (int64_t)1 << a.shift;
     p.shift = a.shift - 6;
     p.q_block = a.Lq; p.runs = 1;
@@ -1869,10 +1884,12 @@ int hn::launch_page_tiles(const attn::PageParams& a, int fmt, void* workspace, h
     }
     const dim3 grid((unsigned)(8 * (int64_t)p.per_xcd));
     if (fmt == HN_KV_FP8) {
-        if (p.uvalid) attn::attn_blocks_kernel<HN_KV_FP8, true, true><<<grid, 256, 0, st>>>(p);
+        if (a.causal) attn::attn_blocks_kernel<HN_KV_FP8, false, true, true><<<grid, 256, 0, st>>>(p);
+        else if (p.uvalid) attn::attn_blocks_kernel<HN_KV_FP8, true, true><<<grid, 256, 0, st>>>(p);
         else attn::attn_blocks_kernel<HN_KV_FP8, false, true><<<grid, 256, 0, st>>>(p);
     } else {
-        if (p.uvalid) attn::attn_blocks_kernel<HN_KV_INT8, true, true><<<grid, 256, 0, st>>>(p);
+        if (a.causal) attn::attn_blocks_kernel<HN_KV_INT8, false, true, true><<<grid, 256, 0, st>>>(p);
+        else if (p.uvalid) attn::attn_blocks_kernel<HN_KV_INT8, true, true><<<grid, 256, 0, st>>>(p);
         else attn::attn_blocks_kernel<HN_KV_INT8, false, true><<<grid, 256, 0, st>>>(p);
     }
     const int rc = check_launch("hn_attn_kv_pages");

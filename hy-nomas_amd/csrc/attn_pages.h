@@ -53,7 +53,8 @@ HN_DEVICE int seq_len(const int32_t* lens, int64_t b, int width, int shift) {
 }
 
 // Causal rows: query i sees tokens below seen_before + i, and below the sequence's length.
-HN_DEVICE int seen_before(const PageParams& p, int b, int len) {
+template <class P>
+HN_DEVICE int seen_before(const P& p, int64_t b, int len) {
     const int first = p.q_start ? __builtin_amdgcn_readfirstlane(p.q_start[b]) : len - (int)p.Lq;
     return (first < len ? first : len) + 1;
 }

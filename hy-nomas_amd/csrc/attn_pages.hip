@@ -524,7 +524,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
 // dealt out evenly to as many workgroups as there are CUs, so that neither the sequences'
 // lengths nor a last round of workgroups leaves any idle (two sequences' 3600 queries x 24
 // heads over 21600 keys and the tail: 2.40 ms, 0.93 PFLOP/s; by runs of 128 rows on 4
-// waves 2.83); parts meet in pages_join_kernel. The part of a tile past a length or a tail, and a page that is none,
+// waves 2.83); parts meet in pages_join_kernel. An item costs 11 us beside its tiles (2.4 us
+// each). The part of a tile past a length or a tail, and a page that is none,
 // read as zeros and are masked by the tile's 64-bit word.
 constexpr int TILE_WAVES = 8;
 constexpr int TILE_ROWS = Shape<TILE_WAVES>::BQ;
@@ -666,8 +667,34 @@ __global__ __launch_bounds__(64 * TILE_WAVES, 1) void attn_page_tiles_kernel(Pag
         if (t_end > t_begin) {
             // ---- prologue: tiles t_begin, + 1 in stages 0, 1, the next one's codes in registers
             int c0 = 0, c1 = 0, c2 = 0;  // keys of tiles t, t + 1, t + 2
+            const bool cached = t_begin + 2 < nc;
+            if (cached) {  // the three tiles' loads in flight together
+                const Place g0 = cache_tile(t_begin), g1 = cache_tile(t_begin + 1), g2 = cache_tile(t_begin + 2);
+                CacheRegs<NW> r0, r1;
+                r0.s = r1.s = 0.0f;
+                load_k<NW, false>(lo, r0, g0.src, g0.count);
+                load_v<NW>(lo, r0, g0.src);
+                load_k<NW, false>(lo, r1, g1.src, g1.count);
+                load_v<NW>(lo, r1, g1.src);
+                fetch_cache_k(g2);
+                load_v<NW>(lo, regs, g2.src);
+                c0 = g0.count;
+                c1 = g1.count;
+                c2 = g2.count;
+                __builtin_amdgcn_s_waitcnt(0);
+                if (threadIdx.x < 2 * BKV) {
+                    sbuf[threadIdx.x] = r0.s;
+                    sbuf[SB_FLOATS + threadIdx.x] = r1.s;
+                }
+                __syncthreads();
+                store_tile<FMT, NW, false>(r0, smem, sbuf);
+                store_tile<FMT, NW, false>(r1, smem + STAGE, sbuf + SB_FLOATS);
+                __syncthreads();
+                if (threadIdx.x < 2 * BKV) sbuf[threadIdx.x] = regs.s;
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
+                if (cached) break;
                 const int t = t_begin + k;
                 int count = 0;
                 if (t < nc) {
@@ -689,19 +716,11 @@ __global__ __launch_bounds__(64 * TILE_WAVES, 1) void attn_page_tiles_kernel(Pag
                 if (k == 0) c0 = count;
                 else c1 = count;
             }
-            {
-                const Place g = cache_tile(t_begin + 2);
-                fetch_cache_k(g);
-                load_v<NW>(lo, regs, g.src);
-                c2 = g.count;
-                if (t_begin + 2 >= nc) {
-                    c2 = tail_keys(t_begin + 2);
-                    fetch_tail(t_begin + 2);
-                }
+            if (!cached) {
+                c2 = tail_keys(t_begin + 2);
+                fetch_tail(t_begin + 2);
+                __builtin_amdgcn_s_waitcnt(0);
             }
-            __builtin_amdgcn_s_waitcnt(0);
-            // (before a tail tile no barrier has ended the reads of tile t_begin's scales)
-            if (t_begin + 2 < nc && threadIdx.x < 2 * BKV) sbuf[threadIdx.x] = regs.s;
             __syncthreads();
             uint64_t mw = word_of(t_begin, c0, smem);
             f32x16 sa = s_block(smem + ka_off, qf), sb;
@@ -915,19 +934,24 @@ __global__ __launch_bounds__(256) void pages_join_kernel(PageParams p, int R) {
 using namespace hn;
 
 struct PagesPlan {
-    int tiles;   // 0: attn_pages_kernel, 4 and 8: the tile kernels of as many waves
+    int tiles;   // 0: attn_pages_kernel; 4, 8: the tile kernel of as many waves
     int rb, runs, whole, wgs, pitch;
     int64_t items;
 };
 
-static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len, int causal) {
+static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t max_len, int64_t cur_len) {
     PagesPlan pl;
     const int64_t rows = Lq * G;
-    // Two sequences x 24 heads x 20000 keys (calls, us): 32 rows 59 in attn_pages_kernel and 95 in
-    // the 4-wave tiles, 64 rows 101 and 99, 128 rows 182 and 107, there 147 in the 8-wave ones; 129
-    // rows 179 against 148, 300 264 and 277, 777 583 and 539, 3600 2293 and 1951; with 3000 keys
-    // 128 rows 38 against 47, 256 48 and 57, 512 81 and 78. Causal rows have no 4-wave tiles.
-    pl.tiles = rows <= 32 ? 0 : rows > 128 ? attn::TILE_WAVES : causal ? 0 : 4;
+    // attn_pages_kernel (0), the 4-wave tiles or the 8-wave ones, calls in us. 33 to 64 rows, 0
+    // against 4: 64 sequences x 8 heads, 300 keys 44 and 23, 1000 keys 82 to 91 and 47, 4000 155 to
+    // 161 and 153; 20000 keys of eight 80 and 100, of two x 24 heads 73 to 78 and 95. 32 rows: 20000
+    // keys 50 and 82 to 92. 128 rows, 20000 keys x 2 x 24 heads: 182 and 107, 8-wave 147. More
+    // rows, 4 against 8, up to 1000 and 4000 keys: 32 sequences x 8 heads, 300 rows 75 and 108, 209
+    // and 229, 1000 rows 187 and 188, 444 and 387; 8 x 8, 600 rows 47 and 67, 117 and 97; up to
+    // 2000 keys 39 and 50 (2 x 24, 300 rows), 121 and 119 (8 x 8, 1200), 272 and 247 (4000). The
+    // same borders for causal rows.
+    const int64_t keys = max_len + cur_len;
+    pl.tiles = rows <= 32 || (rows <= 64 && keys > 4096) ? 0 : rows <= 128 || keys <= 2048 ? 4 : attn::TILE_WAVES;
     if (pl.tiles == attn::TILE_WAVES) {
         pl.runs = (int)((rows + attn::TILE_ROWS - 1) / attn::TILE_ROWS);
         pl.items = B * H * pl.runs;
@@ -993,9 +1017,9 @@ static int64_t plan_bytes(const PagesPlan& pl, int64_t B, int64_t Lq, int64_t Hq
 }
 
 extern "C" int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
-                                                   int64_t cur_len, int causal) {
+                                                   int64_t cur_len) {
     if (!pages_shape_ok(B, Lq, Hq, H, max_len, cur_len)) return 0;
-    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
     return plan_bytes(pl, B, Lq, Hq, H, max_len, cur_len);
 }
 
@@ -1041,7 +1065,7 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
     HN_REQUIRE(width == 0 || n_pages == 0 || (table && kc && vc && ks && vs), HN_E_ARG, "hn_attn_kv_pages: null pool pointer");
     const int64_t max_len = n_pages ? width * page : 0;
     HN_REQUIRE(pages_shape_ok(B, Lq, Hq, H, max_len, cur_len), HN_E_ARG, "hn_attn_kv_pages: too much work");
-    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len, causal);
+    const PagesPlan pl = pages_plan(B, Lq, Hq / H, H, max_len, cur_len);
     const int64_t units = 1 + (max_len + attn::BKV - 1) / attn::BKV + (cur_len + attn::BKV - 1) / attn::BKV;
     HN_REQUIRE(pl.items <= 0x3fffffffLL / units, HN_E_ARG, "hn_attn_kv_pages: too much work for one launch");
     const int64_t need = plan_bytes(pl, B, Lq, Hq, H, max_len, cur_len);

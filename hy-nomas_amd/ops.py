@@ -1363,7 +1363,7 @@ def attn_kv_pages(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
     W = table.shape[1]
     with _on(device):
         lib = L.load()
-        ws_bytes = _pages_workspace(device.index, B, Lq, Hq, H, W * page if P else 0, cur_len, int(causal))
+        ws_bytes = _pages_workspace(device.index, B, Lq, Hq, H, W * page if P else 0, cur_len)
         ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes else None
         L.check(lib.hn_attn_kv_pages(
             fmt, q.data_ptr(), _strides(q), B, Lq, Hq, D, k_codes.data_ptr(), v_codes.data_ptr(), cs,

@@ -473,8 +473,8 @@ int hn_kv_pages_copy(void *const *base, const int64_t *layer_stride, const int64
  * lies behind a sequence's end does not matter.
  *   kcur, vcur, cur_valid, out and lse as in hn_attn_kv_blocks. Probabilities are held to
  *   2^-17 of themselves (the sum of two bf16) where a cached head has up to 32 rows, Lq Hq
- *   / H of them, or up to 128 causal ones, and V is bf16 there; else probabilities and V
- *   are fp16 as in hn_attn_kv_blocks.
+ *   / H of them, or up to 64 and room for more than 4096 keys, and V is bf16 there; else
+ *   probabilities and V are fp16 as in hn_attn_kv_blocks.
  * workspace: hn_attn_kv_pages_workspace_size(.., width * page, ..) bytes, 16-byte aligned. */
 int hn_attn_kv_pages(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,
                      const void *kc, const void *vc, const int64_t *cs, const float *ks, const float *vs,
@@ -487,7 +487,7 @@ int hn_attn_kv_pages(int fmt, const void *q, const int64_t *qs, int64_t B, int64
 /* Bytes of workspace hn_attn_kv_pages needs for these sizes on the current device (0:
  * none); max_len = width * page. */
 int64_t hn_attn_kv_pages_workspace_size(int64_t B, int64_t Lq, int64_t Hq, int64_t H, int64_t max_len,
-                                        int64_t cur_len, int causal);
+                                        int64_t cur_len);
 
 /* Test support; it replaces no reference interface. Writes to out[i] the e4m3
  * byte that the quantizers' hardware conversion (v_cvt_pk_fp8_f32, round to

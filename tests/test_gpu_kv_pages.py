@@ -32,10 +32,15 @@ def _pool(dev, g, pages, page, H, fmt="fp8", layers=None, gain=1.0):
     return pool
 
 
-def _table(dev, g, lens, page, pages, width=None):
+# Tables as wide as their sequences, and with room for many more tokens: which kernel takes
+# a call of more than 32 rows depends on it.
+rooms = pytest.mark.parametrize("room", [0, 5120])
+
+
+def _table(dev, g, lens, page, pages, width=None, room=0):
     """Distinct random pages for every sequence, -1 behind its last."""
     need = [-(-n // page) for n in lens]
-    t = torch.full((len(lens), width or max(1, *need)), -1, dtype=I32)
+    t = torch.full((len(lens), max(width or max(1, *need), room // page)), -1, dtype=I32)
     order = torch.randperm(pages, generator=torch.Generator().manual_seed(int(g.initial_seed()))).tolist()
     for b, n in enumerate(need):
         t[b, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=I32)
@@ -132,30 +137,32 @@ def test_one_token(dev, fmt, H, G, lens):
     _check(got, _reference(q, pool, table, lens), f"{fmt} {H}x{G} {lens}")
 
 
+@rooms
 @pytest.mark.parametrize("page", [64, 256, 1024])
 @pytest.mark.parametrize("Lq,G", [(2, 1), (5, 4), (8, 2), (9, 4), (33, 1), (70, 3), (129, 1), (300, 1), (101, 5)])
-def test_causal(dev, page, Lq, G):
+def test_causal(dev, page, Lq, G, room):
     """Sequences shorter than the queries have rows without a key."""
     _, ca, _ = _mods()
     lens = (Lq, 1000, max(1, Lq // 2), 0, 513 + Lq)
     g = torch.Generator(device=dev).manual_seed(page + Lq)
     pages = sum(-(-n // page) for n in lens) + 1
     pool = _pool(dev, g, pages, page, 2)
-    table = _table(dev, g, lens, page, pages)
+    table = _table(dev, g, lens, page, pages, room=room)
     q = torch.randn(len(lens), Lq, 2 * G, 128, device=dev, generator=g).to(BF16)
     got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
     _check(got, _reference(q, pool, table, lens, causal=True), f"page {page} Lq {Lq} G {G}")
 
 
+@rooms
 @pytest.mark.parametrize("Lq,G", [(1, 1), (7, 2), (40, 1), (200, 2)])
-def test_causal_queries_of_their_own_places(dev, Lq, G):
+def test_causal_queries_of_their_own_places(dev, Lq, G, room):
     """Prompts of different lengths: rows before a sequence's first token see none, rows
     past its last see all of it."""
     _, ca, _ = _mods()
     H, page, lens, first = 2, 64, (700, 230, 64, 5, 0), (700 - Lq // 2, 230 - Lq, 3, -3, 0)
     g = torch.Generator(device=dev).manual_seed(Lq)
     pool = _pool(dev, g, 30, page, H)
-    table = _table(dev, g, lens, page, 30)
+    table = _table(dev, g, lens, page, 30, room=room)
     q = torch.randn(len(lens), Lq, H * G, 128, device=dev, generator=g).to(BF16)
     got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True, q_start=_i32(dev, first))
     _check(got, _reference(q, pool, table, lens, causal=True, first=first), f"{Lq} rows")
@@ -212,10 +219,11 @@ def test_a_pool_without_pages(dev, Lq):
     assert kp.read_pages(pool, "k", table, n, 5).abs().sum().item() == 0
 
 
+@rooms
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
 @pytest.mark.parametrize("Lq,G,Lc", [(1, 1, 1), (1, 4, 70), (31, 1, 200), (130, 1, 0), (129, 2, 129), (300, 1, 64), (65, 1, 1)])
 @pytest.mark.parametrize("masked", [False, True])
-def test_queries_and_tail(dev, fmt, Lq, G, Lc, masked):
+def test_queries_and_tail(dev, fmt, Lq, G, Lc, masked, room):
     """Any number of queries, with the current chunk's keys behind the history, padded
     ones among them, and what a masked key holds without effect."""
     _, ca, _ = _mods()
@@ -223,7 +231,7 @@ def test_queries_and_tail(dev, fmt, Lq, G, Lc, masked):
     g = torch.Generator(device=dev).manual_seed(Lq + G + Lc)
     pages = sum(-(-n // page) for n in lens) + 1
     pool = _pool(dev, g, pages, page, H, fmt)
-    table = _table(dev, g, lens, page, pages)
+    table = _table(dev, g, lens, page, pages, room=room)
     B = len(lens)
     q = torch.randn(B, Lq, H * G, 128, device=dev, generator=g).to(BF16)
     kw = {}
@@ -241,15 +249,16 @@ def test_queries_and_tail(dev, fmt, Lq, G, Lc, masked):
     _check(got, _reference(q, pool, table, lens, **kw), f"{fmt} Lq {Lq} G {G} Lc {Lc} masked {masked}")
 
 
-@pytest.mark.parametrize("Lq", [1, 9, 200])
-def test_what_lies_behind_a_sequence_does_not_matter(dev, Lq):
+@rooms
+@pytest.mark.parametrize("Lq", [1, 9, 40, 200])
+def test_what_lies_behind_a_sequence_does_not_matter(dev, Lq, room):
     """NaN codes and infinite scales behind the end, in unnamed pages and under entries
     that name none; such entries inside a sequence name no keys."""
     _, ca, _ = _mods()
     H, page, lens = 2, 64, (300, 65)
     g = torch.Generator(device=dev).manual_seed(Lq)
     pool = _pool(dev, g, 12, page, H)
-    table = _table(dev, g, lens, page, 12, width=9)
+    table = _table(dev, g, lens, page, 12, width=9, room=room)
     q = torch.randn(2, Lq, H, 128, device=dev, generator=g).to(BF16)
     want = ca.paged_attention(q, pool, table, _i32(dev, lens))
     _check(want, _reference(q, pool, table, lens), "clean")
@@ -283,15 +292,16 @@ def test_what_lies_behind_a_sequence_does_not_matter(dev, Lq):
     assert (got[0][1] == 0).all() and (got[1][1] == -math.inf).all()
 
 
+@rooms
 @pytest.mark.parametrize("Lq", [1, 40, 150])
-def test_nan_and_extreme_logits(dev, Lq):
+def test_nan_and_extreme_logits(dev, Lq, room):
     """A row that meets a NaN gets NaN in output and log-sum-exp; rows of other
     sequences do not. Logits of +-1e4 stay a softmax."""
     _, ca, _ = _mods()
     H, page, lens = 2, 64, (200, 200)
     g = torch.Generator(device=dev).manual_seed(Lq)
     pool = _pool(dev, g, 8, page, H, gain=30.0)
-    table = _table(dev, g, lens, page, 8)
+    table = _table(dev, g, lens, page, 8, room=room)
     q = (torch.randn(2, Lq, H, 128, device=dev, generator=g) * 30).to(BF16)
     got = ca.paged_attention(q, pool, table, _i32(dev, lens))
     _check(got, _reference(q, pool, table, lens), "large logits")

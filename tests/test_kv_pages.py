@@ -190,9 +190,9 @@ def test_c_abi_checks():
                       (dict(cs=odd), "multiples of 16"), (dict(width=2 ** 28), "too many keys"), (dict(q=None), "null"),
                       (dict(width=300), "workspace")):
         assert attend(**kw) == L.HN_E_ARG and match in err(), kw
-    assert lib.hn_attn_kv_pages_workspace_size(1, 1, 4, 2, 128, 0, 0) == 0
-    assert lib.hn_attn_kv_pages_workspace_size(1, 1, 4, 2, 1 << 16, 0, 0) > 0
-    assert lib.hn_attn_kv_pages_workspace_size(0, 1, 4, 2, 128, 0, 0) == 0
+    assert lib.hn_attn_kv_pages_workspace_size(1, 1, 4, 2, 128, 0) == 0
+    assert lib.hn_attn_kv_pages_workspace_size(1, 1, 4, 2, 1 << 16, 0) > 0
+    assert lib.hn_attn_kv_pages_workspace_size(0, 1, 4, 2, 128, 0) == 0
 
     four = ctypes.c_void_p * 4
     sizes = (ctypes.c_int64 * 4)(16384, 16384, 512, 512)
