@@ -153,12 +153,11 @@ struct Block {
 };
 
 //
-// NW 4: the units of all items are dealt out evenly, whatever the sequences' lengths, and
-// parts of an item are joined by a second kernel. NW 8 (WHOLE): a workgroup an item.
-template <int FMT, int RB, bool SV, int NW>
+// The units of all items are dealt out evenly, whatever the sequences' lengths, and parts of
+// an item are joined by a second kernel; or (WHOLE) a workgroup has an item.
+template <int FMT, int RB, bool SV, int NW, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_pages_kernel(PageParams p) {
     constexpr int R = 16 * RB, PITCH = D + 4, UNIT = 32 * NW;
-    constexpr bool WHOLE = NW != 4;
     __shared__ __attribute__((aligned(16))) float so[NW][R][PITCH];
     static_assert(sizeof(so[0]) >= K_TILE, "a wave's K codes fit where its result goes");
     __shared__ float sml[NW][R][2];
@@ -935,7 +934,8 @@ using namespace hn;
 
 struct PagesPlan {
     int tiles;   // 0: attn_pages_kernel; 4, 8: the tile kernel of as many waves
-    int rb, runs, whole, wgs, pitch;
+    int whole;   // of attn_pages_kernel: waves of a workgroup an item; 0: units dealt out
+    int rb, runs, wgs, pitch;
     int64_t items;
 };
 
@@ -965,24 +965,37 @@ static PagesPlan pages_plan(int64_t B, int64_t Lq, int64_t G, int64_t H, int64_t
     pl.runs = (int)((rows + R - 1) / R);
     pl.items = B * H * pl.runs;
     pl.pitch = (int)(rows < R ? rows : R);
-    // A workgroup an item where each has few keys and all are resident at once: calls of
-    // 8 to 256 items of one to four rows, up to 100 keys 6 us against 8.4 to 12.4, 500 8.2 to
-    // 10.6 against 9.1 to 17.1, 1024 11.1 to 16.4 against 11.3 to 24.2, 2048 (eight items) 17.5
-    // against 13.3; twenty rows 500 11.2 against 14.2, 1024 15.3 against 14.6; 1536 items of 100
-    // keys 34.6 against 19.9.
-    const int64_t units = (max_len + 255) / 256 + (cur_len + 255) / 256;
-    pl.wgs = (pl.rb == 1 ? 3 : 2) * device_cus();
-    pl.whole = units * pl.rb <= 4 && pl.items <= 2 * (int64_t)device_cus();
+    // A workgroup an item: of eight waves where each has few keys and all are resident at once
+    // (calls of 8 to 256 items of one to four rows, kernels in us: up to 100 keys 6 against 8.4
+    // to 12.4 dealt out and joined, 500 8.2 to 10.6 against 9.1 to 17.1, 1024 11.1 to 16.4 against
+    // 11.3 to 24.2, 2048 (eight items) 17.5 against 13.3; twenty rows 500 11.2 against 14.2, 1024
+    // 15.3 against 14.6), of four where many items come and go (calls, sequences of n / 8 to n keys
+    // and of n, against dealt out: 2048 items of four rows, n 500 37 and 51 against 63 and 67, 2000
+    // 112 and 178 against 120 and 192, 4000 224 and 333 against 223 and 353; 512 items 1000 21 and 30
+    // against 28 and 35, with eight waves 25; 4000 66 and 88 against 66 and 98, 6000 88 and 128 against
+    // 87 and 141; 256 items 2000 23 and 26 against 26 and 34, 4000 39 and 45 against 38 and 55, twenty
+    // rows there 50 and 59 against 47 and 55).
+    const int64_t units = (max_len + 255) / 256 + (cur_len + 255) / 256, cus = device_cus();
+    pl.wgs = (int)((pl.rb == 1 ? 3 : 2) * cus);
+    if (pl.items < cus) pl.whole = units * pl.rb <= 4 ? 8 : 0;
+    else pl.whole = keys <= (pl.items < 2 * cus ? 2048 : 4096) && pl.items <= 1 << 22 ? 4 : 0;  // (a grid has fewer than 2^32 threads)
     return pl;
 }
 
 // SV: the scales of consecutive tokens are consecutive, four to a load.
-template <int FMT, int NW>
+template <int FMT, int NW, bool WHOLE>
 static void launch_pages(int rb, bool sv, const attn::PageParams& p, unsigned blocks, hipStream_t st) {
-    if (rb == 1 && sv) attn::attn_pages_kernel<FMT, 1, true, NW><<<blocks, 64 * NW, 0, st>>>(p);
-    else if (rb == 1) attn::attn_pages_kernel<FMT, 1, false, NW><<<blocks, 64 * NW, 0, st>>>(p);
-    else if (sv) attn::attn_pages_kernel<FMT, 2, true, NW><<<blocks, 64 * NW, 0, st>>>(p);
-    else attn::attn_pages_kernel<FMT, 2, false, NW><<<blocks, 64 * NW, 0, st>>>(p);
+    if (rb == 1 && sv) attn::attn_pages_kernel<FMT, 1, true, NW, WHOLE><<<blocks, 64 * NW, 0, st>>>(p);
+    else if (rb == 1) attn::attn_pages_kernel<FMT, 1, false, NW, WHOLE><<<blocks, 64 * NW, 0, st>>>(p);
+    else if (sv) attn::attn_pages_kernel<FMT, 2, true, NW, WHOLE><<<blocks, 64 * NW, 0, st>>>(p);
+    else attn::attn_pages_kernel<FMT, 2, false, NW, WHOLE><<<blocks, 64 * NW, 0, st>>>(p);
+}
+
+template <int FMT>
+static void launch_few(const PagesPlan& pl, bool sv, const attn::PageParams& p, unsigned blocks, hipStream_t st) {
+    if (pl.whole == 8) launch_pages<FMT, 8, true>(pl.rb, sv, p, blocks, st);
+    else if (pl.whole) launch_pages<FMT, 4, true>(pl.rb, sv, p, blocks, st);
+    else launch_pages<FMT, 4, false>(pl.rb, sv, p, blocks, st);
 }
 
 template <int FMT>
@@ -1123,13 +1136,8 @@ extern "C" int hn_attn_kv_pages(int fmt, const void* q, const int64_t* qs, int64
         return join_pages<attn::BKV>(pl, p, attn::TILE_ROWS, st);
     }
     const bool sv = ss[1] == 1 && ss[0] % 4 == 0 && ss[2] % 4 == 0 && aligned(p.vs, 16);
-    if (fmt == HN_KV_FP8) {
-        if (pl.whole) launch_pages<HN_KV_FP8, 8>(pl.rb, sv, p, blocks, st);
-        else launch_pages<HN_KV_FP8, 4>(pl.rb, sv, p, blocks, st);
-    } else {
-        if (pl.whole) launch_pages<HN_KV_INT8, 8>(pl.rb, sv, p, blocks, st);
-        else launch_pages<HN_KV_INT8, 4>(pl.rb, sv, p, blocks, st);
-    }
+    if (fmt == HN_KV_FP8) launch_few<HN_KV_FP8>(pl, sv, p, blocks, st);
+    else launch_few<HN_KV_INT8>(pl, sv, p, blocks, st);
     if (const int rc = check_launch("hn_attn_kv_pages"); rc != HN_OK || pl.whole) return rc;
     return join_pages<attn::UNIT>(pl, p, 16 * pl.rb, st);
 }

@@ -336,16 +336,23 @@ def test_strides_scale_and_scratch_of_other_calls(dev):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
-@pytest.mark.parametrize("B,lens", [(70, 130), (300, 40)])
-def test_many_sequences(dev, B, lens):
+@rooms
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("Lq,Lc,causal", [(1, 0, False), (9, 0, True), (2, 70, False), (20, 0, True)])
+@pytest.mark.parametrize("B,lens", [(70, 130), (150, 40), (300, 40)])
+def test_many_sequences(dev, B, lens, Lq, Lc, causal, fmt, room):
     _, ca, _ = _mods()
     n = [(lens * (b + 1) * 7919) % (3 * lens) for b in range(B)]
     g = torch.Generator(device=dev).manual_seed(B)
     pages = sum(-(-x // 64) for x in n) + 1
-    pool = _pool(dev, g, pages, 64, 2)
-    table = _table(dev, g, n, 64, pages)
-    q = torch.randn(B, 1, 4, 128, device=dev, generator=g).to(BF16)
-    _check(ca.paged_attention(q, pool, table, _i32(dev, n)), _reference(q, pool, table, n), f"B {B}")
+    pool = _pool(dev, g, pages, 64, 2, fmt)
+    table = _table(dev, g, n, 64, pages, room=room)
+    q = torch.randn(B, Lq, 4, 128, device=dev, generator=g).to(BF16)
+    kw = dict(causal=causal)
+    if Lc:
+        kv = torch.randn(2, B, Lc, 2, 128, device=dev, generator=g).to(BF16)
+        kw.update(k_cur=kv[0], v_cur=kv[1], cur_valid=torch.rand(B, Lc, device=dev, generator=g) < 0.5)
+    _check(ca.paged_attention(q, pool, table, _i32(dev, n), **kw), _reference(q, pool, table, n, **kw), f"B {B}")
 
 
 @pytest.mark.parametrize("Lq", [1, 5, 150])
