@@ -749,12 +749,13 @@ def _check_keys(codes: torch.Tensor, scale: torch.Tensor, what: str) -> None:
 
 def _one_device(what: str, first: torch.Tensor, *tensors) -> torch.device:
     """The device of ``first``, a GPU, on which every other tensor given is too."""
-    _gpu(first, *tensors)
-    device = first.device
+    index = first.get_device()
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index or index < 0:
+            _gpu(first, *tensors)
             raise RuntimeError(f"{what}: tensors are on different devices")
-    return device
+    _gpu(first)
+    return first.device
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1246,18 +1247,26 @@ def _(codes, scale, table, kv_len, max_len):
     return codes.new_empty((table.shape[0], max_len, *codes.shape[2:]), dtype=torch.bfloat16)
 
 
-def _page_bytes(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+@functools.lru_cache(maxsize=1024)
+def _page_layout(shape: tuple, stride: tuple, size: int):
     """Bytes from layer to layer, from page to page and of a page of [layers, P, page, H,
-    last], whose pages are runs of bytes each (in any order of the tokens and heads)."""
-    size = t.element_size()
+    last] values of ``size`` bytes whose pages are runs of memory each (in any order of the
+    tokens and heads); None where they are not."""
     run = 1
-    for n, s in sorted(((n, s) for n, s in zip(t.shape[2:], t.stride()[2:]) if n != 1), key=lambda x: x[1]):
+    for n, s in sorted(((n, s) for n, s in zip(shape[2:], stride[2:]) if n != 1), key=lambda x: x[1]):
         if s != run:
-            raise ValueError(f"{what}: a page must be one run of memory")
+            return None
         run *= n
     # (a single page or layer lies nowhere relative to another)
-    step = t.stride(1) if t.shape[1] > 1 else run
-    return (t.stride(0) * size if t.shape[0] > 1 else 0), step * size, run * size
+    step = stride[1] if shape[1] > 1 else run
+    return (stride[0] * size if shape[0] > 1 else 0), step * size, run * size
+
+
+def _page_bytes(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    layout = _page_layout(t.shape, t.stride(), t.element_size())
+    if layout is None:
+        raise ValueError(f"{what}: a page must be one run of memory")
+    return layout
 
 
 @eager_op("hy_nomas_amd::kv_pages_copy_", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale"))
@@ -1270,7 +1279,7 @@ def kv_pages_copy_(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.
     _kv_fmt(k_codes)
     if k_codes.ndim == 4:
         k_codes, v_codes, k_scale, v_scale = (t.unsqueeze(0) for t in (k_codes, v_codes, k_scale, v_scale))
-    if k_codes.ndim != 5 or k_scale.dtype != torch.float32 or tuple(k_scale.shape) != (*k_codes.shape[:4], 1):
+    if k_codes.ndim != 5 or k_scale.dtype != torch.float32 or k_scale.shape != (*k_codes.shape[:4], 1):
         raise ValueError(f"{what}: codes [layers, P, page, H, D] with fp32 scales [layers, P, page, H, 1]")
     if (v_codes.dtype != k_codes.dtype or v_codes.shape != k_codes.shape or v_scale.dtype != torch.float32
             or v_scale.shape != k_scale.shape):
@@ -1286,16 +1295,16 @@ def kv_pages_copy_(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.
     if len(to) != len(dst) or not to.isdisjoint(src):
         raise ValueError(f"{what}: a page is written twice, or read and written")
     arrays = (k_codes, v_codes, k_scale, v_scale)
-    _one_device(what, *arrays)
+    device = _one_device(what, *arrays)
     if 0 in k_codes.shape:
         return
     sizes = [_page_bytes(t, what) for t in arrays]
     n = len(src)
-    with _on(k_codes.device):
+    pages = ctypes.c_int32 * n
+    with _on(device):
         L.check(L.load().hn_kv_pages_copy(
-            (ctypes.c_void_p * 4)(*(t.data_ptr() for t in arrays)), *((ctypes.c_int64 * 4)(*col) for col in zip(*sizes)),
-            layers, P, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, _stream(k_codes)),
-            "hn_kv_pages_copy")
+            (ctypes.c_void_p * 4)(*[t.data_ptr() for t in arrays]), *map(_stride_array, zip(*sizes)), layers, P,
+            pages(*src), pages(*dst), n, _stream(k_codes)), "hn_kv_pages_copy")
 
 
 @kv_pages_copy_.register_fake
