@@ -115,6 +115,7 @@ class PagedKVCache:
         self._table: dict[int, list[int]] = {}      # sequence -> its pages
         self._length: dict[int, int] = {}
         self._stamp: dict[int, int] = {}            # changes when a batch's view of the sequence is past
+        self._turn: dict[int, int] = {}             # passes that were opened to add to the sequence
         self._next = 0
 
     def layer(self, i: int) -> dict:
@@ -136,7 +137,7 @@ class PagedKVCache:
     def new(self) -> int:
         """An empty sequence."""
         seq, self._next = self._next, self._next + 1
-        self._table[seq], self._length[seq], self._stamp[seq] = [], 0, 0
+        self._table[seq], self._length[seq], self._stamp[seq], self._turn[seq] = [], 0, 0, 0
         return seq
 
     def fork(self, seq: int) -> int:
@@ -158,7 +159,7 @@ class PagedKVCache:
     def free(self, seq: int) -> None:
         """Forget a sequence; pages that no other one holds are free again."""
         self._drop(self._table.pop(self._known(seq)))
-        del self._length[seq], self._stamp[seq]
+        del self._length[seq], self._stamp[seq], self._turn[seq]
 
     def truncate(self, seq: int, length: int) -> None:
         """Keep the first ``length`` tokens (drafted tokens that were refused go)."""
@@ -175,7 +176,8 @@ class PagedKVCache:
         """A pass of these sequences that adds ``tokens`` tokens to each (a number, or one
         for every sequence; 0: a pass that only reads). Room for them is taken now, and
         pages that they would write but share are copied; ValueError, with nothing
-        changed, if the pool has not enough."""
+        changed, if the pool has not enough. A sequence grows in one pass at a time: an
+        earlier batch that was to add to it is past."""
         seqs = [self._known(s) for s in seqs]
         adds = [tokens] * len(seqs) if isinstance(tokens, int) else list(tokens)
         if len(adds) != len(seqs) or min(adds, default=0) < 0:
@@ -203,6 +205,8 @@ class PagedKVCache:
             self._refs[dst[-1]] = 1
             held[i] = dst[-1]
             self._stamp[s] += 1
+        for s, n in zip(seqs, adds):
+            self._turn[s] += n > 0
         for s, n in grown:
             for _ in range(n):
                 p = heapq.heappop(self._free)
@@ -237,12 +241,14 @@ class PageBatch:
     ``write`` puts a layer's new tokens into the pages, ``attend`` runs a layer's
     attention; ``commit`` makes the new tokens part of the sequences once every layer has
     written them. A batch that is not committed leaves the sequences as they were. Once
-    one of its sequences is committed, cut, freed or moved, it is refused (ValueError)."""
+    one of its sequences is committed, cut, freed or moved, or one that it adds to is opened
+    to grow again, it is refused (ValueError)."""
 
     def __init__(self, cache: PagedKVCache, seqs: list[int], adds: list[int]):
         self.cache, self.seqs, self.adds = cache, seqs, adds
         self.lengths = [cache._length[s] for s in seqs]
         self._stamps = [cache._stamp[s] for s in seqs]
+        self._turns = [(s, cache._turn[s]) for s, a in zip(seqs, adds) if a]
         B, tables = len(seqs), [cache._table[s] for s in seqs]
         width = max((len(t) for t in tables), default=0)
         flat = self.lengths + [n + a for n, a in zip(self.lengths, adds)] + adds
@@ -257,9 +263,11 @@ class PageBatch:
         self.counts = None if len(set(adds)) <= 1 else counts
 
     def _check(self) -> None:
-        stamp = self.cache._stamp
+        stamp, turn = self.cache._stamp, self.cache._turn
         if any(stamp.get(s) != n for s, n in zip(self.seqs, self._stamps)):
             raise ValueError("the batch is past: a sequence was committed, cut, freed or moved since it was opened")
+        if any(turn[s] != n for s, n in self._turns):
+            raise ValueError("the batch is past: a sequence that it adds to was opened to grow again")
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, assume_finite: bool = False,
               status: Optional[torch.Tensor] = None) -> None:

@@ -367,6 +367,36 @@ def test_cache_refusals():
         same.attend(0, torch.zeros(2, 1, 1, 128, dtype=BF16))
 
 
+def test_a_sequence_grows_in_one_pass_at_a_time():
+    """A second pass would write the same places: the first is refused from then on, passes
+    that only read are not, and what the refused one took is the sequence's room."""
+    kp = pkg_module("kv_pages")
+    cache = kp.PagedKVCache(1, 6, 1, device="cpu")
+    a, b = cache.new(), cache.new()
+    cache.open([a, b], [70, 3]).commit()
+    reader, first = cache.open([a, b]), cache.open([a, b], [100, 0])
+    second = cache.open([a], 2)
+    for call in (first.commit, first.discard, lambda: first.attend(0, torch.zeros(2, 1, 1, 128, dtype=BF16))):
+        with pytest.raises(ValueError, match="grow again"):
+            call()
+    other = cache.open([b], 1)  # (first adds nothing to b)
+    reader._check()
+    second.commit()
+    other.commit()
+    assert cache.length(a) == 72 and cache.length(b) == 4
+    with pytest.raises(ValueError, match="past"):
+        reader._check()
+    cache.truncate(a, 72)
+    assert cache.free_pages == 6 - 2 - 1
+    with pytest.raises(ValueError, match="needed"):
+        cache.open([a], 64 * 5)
+    last = cache.open([a], 1)  # (a pass that is refused for want of room leaves others valid)
+    with pytest.raises(ValueError, match="needed"):
+        cache.open([a], 64 * 5)
+    last.commit()
+    assert cache.length(a) == 73
+
+
 def test_model_refusals():
     db = pkg_module("dit_block")
     for kw in (dict(text_len=4), dict(sparse_top_k=2), dict(evict_keep=2)):
