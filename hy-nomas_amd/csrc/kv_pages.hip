@@ -426,12 +426,15 @@ static int pool_args(const char* who, const int64_t* cs, const int64_t* ss, int6
 }
 
 // Tiles of B x L x H rows of `arrays` arrays: as many tokens as there are, up to 16 (eight
-// heads beside them). False: too many for one launch.
+// heads beside them), 32 of up to four heads and 64 of two (two sequences of 46057 tokens x 3
+// heads: a write 69 us, 94 by 16 tokens). False: too many for one launch.
 static bool tiles_of(int64_t B, int64_t L, int64_t H, int arrays, bool token_fast, pages::Tiles& t, dim3& grid) {
     t.B = (int32_t)B; t.L = (int32_t)L; t.H = (int32_t)H;
     t.token_fast = token_fast;
+    int most = 4;  // (6 at most: a tile's tokens lie in two pages)
+    while (most < 6 && (pages::TILE >> (most + 1)) >= H) ++most;
     t.tsh = 0;
-    while (t.tsh < 4 && (1 << t.tsh) < L) ++t.tsh;
+    while (t.tsh < most && (1 << t.tsh) < L) ++t.tsh;
     const int64_t ranges = (L - 1) / (1 << t.tsh) + 1, parts = ((H - 1) / (pages::TILE >> t.tsh) + 1) * arrays;
     if (parts > 0x7fffffffLL || ranges > 0x7fffffffLL / parts) return false;
     t.parts = (int32_t)parts;

@@ -386,8 +386,10 @@ def test_offsets_past_32_bits(dev):
         got = ca.paged_attention(q[:, :lq], pool, table, _i32(dev, [n]))
         _check(got, _reference(q[:, :lq], tail, at, (n,)), f"far pages Lq {lq}")
     big = torch.randn(1, 200, H, 128, device=dev, generator=g).to(BF16)
-    got = ca.paged_attention(big, pool, table, _i32(dev, [n]))
-    _check(got, _reference(big, tail, at, (n,)), "far pages, 200 queries")
+    for room in (0, 10):
+        far = torch.nn.functional.pad(table, (0, room), value=-1)
+        got = ca.paged_attention(big, pool, far, _i32(dev, [n]))
+        _check(got, _reference(big, tail, at, (n,)), "far pages, 200 queries")
     assert torch.equal(kp.read_pages(pool, "k", table, _i32(dev, [n]), n), kp.read_pages(tail, "k", at, _i32(dev, [n]), n))
     kp.copy_pages(pool, [pages - 3], [pages - 1])
     for m in NAMES:
@@ -400,7 +402,7 @@ def test_offsets_past_32_bits(dev):
 
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
 @pytest.mark.parametrize("layout", ["bshd", "bhsd", "qkv"])
-@pytest.mark.parametrize("L,H", [(1, 1), (1, 8), (1, 70), (3, 24), (64, 5), (129, 24), (1000, 2)])
+@pytest.mark.parametrize("L,H", [(1, 1), (1, 8), (1, 70), (3, 24), (64, 5), (129, 24), (1000, 2), (700, 1), (513, 3)])
 def test_write_is_the_contiguous_write(dev, fmt, layout, L, H):
     """Codes and scales are the contiguous cache's, token for token; nothing else of the
     pool changes: rows behind the counts, pages of nobody."""
@@ -545,7 +547,7 @@ def test_tokens_without_a_page_are_dropped(dev):
 
 
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
-@pytest.mark.parametrize("H,page,lens,n", [(3, 64, (0, 1, 200), 200), (8, 256, (700, 9), 1000), (1, 1024, (5,), 3), (2, 64, (64,), 0)])
+@pytest.mark.parametrize("H,page,lens,n", [(3, 64, (0, 1, 200), 200), (8, 256, (700, 9), 1000), (1, 1024, (5,), 3), (2, 64, (64,), 0), (2, 64, (1000, 77), 901), (4, 64, (300,), 333)])
 def test_read(dev, fmt, H, page, lens, n):
     kp, _, _ = _mods()
     g = torch.Generator(device=dev).manual_seed(n)

@@ -173,8 +173,8 @@ def test_c_abi_checks():
         assert write(**kw) == L.HN_E_ARG and match in err(), kw
     assert write(B=0) == 0
     size = lib.hn_kv_pages_write_workspace_size
-    assert size(1, 256, 2) == 0 and size(1, 257, 2) == 48 and size(1, 2 ** 20, 2) == 0 and size(0, 9, 9) == 0
-    for kw in (dict(ws=None, nbytes=48), dict(ws=P, nbytes=47), dict(ws=ctypes.c_void_p(8), nbytes=48)):
+    assert size(1, 256, 2) == 0 and size(1, 257, 2) == 16 and size(1, 65, 8) == 16 and size(2, 65, 9) == 48 and size(1, 2 ** 20, 2) == 0 and size(0, 9, 9) == 0
+    for kw in (dict(ws=None, nbytes=16), dict(ws=P, nbytes=15), dict(ws=ctypes.c_void_p(8), nbytes=16)):
         assert write(n=257, status=P, **kw) == L.HN_E_ARG and "workspace" in err(), kw
 
     def attend(page=64, D=128, Hq=4, causal=0, cur=0, scale=0.1, q=P, cs=st, ws=None, nbytes=0, width=2, Lq=1,
