@@ -626,6 +626,34 @@ def test_captured_calls_follow_the_tables(dev):
         _check((out, lse), _reference(q, pool, table, [x + 1 for x in n]), f"replay {i}")
 
 
+@rooms
+@pytest.mark.parametrize("B,Lq,causal", [(2, 1, False), (2, 40, True), (2, 300, True), (2, 300, False), (150, 1, False), (1, 3, True)])
+def test_every_kernel_captured(dev, B, Lq, causal, room):
+    """One captured call, replayed over other lengths and tables with eager calls between."""
+    _, ca, _ = _mods()
+    H, page, width = 2, 64, max(13, room // 64)
+    g = torch.Generator(device=dev).manual_seed(B + Lq)
+    pool = _pool(dev, g, 13 * B, page, H)
+    table = torch.full((B, width), -1, dtype=I32, device=dev)
+    lens = torch.zeros(B, dtype=I32, device=dev)
+    q = torch.randn(B, Lq, 2 * H, 128, device=dev, generator=g).to(BF16)
+    call = lambda: ca.paged_attention(q, pool, table, lens, causal=causal)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = call()
+    for i in range(4):
+        table[:, :13] = torch.randperm(13 * B, generator=torch.Generator().manual_seed(i)).view(B, 13).to(dev, I32)
+        lens.copy_(torch.randint(0, 13 * page + 1, (B,), generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        got = out.clone(), lse.clone()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+        if i == 3:
+            _check(got, _reference(q, pool, table, lens.tolist(), causal=causal), f"B {B} Lq {Lq}")
+
+
 def test_calls_on_two_streams(dev):
     _, ca, _ = _mods()
     H, page, lens = 2, 64, (3000, 2000)
