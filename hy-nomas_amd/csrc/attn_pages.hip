@@ -95,6 +95,15 @@ HN_DEVICE f32x4_ mfma16_bf16(const bf16x8& a, const bf16x8& b, const f32x4_& c) 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// What a wave's lanes have written to LDS before is there for its other lanes after, and what
+// they have read is read. It binds the compiler: the wave's LDS instructions run in their
+// order as it is, and the kernels are compiled to the same ones with it.
+HN_DEVICE void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // How far (log2) a logit may pass the point that a row's probabilities refer to.
 constexpr float TOP_HIGH = 8.0f;
 
@@ -335,11 +344,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && RB == 1 ? 3 : 2) void attn_page
             const float ks[2] = {x.ks[0], x.ks[1]};
 #pragma unroll
             for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(kt_in + 8 * i * D) = x.k[i];
+            wave_exchange();
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     kx[t][e] = *reinterpret_cast<const uint4*>(kt + (16 * t + r16) * D + 16 * ((g + 4 * e) ^ (r16 & 7)));
+            wave_exchange();  // (the next block's codes, or the item's result, go there)
             __builtin_amdgcn_sched_barrier(0);
             load_k(next);
             __builtin_amdgcn_sched_barrier(0);
