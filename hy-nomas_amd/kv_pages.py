@@ -285,12 +285,13 @@ class PageBatch:
                softmax_scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Attention of q [B, Lq, Hq, D]: with k_cur/v_cur over the tokens before the pass
         and those, without over the tokens written by it too (paged_attention). Causal
-        queries stand as write's rows do: query i is the sequence's i-th new token, and
-        one past them sees what the last does. Fewer or more of them than write's rows are
-        every sequence's last Lq tokens."""
+        queries are every sequence's last Lq tokens. Where the sequences add different
+        numbers of tokens, Lq queries, as many as the longest adds or more (padding), stand
+        as write's rows do: query i is the sequence's i-th new token, and one past them
+        sees what the last does."""
         from .cache_attention import paged_attention
         self._check()
-        rows = causal and self.counts is not None and q.shape[1] == max(self.adds)
+        rows = causal and self.counts is not None and q.shape[1] >= max(self.adds)
         return paged_attention(q, self.cache.layer(layer), self.table, self.end if k_cur is None else self.start,
                                causal=causal, k_cur=k_cur, v_cur=v_cur, cur_valid=cur_valid,
                                softmax_scale=softmax_scale, q_start=self.start if rows else None)

@@ -814,3 +814,36 @@ def test_drafted_tokens(dev):
     batch.write(0, k1, v1)
     again = batch.attend(0, q1)
     assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+
+
+# --------------------------------------------------------------------------
+# padded batches
+
+@rooms
+@pytest.mark.parametrize("adds,rows", [((7, 5), 16), ((40, 0, 3), 100), ((70, 64), 128), ((129, 200, 1), 256)])
+def test_rows_padded_past_the_longest_addition(dev, adds, rows, room):
+    """Writes and causal queries of more rows than any sequence adds: each sequence's rows as
+    alone, whatever the padding holds (few rows, the 4-wave tiles, the 8-wave ones)."""
+    kp, _, _ = _mods()
+    H, G, B = 2, 2, len(adds)
+    g = torch.Generator(device=dev).manual_seed(rows)
+    cache = kp.PagedKVCache(1, 40 + B * (room // 64), H, page=64, device=dev)
+    seqs = [cache.new() for _ in adds]
+    old = [50 + 37 * b + room // 2 for b in range(B)]
+    batch = cache.open(seqs, old)
+    k, v = torch.randn(2, B, max(old), H, 128, device=dev, generator=g).to(BF16)
+    batch.write(0, k, v)
+    batch.commit()
+    batch = cache.open(seqs, adds)
+    k, v = torch.randn(2, B, rows, H, 128, device=dev, generator=g).to(BF16)
+    q = torch.randn(B, rows, H * G, 128, device=dev, generator=g).to(BF16)
+    for b, n in enumerate(adds):
+        k[b, n:], v[b, n:] = float("nan"), float("inf")
+    batch.write(0, k, v)
+    out, lse = batch.attend(0, q, causal=True)
+    batch.commit()
+    for b, (s, n) in enumerate(zip(seqs, adds)):
+        one = cache.open([s])
+        assert cache.length(s) == old[b] + n
+        want = _reference(q[b:b + 1], cache.layer(0), one.table, (old[b] + n,), causal=True, first=(old[b],))
+        _check((out[b:b + 1], lse[b:b + 1]), want, f"adds {adds}, sequence {b}")

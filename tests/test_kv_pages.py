@@ -408,3 +408,24 @@ def test_model_refusals():
             call()
     with pytest.raises(ValueError, match="steps branches"):
         plain.generate_chunk(torch.zeros(1, 4, 256), [], None, [0.0], branches=[0])
+
+
+@pytest.mark.parametrize("adds,rows,at_start", [([7, 5], 7, True), ([7, 5], 16, True), ([7, 0], 8, True),
+                                                ([7, 5], 6, False), ([7, 7], 7, False), ([7, 7], 16, False),
+                                                ([0, 0], 3, False)])
+def test_where_causal_queries_of_a_batch_stand(monkeypatch, adds, rows, at_start):
+    """Sequences that add different numbers of tokens: as many queries as the longest adds,
+    or more of them (padding), start at each sequence's first new token, as write's rows do."""
+    kp, ca = pkg_module("kv_pages"), pkg_module("cache_attention")
+    cache = kp.PagedKVCache(1, 8, 1, page=64, device="cpu")
+    seqs = [cache.new(), cache.new()]
+    cache.open(seqs, [20, 3]).commit()
+    batch, seen = cache.open(seqs, adds), []
+    monkeypatch.setattr(kp, "write_pages", lambda *a, **kw: None)
+    monkeypatch.setattr(ca, "paged_attention", lambda *a, **kw: seen.append((a[3].tolist(), kw["q_start"])))
+    kv = torch.zeros(2, max(max(adds), rows if len(set(adds)) > 1 else 0), 1, 128, dtype=BF16)
+    batch.write(0, kv, kv)
+    batch.attend(0, torch.zeros(2, rows, 1, 128, dtype=BF16), causal=True)
+    (end, start), = seen
+    assert end == [20 + adds[0], 3 + adds[1]]
+    assert (start.tolist() == [20, 3]) if at_start else start is None
