@@ -241,8 +241,8 @@ class PageBatch:
     ``write`` puts a layer's new tokens into the pages, ``attend`` runs a layer's
     attention; ``commit`` makes the new tokens part of the sequences once every layer has
     written them. A batch that is not committed leaves the sequences as they were. Once
-    one of its sequences is committed, cut, freed or moved, or one that it adds to is opened
-    to grow again, it is refused (ValueError)."""
+    it is committed or discarded, one of its sequences grows, is cut, freed or moved, or one
+    that it adds to is opened to grow again, it is refused (ValueError)."""
 
     def __init__(self, cache: PagedKVCache, seqs: list[int], adds: list[int]):
         self.cache, self.seqs, self.adds = cache, seqs, adds
@@ -261,11 +261,14 @@ class PageBatch:
         self.start, self.end, counts = flat[:3 * B].view(3, B).unbind(0)    # tokens before and after the pass
         self.table = flat[3 * B:].view(B, width)
         self.counts = None if len(set(adds)) <= 1 else counts
+        self._over = False
 
     def _check(self) -> None:
+        if self._over:
+            raise ValueError("the batch is past: it was committed or discarded")
         stamp, turn = self.cache._stamp, self.cache._turn
         if any(stamp.get(s) != n for s, n in zip(self.seqs, self._stamps)):
-            raise ValueError("the batch is past: a sequence was committed, cut, freed or moved since it was opened")
+            raise ValueError("the batch is past: a sequence grew, was cut, freed or moved since it was opened")
         if any(turn[s] != n for s, n in self._turns):
             raise ValueError("the batch is past: a sequence that it adds to was opened to grow again")
 
@@ -297,14 +300,19 @@ class PageBatch:
                                softmax_scale=softmax_scale, q_start=self.start if rows else None)
 
     def commit(self) -> None:
-        """The new tokens stand; the batch is of no use afterwards."""
+        """The new tokens stand; the batch is of no use afterwards. Sequences to which it adds
+        nothing, and other passes over those, go on."""
         self._check()
+        self._over = True
         for s, n, a in zip(self.seqs, self.lengths, self.adds):
-            self.cache._length[s] = n + a
-            self.cache._stamp[s] += 1
+            if a:
+                self.cache._length[s] = n + a
+                self.cache._stamp[s] += 1
 
     def discard(self) -> None:
         """Give up the pass: the room that was taken for it is free again."""
         self._check()
-        for s, n in zip(self.seqs, self.lengths):
-            self.cache.truncate(s, n)
+        self._over = True
+        for s, n, a in zip(self.seqs, self.lengths, self.adds):
+            if a:
+                self.cache.truncate(s, n)

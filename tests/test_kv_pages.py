@@ -429,3 +429,24 @@ def test_where_causal_queries_of_a_batch_stand(monkeypatch, adds, rows, at_start
     (end, start), = seen
     assert end == [20 + adds[0], 3 + adds[1]]
     assert (start.tolist() == [20, 3]) if at_start else start is None
+
+
+def test_a_pass_ends_no_pass_of_a_sequence_that_it_only_reads():
+    """commit and discard leave sequences alone to which their batch adds nothing: the room
+    that another pass took for one, and that pass, stand."""
+    kp = pkg_module("kv_pages")
+    for end in ("commit", "discard"):
+        cache = kp.PagedKVCache(1, 12, 1, device="cpu")
+        a, b = cache.new(), cache.new()
+        cache.open([a, b], [70, 3]).commit()
+        grows, reads, twice, mixed = cache.open([b], 200), cache.open([b]), cache.open([a, a]), cache.open([a, b], [9, 0])
+        room, free = list(cache._table[b]), cache.free_pages
+        for batch in (reads, twice, mixed):
+            getattr(batch, end)()
+            assert cache._table[b] == room and cache.free_pages == free
+            with pytest.raises(ValueError, match="past"):  # (it is over itself)
+                getattr(batch, end)()
+        assert cache.length(a) == (79 if end == "commit" else 70) and cache.length(b) == 3
+        grows.commit()
+        assert cache.length(b) == 203
+        _whole(cache)
