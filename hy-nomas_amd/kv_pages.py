@@ -108,7 +108,7 @@ class PagedKVCache:
             raise ValueError("layers and pages must be positive")
         self.pool = make_pages(pages, heads, dim, page=page, layers=layers, code_dtype=code_dtype, device=device)
         self.layers, self.pages, self.page = layers, pages, page
-        self.device = torch.device(device)
+        self.device = self.pool["k"].device  # (with its index)
         self._views = [{n: t[i] for n, t in self.pool.items()} for i in range(layers)]
         self._free = list(range(pages))             # a heap: the lowest number is taken first
         self._refs = [0] * pages

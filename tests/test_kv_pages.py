@@ -450,3 +450,10 @@ def test_a_pass_ends_no_pass_of_a_sequence_that_it_only_reads():
         grows.commit()
         assert cache.length(b) == 203
         _whole(cache)
+
+
+def test_a_cache_is_on_its_pools_device():
+    """Whatever the name that it was given ("cuda" is another device once the current one
+    changes): the tables of later passes go where the pages are."""
+    cache = pkg_module("kv_pages").PagedKVCache(1, 4, 1, device="cpu:0")
+    assert cache.device == cache.pool["k"].device == cache.open([cache.new()], 3).table.device
