@@ -100,7 +100,8 @@ class PagedKVCache:
     commits it; ``free``, ``truncate`` and ``compact`` run between passes.
 
     The pages are the host's: numbers and lengths live there, and a batch brings its
-    tables to the GPU in one copy. All work is ordered on the current stream."""
+    tables to the GPU in one copy. All work is ordered on the current stream; ``open`` and
+    ``compact`` cannot be captured into a graph (RuntimeError)."""
 
     def __init__(self, layers: int, pages: int, heads: int, dim: int = 128, *, page: int = 64,
                  code_dtype: torch.dtype = FP8, device: torch.device | str):
@@ -117,6 +118,11 @@ class PagedKVCache:
         self._stamp: dict[int, int] = {}            # changes when a batch's view of the sequence is past
         self._turn: dict[int, int] = {}             # passes that were opened to add to the sequence
         self._next = 0
+
+    def _not_captured(self) -> None:
+        # (bookkeeping would run once, and the tables' copy replay from memory freed since)
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the pages of a PagedKVCache are the host's: open and compact cannot be captured")
 
     def layer(self, i: int) -> dict:
         """Layer i's pool, as write_pages and paged_attention take it."""
@@ -178,6 +184,7 @@ class PagedKVCache:
         pages that they would write but share are copied; ValueError, with nothing
         changed, if the pool has not enough. A sequence grows in one pass at a time: an
         earlier batch that was to add to it is past."""
+        self._not_captured()
         seqs = [self._known(s) for s in seqs]
         adds = [tokens] * len(seqs) if isinstance(tokens, int) else list(tokens)
         if len(adds) != len(seqs) or min(adds, default=0) < 0:
@@ -219,6 +226,7 @@ class PagedKVCache:
     def compact(self) -> int:
         """Move the pages in use to the lowest numbers (one copy over all layers); returns
         how many were moved. Batches opened before are of no use afterwards."""
+        self._not_captured()
         used = [p for p in range(self.pages) if self._refs[p]]
         n = len(used)
         src = [p for p in used if p >= n]

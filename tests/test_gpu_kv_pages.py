@@ -847,3 +847,42 @@ def test_rows_padded_past_the_longest_addition(dev, adds, rows, room):
         assert cache.length(s) == old[b] + n
         want = _reference(q[b:b + 1], cache.layer(0), one.table, (old[b] + n,), causal=True, first=(old[b],))
         _check((out[b:b + 1], lse[b:b + 1]), want, f"adds {adds}, sequence {b}")
+
+
+def test_a_pass_opened_before_a_capture(dev):
+    """open and compact are refused inside a capture, which goes on; write and attend of a
+    batch from before it replay over new values."""
+    kp, _, _ = _mods()
+    H = 2
+    g = torch.Generator(device=dev).manual_seed(8)
+    cache = kp.PagedKVCache(1, 12, H, page=64, device=dev)
+    seqs = [cache.new(), cache.new()]
+    k, v = torch.randn(2, 2, 100, H, 128, device=dev, generator=g).to(BF16)
+    batch = cache.open(seqs, [100, 64])
+    batch.write(0, k, v)
+    batch.commit()
+    batch = cache.open(seqs, 3)
+    q, k, v = torch.randn(3, 2, 3, H, 128, device=dev, generator=g).to(BF16)
+    status = torch.zeros(1, dtype=I32, device=dev)
+
+    def step():
+        batch.write(0, k, v, status=status)
+        return batch.attend(0, q, causal=True)
+
+    step()
+    graph, free = torch.cuda.CUDAGraph(), cache.free_pages
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.open(seqs, 1), cache.compact):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        out, lse = step()
+    assert cache.free_pages == free
+    for i in range(3):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device=dev, generator=g).to(BF16))
+        graph.replay()
+        got = out.clone(), lse.clone()
+        eager = step()
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1]) and status.item() == 0
+    _check(got, _reference(q, cache.layer(0), batch.table, (103, 67), causal=True), "replayed")
+    batch.commit()

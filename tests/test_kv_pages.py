@@ -457,3 +457,19 @@ def test_a_cache_is_on_its_pools_device():
     changes): the tables of later passes go where the pages are."""
     cache = pkg_module("kv_pages").PagedKVCache(1, 4, 1, device="cpu:0")
     assert cache.device == cache.pool["k"].device == cache.open([cache.new()], 3).table.device
+
+
+def test_no_pass_is_captured(monkeypatch):
+    """A replay would bring the tables of the recorded pass again, from host memory that is
+    another's by then, and repeat its copies: refused, with nothing changed."""
+    cache = pkg_module("kv_pages").PagedKVCache(1, 6, 1, device="cpu")
+    a = cache.new()
+    cache.open([a], 70).commit()
+    b = cache.fork(a)
+    state = list(cache._refs), {s: list(t) for s, t in cache._table.items()}, list(cache._free)
+    monkeypatch.setattr(cache, "device", torch.device("cuda", 0))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: cache.open([b], 1), lambda: cache.open([b]), cache.compact):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    assert state == (cache._refs, cache._table, cache._free)
