@@ -81,7 +81,8 @@ def sparse_chunk_attention(q: torch.Tensor, kv_cache: dict, kv_len: int, block_i
     ended by the first negative entry; None reads the whole cache. Hq may be a
     multiple of the cache's heads. Every listed key is visible to the run's queries;
     cache_valid and cur_valid are as in chunk_attention. A query without a key gets
-    a zero row and lse -inf, one that meets a NaN gets NaN in both.
+    a zero row and lse -inf, one that meets a NaN in itself or a key gets NaN in both, in
+    a value in the output alone.
     """
     if not is_quantized_kv_cache(kv_cache):
         raise TypeError("sparse_chunk_attention reads FP8/INT8 caches")
@@ -103,8 +104,11 @@ def paged_attention(q: torch.Tensor, cache: dict, table: torch.Tensor, kv_len: t
     of the pool's heads. Without ``causal`` every query sees its sequence's tokens and the
     valid tail (cur_valid bool [B or 1, >= Lc]); with it query i is the sequence's token
     q_start[b] + i, written already (int32 [B]; None: the queries are its last Lq tokens),
-    and sees those up to itself. A query without a key gets a zero row and lse -inf, one that meets a NaN gets NaN in both. Entries of
-    the table outside the pool name no keys.
+    and sees those up to itself. A query without a key gets a zero row and lse -inf, one
+    that meets a NaN in itself or a key gets NaN in both, in a value in the output alone.
+    A value that is not finite (a checked write stores none) can make the outputs of causal
+    queries before its token NaN too; finite ones, and any key, have no part in them.
+    Entries of the table outside the pool name no keys.
     """
     if not is_quantized_kv_cache(cache):
         raise TypeError("paged_attention reads FP8/INT8 caches")

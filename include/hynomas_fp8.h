@@ -350,7 +350,7 @@ int64_t hn_select_kv_blocks_workspace_size(int64_t B, int64_t H, int64_t runs, i
  * and the valid tail keys. A list ends at its first negative entry; an entry past
  * the last block is ignored; a block that is listed twice counts twice. idx NULL:
  * every cached token (`top_k` and `is` are unused). A row without a key gets zeros and -inf,
- * a row that meets a NaN gets NaN in both.
+ * one that meets a NaN in its query or a key gets NaN in both, in a V in out alone.
  * What masked keys and the cache past kv_len hold (Inf and NaN included) does not
  * matter.
  *   idx: int32 [B, H, runs, top_k], runs = ceil(Lq / q_block), strides is[3] of
@@ -469,11 +469,15 @@ int hn_kv_pages_copy(void *const *base, const int64_t *layer_stride, const int64
  *   out = softmax(softmax_scale q K^T) V, lse = ln sum exp(softmax_scale q . K).
  * causal (without a tail): query i sees tokens t <= q_start[b] + i (int32 [B]) of the
  * sequence; with q_start null the queries are its last Lq tokens, q_start[b] = lens[b] -
- * Lq. A row without a key gets zeros and -inf, one that meets a NaN gets NaN in both. What
- * lies behind a sequence's end does not matter.
+ * Lq. A row without a key gets zeros and -inf, one that meets a NaN in its query or a key
+ * gets NaN in both, in a V in out alone (lse is the keys'). What lies behind a sequence's
+ * end does not matter. Nor do keys and finite values of later tokens to a causal row; a V
+ * that is NaN or Inf (hn_kv_pages_write with a status stores none) can reach, as 0 * V, the
+ * output of rows before its token.
  *   kcur, vcur, cur_valid, out and lse as in hn_attn_kv_blocks. Probabilities are held to
  *   2^-17 of themselves (the sum of two bf16) where a cached head has up to 32 rows, Lq Hq
- *   / H of them, or up to 64 and room for more than 4096 keys, and V is bf16 there; else
+ *   / H of them, or up to 64 and room for more than 4096 keys, and V is bf16 there (its
+ *   fp32 sums hold up to 2^8 |V| a key); else
  *   probabilities and V are fp16 as in hn_attn_kv_blocks.
  * workspace: hn_attn_kv_pages_workspace_size(.., width * page, ..) bytes, 16-byte aligned. */
 int hn_attn_kv_pages(int fmt, const void *q, const int64_t *qs, int64_t B, int64_t Lq, int64_t Hq, int64_t D,

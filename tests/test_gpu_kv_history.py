@@ -1114,3 +1114,23 @@ def test_attention_of_small_values(dev, Lq, q_block):
     if q_block == 1:
         bound = ref[2] - 2.0 ** -24                        # without the term for V's last place
         assert ((got[0].to(F64) - ref[0]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("kv", [500, 20000])
+@pytest.mark.parametrize("Lq,q_block", [(4, 1), (20, 20), (50, 50), (100, 100)])
+def test_attention_of_a_nan_value(dev, Lq, q_block, kv):
+    """A NaN among the values is in the outputs of the head's rows alone: the log-sum-exp is
+    the keys'."""
+    ca = pkg_module("cache_attention")
+    g = _gen(dev, 190 + Lq)
+    cache = _cache(dev, 1, kv, 2, "fp8", g)
+    q = torch.randn(1, Lq, 2, D, device=dev, generator=g).to(BF16)
+    n = -(-kv // 64)
+    idx = torch.arange(n, dtype=torch.int32, device=dev).expand(1, 2, -(-Lq // q_block), n)
+    ref = _attend(q, cache, kv, idx, 64, q_block, None, None, None, None)
+    cache["v_scale"][0, 77, 1] = float("nan")
+    for lists in (idx, None):
+        out, lse = ca.sparse_chunk_attention(q, cache, kv, lists, q_block=q_block)
+        assert torch.isnan(out[:, :, 1]).all()
+        assert ((out[:, :, 0].to(F64) - ref[0][:, :, 0]).abs() <= ref[2][:, :, 0]).all()
+        assert ((lse.to(F64) - ref[1]).abs() <= ref[3]).all()

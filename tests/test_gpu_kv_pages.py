@@ -886,3 +886,59 @@ def test_a_pass_opened_before_a_capture(dev):
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1]) and status.item() == 0
     _check(got, _reference(q, cache.layer(0), batch.table, (103, 67), causal=True), "replayed")
     batch.commit()
+
+
+# --------------------------------------------------------------------------
+# what is not finite, and causal rows before it
+
+def _before_and_after(fmt, Lq, G, room, dev):
+    _, ca, _ = _mods()
+    H, page, lens = 2, 64, (700, 230)
+    g = torch.Generator(device=dev).manual_seed(Lq + G)
+    pool = _pool(dev, g, 20, page, H, fmt)
+    table = _table(dev, g, lens, page, 20, room=room)
+    q = torch.randn(2, Lq, H * G, 128, device=dev, generator=g).to(BF16)
+    at = max(1, Lq // 2)  # the row from which on sequence 0's special token is seen
+    place = lens[0] - Lq + at
+    where = table[0, place // page].item(), place % page, 1
+    return ca, pool, table, q, lens, at, where
+
+
+few_and_tiles = pytest.mark.parametrize("Lq,G", [(8, 1), (9, 3), (40, 1), (70, 1), (33, 5), (300, 1)])
+
+
+@rooms
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@few_and_tiles
+def test_a_nan_key_reaches_the_rows_that_see_it(dev, fmt, Lq, G, room):
+    """NaN in both outputs of those rows and that cached head, no other row differs."""
+    ca, pool, table, q, lens, at, where = _before_and_after(fmt, Lq, G, room, dev)
+    want = _reference(q, pool, table, lens, causal=True)
+    pool["k_scale"][where] = float("nan")
+    out, lse = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
+    assert torch.isnan(out[0, at:, G:]).all() and torch.isnan(lse[0, G:, at:]).all()
+    out[0, at:, G:], lse[0, G:, at:] = want[0][0, at:, G:].to(BF16), want[1][0, G:, at:].float()
+    _check((out, lse), want, f"{fmt} Lq {Lq} G {G}")
+
+
+@rooms
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@few_and_tiles
+def test_values_that_causal_rows_do_not_see(dev, fmt, Lq, G, room):
+    """A finite V, past fp16's range too, has no part in the rows before its token. A NaN one
+    makes the outputs NaN of the rows that see it; the log-sum-exp is the keys' alone."""
+    ca, pool, table, q, lens, at, where = _before_and_after(fmt, Lq, G, room, dev)
+    want = _reference(q, pool, table, lens, causal=True)
+    n = _i32(dev, lens)
+    for big in (70000.0, 1e30, 3e38):
+        pool["v_scale"][where] = big / (448 if fmt == "fp8" else 127)
+        out, lse = ca.paged_attention(q, pool, table, n, causal=True)
+        out[0, at:, G:] = want[0][0, at:, G:].to(BF16)  # (rows that see it have sums of their own range)
+        _check((out, lse), want, f"V {big}, {fmt} Lq {Lq} G {G}")
+    for bad in (float("nan"), float("inf")):
+        pool["v_scale"][where] = bad
+        out, lse = ca.paged_attention(q, pool, table, n, causal=True)
+        seen = out[0, at:, G:]
+        assert (torch.isnan(seen) if bad != bad else ~torch.isfinite(seen)).all()
+        out[0, :, G:] = want[0][0, :, G:].to(BF16)
+        _check((out, lse), want, f"V {bad}, {fmt} Lq {Lq} G {G}")
