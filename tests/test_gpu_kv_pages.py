@@ -942,3 +942,99 @@ def test_values_that_causal_rows_do_not_see(dev, fmt, Lq, G, room):
         assert (torch.isnan(seen) if bad != bad else ~torch.isfinite(seen)).all()
         out[0, :, G:] = want[0][0, :, G:].to(BF16)
         _check((out, lse), want, f"V {bad}, {fmt} Lq {Lq} G {G}")
+
+
+# --------------------------------------------------------------------------
+# instances and promises that the tests above leave open
+
+@rooms
+@pytest.mark.parametrize("page", [64, 256])
+@pytest.mark.parametrize("Lq,G", [(5, 4), (9, 4), (33, 1), (70, 3), (129, 1), (300, 1), (101, 5)])
+def test_causal_int8(dev, page, Lq, G, room):
+    _, ca, _ = _mods()
+    lens = (Lq, 1000, max(1, Lq // 2), 0, 513 + Lq)
+    g = torch.Generator(device=dev).manual_seed(page + Lq)
+    pages = sum(-(-n // page) for n in lens) + 1
+    pool = _pool(dev, g, pages, page, 2, "int8")
+    table = _table(dev, g, lens, page, pages, room=room)
+    q = torch.randn(len(lens), Lq, 2 * G, 128, device=dev, generator=g).to(BF16)
+    got = ca.paged_attention(q, pool, table, _i32(dev, lens), causal=True)
+    _check(got, _reference(q, pool, table, lens, causal=True), f"page {page} Lq {Lq} G {G}")
+
+
+@rooms
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("B,Lq,Lc,masked,causal", [(2, 1, 70, True, False), (2, 20, 0, False, True), (2, 40, 65, False, False),
+                                                   (2, 40, 65, True, False), (2, 300, 65, False, False),
+                                                   (2, 300, 65, True, False), (2, 300, 0, False, True),
+                                                   (150, 1, 3, True, False), (150, 16, 0, False, True)])
+def test_tails_and_formats_captured(dev, fmt, B, Lq, Lc, masked, causal, room):
+    """One captured call of each form, replayed over other lengths, tables and masks with eager
+    calls between."""
+    _, ca, _ = _mods()
+    H, page, width = 2, 64, max(13, room // 64)
+    g = torch.Generator(device=dev).manual_seed(B + Lq + Lc)
+    pool = _pool(dev, g, 13 * B, page, H, fmt)
+    table = torch.full((B, width), -1, dtype=I32, device=dev)
+    lens = torch.zeros(B, dtype=I32, device=dev)
+    q = torch.randn(B, Lq, 2 * H, 128, device=dev, generator=g).to(BF16)
+    kw = dict(causal=causal)
+    if Lc:
+        kv = torch.randn(2, B, Lc, H, 128, device=dev, generator=g).to(BF16)
+        kw.update(k_cur=kv[0], v_cur=kv[1])
+    if masked:
+        kw["cur_valid"] = torch.ones(B, Lc, dtype=torch.bool, device=dev)
+    call = lambda: ca.paged_attention(q, pool, table, lens, **kw)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = call()
+    for i in range(3):
+        now = torch.Generator().manual_seed(i)
+        table[:, :13] = torch.randperm(13 * B, generator=now).view(B, 13).to(dev, I32)
+        lens.copy_(torch.randint(0, 13 * page + 1, (B,), generator=now))
+        if masked:
+            kw["cur_valid"].copy_(torch.rand(B, Lc, generator=now) < 0.6)
+        graph.replay()
+        got = out.clone(), lse.clone()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+    if B < 10:
+        _check(got, _reference(q, pool, table, lens.tolist(), **kw), f"{fmt} Lq {Lq} Lc {Lc}")
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("Lq,G,room", [(1, 1, 0), (1, 16, 5120), (4, 8, 0), (4, 8, 5120), (1, 64, 5120), (64, 1, 5120)])
+def test_probabilities_of_few_rows(dev, fmt, Lq, G, room):
+    """Two or a few keys of nearly equal weight whose values cancel: what the probabilities'
+    rounding leaves is the output. They are held to 2^-17 of themselves (two bf16); beside it
+    the logit's fp32 sum of 128 terms, exp2 and the sums (2^-20), and half a step of bf16 at
+    the result. One bf16 would be far off."""
+    _, ca, _ = _mods()
+    H, page, lens = 2, 64, (2, 8, 34, 300)
+    B = len(lens)
+    g = torch.Generator(device=dev).manual_seed(Lq + G)
+    pool = _pool(dev, g, 9, page, H, fmt)
+    for n in ("v", "v_scale"):  # odd tokens: the values of the one before, negated
+        pool[n][:, 1::2] = pool[n][:, ::2]
+    pool["v_scale"][:, 1::2] *= -1
+    table = _table(dev, g, lens, page, 9, room=room)
+    q = (torch.randn(B, Lq, H * G, 128, device=dev, generator=g) * 0.05).to(BF16)
+    out, lse = ca.paged_attention(q, pool, table, _i32(dev, lens))
+    ref, rlse, spread, terms = _reference(q, pool, table, lens)
+    rel = (2.0 ** -17 + 2.0 ** -20 + 2 * 129 * 2.0 ** -24 * terms).transpose(1, 2)[..., None]
+    tol = rel * spread + (ref.abs() + rel * spread) * 2.0 ** -8 + 1e-30  # (values whose codes are 0: exactly 0)
+    worst = ((out.to(F64) - ref).abs() / tol).max().item()
+    print(f"[pages] probabilities {fmt} Lq {Lq} G {G}: {worst:.2f} of the tolerance", flush=True)
+    assert worst <= 1.0
+    assert ((lse.to(F64) - rlse).abs() <= 129 * 2.0 ** -24 * terms + 2.0 ** -20 + rlse.abs() * 2.0 ** -22).all()
+    off = 0.0  # (the tolerance tells one bf16 from two)
+    for b, n in enumerate(lens):
+        k, v = (_held(pool, key, table, b, n) for key in "kv")
+        for h in range(H * G):
+            s = q[b, :, h].to(F64) @ k[:, h // G].T * 128 ** -0.5
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            once = (p.to(BF16).to(F64) @ v[:, h // G]) / p.sum(-1, keepdim=True)
+            off = max(off, ((once - ref[b, :, h]).abs() / tol[b, :, h]).max().item())
+    assert off > 1.0, off
