@@ -1038,3 +1038,56 @@ def test_probabilities_of_few_rows(dev, fmt, Lq, G, room):
             once = (p.to(BF16).to(F64) @ v[:, h // G]) / p.sum(-1, keepdim=True)
             off = max(off, ((once - ref[b, :, h]).abs() / tol[b, :, h]).max().item())
     assert off > 1.0, off
+
+
+def test_compiled_calls(dev):
+    """torch.compile keeps each op as one node; the registered ops, and calls that a profiler
+    sees, are the eager ones."""
+    kp, ca, _ = _mods()
+    H, page = 2, 64
+    g = torch.Generator(device=dev).manual_seed(11)
+    pool = _pool(dev, g, 8, page, H)
+    table = _i32(dev, [[0, 1, 2], [3, 4, 5]])
+    start, lens = _i32(dev, [5, 70]), _i32(dev, [15, 80])
+    q, k, v = torch.randn(3, 2, 10, H, 128, device=dev, generator=g).to(BF16)
+    status = torch.zeros(1, dtype=I32, device=dev)
+
+    def step(pool, q, k, v):
+        kp.write_pages(pool, k, v, table, start, status=status)
+        kp.copy_pages(pool, [1, 4], [6, 7])
+        out, lse = ca.paged_attention(q, pool, table, lens, causal=True, q_start=start)
+        tail, _ = ca.paged_attention(q, pool, table, start, k_cur=k, v_cur=v)
+        return out, lse, tail, kp.read_pages(pool, "v", table, lens, 90)
+
+    pools = [{n: t.clone() for n, t in pool.items()} for _ in range(3)]
+    eager = step(pools[0], q, k, v)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)(pools[1], q, k, v)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        seen = step(pools[2], q, k, v)
+    names = {e.key for e in prof.key_averages()}
+    assert {"hy_nomas_amd::" + n for n in ("kv_pages_write_", "kv_pages_copy_", "attn_kv_pages", "kv_pages_read")} <= names
+    for got, cache in ((compiled, pools[1]), (seen, pools[2])):
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+        for n in NAMES:
+            a, b = (x.view(torch.uint8) if n in "kv" else x for x in (cache[n], pools[0][n]))
+            assert torch.equal(a, b)
+
+
+@rooms
+@pytest.mark.parametrize("Lq", [1, 20, 40, 300])
+def test_masks_tables_and_queries_of_many_shapes(dev, Lq, room):
+    """One mask for all sequences, wider than the tail, of bytes; one table row for all; every
+    sequence's queries the same memory; a table that is part of a wider one."""
+    _, ca, _ = _mods()
+    H, page, lens, Lc = 2, 64, (300, 77, 0), 70
+    g = torch.Generator(device=dev).manual_seed(Lq)
+    pool = _pool(dev, g, 6, page, H)
+    row = torch.full((1, 9 + room // page), -1, dtype=I32, device=dev)
+    row[0, 2:7] = _i32(dev, [5, 0, 3, 1, 2])
+    table, n = row[:, 2:].expand(3, -1), _i32(dev, lens)
+    q = torch.randn(1, Lq, H, 128, device=dev, generator=g).to(BF16).expand(3, -1, -1, -1)
+    k, v = torch.randn(2, 1, Lc, H, 128, device=dev, generator=g).to(BF16).expand(2, 3, -1, -1, -1)
+    mask = (torch.rand(1, 200, device=dev, generator=g) < 0.5).to(torch.uint8)
+    want = _reference(q, pool, table, lens, k_cur=k, v_cur=v, cur_valid=mask)
+    for m in (mask, mask.bool(), mask[:, :Lc].expand(3, -1), torch.stack([mask, mask], 2)[:, :, 0]):
+        _check(ca.paged_attention(q, pool, table, n, k_cur=k, v_cur=v, cur_valid=m), want, f"{Lq} rows")
