@@ -109,6 +109,11 @@ def paged_attention(q: torch.Tensor, cache: dict, table: torch.Tensor, kv_len: t
     A value that is not finite (a checked write stores none) can make the outputs of causal
     queries before its token NaN too; finite ones, and any key, have no part in them.
     Entries of the table outside the pool name no keys.
+
+    Up to 32 rows a cached head (Lq Hq / H), and up to 64 where the table has room for more
+    than 4096 keys (W pages and the tail, whatever kv_len says), are weighed by probabilities
+    of 2^-17 over bf16 values, more by fp16 of both: a wider table can change an output's
+    last bits.
     """
     if not is_quantized_kv_cache(cache):
         raise TypeError("paged_attention reads FP8/INT8 caches")
